@@ -73,7 +73,10 @@ typedef enum uor_b200_dtype {
     UOR_B200_TROP_I8 = 8,
     UOR_B200_TROP_I16 = 9,
     UOR_B200_TROP_I32 = 10,
-    UOR_B200_TROP_I64 = 11
+    UOR_B200_TROP_I64 = 11,
+    /* 16-bit floats: activations, outputs and scales of the 4-bit family and the router only. */
+    UOR_B200_BF16 = 12,
+    UOR_B200_F16 = 13
 } uor_b200_dtype;
 
 /* ----------------------------------------------------------------- context */
@@ -108,7 +111,9 @@ typedef enum uor_b200_kernel {
     UOR_B200_KERNEL_CODED_TCGEN05 = 4, /* K1C: codebook decode feeding K1's MMA */
     UOR_B200_KERNEL_FLOAT_EXACT = 5,   /* K6+K7: exact float, one rounding */
     UOR_B200_KERNEL_EPILOGUE_ONLY = 6, /* k == 0: C := encode(beta * C) */
-    UOR_B200_KERNEL_SKINNY = 7         /* <= 16 rows or columns: dp4a reduce / column kernels */
+    UOR_B200_KERNEL_SKINNY = 7,        /* <= 16 rows or columns: dp4a reduce / column kernels */
+    UOR_B200_KERNEL_Q4 = 8,            /* 4-bit weights with group scales */
+    UOR_B200_KERNEL_ROUTER = 9         /* the experts' router and its gradient */
 } uor_b200_kernel;
 
 typedef struct uor_b200_route {
@@ -427,6 +432,93 @@ int uor_b200_arena_gemm(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_
  * *distinct receives their count, values[0 .. *distinct) is the Arena table. -0.0 and
  * +0.0, and NaNs with different payloads, are distinct symbols. Host only. */
 int uor_b200_arena_canonicalize(uor_b200_dtype elem, void *values, size_t len, size_t *distinct);
+
+/* ------------------------------------- 4-bit weights with group scales */
+
+/* Weights of `rows` x `cols` (outputs x reduction) in 4 bits:
+ *   w[j][p] = scale[j][p / group] * (code[j][p] - zero[j][p / group]),
+ * codes 0..15 two per byte, low nibble first (the order of Packed<Grid<16>, 2>), a row
+ * beginning on a byte of its own; without zero points the zero is 8. This family is not exact
+ * like the rest of the library: the products are of 16-bit floats, sums are held in f32 in an
+ * order that depends on the shapes alone (the same call gives the same bytes), and the result
+ * is rounded once to `out`. Non-finite activations and scales spread as the formula has them.
+ * No reference counterpart: the reference's codecs carry no scales. */
+typedef struct uor_b200_q4 {
+    const uint8_t *codes;
+    size_t codes_len;      /* bytes */
+    size_t rows, cols;
+    size_t row_bytes;      /* bytes from one row's codes to the next's */
+    const void *scales;    /* [rows][ceil(cols / group)] of scale_type */
+    size_t scales_len;     /* elements */
+    uint32_t scale_type;   /* F32, BF16 or F16 */
+    uint32_t group;        /* reduction positions that share a scale: a multiple of 32 */
+    size_t groups_rs;      /* elements from one row's scales (and zeros) to the next's */
+    const uint8_t *zeros;  /* one byte per scale, its low four bits read; NULL: 8 */
+    size_t zeros_len;      /* bytes; 0 with NULL */
+} uor_b200_q4;
+
+/* C := A dequant(W)^T: A m x k of elem (BF16 or F16), W k wide with n rows, C m x n of out
+ * (elem or F32). k == 0 gives zeros. DOES_NOT_FIT where the codes, scales or zeros are shorter
+ * than their shape; INVALID_ARGUMENT for a group that is no multiple of 32; only
+ * encode NEAREST is supported. */
+int uor_b200_q4_gemm(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_view *a,
+                     const uor_b200_q4 *w, const uor_b200_view_mut *c, const uor_b200_call *call);
+
+/* ------------------------------------------------ mixture of experts */
+
+typedef enum uor_b200_score {
+    UOR_B200_SOFTMAX = 0,  /* over a row's open experts */
+    UOR_B200_SIGMOID = 1
+} uor_b200_score;
+
+/* How a row of logits becomes a choice of experts. */
+typedef struct uor_b200_router {
+    uint32_t experts;     /* 1 .. 1024 */
+    uint32_t top_k;       /* 1 .. 32, at most the experts of top_groups groups */
+    uint32_t score;       /* uor_b200_score */
+    uint32_t groups;      /* equal runs of experts, at most 32; 1: no groups */
+    uint32_t top_groups;  /* groups whose experts may be chosen */
+    uint32_t renormalize; /* 1: the chosen weights are divided by their sum */
+    float scale;          /* the weights are multiplied by it, after that */
+} uor_b200_router;
+
+/* For each row (a token) of logits (tokens x experts, elem F32, BF16 or F16):
+ *   score[e] = softmax(logits)[e] or 1 / (1 + exp(-logit[e])), in f32;
+ *   key[e]   = score[e] + bias[e] (bias: experts floats, or NULL); the bias steers the choice
+ *              and is no part of the weights;
+ *   with top_groups < groups: a group's score is the sum of its two largest keys (its one,
+ *              in groups of one), and only experts of the top_groups best groups stay open;
+ *   ids[t][..] (int32) = the top_k largest keys' experts, largest first, ties to the lowest
+ *              index; weights[t][..] (f32) = their scores, renormalised and scaled.
+ * An expert whose logit is -inf or NaN, or whose key is, is closed: it is never chosen, and its
+ * score is 0. Where fewer than top_k are open the rest have id -1 and weight 0. Renormalised
+ * weights are shares of the true scores, also where f32 has those as 0; where no chosen score
+ * is above exp(-700) (logits of the type's lowest value) a sigmoid's are 0. */
+int uor_b200_expert_route(uor_b200_dtype elem, const uor_b200_router *router,
+                          const uor_b200_view *logits, const float *bias, size_t bias_len,
+                          const uor_b200_view_mut *ids, const uor_b200_view_mut *weights,
+                          const uor_b200_call *call);
+
+/* The gradient of the logits (tokens x experts, of elem) from that of the weights (tokens x
+ * top_k, f32), with the choice `ids` held fixed: the choice, and so the bias, has no gradient.
+ * ids outside [0, experts) take no part; every element of dlogits is written. */
+int uor_b200_expert_route_backward(uor_b200_dtype elem, const uor_b200_router *router,
+                                   const uor_b200_view *logits, const uor_b200_view *ids,
+                                   const uor_b200_view *dweights, const uor_b200_view_mut *dlogits,
+                                   const uor_b200_call *call);
+
+/* The chosen experts' gated feed-forward layer over 4-bit weights:
+ *   y[t] = sum_s weights[t][s] * down_e (silu(gate_e x[t]) * (up_e x[t])),  e = ids[t][s],
+ * silu(v) = v / (1 + exp(-v)). x is tokens x d of elem (BF16 or F16), y tokens x d of out (elem
+ * or F32). `up` holds every expert's gate rows and then its up rows: experts * 2 f rows of d;
+ * `down` experts * d rows of f. ids (int32) and weights (f32) are tokens x top_k; an id outside
+ * [0, experts) is skipped, whatever its weight, and a token without any gets zeros. The inner
+ * activations are rounded once to elem between the two products. */
+int uor_b200_expert_q4_ffn(uor_b200_dtype elem, uor_b200_dtype out, size_t experts,
+                           const uor_b200_view *x, const uor_b200_view *ids,
+                           const uor_b200_view *weights, const uor_b200_q4 *up,
+                           const uor_b200_q4 *down, const uor_b200_view_mut *y,
+                           const uor_b200_call *call);
 
 /* ------------------------------------------------- split-K across devices */
 

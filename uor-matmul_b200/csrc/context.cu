@@ -26,6 +26,8 @@ size_t dtype_size(uor_b200_dtype t) {
     case UOR_B200_TROP_I16: return 4;
     case UOR_B200_TROP_I32: return 8;
     case UOR_B200_TROP_I64: return 16;
+    case UOR_B200_BF16: return 2;
+    case UOR_B200_F16: return 2;
     default: return 0;
     }
 }

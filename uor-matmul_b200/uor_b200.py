@@ -22,13 +22,14 @@ LIB_PATH = os.path.join(HERE, "libuor_b200.so")
 OK, NONCONFORMANT, OUTPUT_ALIASES, DEVICE_ERROR, TIMEOUT, NCCL_ERROR, DOES_NOT_FIT, \
     INVALID_ARGUMENT, UNSUPPORTED = range(9)
 NEAREST, TOWARD_ZERO, SATURATING, WRAPPING = range(4)
-I8, I16, I32, I64, I128, F32, F64, TROP_I8, TROP_I16, TROP_I32, TROP_I64 = range(1, 12)
+I8, I16, I32, I64, I128, F32, F64, TROP_I8, TROP_I16, TROP_I32, TROP_I64, BF16, F16 = range(1, 14)
 DEVICE_POINTERS, ASYNC, DIGIT_SLICES, MODULAR, CODEC_ON_CHIP = 1, 2, 4, 8, 16
 KERNEL_NAMES = {0: "none", 1: "i8_tcgen05", 2: "limb_tcgen05", 3: "tropical",
-                4: "coded_tcgen05", 5: "float_exact", 6: "epilogue_only", 7: "skinny_dp4a"}
+                4: "coded_tcgen05", 5: "float_exact", 6: "epilogue_only", 7: "skinny_dp4a",
+                8: "q4", 9: "router"}
 
 DTYPE_SIZE = {I8: 1, I16: 2, I32: 4, I64: 8, I128: 16, F32: 4, F64: 8,
-              TROP_I8: 2, TROP_I16: 4, TROP_I32: 8, TROP_I64: 16}
+              TROP_I8: 2, TROP_I16: 4, TROP_I32: 8, TROP_I64: 16, BF16: 2, F16: 2}
 
 
 class UorError(RuntimeError):
@@ -73,6 +74,45 @@ class Codec(ctypes.Structure):
 
 
 TIER_GRID, TIER_SIGN, TIER_TERNARY, TIER_BOOK = range(4)
+
+
+class Q4(ctypes.Structure):
+    """uor_b200_q4: rows x cols weights in 4 bits, codes two per byte, low nibble first, with a
+    scale (and a zero point, else 8) per row and `group` positions of the reduction. Holds the
+    arrays it describes, so one descriptor serves as many calls as its program makes."""
+    _fields_ = [("codes", ctypes.c_void_p), ("codes_len", ctypes.c_size_t),
+                ("rows", ctypes.c_size_t), ("cols", ctypes.c_size_t),
+                ("row_bytes", ctypes.c_size_t), ("scales", ctypes.c_void_p),
+                ("scales_len", ctypes.c_size_t), ("scale_type", ctypes.c_uint32),
+                ("group", ctypes.c_uint32), ("groups_rs", ctypes.c_size_t),
+                ("zeros", ctypes.c_void_p), ("zeros_len", ctypes.c_size_t)]
+
+    def __init__(self, codes, scales, scale_type, rows, cols, group, zeros=None, row_bytes=None,
+                 groups_rs=None):
+        pc, lc, dev = _buffer(codes)
+        ps, ls, _ = _buffer(scales)
+        pz, lz = _buffer(zeros)[:2] if zeros is not None else (None, 0)
+        if (_on_device(codes, scales) if zeros is None else _on_device(codes, scales, zeros)) != dev:
+            raise ValueError("operands must all be host arrays or all be CUDA tensors")
+        super().__init__(pc, lc, rows, cols, (cols + 1) // 2 if row_bytes is None else row_bytes,
+                         ps, ls, scale_type, group,
+                         -(-cols // max(group, 1)) if groups_rs is None else groups_rs, pz, lz)
+        self.arrays, self.on_device = (codes, scales, zeros), dev
+
+
+SOFTMAX, SIGMOID = range(2)
+
+
+class Router(ctypes.Structure):
+    """uor_b200_router: how a row of logits becomes a choice of experts."""
+    _fields_ = [("experts", ctypes.c_uint32), ("top_k", ctypes.c_uint32),
+                ("score", ctypes.c_uint32), ("groups", ctypes.c_uint32),
+                ("top_groups", ctypes.c_uint32), ("renormalize", ctypes.c_uint32),
+                ("scale", ctypes.c_float)]
+
+    def __init__(self, experts, top_k, score=SOFTMAX, groups=1, top_groups=1, renormalize=True,
+                 scale=1.0):
+        super().__init__(experts, top_k, score, groups, top_groups, int(renormalize), scale)
 
 
 class Call(ctypes.Structure):
@@ -140,6 +180,11 @@ def lib():
             "uor_b200_nccl_unique_id": ([P, Z], I),
             "uor_b200_nccl_comm_init": ([P, I, P, Z, I, ctypes.POINTER(P)], I),
             "uor_b200_nccl_comm_destroy": ([P], I),
+            "uor_b200_q4_gemm": ([I, I, VP, ctypes.POINTER(Q4), VP, CP], I),
+            "uor_b200_expert_route": ([I, ctypes.POINTER(Router), VP, P, Z, VP, VP, CP], I),
+            "uor_b200_expert_route_backward": ([I, ctypes.POINTER(Router), VP, VP, VP, VP, CP], I),
+            "uor_b200_expert_q4_ffn": ([I, I, Z, VP, VP, VP, ctypes.POINTER(Q4),
+                                        ctypes.POINTER(Q4), VP, CP], I),
             "uor_b200_status_string": ([I], ctypes.c_char_p),
             "uor_b200_version": ([], I),
             "uor_b200_selftest_wait_timeout": ([P, U64], I),
@@ -480,6 +525,60 @@ def arena_canonicalize(values):
     _check(lib().uor_b200_arena_canonicalize(elem, values.ctypes.data, values.size,
                                              ctypes.byref(n)), "arena_canonicalize")
     return n.value
+
+
+# ------------------------------------------------------------------ 4-bit weights, experts
+
+def q4_gemm(elem, out, a, av, w, c, cv, ctx=None, route=None, asynchronous=False):
+    """C := A dequant(W)^T for a Q4 descriptor w: elem BF16 or F16, out elem or F32; f32 sums,
+    rounded once. NumPy has no bfloat16: its bits pass as uint16 arrays."""
+    dev = _on_device(a, c)
+    if dev != w.on_device:
+        raise ValueError("operands must all be host arrays or all be CUDA tensors")
+    A, C = view(a, *av), view(c, *cv)
+    call = make_call(NEAREST, dev, ctx, route, asynchronous)
+    _check(lib().uor_b200_q4_gemm(elem, out, ctypes.byref(A), ctypes.byref(w), ctypes.byref(C),
+                                  ctypes.byref(call)), "q4_gemm")
+
+
+def expert_route(elem, router, logits, lv, bias, ids, iv, weights, wv, ctx=None, route=None,
+                 asynchronous=False):
+    """Each row's top_k experts (int32, -1 where none is left) and their f32 weights; bias is
+    None or one float per expert, added for the choice alone."""
+    dev = _on_device(logits, ids, weights) if bias is None else \
+        _on_device(logits, ids, weights, bias)
+    L, IDS, W = view(logits, *lv), view(ids, *iv), view(weights, *wv)
+    pb, lb = _buffer(bias)[:2] if bias is not None else (None, 0)
+    call = make_call(NEAREST, dev, ctx, route, asynchronous)
+    _check(lib().uor_b200_expert_route(elem, ctypes.byref(router), ctypes.byref(L), pb, lb,
+                                       ctypes.byref(IDS), ctypes.byref(W), ctypes.byref(call)),
+           "expert_route")
+
+
+def expert_route_backward(elem, router, logits, lv, ids, iv, dweights, gv, dlogits, dv, ctx=None,
+                          route=None, asynchronous=False):
+    """The logits' gradient from the weights', the choice ids held fixed."""
+    dev = _on_device(logits, ids, dweights, dlogits)
+    L, IDS, G, D = view(logits, *lv), view(ids, *iv), view(dweights, *gv), view(dlogits, *dv)
+    call = make_call(NEAREST, dev, ctx, route, asynchronous)
+    _check(lib().uor_b200_expert_route_backward(elem, ctypes.byref(router), ctypes.byref(L),
+                                                ctypes.byref(IDS), ctypes.byref(G),
+                                                ctypes.byref(D), ctypes.byref(call)),
+           "expert_route_backward")
+
+
+def expert_q4_ffn(elem, out, experts, x, xv, ids, iv, weights, wv, up, down, y, yv, ctx=None,
+                  route=None, asynchronous=False):
+    """y[t] = sum_s weights[t][s] down_e (silu(gate_e x[t]) * (up_e x[t])), e = ids[t][s], over
+    Q4 descriptors: up holds experts * 2 f rows (each expert's gate rows, then its up rows)."""
+    dev = _on_device(x, ids, weights, y)
+    if dev != up.on_device or dev != down.on_device:
+        raise ValueError("operands must all be host arrays or all be CUDA tensors")
+    X, IDS, W, Y = view(x, *xv), view(ids, *iv), view(weights, *wv), view(y, *yv)
+    call = make_call(NEAREST, dev, ctx, route, asynchronous)
+    _check(lib().uor_b200_expert_q4_ffn(elem, out, experts, ctypes.byref(X), ctypes.byref(IDS),
+                                        ctypes.byref(W), ctypes.byref(up), ctypes.byref(down),
+                                        ctypes.byref(Y), ctypes.byref(call)), "expert_q4_ffn")
 
 
 # ------------------------------------------------------------------ split-K exchange
