@@ -3,6 +3,7 @@
 // y[i][j] = sum_p x[i][p] scale[j][p / g] (code[j][p] - zero[j][p / g]). The plainest kernel: a
 // warp per output, lanes over the reduction's bytes, f32 sums, a shuffle tree at the end.
 #include "q4.cuh"
+#include "q4_few.cuh"
 
 namespace uor {
 
@@ -70,11 +71,29 @@ __global__ void ffn_down_simple(FfnArgs a, const T* h) {
     if (lane == 0) store_f32(a.y.p, t * a.y.rs + j * a.y.cs, a.y.type, total);
 }
 
+// What the few-rows kernel's vector loads may rely on.
+static void few_align(FewParams* p) {
+    const uint64_t codes = reinterpret_cast<uint64_t>(p->w.codes) | static_cast<uint64_t>(p->w.row_bytes);
+    p->codes_align = codes % 16 == 0 ? 16 : codes % 4 == 0 ? 4 : 1;
+    p->x_vec = (reinterpret_cast<uint64_t>(p->x) | static_cast<uint64_t>(p->x_rs * 2)) % 16 == 0;
+}
+
 static unsigned blocks_for(int64_t warps) { return static_cast<unsigned>((warps + 7) / 8); }
 
 int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4Dev& w, const MatOut& y,
                 uor_b200_route* route) {
     route->kernel = UOR_B200_KERNEL_Q4;
+    if (m <= 8 && x.cs == 1 && w.cols > 0) {
+        FewParams p{};
+        p.w = w;
+        p.x = x.p;
+        p.x_rs = x.rs;
+        p.m = m;
+        p.n = w.rows;
+        p.y = y;
+        few_align(&p);
+        return few_launch(ctx, elem, FEW_DENSE, p, false);
+    }
     const unsigned grid = blocks_for(m * w.rows);
     if (elem == UOR_B200_BF16)
         q4_simple<__nv_bfloat16><<<grid, 256, 0, ctx->stream>>>(x, w, y, m);
@@ -96,6 +115,30 @@ static int ffn_typed(uor_b200_ctx* ctx, const FfnArgs& a) {
 
 int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     route->kernel = UOR_B200_KERNEL_Q4;
+    if (a.tokens <= FEW_MAX_TOKENS && a.tokens * a.top_k <= FEW_MAX_PAIRS && a.top_k > 0 && a.f > 0 && a.x.cs == 1) {
+        int st = UOR_B200_OK;
+        FewParams p{};
+        p.h = ctx_buffer(ctx, SLOT_WS, static_cast<size_t>(a.tokens) * a.top_k * a.f * 2, &st);
+        if (!p.h) return st;
+        p.w = a.up;
+        p.x = a.x.p;
+        p.x_rs = a.x.rs;
+        p.n = a.f;
+        p.ids = a.ids;
+        p.weights = a.weights;
+        p.tokens = static_cast<int>(a.tokens);
+        p.top_k = a.top_k;
+        p.experts = a.experts;
+        few_align(&p);
+        if ((st = few_launch(ctx, a.elem, FEW_UP, p, false))) return st;
+        p.w = a.down;
+        p.x = p.h;
+        p.x_rs = a.f;
+        p.n = a.d;
+        p.y = a.y;
+        few_align(&p);
+        return few_launch(ctx, a.elem, FEW_DOWN, p, true);
+    }
     return a.elem == UOR_B200_BF16 ? ffn_typed<__nv_bfloat16>(ctx, a) : ffn_typed<__half>(ctx, a);
 }
 
