@@ -20,14 +20,19 @@ struct FewParams {
     MatOut y;            // dense and down
     Mat ids, weights;    // experts
     int tokens, top_k, experts;
-    void* h;             // up: [tokens * top_k][n]
-    int codes_align;     // 16, 4 or 1: what every row of codes begins at a multiple of
+    void* h;             // up: [tokens * top_k][h_rs], every eight in the operands' order
+    int64_t h_rs;        // n rounded up to 8
+    int codes_align;     // 16 if every row of codes begins at a multiple of 16 bytes
     int x_vec;           // rows of x begin at multiples of 16 bytes
+    // Set by the launch:
+    int panel;           // chunks whose activations are resident
+    int group_shift;     // log2 of the group, or -1
+    int quants_vec;      // a chunk's scales, and its zero points, are one vector each
 };
 
 constexpr int FEW_MAX_PAIRS = 256;  // tokens * top_k of the experts' modes
 constexpr int FEW_MAX_TOKENS = 8;
 
-int few_launch(uor_b200_ctx* ctx, int elem, FewMode mode, const FewParams& p, bool after_up);
+int few_launch(uor_b200_ctx* ctx, int elem, FewMode mode, FewParams p, bool after_up);
 
 }  // namespace uor

@@ -74,7 +74,7 @@ __global__ void ffn_down_simple(FfnArgs a, const T* h) {
 // What the few-rows kernel's vector loads may rely on.
 static void few_align(FewParams* p) {
     const uint64_t codes = reinterpret_cast<uint64_t>(p->w.codes) | static_cast<uint64_t>(p->w.row_bytes);
-    p->codes_align = codes % 16 == 0 ? 16 : codes % 4 == 0 ? 4 : 1;
+    p->codes_align = codes % 16 == 0 ? 16 : 1;
     p->x_vec = (reinterpret_cast<uint64_t>(p->x) | static_cast<uint64_t>(p->x_rs * 2)) % 16 == 0;
 }
 
@@ -118,8 +118,9 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     if (a.tokens <= FEW_MAX_TOKENS && a.tokens * a.top_k <= FEW_MAX_PAIRS && a.top_k > 0 && a.f > 0 && a.x.cs == 1) {
         int st = UOR_B200_OK;
         FewParams p{};
-        p.h = ctx_buffer(ctx, SLOT_WS, static_cast<size_t>(a.tokens) * a.top_k * a.f * 2, &st);
+        p.h = ctx_buffer(ctx, SLOT_WS, static_cast<size_t>(a.tokens) * a.top_k * ((a.f + 7) / 8 * 8) * 2, &st);
         if (!p.h) return st;
+        p.h_rs = (a.f + 7) / 8 * 8;
         p.w = a.up;
         p.x = a.x.p;
         p.x_rs = a.x.rs;
@@ -133,7 +134,7 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
         if ((st = few_launch(ctx, a.elem, FEW_UP, p, false))) return st;
         p.w = a.down;
         p.x = p.h;
-        p.x_rs = a.f;
+        p.x_rs = p.h_rs;
         p.n = a.d;
         p.y = a.y;
         few_align(&p);
