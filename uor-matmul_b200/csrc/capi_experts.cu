@@ -273,7 +273,7 @@ int uor_b200_expert_q4_ffn(uor_b200_dtype elem, uor_b200_dtype out, size_t exper
         (st = place(ids, 4, &I)) || (st = place(weights, 4, &W)))
         return st;
     const size_t t = x->rows, d = x->cols, f = down->cols, k = ids->cols;
-    if (experts > MOST) return UOR_B200_UNSUPPORTED;
+    if (experts > 1024) return UOR_B200_UNSUPPORTED;
     if (up->cols != d || up->rows != experts * 2 * f || down->rows != experts * d || ids->rows != t ||
         weights->rows != t || weights->cols != k || y->rows != t || y->cols != d)
         return UOR_B200_NONCONFORMANT;

@@ -1,129 +1,266 @@
-// q4_gemm.cu -- products with 4-bit weights and group scales.
-//
-// y[i][j] = sum_p x[i][p] scale[j][p / g] (code[j][p] - zero[j][p / g]). The plainest kernel: a
-// warp per output, lanes over the reduction's bytes, f32 sums, a shuffle tree at the end.
+// q4_gemm.cu -- 4-bit weights with group scales and the experts' layer: which kernels a call runs,
+// and the small ones around the products (rows brought together, choices sorted, parts added).
+#include <cstring>
+
 #include "q4.cuh"
 #include "q4_few.cuh"
+#include "q4_many.cuh"
 
 namespace uor {
 
-// One lane's share of sum_p x[p cs] w[row][p].
-template <typename T>
-__device__ __forceinline__ float q4_dot(const T* x, int64_t cs, const Q4Dev& w, int64_t row, int lane) {
-    const uint8_t* codes = w.codes + row * w.row_bytes;
-    float sum = 0;
-    for (int b = lane; b < (w.cols + 1) / 2; b += 32) {
-        const int g = 2 * b / w.group;
-        const float scale = load_f32(w.scales, row * w.groups_rs + g, w.scale_type);
-        const int zero = w.zeros ? w.zeros[row * w.groups_rs + g] & 15 : 8;
-        const int code = codes[b];
-        float part = to_f32(x[2 * b * cs]) * static_cast<float>((code & 15) - zero);
-        if (2 * b + 1 < w.cols)
-            part = fmaf(to_f32(x[(2 * b + 1) * cs]), static_cast<float>((code >> 4) - zero), part);
-        sum = fmaf(part, scale, sum);
+namespace {
+
+// Rows of x, strided anyhow, as contiguous ones of `pitch` elements; row i is x's row
+// perm[i] / top_k where there is a permutation, and then only offsets[experts] rows exist.
+// Eight elements to a thread.
+__global__ void rows_kernel(Mat x, int cols, int pitch, int64_t rows, const int* perm, int top_k, const int* total, bool vec,
+                            uint16_t* to) {
+    const int per_row = pitch / 8;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const int64_t i = at / per_row;
+    if (i >= (total ? min(static_cast<int64_t>(*total), rows) : rows)) return;
+    const int c = static_cast<int>(at - i * per_row) * 8;
+    const int64_t row = perm ? perm[i] / top_k : i;
+    const auto* from = static_cast<const uint16_t*>(x.p) + row * x.rs;
+    uint4 v;
+    if (vec && c + 8 <= cols) {
+        v = *reinterpret_cast<const uint4*>(from + c);
+    } else {
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int b = 0; b < 8; ++b)
+            if (c + b < cols) w[b >> 1] |= static_cast<uint32_t>(from[(c + b) * x.cs]) << (16 * (b & 1));
+        v = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    return sum;
+    *reinterpret_cast<uint4*>(to + i * pitch + c) = v;
 }
 
-__device__ __forceinline__ float warp_sum(float v) {
-    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+// Rows of codes at any address and distance as rows of `pitch` bytes, a multiple of 16.
+__global__ void codes_kernel(const uint8_t* codes, int64_t row_bytes, int64_t rows, int row_len, int pitch, uint8_t* to) {
+    const int per_row = pitch / 16;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const int64_t i = at / per_row;
+    if (i >= rows) return;
+    const int c = static_cast<int>(at - i * per_row) * 16;
+    const uint8_t* from = codes + i * row_bytes + c;
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int b = 0; b < 16; ++b)
+        if (c + b < row_len) w[b >> 2] |= static_cast<uint32_t>(from[b]) << (8 * (b & 3));
+    *reinterpret_cast<uint4*>(to + i * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T>
-__global__ void q4_simple(Mat x, Q4Dev w, MatOut y, int64_t m) {
-    const int lane = threadIdx.x & 31;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int64_t i = at / w.rows, j = at % w.rows;
-    if (i >= m) return;
-    const float s = warp_sum(q4_dot(static_cast<const T*>(x.p) + i * x.rs, x.cs, w, j, lane));
-    if (lane == 0) store_f32(y.p, i * y.rs + j * y.cs, y.type, s);
+constexpr int SORT_THREADS = 256;
+
+// The pairs (token, choice) of one expert per block, in their own order, behind those of the
+// experts before it: offsets[e] counts the pairs of lower experts. Ids outside the experts have
+// no place. Every thread counts and then places a run of pairs of its own.
+__global__ void __launch_bounds__(SORT_THREADS) sort_kernel(Mat ids, int pairs, int top_k, int experts, int* offsets, int* perm) {
+    __shared__ int warp_less[SORT_THREADS / 32], warp_same[SORT_THREADS / 32];
+    const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int run = (pairs + SORT_THREADS - 1) / SORT_THREADS;
+    const int first = min(pairs, static_cast<int>(threadIdx.x) * run), last = min(pairs, first + run);
+    auto id = [&](int i) {
+        const int t = i / top_k;
+        return static_cast<const int32_t*>(ids.p)[t * ids.rs + (i - t * top_k) * ids.cs];
+    };
+    int less = 0, same = 0;
+#pragma unroll 8
+    for (int i = first; i < last; ++i) {
+        const int v = id(i);
+        less += v >= 0 && v < e;
+        same += v == e;
+    }
+    int before = same;  // pairs of this expert in the runs up to this one's end
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += v;
+    }
+    less = __reduce_add_sync(0xffffffffu, less);
+    if (lane == 31) warp_less[warp] = less, warp_same[warp] = before;
+    __syncthreads();
+    int begin = 0, here = 0, all = 0;
+    for (int w = 0; w < SORT_THREADS / 32; ++w) {
+        begin += warp_less[w];
+        if (w < warp) here += warp_same[w];
+        all += warp_same[w];
+    }
+    if (threadIdx.x == 0) {
+        offsets[e] = begin;
+        if (e == experts - 1) offsets[experts] = begin + all;
+    }
+    int at = begin + here + before - same;
+    for (int i = first; i < last; ++i)
+        if (id(i) == e) perm[at++] = i;
 }
 
-template <typename T>
-__global__ void ffn_up_simple(FfnArgs a, T* h) {
-    const int lane = threadIdx.x & 31;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int64_t pair = at / a.f, j = at % a.f, t = pair / a.top_k;
+// y[i][j] = the parts' sum, in their order (no parts: 0).
+__global__ void add_parts_kernel(const float* part, int splits, int64_t rows, int n, MatOut y) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (at >= rows * n) return;
+    const int64_t i = at / n, j = at - i * n;
+    float v = 0;
+    for (int s = 0; s < splits; ++s) v += part[s * rows * n + at];
+    store_f32(y.p, i * y.rs + j * y.cs, y.type, v);
+}
+
+// y[t][j] = the token's choices' products, each times its weight, in the choices' order.
+__global__ void combine_kernel(const float* part, int splits, FfnArgs a) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const int64_t t = at / a.d, j = at - t * a.d;
     if (t >= a.tokens) return;
-    const int64_t e = static_cast<const int32_t*>(a.ids.p)[t * a.ids.rs + pair % a.top_k * a.ids.cs];
-    if (e < 0 || e >= a.experts) return;
-    const T* x = static_cast<const T*>(a.x.p) + t * a.x.rs;
-    const float gate = warp_sum(q4_dot(x, a.x.cs, a.up, e * 2 * a.f + j, lane));
-    const float up = warp_sum(q4_dot(x, a.x.cs, a.up, e * 2 * a.f + a.f + j, lane));
-    if (lane == 0) h[pair * a.f + j] = from_f32<T>(silu(gate) * up);
-}
-
-template <typename T>
-__global__ void ffn_down_simple(FfnArgs a, const T* h) {
-    const int lane = threadIdx.x & 31;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int64_t t = at / a.d, j = at % a.d;
-    if (t >= a.tokens) return;
-    float total = 0;
+    const int64_t step = a.tokens * a.top_k * a.d;
+    float v = 0;
     for (int s = 0; s < a.top_k; ++s) {
-        const int64_t e = static_cast<const int32_t*>(a.ids.p)[t * a.ids.rs + s * a.ids.cs];
+        const int e = static_cast<const int32_t*>(a.ids.p)[t * a.ids.rs + s * a.ids.cs];
         if (e < 0 || e >= a.experts) continue;
-        const float weight = static_cast<const float*>(a.weights.p)[t * a.weights.rs + s * a.weights.cs];
-        const float v = warp_sum(q4_dot(h + (t * a.top_k + s) * a.f, 1, a.down, e * a.d + j, lane));
-        total = fmaf(weight, v, total);
+        const float w = static_cast<const float*>(a.weights.p)[t * a.weights.rs + s * a.weights.cs];
+        const float* from = part + (t * a.top_k + s) * a.d + j;
+        float sum = from[0];
+        for (int c = 1; c < splits; ++c) sum += from[c * step];
+        v = fmaf(w, sum, v);
     }
-    if (lane == 0) store_f32(a.y.p, t * a.y.rs + j * a.y.cs, a.y.type, total);
+    store_f32(a.y.p, t * a.y.rs + j * a.y.cs, a.y.type, v);
+}
+
+constexpr int THREADS = 256;
+unsigned blocks_for(int64_t threads) { return static_cast<unsigned>((threads + THREADS - 1) / THREADS); }
+
+int up_to(int v, int by) { return (v + by - 1) / by * by; }
+
+bool rows_aligned(const void* p, int64_t stride_bytes) {
+    return (reinterpret_cast<uint64_t>(p) | static_cast<uint64_t>(stride_bytes)) % 16 == 0;
+}
+
+// What the kernels with TMA read must lie in rows of whole 16 bytes that do not overlap.
+bool x_in_place(const Mat& x, int cols) { return x.cs == 1 && rows_aligned(x.p, x.rs * 2) && x.rs >= cols; }
+bool codes_in_place(const Q4Dev& w) {
+    return rows_aligned(w.codes, w.row_bytes) && w.row_bytes >= (w.cols + 1) / 2 && w.row_bytes < (int64_t(1) << 40);
+}
+
+// A call's pieces of the context's workspace.
+class Pieces {
+  public:
+    size_t add(size_t bytes) {
+        const size_t at = total_;
+        total_ += (bytes + 1023) / 1024 * 1024;
+        return at;
+    }
+    uint8_t* get(uor_b200_ctx* ctx, int* st) { return static_cast<uint8_t*>(ctx_buffer(ctx, SLOT_WS, total_, st)); }
+
+  private:
+    size_t total_ = 0;
+};
+
+size_t codes_copy_bytes(const Q4Dev& w) {
+    return codes_in_place(w) ? 0 : static_cast<size_t>(w.rows) * up_to((w.cols + 1) / 2, 16);
+}
+void copy_codes(uor_b200_ctx* ctx, Q4Dev* w, uint8_t* to) {
+    if (codes_in_place(*w)) return;
+    const int pitch = up_to((w->cols + 1) / 2, 16);
+    codes_kernel<<<blocks_for(static_cast<int64_t>(w->rows) * (pitch / 16)), THREADS, 0, ctx->stream>>>(
+        w->codes, w->row_bytes, w->rows, (w->cols + 1) / 2, pitch, to);
+    w->codes = to;
+    w->row_bytes = pitch;
+}
+void copy_rows(uor_b200_ctx* ctx, const Mat& x, int cols, int64_t rows, const int* perm, int top_k, const int* total, void* to) {
+    const int pitch = up_to(cols, 8);
+    rows_kernel<<<blocks_for(rows * (pitch / 8)), THREADS, 0, ctx->stream>>>(
+        x, cols, pitch, rows, perm, top_k, total, x.cs == 1 && rows_aligned(x.p, x.rs * 2), static_cast<uint16_t*>(to));
 }
 
 // What the few-rows kernel's vector loads may rely on.
-static void few_align(FewParams* p) {
-    const uint64_t codes = reinterpret_cast<uint64_t>(p->w.codes) | static_cast<uint64_t>(p->w.row_bytes);
-    p->codes_align = codes % 16 == 0 ? 16 : 1;
-    p->x_vec = (reinterpret_cast<uint64_t>(p->x) | static_cast<uint64_t>(p->x_rs * 2)) % 16 == 0;
+void few_align(FewParams* p) {
+    p->codes_align = rows_aligned(p->w.codes, p->w.row_bytes) ? 16 : 1;
+    p->x_vec = rows_aligned(p->x, p->x_rs * 2);
 }
 
-static unsigned blocks_for(int64_t warps) { return static_cast<unsigned>((warps + 7) / 8); }
+int zeros_out(uor_b200_ctx* ctx, int64_t rows, int n, const MatOut& y) {
+    add_parts_kernel<<<blocks_for(rows * n), THREADS, 0, ctx->stream>>>(nullptr, 0, rows, n, y);
+    return cuda_status(cudaGetLastError());
+}
+
+}  // namespace
 
 int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4Dev& w, const MatOut& y,
                 uor_b200_route* route) {
     route->kernel = UOR_B200_KERNEL_Q4;
-    if (m <= 8 && x.cs == 1 && w.cols > 0) {
+    if (w.cols == 0) return zeros_out(ctx, m, w.rows, y);
+    int st = UOR_B200_OK;
+    const bool few = m <= FEW_MAX_TOKENS;
+    Pieces pieces;
+    // The few-rows kernel reads any row whose elements follow one another.
+    const bool own_rows = few ? x.cs != 1 : !x_in_place(x, w.cols);
+    const size_t x_at = pieces.add(own_rows ? static_cast<size_t>(m) * up_to(w.cols, 8) * 2 : 0);
+    ManyParams many{};
+    many.w = w;
+    many.mode = MANY_DENSE;
+    many.n = w.rows;
+    many.experts = 1;
+    many.m = static_cast<int>(m);
+    many.row_bound = many.m;
+    many.y = y;
+    many.part_rows = m;
+    const int splits = few ? 1 : many_splits(ctx, many);
+    const size_t codes_at = pieces.add(few ? 0 : codes_copy_bytes(w));
+    const size_t part_at = pieces.add(splits > 1 ? static_cast<size_t>(splits) * m * w.rows * 4 : 0);
+    uint8_t* ws = pieces.get(ctx, &st);
+    if (!ws) return st;
+    Mat rows = x;
+    if (own_rows) {
+        copy_rows(ctx, x, w.cols, m, nullptr, 1, nullptr, ws + x_at);
+        rows = Mat{ws + x_at, up_to(w.cols, 8), 1};
+    }
+    if (few) {
         FewParams p{};
         p.w = w;
-        p.x = x.p;
-        p.x_rs = x.rs;
+        p.x = rows.p;
+        p.x_rs = rows.rs;
         p.m = m;
         p.n = w.rows;
         p.y = y;
         few_align(&p);
+        route->tile_m = 16, route->tile_n = 8, route->tile_k = 256;
         return few_launch(ctx, elem, FEW_DENSE, p, false);
     }
-    const unsigned grid = blocks_for(m * w.rows);
-    if (elem == UOR_B200_BF16)
-        q4_simple<__nv_bfloat16><<<grid, 256, 0, ctx->stream>>>(x, w, y, m);
-    else
-        q4_simple<__half><<<grid, 256, 0, ctx->stream>>>(x, w, y, m);
-    return cuda_status(cudaGetLastError());
-}
-
-template <typename T>
-static int ffn_typed(uor_b200_ctx* ctx, const FfnArgs& a) {
-    int st = UOR_B200_OK;
-    T* h = static_cast<T*>(ctx_buffer(ctx, SLOT_WS, static_cast<size_t>(a.tokens) * a.top_k * a.f * 2, &st));
-    if (!h) return st;
-    if (a.top_k && a.f)
-        ffn_up_simple<T><<<blocks_for(a.tokens * a.top_k * a.f), 256, 0, ctx->stream>>>(a, h);
-    ffn_down_simple<T><<<blocks_for(a.tokens * a.d), 256, 0, ctx->stream>>>(a, h);
-    return cuda_status(cudaGetLastError());
+    copy_codes(ctx, &many.w, ws + codes_at);
+    many.x = rows.p;
+    many.x_rs = rows.rs;
+    many.x_rows = m;
+    many.part = reinterpret_cast<float*>(ws + part_at);
+    route->tile_m = 128, route->tile_n = 256, route->tile_k = 64;
+    route->k_chunks = splits;
+    if ((st = many_launch(ctx, elem, many))) return st;
+    if (splits > 1) {
+        add_parts_kernel<<<blocks_for(m * w.rows), THREADS, 0, ctx->stream>>>(many.part, splits, m, w.rows, y);
+        return cuda_status(cudaGetLastError());
+    }
+    return UOR_B200_OK;
 }
 
 int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     route->kernel = UOR_B200_KERNEL_Q4;
-    if (a.tokens <= FEW_MAX_TOKENS && a.tokens * a.top_k <= FEW_MAX_PAIRS && a.top_k > 0 && a.f > 0 && a.x.cs == 1) {
-        int st = UOR_B200_OK;
+    if (a.top_k == 0 || a.f == 0) return zeros_out(ctx, a.tokens, a.d, a.y);
+    int st = UOR_B200_OK;
+    const int64_t pairs = a.tokens * a.top_k;
+    const int h_rs = up_to(a.f, 8), x_rs = up_to(a.d, 8);
+    Pieces pieces;
+    const size_t h_at = pieces.add(static_cast<size_t>(pairs) * h_rs * 2);
+    if (a.tokens <= FEW_MAX_TOKENS && pairs <= FEW_MAX_PAIRS) {
+        const size_t x_at = pieces.add(a.x.cs == 1 ? 0 : static_cast<size_t>(a.tokens) * x_rs * 2);
+        uint8_t* ws = pieces.get(ctx, &st);
+        if (!ws) return st;
         FewParams p{};
-        p.h = ctx_buffer(ctx, SLOT_WS, static_cast<size_t>(a.tokens) * a.top_k * ((a.f + 7) / 8 * 8) * 2, &st);
-        if (!p.h) return st;
-        p.h_rs = (a.f + 7) / 8 * 8;
+        p.h = ws + h_at;
+        p.h_rs = h_rs;
         p.w = a.up;
         p.x = a.x.p;
         p.x_rs = a.x.rs;
+        if (a.x.cs != 1) {
+            copy_rows(ctx, a.x, a.d, a.tokens, nullptr, 1, nullptr, ws + x_at);
+            p.x = ws + x_at;
+            p.x_rs = x_rs;
+        }
         p.n = a.f;
         p.ids = a.ids;
         p.weights = a.weights;
@@ -131,16 +268,55 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
         p.top_k = a.top_k;
         p.experts = a.experts;
         few_align(&p);
+        route->tile_m = 16, route->tile_n = 8, route->tile_k = 256;
         if ((st = few_launch(ctx, a.elem, FEW_UP, p, false))) return st;
         p.w = a.down;
         p.x = p.h;
-        p.x_rs = p.h_rs;
+        p.x_rs = h_rs;
         p.n = a.d;
         p.y = a.y;
         few_align(&p);
         return few_launch(ctx, a.elem, FEW_DOWN, p, true);
     }
-    return a.elem == UOR_B200_BF16 ? ffn_typed<__nv_bfloat16>(ctx, a) : ffn_typed<__half>(ctx, a);
+
+    ManyParams up{};
+    up.w = a.up;
+    up.mode = MANY_UP;
+    up.n = a.f;
+    up.experts = a.experts;
+    up.row_bound = static_cast<int>(a.tokens);  // an expert's rows: at most one of each token, usually
+    up.x_rs = x_rs;
+    up.x_rows = pairs;
+    up.h_rs = h_rs;
+    ManyParams down = up;
+    down.w = a.down;
+    down.mode = MANY_DOWN;
+    down.n = a.d;
+    down.x_rs = h_rs;
+    down.part_rows = pairs;
+    const int splits = many_splits(ctx, down);
+    const size_t x_at = pieces.add(static_cast<size_t>(pairs) * x_rs * 2);
+    const size_t part_at = pieces.add(static_cast<size_t>(splits) * pairs * a.d * 4);
+    const size_t up_at = pieces.add(codes_copy_bytes(a.up)), down_at = pieces.add(codes_copy_bytes(a.down));
+    const size_t offsets_at = pieces.add((a.experts + 1) * sizeof(int)), perm_at = pieces.add(pairs * sizeof(int));
+    uint8_t* ws = pieces.get(ctx, &st);
+    if (!ws) return st;
+    int* offsets = reinterpret_cast<int*>(ws + offsets_at);
+    int* perm = reinterpret_cast<int*>(ws + perm_at);
+    sort_kernel<<<a.experts, SORT_THREADS, 0, ctx->stream>>>(a.ids, static_cast<int>(pairs), a.top_k, a.experts, offsets, perm);
+    copy_rows(ctx, a.x, a.d, pairs, perm, a.top_k, offsets + a.experts, ws + x_at);
+    copy_codes(ctx, &up.w, ws + up_at);
+    copy_codes(ctx, &down.w, ws + down_at);
+    up.offsets = down.offsets = offsets;
+    up.perm = down.perm = perm;
+    up.x = ws + x_at;
+    up.h = ws + h_at;
+    down.x = ws + h_at;
+    down.part = reinterpret_cast<float*>(ws + part_at);
+    route->tile_m = 128, route->tile_n = 256, route->tile_k = 64;
+    if ((st = many_launch(ctx, a.elem, up)) || (st = many_launch(ctx, a.elem, down))) return st;
+    combine_kernel<<<blocks_for(a.tokens * a.d), THREADS, 0, ctx->stream>>>(down.part, splits, a);
+    return cuda_status(cudaGetLastError());
 }
 
 }  // namespace uor
