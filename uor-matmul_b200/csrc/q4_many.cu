@@ -36,12 +36,12 @@ template <bool WIDE>
 struct Shape {
     static constexpr int COLS = WIDE ? 256 : 128;
     static constexpr int STAGES = WIDE ? 4 : 5;
-    static constexpr int CSTAGES = WIDE ? 3 : 4;
+    static constexpr int CSTAGES = WIDE ? 2 : 4;
     static constexpr int X_BYTES = COLS * BK * 2;
     static constexpr int STAGE_BYTES = X_BYTES + A_BYTES;
     static constexpr int DECODERS = WIDE ? 4 : 8;  // warps
     static constexpr int SUMMERS = WIDE ? 8 : 4;
-    static constexpr int EXCHANGE = (WIDE ? 2 : 1) * 64 * 8 * 4;
+    static constexpr int EXCHANGE = (WIDE ? 2 : 1) * BM * 8 * 4;
     static constexpr int SMEM = STAGES * STAGE_BYTES + CSTAGES * C_BYTES + EXCHANGE + (MANY_MAX_EXPERTS + 1) * 4 + 256 + 1024;
 };
 static_assert(Shape<true>::SMEM <= 232448 && Shape<false>::SMEM <= 232448, "shared memory of a block");
@@ -123,6 +123,59 @@ __device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, ui
 }
 __device__ __forceinline__ float half_of(uint64_t v, int i) {
     return __uint_as_float(static_cast<uint32_t>(i ? v >> 32 : v));
+}
+
+// Four inner activations from their gates' and ups' sums.
+template <typename T>
+__device__ __noinline__ void up_out(const float* gate, int valid, T* to) {
+    const float4 g = *reinterpret_cast<const float4*>(gate), u = *reinterpret_cast<const float4*>(gate + 64);
+    const float v[4] = {silu(g.x) * u.x, silu(g.y) * u.y, silu(g.z) * u.z, silu(g.w) * u.w};
+    if (valid == 4) {  // rows of h begin at multiples of 16 bytes
+        T t[4] = {from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
+        uint2 bits;
+        memcpy(&bits, t, 8);
+        *reinterpret_cast<uint2*>(to) = bits;
+    } else {
+        for (int i = 0; i < valid; ++i) to[i] = from_f32<T>(i == 0 ? v[0] : i == 1 ? v[1] : v[2]);
+    }
+}
+
+// Eight neighbouring outputs of activation row i from output j on, to where this launch's go.
+__device__ __noinline__ void out(const ManyParams& p, const Item& it, int64_t i, int j, const float* from, int valid) {
+    const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
+    void* to = p.part;
+    int64_t at, step = 1;
+    int type = UOR_B200_F32;
+    if (p.mode == MANY_DOWN || p.splits > 1) {
+        at = (it.split * p.part_rows + (p.mode == MANY_DOWN ? p.perm[i] : i)) * p.n + j;
+    } else {
+        to = p.y.p;
+        type = p.y.type;
+        step = p.y.cs;
+        at = i * p.y.rs + j * step;
+    }
+    const int size = type == UOR_B200_F32 ? 4 : 2;
+    char* c = static_cast<char*>(to) + at * size;
+    if (valid == 8 && step == 1 && reinterpret_cast<uint64_t>(c) % 16 == 0) {
+        if (type == UOR_B200_F32) {
+            reinterpret_cast<float4*>(c)[0] = a;
+            reinterpret_cast<float4*>(c)[1] = b;
+        } else {
+            uint4 w;
+            if (type == UOR_B200_BF16) {
+                const __nv_bfloat162 t[4] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w),
+                                             __floats2bfloat162_rn(b.x, b.y), __floats2bfloat162_rn(b.z, b.w)};
+                memcpy(&w, t, 16);
+            } else {
+                const __half2 t[4] = {__floats2half2_rn(a.x, a.y), __floats2half2_rn(a.z, a.w), __floats2half2_rn(b.x, b.y),
+                                      __floats2half2_rn(b.z, b.w)};
+                memcpy(&w, t, 16);
+            }
+            *reinterpret_cast<uint4*>(c) = w;
+        }
+    } else {
+        for (int k = 0; k < valid; ++k) store_f32(to, at + k * step, type, from[k]);
+    }
 }
 
 template <int N>
@@ -415,43 +468,38 @@ __global__ void __launch_bounds__(THREADS, 1)
             // The warpgroup stores together or not at all: a warp that gave up meets the others here.
             ok = bar_and_all(1 + part, 128, ok);
             if (!ok) break;
+            // Sums leave through shared memory eight columns at a time, [column][row], so that a
+            // thread stores neighbouring outputs of one column at once.
             const int left = it.cols - part * 128;  // this warpgroup's existing columns
+            float* swap = exchange + part * (BM * 8);
+            const int col = r >> 4;  // the column of eight that this thread stores
             if (p.mode == MANY_UP) {
-                // Rows 0 .. 63 are gates, 64 .. 127 the same outputs' ups, which pass through
-                // shared memory eight columns at a time.
-                float* swap = exchange + part * (64 * 8);
-                const int j = it.j0 + r;
+                // Rows 0 .. 63 are gates, 64 .. 127 the same outputs' ups.
+                const int j = (r & 15) * 4;
+                const float* gate = swap + col * BM + j;
+                T* to = static_cast<T*>(p.h) + (it.p0 + part * 128 + col) * p.h_rs + it.j0 + j;
+                const int valid = min(4, p.n - it.j0 - j);
 #pragma unroll
-                for (int c = 0; c < 128; c += 8) {
+                for (int c = 0; c < 128; c += 8)
                     if (c < left) {
-                        if (r >= 64) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) swap[i * 64 + r - 64] = half_of(acc[(c + i) / 2], i & 1);
-                        }
+                        for (int i = 0; i < 8; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
                         asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                        if (r < 64 && j < p.n) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (c + i < left)
-                                    static_cast<T*>(p.h)[(it.p0 + part * 128 + c + i) * p.h_rs + j] =
-                                        from_f32<T>(silu(half_of(acc[(c + i) / 2], i & 1)) * swap[i * 64 + r]);
-                        }
+                        if (c + col < left && valid > 0) up_out(gate, valid, to + c * p.h_rs);
                         asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
                     }
-                }
-            } else if (it.j0 + r < p.n) {
-                const int64_t j = it.j0 + r;
+            } else {
+                const int j = (r & 15) * 8;
+                const float* from = swap + col * BM + j;
+                const int valid = min(8, p.n - it.j0 - j);
 #pragma unroll
-                for (int c = 0; c < 128; ++c)
+                for (int c = 0; c < 128; c += 8)
                     if (c < left) {
-                        const float v = half_of(acc[c / 2], c & 1);
-                        const int64_t i = it.p0 + part * 128 + c;
-                        if (p.mode == MANY_DOWN)
-                            p.part[(it.split * p.part_rows + p.perm[i]) * p.n + j] = v;
-                        else if (p.splits > 1)
-                            p.part[(it.split * p.part_rows + i) * p.n + j] = v;
-                        else
-                            store_f32(p.y.p, i * p.y.rs + j * p.y.cs, p.y.type, v);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
+                        if (c + col < left && valid > 0) out(p, it, it.p0 + part * 128 + c + col, it.j0 + j, from, valid);
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
                     }
             }
         }
