@@ -86,6 +86,10 @@ int cuda_status(cudaError_t e);
 bool make_tmap_u8(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1,
                   uint64_t stride1, uint32_t box0, uint32_t box1, bool swizzle128 = true);
 
+// The same with 64-byte swizzle (box0 at most 64).
+bool make_tmap_u8_sw64(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1,
+                       uint64_t stride1, uint32_t box0, uint32_t box1);
+
 // A 2-D tensor map of 16-bit elements, 128-byte swizzle, zero fill out of range.
 bool make_tmap_u16(CUtensorMap* map, const void* base, uint64_t dim0, uint64_t dim1,
                    uint64_t stride1_bytes, uint32_t box0, uint32_t box1);

@@ -1,17 +1,24 @@
 // q4_many.cu -- products of many rows with 4-bit weights and group scales.
 //
-// Bound by the tensor cores: 2 m n k operations on 16-bit floats. A work item is a tile of 128
-// weight rows by up to 256 activation rows; the weights are the instruction's M side, so that a
-// thread of the epilogue owns one weight row and a group's scale is one number per thread.
+// Bound by the tensor cores: 2 m n k operations on 16-bit floats. A work item is a tile of 256
+// weight rows by up to 192 activation rows, on a pair of CTAs (tcgen05.mma.cta_group::2): each
+// CTA holds 128 of the weight rows and brings half of the activation rows. The weights are the
+// instruction's M side, so that a thread of the epilogue owns one weight row and a group's scale
+// is one number per thread.
 //
 // The roles of a CTA: a warp brings 64-position stages of activations by TMA, another the codes of
-// 128 positions; a warpgroup (two where tiles have at most 128 columns) turns each code into a
-// 16-bit float, exactly (code - zero), in the swizzled layout of the operand; one thread issues
-// the tcgen05.mma; two warpgroups (one) hold the sums. A group's products are summed in tensor
+// 128 positions; two warpgroups turn each code into a 16-bit float, exactly (code - zero), and
+// store it to tensor memory, where the instruction takes its A side from; one thread of the pair
+// issues the tcgen05.mma; two warpgroups hold the sums. A group's products are summed in tensor
 // memory, and at the group's end these warpgroups add scale x sum to their f32 registers, while the
-// next group runs in the other half of tensor memory. So no weight is rounded: rounding scale x
-// code to 16 bits would cost as much precision as rounding the output does. That costs the reads
-// of tensor memory: a multiply-add per group, row and column, two in one instruction.
+// next group runs in the other of two accumulators. So no weight is rounded: rounding scale x
+// code to 16 bits would cost as much precision as rounding the output does.
+//
+// Why this shape. With the weights in shared memory and one CTA per 128 x 256 tile, the operands'
+// reads, the TMA's and the decoders' writes came to 104 KB a stage, 830 cycles at 128 bytes a
+// cycle, for 512 cycles of multiplication (2048 x 8192 x 8192: 366 us, 295 us without decoding
+// and scaling). Here a stage moves 4 x 3 KB of operands, 12 KB of TMA and 8 KB of codes for 384.
+// Tensor memory's 512 columns hold two accumulators of 192 and four stages of weights of 32.
 //
 // Every wait is bounded; a role that gives up records it, and every other role leaves after it.
 #include "q4_many.cuh"
@@ -25,26 +32,28 @@ namespace uor {
 
 namespace {
 
-constexpr int BM = 128;        // weight rows of a tile
+constexpr int BM = 128;        // weight rows of a CTA's half of a tile
 constexpr int BK = 64;         // reduction positions of a stage: 128 bytes of a row
 constexpr int CODES_K = 128;   // of a stage of codes
-constexpr int A_BYTES = BM * BK * 2;
+constexpr int MAX_COLS = 192;  // activation rows of a tile
+constexpr int X_BOX = 32;      // activation rows of one TMA copy
+constexpr int X_BOX_BYTES = X_BOX * BK * 2;
+constexpr int X_BYTES = MAX_COLS / 2 * BK * 2;
 constexpr int C_BYTES = BM * CODES_K / 2;
-constexpr int THREADS = 512;
-
-template <bool WIDE>
-struct Shape {
-    static constexpr int COLS = WIDE ? 256 : 128;
-    static constexpr int STAGES = WIDE ? 4 : 5;
-    static constexpr int CSTAGES = WIDE ? 2 : 4;
-    static constexpr int X_BYTES = COLS * BK * 2;
-    static constexpr int STAGE_BYTES = X_BYTES + A_BYTES;
-    static constexpr int DECODERS = WIDE ? 4 : 8;  // warps
-    static constexpr int SUMMERS = WIDE ? 8 : 4;
-    static constexpr int EXCHANGE = (WIDE ? 2 : 1) * BM * 8 * 4;
-    static constexpr int SMEM = STAGES * STAGE_BYTES + CSTAGES * C_BYTES + EXCHANGE + (MANY_MAX_EXPERTS + 1) * 4 + 256 + 1024;
-};
-static_assert(Shape<true>::SMEM <= 232448 && Shape<false>::SMEM <= 232448, "shared memory of a block");
+constexpr int XSTAGES = 8, CSTAGES = 6, ASTAGES = 4;
+constexpr int A_COLS = BK / 2;                       // tensor-memory columns of a stage of weights
+constexpr int A_FIRST = 2 * MAX_COLS;
+constexpr int DECODERS = 8, SUMMERS = 8;             // warps of a CTA
+constexpr int PART = MAX_COLS / 2;                   // columns of a summing warpgroup
+constexpr int EXCHANGE = BM * 8 * 4;                 // bytes, per summing warpgroup
+constexpr int BARS = 2 * XSTAGES + 2 * CSTAGES + 2 * ASTAGES + 5;
+constexpr int SMEM = XSTAGES * X_BYTES + CSTAGES * C_BYTES + 2 * EXCHANGE + (BARS + 1) * 8 + (MANY_MAX_EXPERTS + 1) * 4 + 1024;
+// Warpgroup 0: TMA, MMA; 1 and 2: decoders; 3 and 4: sums. Registers: 96 a thread at launch.
+constexpr int THREADS = 640;
+constexpr int REGS_CONTROL = 48, REGS_DECODE = 48, REGS_SUM = 160;
+static_assert(SMEM <= 232448, "shared memory of a block");
+static_assert(A_FIRST + ASTAGES * A_COLS == 512, "tensor memory");
+static_assert(REGS_CONTROL + 2 * REGS_DECODE + 2 * REGS_SUM <= 5 * 96, "registers of the launch");
 
 struct Item {
     int expert, cols, n;      // cols: existing activation rows; n: the instruction's
@@ -58,7 +67,7 @@ struct Item {
 __device__ __forceinline__ int tiles_of(int count, int max_cols) { return (count + max_cols - 1) / max_cols; }
 
 // Item u: row tiles run fastest, then the experts' tiles of activations, then the splits.
-__device__ __forceinline__ bool item_at(int u, const ManyParams& p, const int* first_tile, Item* it) {
+__device__ __forceinline__ bool item_at(int u, const ManyParams& p, const int* first_tile, int rank, Item* it) {
     const int rt = u % p.row_tiles;
     const int rest = u / p.row_tiles;
     const int tiles = first_tile[p.experts];
@@ -73,14 +82,14 @@ __device__ __forceinline__ bool item_at(int u, const ManyParams& p, const int* f
     const int begin = p.offsets ? p.offsets[lo] : 0;
     const int count = p.offsets ? p.offsets[lo + 1] - begin : p.m;
     const int parts = tiles_of(count, p.max_cols);
-    const int size = ((count + parts - 1) / parts + 15) & ~15;  // even shares, in whole instructions
+    const int size = ((count + parts - 1) / parts + 31) & ~31;  // even shares, in whole instructions
     const int i = tt - first_tile[lo];
     it->expert = lo;
     it->cols = min(size, count - i * size);
-    it->n = (it->cols + 15) & ~15;
+    it->n = (it->cols + 31) & ~31;
     it->p0 = begin + static_cast<int64_t>(i) * size;
-    const int outputs = p.mode == MANY_UP ? BM / 2 : BM;
-    it->j0 = rt * outputs;
+    const int outputs = p.mode == MANY_UP ? BM / 2 : BM;  // of a CTA
+    it->j0 = (2 * rt + rank) * outputs;
     it->row0 = static_cast<int64_t>(lo) * (p.mode == MANY_UP ? 2 * p.n : p.n) + it->j0;
     it->kb0 = it->split * p.kb_per_split;
     it->kbs = min(p.kb_per_split, (p.w.cols + BK - 1) / BK - it->kb0);
@@ -183,43 +192,49 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <typename T, int SEG, bool WIDE>
+template <typename T, int SEG>
 __global__ void __launch_bounds__(THREADS, 1)
     many_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_x,
                 const __grid_constant__ ManyParams p) {
-    using S = Shape<WIDE>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t* codes_at = smem + S::STAGES * S::STAGE_BYTES;
-    float* exchange = reinterpret_cast<float*>(codes_at + S::CSTAGES * C_BYTES);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(exchange) + S::EXCHANGE);
-    int* first_tile = reinterpret_cast<int*>(bars + 32);
-    const uint32_t xfull = smem_u32(bars), afull = xfull + 8 * S::STAGES, empty = afull + 8 * S::STAGES;
-    const uint32_t cfull = empty + 8 * S::STAGES, cempty = cfull + 8 * S::CSTAGES;
-    const uint32_t tfull = cempty + 8 * S::CSTAGES, tempty = tfull + 16, drain = tempty + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 31);
+    uint8_t* codes_at = smem + XSTAGES * X_BYTES;
+    float* exchange = reinterpret_cast<float*>(codes_at + CSTAGES * C_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + 2 * BM * 8);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
+    int* first_tile = reinterpret_cast<int*>(bars + BARS + 1);
+    const uint32_t xfull = smem_u32(bars), xempty = xfull + 8 * XSTAGES;  // xfull: the leader's, both CTAs' bytes
+    const uint32_t cfull = xempty + 8 * XSTAGES, cempty = cfull + 8 * CSTAGES;
+    const uint32_t afull = cempty + 8 * CSTAGES, aempty = afull + 8 * ASTAGES;  // afull: the leader's
+    const uint32_t tfull = aempty + 8 * ASTAGES, tempty = tfull + 16, drain = tempty + 16;  // tempty: the leader's
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
+    const uint32_t rank = cluster_ctarank();
+    const bool leader = rank == 0;
+    const int pair = static_cast<int>(cluster_id_x()), pairs = static_cast<int>(nclusters_x());
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::STAGES; ++s) {
+        for (int s = 0; s < XSTAGES; ++s) {
             mbar_init(xfull + 8 * s, 1);
-            mbar_init(afull + 8 * s, S::DECODERS);
-            mbar_init(empty + 8 * s, 1);
+            mbar_init(xempty + 8 * s, 1);
         }
-        for (int s = 0; s < S::CSTAGES; ++s) {
+        for (int s = 0; s < CSTAGES; ++s) {
             mbar_init(cfull + 8 * s, 1);
-            mbar_init(cempty + 8 * s, S::DECODERS);
+            mbar_init(cempty + 8 * s, DECODERS);
+        }
+        for (int s = 0; s < ASTAGES; ++s) {
+            mbar_init(afull + 8 * s, DECODERS);  // one warpgroup of each CTA
+            mbar_init(aempty + 8 * s, 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(tfull + 8 * b, 1);
-            mbar_init(tempty + 8 * b, S::SUMMERS);
+            mbar_init(tempty + 8 * b, 2 * SUMMERS);
         }
         mbar_init(drain, 1);
         fence_barrier_init();
         tma_prefetch_desc(&tm_codes);
         tma_prefetch_desc(&tm_x);
     }
-    if (warp == 3) tmem_alloc(smem_u32(tmem_slot), 2 * S::COLS);
+    if (warp == 3) tmem_alloc_pair(smem_u32(tmem_slot), 512);
     if (warp == 4) {  // tiles of activations before each expert's
         int before = 0;
         for (int e0 = 0; e0 <= p.experts; e0 += 32) {
@@ -237,39 +252,43 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     tc_fence_before();
     __syncthreads();
+    cluster_sync();  // both CTAs' barriers exist before either signals the other
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int items = p.row_tiles * first_tile[p.experts] * p.splits;
     Item it;
 
     if (wg == 0) {
-        regs_down<32>();
-        if (warp == 0) {  // activations
+        regs_down<REGS_CONTROL>();
+        if (warp == 0) {  // activations: this CTA's half of the tile's
             if (elect_one()) {
                 const uint64_t policy = l2_policy_evict_last();
                 int s = 0;
                 uint32_t phase = 0, armed = 0, armed_phase = 0;
                 bool ok = true;
-                for (int u = blockIdx.x; u < items && ok; u += gridDim.x) {
-                    if (!item_at(u, p, first_tile, &it)) continue;
-                    const int boxes = (it.n + 63) / 64;
+                for (int u = pair; u < items && ok; u += pairs) {
+                    if (!item_at(u, p, first_tile, rank, &it)) continue;
+                    const int boxes = (it.n / 2 + X_BOX - 1) / X_BOX;
+                    const int row = static_cast<int>(it.p0) + static_cast<int>(rank) * (it.n / 2);
                     for (int kb = 0; kb < it.kbs; ++kb) {
-                        if (!mbar_wait(empty + 8 * s, phase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) {
+                        if (!mbar_wait(xempty + 8 * s, phase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) {
                             ok = false;
                             break;
                         }
-                        mbar_expect_tx(xfull + 8 * s, boxes * 64 * BK * 2);
-                        armed |= 1u << s;
-                        armed_phase = (armed_phase & ~(1u << s)) | phase << s;
-                        const uint32_t dst = smem_u32(smem + s * S::STAGE_BYTES);
+                        if (leader) {
+                            mbar_expect_tx(xfull + 8 * s, 2 * boxes * X_BOX_BYTES);
+                            armed |= 1u << s;
+                            armed_phase = (armed_phase & ~(1u << s)) | phase << s;
+                        }
+                        const uint32_t full = mapa_shared(xfull + 8 * s, 0);
+                        const uint32_t dst = smem_u32(smem + s * X_BYTES);
                         for (int b = 0; b < boxes; ++b)
-                            tma_load_2d(dst + b * (64 * BK * 2), &tm_x, xfull + 8 * s, (it.kb0 + kb) * BK,
-                                        static_cast<int>(it.p0) + b * 64, policy);
-                        if (++s == S::STAGES) s = 0, phase ^= 1;
+                            tma_load_2d_pair(dst + b * X_BOX_BYTES, &tm_x, full, (it.kb0 + kb) * BK, row + b * X_BOX, policy);
+                        if (++s == XSTAGES) s = 0, phase ^= 1;
                     }
                 }
-                if (!ok)
-                    for (int i = 0; i < S::STAGES; ++i)
+                if (!ok && leader)
+                    for (int i = 0; i < XSTAGES; ++i)
                         if (armed >> i & 1)
                             mbar_wait(xfull + 8 * i, armed_phase >> i & 1, p.budget_ns, p.status, KERR_TIMEOUT_DRAIN);
             }
@@ -280,8 +299,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 int s = 0;
                 uint32_t phase = 0, armed = 0, armed_phase = 0;
                 bool ok = true;
-                for (int u = blockIdx.x; u < items && ok; u += gridDim.x) {
-                    if (!item_at(u, p, first_tile, &it)) continue;
+                for (int u = pair; u < items && ok; u += pairs) {
+                    if (!item_at(u, p, first_tile, rank, &it)) continue;
                     const int second = static_cast<int>(it.row0) + (p.mode == MANY_UP ? p.n : 64);
                     for (int kb = 0; kb < it.kbs; kb += 2) {
                         if (!mbar_wait(cempty + 8 * s, phase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) {
@@ -295,31 +314,31 @@ __global__ void __launch_bounds__(THREADS, 1)
                         const int byte = (it.kb0 + kb) * (BK / 2);
                         tma_load_2d(dst, &tm_codes, cfull + 8 * s, byte, static_cast<int>(it.row0), policy);
                         tma_load_2d(dst + C_BYTES / 2, &tm_codes, cfull + 8 * s, byte, second, policy);
-                        if (++s == S::CSTAGES) s = 0, phase ^= 1;
+                        if (++s == CSTAGES) s = 0, phase ^= 1;
                     }
                 }
                 if (!ok)
-                    for (int i = 0; i < S::CSTAGES; ++i)
+                    for (int i = 0; i < CSTAGES; ++i)
                         if (armed >> i & 1)
                             mbar_wait(cfull + 8 * i, armed_phase >> i & 1, p.budget_ns, p.status, KERR_TIMEOUT_DRAIN);
             }
             __syncwarp();
-        } else if (warp == 1) {  // the tensor cores
-            int s = 0, b = 0;
-            uint32_t phase = 0, bphase = 0;
+        } else if (warp == 1 && leader) {  // the tensor cores of both CTAs
+            int s = 0, a = 0, b = 0;
+            uint32_t phase = 0, aphase = 0, bphase = 0;
             bool ok = true, issued = false;
             constexpr int PER_STAGE = SEG >= BK ? 1 : BK / SEG;  // groups' pieces in a stage
             constexpr int MMAS = BK / 16 / PER_STAGE;
-            for (int u = blockIdx.x; u < items && ok; u += gridDim.x) {
-                if (!item_at(u, p, first_tile, &it)) continue;
-                const uint32_t idesc = idesc_f16(BM, it.n, std::is_same<T, __nv_bfloat16>::value);
+            for (int u = pair; u < items && ok; u += pairs) {
+                if (!item_at(u, p, first_tile, rank, &it)) continue;
+                const uint32_t idesc = idesc_f16(2 * BM, it.n, std::is_same<T, __nv_bfloat16>::value);
                 for (int kb = 0; kb < it.kbs && ok; ++kb) {
                     if (!mbar_wait_warp(xfull + 8 * s, phase, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL) ||
-                        !mbar_wait_warp(afull + 8 * s, phase, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL)) {
+                        !mbar_wait_warp(afull + 8 * a, aphase, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL)) {
                         ok = false;
                         break;
                     }
-                    const uint32_t sx = smem_u32(smem + s * S::STAGE_BYTES), sa = sx + S::X_BYTES;
+                    const uint32_t sx = smem_u32(smem + s * X_BYTES), sa = tmem + A_FIRST + a * A_COLS;
                     const bool first = SEG != 128 || (kb & 1) == 0;
                     const bool last = SEG != 128 || (kb & 1) == 1 || kb == it.kbs - 1;
                     for (int h = 0; h < PER_STAGE; ++h) {
@@ -331,12 +350,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                         tc_fence_after();
                         if (elect_one()) {
 #pragma unroll
-                            for (int i = 0; i < MMAS; ++i) {
-                                const int at = (h * MMAS + i) * 32;
-                                mma_f16(tmem + b * S::COLS, smem_desc_sw128(sa + at, 16, 1024), smem_desc_sw128(sx + at, 16, 1024),
-                                        idesc, !first || i != 0);
-                            }
-                            if (last) mma_commit(tfull + 8 * b);
+                            for (int i = 0; i < MMAS; ++i)
+                                mma_f16_pair_ts(tmem + b * MAX_COLS, sa + (h * MMAS + i) * 8,
+                                                smem_desc_sw128(sx + (h * MMAS + i) * 32, 16, 1024), idesc, !first || i != 0);
+                            if (last) mma_commit_pair(tfull + 8 * b, 0x3);
                             issued = true;
                         }
                         __syncwarp();
@@ -346,98 +363,105 @@ __global__ void __launch_bounds__(THREADS, 1)
                         }
                     }
                     if (!ok) break;
-                    if (elect_one()) mma_commit(empty + 8 * s);
+                    if (elect_one()) {
+                        mma_commit_pair(xempty + 8 * s, 0x3);
+                        mma_commit_pair(aempty + 8 * a, 0x3);
+                    }
                     __syncwarp();
-                    if (++s == S::STAGES) s = 0, phase ^= 1;
+                    if (++s == XSTAGES) s = 0, phase ^= 1;
+                    if (++a == ASTAGES) a = 0, aphase ^= 1;
                 }
             }
             if (!ok) {
                 if (elect_one() && issued) {
-                    mma_commit(drain);
+                    mma_commit_pair(drain, 0x1);
                     mbar_wait(drain, 0, p.budget_ns, p.status, KERR_TIMEOUT_DRAIN);
                 }
                 __syncwarp();
             }
         }
-    } else if (wg == 1 || (!WIDE && wg == 3)) {
-        if constexpr (WIDE) regs_down<80>();
-        else regs_down<104>();
-        // A thread turns its row's codes into the operand: all of a stage's 64 positions, or half.
-        const int r = threadIdx.x & 127;
-        constexpr int SPAN = WIDE ? BK : BK / 2;
-        const int k0 = WIDE || wg == 1 ? 0 : SPAN;
-        int s = 0, q = 0;
-        uint32_t phase = 0, qphase = 0;
+    } else if (wg <= 2) {
+        regs_down<REGS_DECODE>();
+        // A thread turns its row's codes into the operand's row, lane r of tensor memory. The two
+        // warpgroups take the two stages of each stage of codes.
+        const int r = threadIdx.x & 127, odd = wg - 1;
+        const uint32_t to = tmem + (static_cast<uint32_t>(r & ~31) << 16) + A_FIRST;
+        const uint8_t* from = codes_at + r * (CODES_K / 2);
+        const int turn = (r >> 1) & 3;  // the 64-byte swizzle's
+        int q = 0;
+        uint32_t qphase = 0, n = 0;  // n: stages of weights so far
         const int groups = (p.w.cols + p.w.group - 1) / p.w.group;
         bool ok = true;
-        for (int u = blockIdx.x; u < items && ok; u += gridDim.x) {
-            if (!item_at(u, p, first_tile, &it)) continue;
+        for (int u = pair; u < items && ok; u += pairs) {
+            if (!item_at(u, p, first_tile, rank, &it)) continue;
             const int64_t row = min(it.row0 + (r < 64 ? r : r - 64 + (p.mode == MANY_UP ? p.n : 64)), static_cast<int64_t>(p.w.rows) - 1);
             const uint8_t* zeros = p.w.zeros ? p.w.zeros + row * p.w.groups_rs : nullptr;
-            // this row's zero point at position k
-            auto zero_at = [&](int k) {
-                return zeros ? static_cast<uint32_t>(zeros[min(k / p.w.group, groups - 1)]) & 15u : 8u;
+            constexpr int PIECE = SEG < BK ? SEG : BK;  // positions under one zero point
+            constexpr int PIECES = BK / PIECE;
+            uint32_t next[PIECES];
+            auto fetch = [&](int kb) {  // this row's zero points of stage kb
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i)
+                    next[i] = zeros ? zeros[min(((it.kb0 + kb) * BK + i * PIECE) / p.w.group, groups - 1)] & 15u : 8u;
             };
-            constexpr int PIECE = SEG < SPAN ? SEG : SPAN;  // positions under one zero point
-            constexpr int PIECES = SPAN / PIECE;
-            uint32_t z[PIECES], next[PIECES];
-#pragma unroll
-            for (int i = 0; i < PIECES; ++i) next[i] = zero_at(it.kb0 * BK + k0 + i * PIECE);
-            for (int kb = 0; kb < it.kbs; ++kb) {
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i) {
-                    z[i] = zero_pair<T>(next[i]);
-                    if (zeros) next[i] = zero_at((it.kb0 + kb + 1) * BK + k0 + i * PIECE);
-                }
-                if ((kb & 1) == 0 &&
-                    !mbar_wait_warp(cfull + 8 * q, qphase, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL)) {
+            fetch(odd);
+            for (int kb = odd; kb - odd < it.kbs; kb += 2) {
+                if (!mbar_wait_warp(cfull + 8 * q, qphase, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL)) {
                     ok = false;
                     break;
                 }
-                const uint8_t* from = codes_at + q * C_BYTES + r * (CODES_K / 2) + ((kb & 1) * BK + k0) / 2;
-                uint4 c[SPAN / 32];
-#pragma unroll
-                for (int i = 0; i < SPAN / 32; ++i) c[i] = reinterpret_cast<const uint4*>(from)[i];
-                if ((kb & 1) == 1 || kb == it.kbs - 1) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(cempty + 8 * q);
-                    if (++q == S::CSTAGES) q = 0, qphase ^= 1;
-                }
-                if (!mbar_wait_warp(empty + 8 * s, phase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) {
-                    ok = false;
-                    break;
-                }
-                uint8_t* to = smem + s * S::STAGE_BYTES + S::X_BYTES + r * (BK * 2);
-#pragma unroll
-                for (int i = 0; i < SPAN / 8; ++i) {
-                    const uint32_t w = i % 4 == 0 ? c[i / 4].x : i % 4 == 1 ? c[i / 4].y : i % 4 == 2 ? c[i / 4].z : c[i / 4].w;
-                    *reinterpret_cast<uint4*>(to + (((k0 / 8 + i) ^ (r & 7)) << 4)) = decode8<T>(w, z[i * 8 / PIECE]);
-                }
-                fence_proxy_async();
+                const uint4 c0 = *reinterpret_cast<const uint4*>(from + q * C_BYTES + (((2 * odd) ^ turn) << 4));
+                const uint4 c1 = *reinterpret_cast<const uint4*>(from + q * C_BYTES + (((2 * odd + 1) ^ turn) << 4));
                 __syncwarp();
-                if (lane == 0) mbar_arrive(afull + 8 * s);
-                if (++s == S::STAGES) s = 0, phase ^= 1;
+                if (lane == 0) mbar_arrive(cempty + 8 * q);
+                if (++q == CSTAGES) q = 0, qphase ^= 1;
+                if (kb >= it.kbs) break;  // the last stage of codes was half a one
+                const uint32_t z0 = zero_pair<T>(next[0]), z1 = zero_pair<T>(next[PIECES - 1]);
+                if (zeros) fetch(kb + 2);
+                const uint32_t a = (n + kb) % ASTAGES, aphase = (n + kb) / ASTAGES & 1;
+                if (!mbar_wait_warp(aempty + 8 * a, aphase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                uint32_t v[16];
+                auto put = [&](const uint4& c, uint32_t z, int at) {
+                    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 d = decode8<T>(w[i], z);
+                        v[4 * i] = d.x, v[4 * i + 1] = d.y, v[4 * i + 2] = d.z, v[4 * i + 3] = d.w;
+                    }
+                    __syncwarp();
+                    tmem_st16(to + a * A_COLS + at, v);
+                };
+                put(c0, z0, 0);
+                put(c1, z1, 16);
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_pair(mapa_shared(afull + 8 * a, 0));
             }
+            n += it.kbs;
         }
     } else {
-        if constexpr (WIDE) regs_up<200>();
-        else regs_up<208>();
-        const int r = threadIdx.x & 127, part = WIDE ? wg - 2 : 0;
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(r & ~31) << 16) + part * 128;
+        regs_up<REGS_SUM>();
+        const int r = threadIdx.x & 127, part = wg - 3;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(r & ~31) << 16) + part * PART;
         const int groups = (p.w.cols + p.w.group - 1) / p.w.group;
         int b = 0;
         uint32_t bphase = 0;
         bool ok = true;
-        for (int u = blockIdx.x; u < items && ok; u += gridDim.x) {
-            if (!item_at(u, p, first_tile, &it)) continue;
+        for (int u = pair; u < items && ok; u += pairs) {
+            if (!item_at(u, p, first_tile, rank, &it)) continue;
             const int64_t row = min(it.row0 + (r < 64 ? r : r - 64 + (p.mode == MANY_UP ? p.n : 64)), static_cast<int64_t>(p.w.rows) - 1);
             const int64_t scales = row * p.w.groups_rs;
             const int from = it.kb0 * BK, to = min(p.w.cols, from + it.kbs * BK);
             auto scale_at = [&](int k) { return load_f32(p.w.scales, scales + min(k / p.w.group, groups - 1), p.w.scale_type); };
-            uint64_t acc[64];
+            uint64_t acc[PART / 2];
 #pragma unroll
-            for (int i = 0; i < 64; ++i) acc[i] = 0;
-            const int mine = it.n - part * 128;  // this warpgroup's columns
+            for (int i = 0; i < PART / 2; ++i) acc[i] = 0;
+            const int mine = it.n - part * PART;  // this warpgroup's columns
             float next = scale_at(from);
             for (int k = from; k < to; k += SEG) {
                 const uint32_t sb = __float_as_uint(next);
@@ -448,20 +472,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                     break;
                 }
                 tc_fence_after();
+                // Sixteen columns travel while the sixteen before them are added.
+                uint32_t v[2][16];
+                __syncwarp();
+                if (mine > 0) tmem_ld16(lanes + b * MAX_COLS, v[0]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    if (c * 32 < mine) {
-                        uint32_t v[32];
-                        __syncwarp();
-                        tmem_ld32(lanes + b * S::COLS + c * 32, v);
+                for (int c = 0; c < PART / 16; ++c) {
+                    if (c * 16 < mine) {
                         tmem_ld_wait();
+                        if (c + 1 < PART / 16 && (c + 1) * 16 < mine) tmem_ld16(lanes + b * MAX_COLS + (c + 1) * 16, v[(c + 1) & 1]);
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], v[2 * i], v[2 * i + 1], scale);
+                        for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], scale);
                     }
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(tempty + 8 * b);
+                if (lane == 0) mbar_arrive_pair(mapa_shared(tempty + 8 * b, 0));
                 b ^= 1;
                 if (b == 0) bphase ^= 1;
             }
@@ -470,17 +496,17 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!ok) break;
             // Sums leave through shared memory eight columns at a time, [column][row], so that a
             // thread stores neighbouring outputs of one column at once.
-            const int left = it.cols - part * 128;  // this warpgroup's existing columns
+            const int left = it.cols - part * PART;  // this warpgroup's existing columns
             float* swap = exchange + part * (BM * 8);
             const int col = r >> 4;  // the column of eight that this thread stores
             if (p.mode == MANY_UP) {
                 // Rows 0 .. 63 are gates, 64 .. 127 the same outputs' ups.
                 const int j = (r & 15) * 4;
                 const float* gate = swap + col * BM + j;
-                T* to = static_cast<T*>(p.h) + (it.p0 + part * 128 + col) * p.h_rs + it.j0 + j;
+                T* to = static_cast<T*>(p.h) + (it.p0 + part * PART + col) * p.h_rs + it.j0 + j;
                 const int valid = min(4, p.n - it.j0 - j);
 #pragma unroll
-                for (int c = 0; c < 128; c += 8)
+                for (int c = 0; c < PART; c += 8)
                     if (c < left) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
@@ -493,12 +519,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const float* from = swap + col * BM + j;
                 const int valid = min(8, p.n - it.j0 - j);
 #pragma unroll
-                for (int c = 0; c < 128; c += 8)
+                for (int c = 0; c < PART; c += 8)
                     if (c < left) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
                         asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                        if (c + col < left && valid > 0) out(p, it, it.p0 + part * 128 + c + col, it.j0 + j, from, valid);
+                        if (c + col < left && valid > 0) out(p, it, it.p0 + part * PART + c + col, it.j0 + j, from, valid);
                         asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
                     }
             }
@@ -507,39 +533,39 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     tc_fence_before();
     __syncthreads();
+    cluster_sync();  // neither CTA leaves while the other may still signal it
     if (warp == 3) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * S::COLS);
+        tmem_dealloc_pair(tmem, 512);
     }
 }
 
-// A launch's tile width and splits. Rows of x are spread evenly over their tiles, so a tile is
-// as wide as the rows allow up to 256 (or 128, where none needs more: the second warpgroup of
-// decoders then halves the time a stage's codes take). For one matrix the width is chosen by the
-// time of whole waves of tiles.
+int resident_pairs(const uor_b200_ctx* ctx);
+
+// A launch's tile width and splits. An expert's rows are spread evenly over their tiles; for one
+// matrix the width is chosen by the time of whole waves of tiles.
 void plan(const uor_b200_ctx* ctx, ManyParams* p) {
-    const int outputs = p->mode == MANY_UP ? BM / 2 : BM;
+    const int outputs = p->mode == MANY_UP ? BM : 2 * BM;
+    const int clusters = resident_pairs(ctx);
     p->row_tiles = (p->n + outputs - 1) / outputs;
     const int kbs = (p->w.cols + BK - 1) / BK;
     p->splits = 1;
-    p->max_cols = p->row_bound <= 128 ? 128 : 256;
+    p->max_cols = MAX_COLS;
     int64_t tiles = p->experts;
     if (p->mode == MANY_DENSE) {
-        if (p->m > 256) {
-            double best = 0;
-            for (int width = 256; width >= 160; width -= 16) {
-                const int64_t tt = (p->m + width - 1) / width;
-                const int64_t each = ((p->m + tt - 1) / tt + 15) & ~15ll;
-                const int64_t waves = (tt * p->row_tiles + ctx->sm_count - 1) / ctx->sm_count;
-                const double cost = static_cast<double>(waves) * (each + 24);  // a tile's fixed part
-                if (best == 0 || cost < best) best = cost, p->max_cols = width;
-            }
+        double best = 0;
+        for (int width = MAX_COLS; width >= 96 && p->m > MAX_COLS; width -= 32) {
+            const int64_t tt = (p->m + width - 1) / width;
+            const int64_t each = ((p->m + tt - 1) / tt + 31) & ~31ll;
+            const int64_t waves = (tt * p->row_tiles + clusters - 1) / clusters;
+            const double cost = static_cast<double>(waves) * (each + 24);  // a tile's fixed part
+            if (best == 0 || cost < best) best = cost, p->max_cols = width;
         }
         tiles = (p->m + p->max_cols - 1) / p->max_cols;
     }
     if (p->mode != MANY_UP) {
         // Whole stages of codes to a split, and eight of them at least.
-        int64_t want = ctx->sm_count / (tiles * p->row_tiles);
+        int64_t want = clusters / (tiles * p->row_tiles);
         const int64_t most = kbs / 16;
         if (want > most) want = most;
         if (want > 8) want = 8;
@@ -549,34 +575,66 @@ void plan(const uor_b200_ctx* ctx, ManyParams* p) {
     p->splits = (kbs + p->kb_per_split - 1) / p->kb_per_split;
 }
 
-template <typename T, int SEG, bool WIDE>
-int launch_many(uor_b200_ctx* ctx, ManyParams& p) {
-    CUtensorMap tm_codes, tm_x;
-    const uint64_t rows = static_cast<uint64_t>(p.w.rows);
-    if (!make_tmap_u8(&tm_codes, p.w.codes, (p.w.cols + 1) / 2, rows, p.w.row_bytes, CODES_K / 2, 64, false) ||
-        !make_tmap_u16(&tm_x, p.x, p.w.cols, p.x_rows, p.x_rs * 2, BK, 64))
-        return UOR_B200_DEVICE_ERROR;
-    auto* kernel = many_kernel<T, SEG, WIDE>;
-    static bool ready[64] = {};
-    if (!ready[ctx->device & 63]) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<WIDE>::SMEM) != cudaSuccess)
-            return UOR_B200_DEVICE_ERROR;
-        ready[ctx->device & 63] = true;
+// The pairs that run at one time. All instances have the same resources.
+int resident_pairs(const uor_b200_ctx* ctx) {
+    static int most[64] = {};
+    int& n = most[ctx->device & 63];
+    if (n) return n;
+    auto* kernel = many_kernel<__nv_bfloat16, 128>;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(ctx->sm_count / 2 * 2);
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = SMEM;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    c.attrs = &attr;
+    c.numAttrs = 1;
+    int found = 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&found, kernel, &c) != cudaSuccess || found < 1) {
+        cudaGetLastError();
+        found = ctx->sm_count / 2;
     }
-    kernel<<<ctx->sm_count, THREADS, Shape<WIDE>::SMEM, ctx->stream>>>(tm_codes, tm_x, p);
-    return cuda_status(cudaGetLastError());
+    return n = found;
 }
 
 template <typename T, int SEG>
-int by_width(uor_b200_ctx* ctx, ManyParams& p) {
-    return p.max_cols > 128 ? launch_many<T, SEG, true>(ctx, p) : launch_many<T, SEG, false>(ctx, p);
+int launch_many(uor_b200_ctx* ctx, ManyParams& p) {
+    CUtensorMap tm_codes, tm_x;
+    const uint64_t rows = static_cast<uint64_t>(p.w.rows);
+    if (!make_tmap_u8_sw64(&tm_codes, p.w.codes, (p.w.cols + 1) / 2, rows, p.w.row_bytes, CODES_K / 2, 64) ||
+        !make_tmap_u16(&tm_x, p.x, p.w.cols, p.x_rows, p.x_rs * 2, BK, X_BOX))
+        return UOR_B200_DEVICE_ERROR;
+    auto* kernel = many_kernel<T, SEG>;
+    static bool ready[64] = {};
+    if (!ready[ctx->device & 63]) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM) != cudaSuccess)
+            return UOR_B200_DEVICE_ERROR;
+        ready[ctx->device & 63] = true;
+    }
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(2 * resident_pairs(ctx));
+    c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = SMEM;
+    c.stream = ctx->stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    c.attrs = &attr;
+    c.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&c, kernel, tm_codes, tm_x, p));
 }
 
 template <typename T>
 int by_segment(uor_b200_ctx* ctx, ManyParams& p) {
-    if (p.w.group % 128 == 0) return by_width<T, 128>(ctx, p);
-    if (p.w.group % 64 == 0) return by_width<T, 64>(ctx, p);
-    return by_width<T, 32>(ctx, p);
+    if (p.w.group % 128 == 0) return launch_many<T, 128>(ctx, p);
+    if (p.w.group % 64 == 0) return launch_many<T, 64>(ctx, p);
+    return launch_many<T, 32>(ctx, p);
 }
 
 }  // namespace

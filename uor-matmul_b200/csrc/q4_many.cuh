@@ -23,14 +23,13 @@ struct ManyParams {
     const int* offsets;   // [experts + 1] first sorted row of each expert; null for dense
     const int* perm;      // the pair behind each sorted row
     int m;                // dense: rows of x
-    int row_bound;        // at least the rows of any launch, for choosing a tile (dense: m)
     MatOut y;             // dense, without splits
     float* part;          // dense with splits: [splits][m][n]; down: [splits][pairs][n]
     int64_t part_rows;    // m or pairs
     void* h;              // up: [sorted rows][h_rs]
     int64_t h_rs;
     // Set by the launch:
-    int max_cols;         // rows of x in a tile, a multiple of 16
+    int max_cols;         // rows of x in a tile, a multiple of 32
     int row_tiles, splits, kb_per_split;
     int* status;
     uint64_t budget_ns;
