@@ -6,19 +6,22 @@
 // instruction's M side, so that a thread of the epilogue owns one weight row and a group's scale
 // is one number per thread.
 //
-// The roles of a CTA: a warp brings 64-position stages of activations by TMA, another the codes of
-// 128 positions; two warpgroups turn each code into a 16-bit float, exactly (code - zero), and
-// store it to tensor memory, where the instruction takes its A side from; one thread of the pair
-// issues the tcgen05.mma; two warpgroups hold the sums. A group's products are summed in tensor
-// memory, and at the group's end these warpgroups add scale x sum to their f32 registers, while the
-// next group runs in the other of two accumulators. So no weight is rounded: rounding scale x
-// code to 16 bits would cost as much precision as rounding the output does.
+// The roles of a CTA: a warp brings 128-position stages of activations by TMA, another the codes;
+// two warpgroups turn each code into a 16-bit float, exactly (code - zero), and store it to tensor
+// memory, where the instruction takes its A side from; one thread of the pair issues the
+// tcgen05.mma; two warpgroups hold the sums. A group's products are summed in tensor memory, and
+// at the group's end these warpgroups add scale x sum to their f32 registers, while the next group
+// runs in the other of two accumulators. So no weight is rounded: rounding scale x code to 16
+// bits would cost as much precision as rounding the output does.
 //
 // Why this shape. With the weights in shared memory and one CTA per 128 x 256 tile, the operands'
-// reads, the TMA's and the decoders' writes came to 104 KB a stage, 830 cycles at 128 bytes a
-// cycle, for 512 cycles of multiplication (2048 x 8192 x 8192: 366 us, 295 us without decoding
-// and scaling). Here a stage moves 4 x 3 KB of operands, 12 KB of TMA and 8 KB of codes for 384.
-// Tensor memory's 512 columns hold two accumulators of 192 and four stages of weights of 32.
+// reads, the TMA's and the decoders' writes came to 104 KB per 64 positions, 830 cycles at 128
+// bytes a cycle, for 512 cycles of multiplication (2048 x 8192 x 8192: 366 us, 295 us without
+// decoding and scaling). Here 64 positions move 4 x 3 KB of operands, 12 KB of TMA and 8 KB of
+// codes for 384. Beside that it is instructions that count, and waiting ones among them: one
+// arrival and one commit per 128 positions, waits that sleep, and no release at cluster scope.
+// Tensor memory's 512 columns hold two accumulators of 192 and two stages of weights of 64, or
+// two of 128 and four where tiles have at most 128 columns.
 //
 // Every wait is bounded; a role that gives up records it, and every other role leaves after it.
 #include "q4_many.cuh"
@@ -33,26 +36,28 @@ namespace uor {
 namespace {
 
 constexpr int BM = 128;        // weight rows of a CTA's half of a tile
-constexpr int BK = 64;         // reduction positions of a stage: 128 bytes of a row
-constexpr int CODES_K = 128;   // of a stage of codes
+constexpr int BK = 128;        // reduction positions of a stage
+constexpr int ATOM = 64;       // positions in the 128 bytes that the activations' swizzle spans
 constexpr int MAX_COLS = 192;  // activation rows of a tile
 constexpr int X_BOX = 32;      // activation rows of one TMA copy
-constexpr int X_BOX_BYTES = X_BOX * BK * 2;
-constexpr int X_BYTES = MAX_COLS / 2 * BK * 2;
-constexpr int C_BYTES = BM * CODES_K / 2;
-constexpr int XSTAGES = 8, CSTAGES = 6, ASTAGES = 4;
+constexpr int X_BOX_BYTES = X_BOX * ATOM * 2;
+constexpr int ATOM_BYTES = MAX_COLS / 2 * ATOM * 2;
+constexpr int X_BYTES = ATOM_BYTES * BK / ATOM;
+constexpr int C_BYTES = BM * BK / 2;
+constexpr int STAGES = 4, CSTAGES = 6, MOST_ASTAGES = 4;
 constexpr int A_COLS = BK / 2;                       // tensor-memory columns of a stage of weights
-constexpr int A_FIRST = 2 * MAX_COLS;
 constexpr int DECODERS = 8, SUMMERS = 8;             // warps of a CTA
 constexpr int PART = MAX_COLS / 2;                   // columns of a summing warpgroup
-constexpr int EXCHANGE = BM * 8 * 4;                 // bytes, per summing warpgroup
-constexpr int BARS = 2 * XSTAGES + 2 * CSTAGES + 2 * ASTAGES + 5;
-constexpr int SMEM = XSTAGES * X_BYTES + CSTAGES * C_BYTES + 2 * EXCHANGE + (BARS + 1) * 8 + (MANY_MAX_EXPERTS + 1) * 4 + 1024;
+constexpr int OUT_COLS = 32;                         // columns that leave at a time
+constexpr int EXCHANGE = BM * OUT_COLS * 4;          // bytes, per summing warpgroup
+constexpr int BARS = 2 * STAGES + 2 * CSTAGES + MOST_ASTAGES + 5;
+constexpr int SMEM = STAGES * X_BYTES + CSTAGES * C_BYTES + 2 * EXCHANGE + (BARS + 1) * 8 + (MANY_MAX_EXPERTS + 1) * 4 + 1024;
+constexpr uint32_t NAP_NS = 1000;  // a wait's sleep between looks; an arrival ends it at once
 // Warpgroup 0: TMA, MMA; 1 and 2: decoders; 3 and 4: sums. Registers: 96 a thread at launch.
 constexpr int THREADS = 640;
-constexpr int REGS_CONTROL = 48, REGS_DECODE = 48, REGS_SUM = 160;
+constexpr int REGS_CONTROL = 32, REGS_DECODE = 56, REGS_SUM = 168;
 static_assert(SMEM <= 232448, "shared memory of a block");
-static_assert(A_FIRST + ASTAGES * A_COLS == 512, "tensor memory");
+static_assert(2 * MAX_COLS + 2 * A_COLS <= 512 && 2 * 128 + 4 * A_COLS <= 512, "tensor memory");
 static_assert(REGS_CONTROL + 2 * REGS_DECODE + 2 * REGS_SUM <= 5 * 96, "registers of the launch");
 
 struct Item {
@@ -126,6 +131,18 @@ __device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
     return (std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u) | (z << 16) | z;
 }
 
+// Steps along a row's scales (or zero points) by a piece of a group at a time.
+struct GroupWalk {
+    int at, pos, group, last;
+    __device__ __forceinline__ GroupWalk(int k, int group, int cols)
+        : at(k / group), pos(k - k / group * group), group(group), last((cols + group - 1) / group - 1) {}
+    __device__ __forceinline__ int index() const { return min(at, last); }
+    __device__ __forceinline__ void step(int by) {
+        pos += by;
+        while (pos >= group) pos -= group, ++at;
+    }
+};
+
 // acc += v * s on two floats at once.
 __device__ __forceinline__ void fma2(uint64_t& acc, uint32_t lo, uint32_t hi, uint64_t s) {
     asm("{\n .reg .b64 v;\n mov.b64 v, {%1, %2};\n fma.rn.f32x2 %0, v, %3, %0;\n}\n" : "+l"(acc) : "r"(lo), "r"(hi), "l"(s));
@@ -134,56 +151,61 @@ __device__ __forceinline__ float half_of(uint64_t v, int i) {
     return __uint_as_float(static_cast<uint32_t>(i ? v >> 32 : v));
 }
 
-// Four inner activations from their gates' and ups' sums.
+// The sums of `cols` activation rows from row i0 on, [column][row] in shared memory, to where
+// this launch's outputs go; 128 threads, `r` this one. Each stores eight neighbouring outputs of a
+// column (four with gates and ups), as one vector where they lie so.
 template <typename T>
-__device__ __noinline__ void up_out(const float* gate, int valid, T* to) {
-    const float4 g = *reinterpret_cast<const float4*>(gate), u = *reinterpret_cast<const float4*>(gate + 64);
-    const float v[4] = {silu(g.x) * u.x, silu(g.y) * u.y, silu(g.z) * u.z, silu(g.w) * u.w};
-    if (valid == 4) {  // rows of h begin at multiples of 16 bytes
-        T t[4] = {from_f32<T>(v[0]), from_f32<T>(v[1]), from_f32<T>(v[2]), from_f32<T>(v[3])};
-        uint2 bits;
-        memcpy(&bits, t, 8);
-        *reinterpret_cast<uint2*>(to) = bits;
-    } else {
-        for (int i = 0; i < valid; ++i) to[i] = from_f32<T>(i == 0 ? v[0] : i == 1 ? v[1] : v[2]);
-    }
-}
-
-// Eight neighbouring outputs of activation row i from output j on, to where this launch's go.
-__device__ __noinline__ void out(const ManyParams& p, const Item& it, int64_t i, int j, const float* from, int valid) {
-    const float4 a = *reinterpret_cast<const float4*>(from), b = *reinterpret_cast<const float4*>(from + 4);
-    void* to = p.part;
-    int64_t at, step = 1;
-    int type = UOR_B200_F32;
-    if (p.mode == MANY_DOWN || p.splits > 1) {
-        at = (it.split * p.part_rows + (p.mode == MANY_DOWN ? p.perm[i] : i)) * p.n + j;
-    } else {
-        to = p.y.p;
-        type = p.y.type;
-        step = p.y.cs;
-        at = i * p.y.rs + j * step;
-    }
-    const int size = type == UOR_B200_F32 ? 4 : 2;
-    char* c = static_cast<char*>(to) + at * size;
-    if (valid == 8 && step == 1 && reinterpret_cast<uint64_t>(c) % 16 == 0) {
-        if (type == UOR_B200_F32) {
-            reinterpret_cast<float4*>(c)[0] = a;
-            reinterpret_cast<float4*>(c)[1] = b;
-        } else {
-            uint4 w;
-            if (type == UOR_B200_BF16) {
-                const __nv_bfloat162 t[4] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w),
-                                             __floats2bfloat162_rn(b.x, b.y), __floats2bfloat162_rn(b.z, b.w)};
-                memcpy(&w, t, 16);
+__device__ __noinline__ void sums_out(const ManyParams& p, const Item& it, const float* swap, int64_t i0, int cols, int r) {
+    if (p.mode == MANY_UP) {
+        // Rows 0 .. 63 are gates, 64 .. 127 the same outputs' ups.
+        const int j = (r & 15) * 4, valid = min(4, p.n - it.j0 - j);
+        T* to = static_cast<T*>(p.h) + i0 * p.h_rs + it.j0 + j;
+        for (int c = r >> 4; c < cols && valid > 0; c += 8) {
+            const float4 g = *reinterpret_cast<const float4*>(swap + c * BM + j);
+            const float4 u = *reinterpret_cast<const float4*>(swap + c * BM + j + 64);
+            const T v[4] = {from_f32<T>(silu(g.x) * u.x), from_f32<T>(silu(g.y) * u.y), from_f32<T>(silu(g.z) * u.z),
+                            from_f32<T>(silu(g.w) * u.w)};
+            if (valid == 4) {  // rows of h begin at multiples of 16 bytes
+                uint2 bits;
+                memcpy(&bits, v, 8);
+                *reinterpret_cast<uint2*>(to + c * p.h_rs) = bits;
             } else {
-                const __half2 t[4] = {__floats2half2_rn(a.x, a.y), __floats2half2_rn(a.z, a.w), __floats2half2_rn(b.x, b.y),
-                                      __floats2half2_rn(b.z, b.w)};
-                memcpy(&w, t, 16);
+                for (int k = 0; k < valid; ++k) to[c * p.h_rs + k] = k == 0 ? v[0] : k == 1 ? v[1] : v[2];
             }
-            *reinterpret_cast<uint4*>(c) = w;
         }
-    } else {
-        for (int k = 0; k < valid; ++k) store_f32(to, at + k * step, type, from[k]);
+        return;
+    }
+    const int j = (r & 15) * 8, valid = min(8, p.n - it.j0 - j);
+    const bool parts = p.mode == MANY_DOWN || p.splits > 1;
+    const int type = parts ? UOR_B200_F32 : p.y.type;
+    const int64_t rs = parts ? p.n : p.y.rs, step = parts ? 1 : p.y.cs;
+    void* to = parts ? p.part + it.split * p.part_rows * p.n : p.y.p;
+    for (int c = r >> 4; c < cols && valid > 0; c += 8) {
+        const float4 a = *reinterpret_cast<const float4*>(swap + c * BM + j);
+        const float4 b = *reinterpret_cast<const float4*>(swap + c * BM + j + 4);
+        const int64_t i = p.mode == MANY_DOWN ? p.perm[i0 + c] : i0 + c;
+        const int64_t at = i * rs + (it.j0 + j) * step;
+        char* first = static_cast<char*>(to) + at * (type == UOR_B200_F32 ? 4 : 2);
+        if (valid == 8 && step == 1 && reinterpret_cast<uint64_t>(first) % 16 == 0) {
+            if (type == UOR_B200_F32) {
+                reinterpret_cast<float4*>(first)[0] = a;
+                reinterpret_cast<float4*>(first)[1] = b;
+            } else {
+                uint4 w;
+                if (type == UOR_B200_BF16) {
+                    const __nv_bfloat162 t[4] = {__floats2bfloat162_rn(a.x, a.y), __floats2bfloat162_rn(a.z, a.w),
+                                                 __floats2bfloat162_rn(b.x, b.y), __floats2bfloat162_rn(b.z, b.w)};
+                    memcpy(&w, t, 16);
+                } else {
+                    const __half2 t[4] = {__floats2half2_rn(a.x, a.y), __floats2half2_rn(a.z, a.w), __floats2half2_rn(b.x, b.y),
+                                          __floats2half2_rn(b.z, b.w)};
+                    memcpy(&w, t, 16);
+                }
+                *reinterpret_cast<uint4*>(first) = w;
+            }
+        } else {
+            for (int k = 0; k < valid; ++k) store_f32(to, at + k * step, type, swap[c * BM + j + k]);
+        }
     }
 }
 
@@ -198,33 +220,34 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const __grid_constant__ ManyParams p) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-    uint8_t* codes_at = smem + XSTAGES * X_BYTES;
+    uint8_t* codes_at = smem + STAGES * X_BYTES;
     float* exchange = reinterpret_cast<float*>(codes_at + CSTAGES * C_BYTES);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + 2 * BM * 8);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + 2 * BM * OUT_COLS);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
     int* first_tile = reinterpret_cast<int*>(bars + BARS + 1);
-    const uint32_t xfull = smem_u32(bars), xempty = xfull + 8 * XSTAGES;  // xfull: the leader's, both CTAs' bytes
-    const uint32_t cfull = xempty + 8 * XSTAGES, cempty = cfull + 8 * CSTAGES;
-    const uint32_t afull = cempty + 8 * CSTAGES, aempty = afull + 8 * ASTAGES;  // afull: the leader's
-    const uint32_t tfull = aempty + 8 * ASTAGES, tempty = tfull + 16, drain = tempty + 16;  // tempty: the leader's
+    // xfull, afull and tempty count on the leader, for both CTAs. done: a stage's products are
+    // complete, which frees its activations and its weights, and with one group to a stage is the
+    // sums' signal too (tfull otherwise).
+    const uint32_t xfull = smem_u32(bars), done = xfull + 8 * STAGES;
+    const uint32_t cfull = done + 8 * STAGES, cempty = cfull + 8 * CSTAGES;
+    const uint32_t afull = cempty + 8 * CSTAGES;
+    const uint32_t tfull = afull + 8 * MOST_ASTAGES, tempty = tfull + 16, drain = tempty + 16;
+    constexpr int GROUPS = BK / SEG;  // of a stage
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
     const uint32_t rank = cluster_ctarank();
     const bool leader = rank == 0;
     const int pair = static_cast<int>(cluster_id_x()), pairs = static_cast<int>(nclusters_x());
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < XSTAGES; ++s) {
+        for (int s = 0; s < STAGES; ++s) {
             mbar_init(xfull + 8 * s, 1);
-            mbar_init(xempty + 8 * s, 1);
+            mbar_init(done + 8 * s, 1);
         }
         for (int s = 0; s < CSTAGES; ++s) {
             mbar_init(cfull + 8 * s, 1);
             mbar_init(cempty + 8 * s, DECODERS);
         }
-        for (int s = 0; s < ASTAGES; ++s) {
-            mbar_init(afull + 8 * s, DECODERS);  // one warpgroup of each CTA
-            mbar_init(aempty + 8 * s, 1);
-        }
+        for (int s = 0; s < MOST_ASTAGES; ++s) mbar_init(afull + 8 * s, 2 * DECODERS);
         for (int b = 0; b < 2; ++b) {
             mbar_init(tfull + 8 * b, 1);
             mbar_init(tempty + 8 * b, 2 * SUMMERS);
@@ -256,6 +279,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int items = p.row_tiles * first_tile[p.experts] * p.splits;
+    const int acc_cols = p.max_cols > 128 ? MAX_COLS : 128;
+    const uint32_t a_stages = p.max_cols > 128 ? 2 : 4;
     Item it;
 
     if (wg == 0) {
@@ -263,32 +288,33 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (warp == 0) {  // activations: this CTA's half of the tile's
             if (elect_one()) {
                 const uint64_t policy = l2_policy_evict_last();
-                int s = 0;
-                uint32_t phase = 0, armed = 0, armed_phase = 0;
+                uint32_t n = 0, armed = 0, armed_phase = 0;  // n: stages so far
                 bool ok = true;
                 for (int u = pair; u < items && ok; u += pairs) {
                     if (!item_at(u, p, first_tile, rank, &it)) continue;
                     const int boxes = (it.n / 2 + X_BOX - 1) / X_BOX;
                     const int row = static_cast<int>(it.p0) + static_cast<int>(rank) * (it.n / 2);
-                    for (int kb = 0; kb < it.kbs; ++kb) {
-                        if (!mbar_wait(xempty + 8 * s, phase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) {
+                    for (int kb = 0; kb < it.kbs; ++kb, ++n) {
+                        const uint32_t s = n % STAGES, phase = n / STAGES & 1;
+                        if (!mbar_wait_hint(done + 8 * s, phase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER, NAP_NS)) {
                             ok = false;
                             break;
                         }
                         if (leader) {
-                            mbar_expect_tx(xfull + 8 * s, 2 * boxes * X_BOX_BYTES);
+                            mbar_expect_tx(xfull + 8 * s, 2 * (BK / ATOM) * boxes * X_BOX_BYTES);
                             armed |= 1u << s;
                             armed_phase = (armed_phase & ~(1u << s)) | phase << s;
                         }
                         const uint32_t full = mapa_shared(xfull + 8 * s, 0);
                         const uint32_t dst = smem_u32(smem + s * X_BYTES);
-                        for (int b = 0; b < boxes; ++b)
-                            tma_load_2d_pair(dst + b * X_BOX_BYTES, &tm_x, full, (it.kb0 + kb) * BK, row + b * X_BOX, policy);
-                        if (++s == XSTAGES) s = 0, phase ^= 1;
+                        for (int h = 0; h < BK / ATOM; ++h)
+                            for (int b = 0; b < boxes; ++b)
+                                tma_load_2d_pair(dst + h * ATOM_BYTES + b * X_BOX_BYTES, &tm_x, full,
+                                                 (it.kb0 + kb) * BK + h * ATOM, row + b * X_BOX, policy);
                     }
                 }
                 if (!ok && leader)
-                    for (int i = 0; i < XSTAGES; ++i)
+                    for (int i = 0; i < STAGES; ++i)
                         if (armed >> i & 1)
                             mbar_wait(xfull + 8 * i, armed_phase >> i & 1, p.budget_ns, p.status, KERR_TIMEOUT_DRAIN);
             }
@@ -302,8 +328,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 for (int u = pair; u < items && ok; u += pairs) {
                     if (!item_at(u, p, first_tile, rank, &it)) continue;
                     const int second = static_cast<int>(it.row0) + (p.mode == MANY_UP ? p.n : 64);
-                    for (int kb = 0; kb < it.kbs; kb += 2) {
-                        if (!mbar_wait(cempty + 8 * s, phase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) {
+                    for (int kb = 0; kb < it.kbs; ++kb) {
+                        if (!mbar_wait_hint(cempty + 8 * s, phase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER, NAP_NS)) {
                             ok = false;
                             break;
                         }
@@ -324,102 +350,89 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             __syncwarp();
         } else if (warp == 1 && leader) {  // the tensor cores of both CTAs
-            int s = 0, a = 0, b = 0;
-            uint32_t phase = 0, aphase = 0, bphase = 0;
-            bool ok = true, issued = false;
-            constexpr int PER_STAGE = SEG >= BK ? 1 : BK / SEG;  // groups' pieces in a stage
-            constexpr int MMAS = BK / 16 / PER_STAGE;
-            for (int u = pair; u < items && ok; u += pairs) {
-                if (!item_at(u, p, first_tile, rank, &it)) continue;
-                const uint32_t idesc = idesc_f16(2 * BM, it.n, std::is_same<T, __nv_bfloat16>::value);
-                for (int kb = 0; kb < it.kbs && ok; ++kb) {
-                    if (!mbar_wait_warp(xfull + 8 * s, phase, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL) ||
-                        !mbar_wait_warp(afull + 8 * a, aphase, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL)) {
-                        ok = false;
-                        break;
-                    }
-                    const uint32_t sx = smem_u32(smem + s * X_BYTES), sa = tmem + A_FIRST + a * A_COLS;
-                    const bool first = SEG != 128 || (kb & 1) == 0;
-                    const bool last = SEG != 128 || (kb & 1) == 1 || kb == it.kbs - 1;
-                    for (int h = 0; h < PER_STAGE; ++h) {
-                        if (h && (it.kb0 + kb) * BK + h * SEG >= p.w.cols) break;
-                        if (first && !mbar_wait_warp(tempty + 8 * b, bphase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_ACC)) {
-                            ok = false;
-                            break;
-                        }
-                        tc_fence_after();
-                        if (elect_one()) {
+            if (elect_one()) {
+                uint32_t n = 0, g = 0;  // stages and groups so far
+                bool ok = true;
+                for (int u = pair; u < items && ok; u += pairs) {
+                    if (!item_at(u, p, first_tile, rank, &it)) continue;
+                    const uint32_t idesc = idesc_f16(2 * BM, it.n, std::is_same<T, __nv_bfloat16>::value);
+                    for (int kb = 0; kb < it.kbs && ok; ++kb, ++n) {
+                        const uint32_t s = n % STAGES, a = n % a_stages;
+                        ok = mbar_wait(xfull + 8 * s, n / STAGES & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL) &&
+                             mbar_wait(afull + 8 * a, n / a_stages & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL);
+                        const uint32_t sx = smem_u32(smem + s * X_BYTES), sa = tmem + 2 * acc_cols + a * A_COLS;
 #pragma unroll
-                            for (int i = 0; i < MMAS; ++i)
-                                mma_f16_pair_ts(tmem + b * MAX_COLS, sa + (h * MMAS + i) * 8,
-                                                smem_desc_sw128(sx + (h * MMAS + i) * 32, 16, 1024), idesc, !first || i != 0);
-                            if (last) mma_commit_pair(tfull + 8 * b, 0x3);
-                            issued = true;
+                        for (int h = 0; h < GROUPS; ++h) {
+                            if (!ok || (h && (it.kb0 + kb) * BK + h * SEG >= p.w.cols)) break;
+                            const uint32_t b = g & 1;
+                            ok = mbar_wait(tempty + 8 * b, (g >> 1 & 1) ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_ACC);
+                            if (!ok) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int i = 0; i < SEG / 16; ++i) {
+                                const int k16 = h * (SEG / 16) + i;
+                                mma_f16_pair_ts(tmem + b * acc_cols, sa + k16 * 8,
+                                                smem_desc_sw128(sx + k16 / 4 * ATOM_BYTES + k16 % 4 * 32, 16, 1024), idesc, i != 0);
+                            }
+                            if (GROUPS > 1) mma_commit_pair(tfull + 8 * b, 0x3);
+                            ++g;
                         }
-                        __syncwarp();
-                        if (last) {
-                            b ^= 1;
-                            if (b == 0) bphase ^= 1;
-                        }
+                        if (ok) mma_commit_pair(done + 8 * s, 0x3);
                     }
-                    if (!ok) break;
-                    if (elect_one()) {
-                        mma_commit_pair(xempty + 8 * s, 0x3);
-                        mma_commit_pair(aempty + 8 * a, 0x3);
-                    }
-                    __syncwarp();
-                    if (++s == XSTAGES) s = 0, phase ^= 1;
-                    if (++a == ASTAGES) a = 0, aphase ^= 1;
                 }
-            }
-            if (!ok) {
-                if (elect_one() && issued) {
+                if (!ok && g) {
                     mma_commit_pair(drain, 0x1);
                     mbar_wait(drain, 0, p.budget_ns, p.status, KERR_TIMEOUT_DRAIN);
                 }
-                __syncwarp();
             }
+            __syncwarp();
         }
     } else if (wg <= 2) {
         regs_down<REGS_DECODE>();
-        // A thread turns its row's codes into the operand's row, lane r of tensor memory. The two
-        // warpgroups take the two stages of each stage of codes.
-        const int r = threadIdx.x & 127, odd = wg - 1;
-        const uint32_t to = tmem + (static_cast<uint32_t>(r & ~31) << 16) + A_FIRST;
-        const uint8_t* from = codes_at + r * (CODES_K / 2);
+        // A thread turns its row's codes into the operand's row, lane r of tensor memory: one
+        // warpgroup the first half of a stage's positions, the other the second.
+        const int r = threadIdx.x & 127, part = wg - 1;
+        const uint32_t to = tmem + (static_cast<uint32_t>(r & ~31) << 16) + 2 * acc_cols + part * (A_COLS / 2);
         const int turn = (r >> 1) & 3;  // the 64-byte swizzle's
+        const uint8_t* from = codes_at + r * (BK / 2);
+        const int at0 = ((2 * part) ^ turn) << 4, at1 = ((2 * part + 1) ^ turn) << 4;
         int q = 0;
-        uint32_t qphase = 0, n = 0;  // n: stages of weights so far
-        const int groups = (p.w.cols + p.w.group - 1) / p.w.group;
+        uint32_t qphase = 0, n = 0;  // n: stages so far
         bool ok = true;
         for (int u = pair; u < items && ok; u += pairs) {
             if (!item_at(u, p, first_tile, rank, &it)) continue;
             const int64_t row = min(it.row0 + (r < 64 ? r : r - 64 + (p.mode == MANY_UP ? p.n : 64)), static_cast<int64_t>(p.w.rows) - 1);
             const uint8_t* zeros = p.w.zeros ? p.w.zeros + row * p.w.groups_rs : nullptr;
-            constexpr int PIECE = SEG < BK ? SEG : BK;  // positions under one zero point
-            constexpr int PIECES = BK / PIECE;
-            uint32_t next[PIECES];
-            auto fetch = [&](int kb) {  // this row's zero points of stage kb
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i)
-                    next[i] = zeros ? zeros[min(((it.kb0 + kb) * BK + i * PIECE) / p.w.group, groups - 1)] & 15u : 8u;
+            uint32_t next0 = 8, next1 = 8;  // the zero points of this half's two 32 positions
+            GroupWalk walk(it.kb0 * BK + part * (BK / 2), p.w.group, p.w.cols);
+            auto fetch = [&]() {
+                if (!zeros) return;
+                next0 = next1 = zeros[walk.index()];
+                if (SEG == 32) {
+                    walk.step(32);
+                    next1 = zeros[walk.index()];
+                    walk.step(BK - 32);
+                } else {
+                    walk.step(BK);
+                }
             };
-            fetch(odd);
-            for (int kb = odd; kb - odd < it.kbs; kb += 2) {
-                if (!mbar_wait_warp(cfull + 8 * q, qphase, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL)) {
+            fetch();
+            for (int kb = 0; kb < it.kbs; ++kb, ++n) {
+                if (!mbar_wait_warp_hint(cfull + 8 * q, qphase, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL, NAP_NS)) {
                     ok = false;
                     break;
                 }
-                const uint4 c0 = *reinterpret_cast<const uint4*>(from + q * C_BYTES + (((2 * odd) ^ turn) << 4));
-                const uint4 c1 = *reinterpret_cast<const uint4*>(from + q * C_BYTES + (((2 * odd + 1) ^ turn) << 4));
+                const uint4 c0 = *reinterpret_cast<const uint4*>(from + q * C_BYTES + at0);
+                const uint4 c1 = *reinterpret_cast<const uint4*>(from + q * C_BYTES + at1);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(cempty + 8 * q);
                 if (++q == CSTAGES) q = 0, qphase ^= 1;
-                if (kb >= it.kbs) break;  // the last stage of codes was half a one
-                const uint32_t z0 = zero_pair<T>(next[0]), z1 = zero_pair<T>(next[PIECES - 1]);
-                if (zeros) fetch(kb + 2);
-                const uint32_t a = (n + kb) % ASTAGES, aphase = (n + kb) / ASTAGES & 1;
-                if (!mbar_wait_warp(aempty + 8 * a, aphase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) {
+                const uint32_t z0 = zero_pair<T>(next0 & 15u), z1 = zero_pair<T>(next1 & 15u);
+                fetch();
+                // the stage that used this one's columns is `a_stages` back
+                const uint32_t a = n % a_stages, before = n - a_stages;
+                if (n >= a_stages && !mbar_wait_warp_hint(done + 8 * (before % STAGES), before / STAGES & 1, p.budget_ns, p.status,
+                                                          KERR_TIMEOUT_PRODUCER, NAP_NS)) {
                     ok = false;
                     break;
                 }
@@ -442,92 +455,83 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive_pair(mapa_shared(afull + 8 * a, 0));
             }
-            n += it.kbs;
         }
     } else {
         regs_up<REGS_SUM>();
         const int r = threadIdx.x & 127, part = wg - 3;
-        const uint32_t lanes = tmem + (static_cast<uint32_t>(r & ~31) << 16) + part * PART;
-        const int groups = (p.w.cols + p.w.group - 1) / p.w.group;
-        int b = 0;
-        uint32_t bphase = 0;
+        const uint32_t lanes = tmem + (static_cast<uint32_t>(r & ~31) << 16);
+        uint32_t g = 0;  // groups so far
         bool ok = true;
         for (int u = pair; u < items && ok; u += pairs) {
             if (!item_at(u, p, first_tile, rank, &it)) continue;
             const int64_t row = min(it.row0 + (r < 64 ? r : r - 64 + (p.mode == MANY_UP ? p.n : 64)), static_cast<int64_t>(p.w.rows) - 1);
-            const int64_t scales = row * p.w.groups_rs;
             const int from = it.kb0 * BK, to = min(p.w.cols, from + it.kbs * BK);
-            auto scale_at = [&](int k) { return load_f32(p.w.scales, scales + min(k / p.w.group, groups - 1), p.w.scale_type); };
+            GroupWalk walk(from, p.w.group, p.w.cols);
+            const bool wide = p.w.scale_type == UOR_B200_F32, bf16 = p.w.scale_type == UOR_B200_BF16;
+            const char* scales = static_cast<const char*>(p.w.scales) + row * p.w.groups_rs * (wide ? 4 : 2);
+            uint32_t next;
+            auto fetch = [&]() {
+                if (wide) next = reinterpret_cast<const uint32_t*>(scales)[walk.index()];
+                else next = reinterpret_cast<const uint16_t*>(scales)[walk.index()];
+                walk.step(SEG);
+            };
             uint64_t acc[PART / 2];
 #pragma unroll
             for (int i = 0; i < PART / 2; ++i) acc[i] = 0;
-            const int mine = it.n - part * PART;  // this warpgroup's columns
-            float next = scale_at(from);
-            for (int k = from; k < to; k += SEG) {
-                const uint32_t sb = __float_as_uint(next);
+            const int mine = it.n / 2;  // this warpgroup's columns: sixteens
+            const uint32_t sums = lanes + part * mine;
+            fetch();
+            for (int k = from; k < to; k += SEG, ++g) {
+                const uint32_t b = g & 1;
+                const uint32_t sb = wide ? next
+                                    : bf16 ? next << 16
+                                           : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(next))));
                 const uint64_t scale = static_cast<uint64_t>(sb) << 32 | sb;
-                if (k + SEG < to) next = scale_at(k + SEG);
-                if (!mbar_wait_warp(tfull + 8 * b, bphase, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE)) {
+                if (k + SEG < to) fetch();
+                const uint32_t bar = GROUPS == 1 ? done + 8 * (g % STAGES) : tfull + 8 * b;
+                const uint32_t phase = GROUPS == 1 ? g / STAGES & 1 : g >> 1 & 1;
+                if (!mbar_wait_warp_hint(bar, phase, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE, NAP_NS)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                // Sixteen columns travel while the sixteen before them are added.
-                uint32_t v[2][16];
+                // Half of the columns travel at a time: a read takes some 250 cycles, however many
+                // are under way.
                 __syncwarp();
-                if (mine > 0) tmem_ld16(lanes + b * MAX_COLS, v[0]);
 #pragma unroll
-                for (int c = 0; c < PART / 16; ++c) {
-                    if (c * 16 < mine) {
-                        tmem_ld_wait();
-                        if (c + 1 < PART / 16 && (c + 1) * 16 < mine) tmem_ld16(lanes + b * MAX_COLS + (c + 1) * 16, v[(c + 1) & 1]);
+                for (int h = 0; h < PART; h += 48) {
+                    uint32_t v[3][16];
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], v[c & 1][2 * i], v[c & 1][2 * i + 1], scale);
-                    }
+                    for (int c = 0; c < 3; ++c)
+                        if (h + c * 16 < mine) tmem_ld16(sums + b * acc_cols + h + c * 16, v[c]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 3; ++c)
+                        if (h + c * 16 < mine) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) fma2(acc[h / 2 + c * 8 + i], v[c][2 * i], v[c][2 * i + 1], scale);
+                        }
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_pair(mapa_shared(tempty + 8 * b, 0));
-                b ^= 1;
-                if (b == 0) bphase ^= 1;
             }
             // The warpgroup stores together or not at all: a warp that gave up meets the others here.
             ok = bar_and_all(1 + part, 128, ok);
             if (!ok) break;
-            // Sums leave through shared memory eight columns at a time, [column][row], so that a
+            // Sums leave through shared memory 32 columns at a time, [column][row], so that a
             // thread stores neighbouring outputs of one column at once.
-            const int left = it.cols - part * PART;  // this warpgroup's existing columns
-            float* swap = exchange + part * (BM * 8);
-            const int col = r >> 4;  // the column of eight that this thread stores
-            if (p.mode == MANY_UP) {
-                // Rows 0 .. 63 are gates, 64 .. 127 the same outputs' ups.
-                const int j = (r & 15) * 4;
-                const float* gate = swap + col * BM + j;
-                T* to = static_cast<T*>(p.h) + (it.p0 + part * PART + col) * p.h_rs + it.j0 + j;
-                const int valid = min(4, p.n - it.j0 - j);
+            const int left = min(mine, it.cols - part * mine);  // this warpgroup's existing columns
+            float* swap = exchange + part * (BM * OUT_COLS);
 #pragma unroll
-                for (int c = 0; c < PART; c += 8)
-                    if (c < left) {
+            for (int c = 0; c < PART; c += OUT_COLS)
+                if (c < left) {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                        if (c + col < left && valid > 0) up_out(gate, valid, to + c * p.h_rs);
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                    }
-            } else {
-                const int j = (r & 15) * 8;
-                const float* from = swap + col * BM + j;
-                const int valid = min(8, p.n - it.j0 - j);
-#pragma unroll
-                for (int c = 0; c < PART; c += 8)
-                    if (c < left) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                        if (c + col < left && valid > 0) out(p, it, it.p0 + part * PART + c + col, it.j0 + j, from, valid);
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                    }
-            }
+                    for (int i = 0; i < OUT_COLS; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
+                    sums_out<T>(p, it, swap, it.p0 + part * mine + c, min(OUT_COLS, left - c), r);
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
+                }
         }
     }
 
@@ -558,20 +562,21 @@ void plan(const uor_b200_ctx* ctx, ManyParams* p) {
             const int64_t tt = (p->m + width - 1) / width;
             const int64_t each = ((p->m + tt - 1) / tt + 31) & ~31ll;
             const int64_t waves = (tt * p->row_tiles + clusters - 1) / clusters;
-            const double cost = static_cast<double>(waves) * (each + 24);  // a tile's fixed part
+            // a tile's fixed part, and decoding, which takes as long as 144 columns' products
+            const double cost = static_cast<double>(waves) * ((each > 144 ? each : 144) + 24);
             if (best == 0 || cost < best) best = cost, p->max_cols = width;
         }
         tiles = (p->m + p->max_cols - 1) / p->max_cols;
     }
     if (p->mode != MANY_UP) {
-        // Whole stages of codes to a split, and eight of them at least.
+        // Eight stages to a split at least.
         int64_t want = clusters / (tiles * p->row_tiles);
-        const int64_t most = kbs / 16;
+        const int64_t most = kbs / 8;
         if (want > most) want = most;
         if (want > 8) want = 8;
         if (want > 1) p->splits = static_cast<int>(want);
     }
-    p->kb_per_split = ((kbs + p->splits - 1) / p->splits + 1) & ~1;
+    p->kb_per_split = (kbs + p->splits - 1) / p->splits;
     p->splits = (kbs + p->kb_per_split - 1) / p->kb_per_split;
 }
 
@@ -605,8 +610,8 @@ template <typename T, int SEG>
 int launch_many(uor_b200_ctx* ctx, ManyParams& p) {
     CUtensorMap tm_codes, tm_x;
     const uint64_t rows = static_cast<uint64_t>(p.w.rows);
-    if (!make_tmap_u8_sw64(&tm_codes, p.w.codes, (p.w.cols + 1) / 2, rows, p.w.row_bytes, CODES_K / 2, 64) ||
-        !make_tmap_u16(&tm_x, p.x, p.w.cols, p.x_rows, p.x_rs * 2, BK, X_BOX))
+    if (!make_tmap_u8_sw64(&tm_codes, p.w.codes, (p.w.cols + 1) / 2, rows, p.w.row_bytes, BK / 2, 64) ||
+        !make_tmap_u16(&tm_x, p.x, p.w.cols, p.x_rows, p.x_rs * 2, ATOM, X_BOX))
         return UOR_B200_DEVICE_ERROR;
     auto* kernel = many_kernel<T, SEG>;
     static bool ready[64] = {};
