@@ -227,7 +227,7 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     many.x_rs = rows.rs;
     many.x_rows = m;
     many.part = reinterpret_cast<float*>(ws + part_at);
-    route->tile_m = 256, route->tile_n = 192, route->tile_k = 64;
+    route->tile_m = 256, route->tile_n = 256, route->tile_k = 64;
     route->k_chunks = splits;
     if ((st = many_launch(ctx, elem, many))) return st;
     if (splits > 1) {
@@ -311,7 +311,7 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     up.h = ws + h_at;
     down.x = ws + h_at;
     down.part = reinterpret_cast<float*>(ws + part_at);
-    route->tile_m = 256, route->tile_n = 192, route->tile_k = 64;
+    route->tile_m = 256, route->tile_n = 256, route->tile_k = 64;
     if ((st = many_launch(ctx, a.elem, up)) || (st = many_launch(ctx, a.elem, down))) return st;
     combine_kernel<<<blocks_for(a.tokens * a.d), THREADS, 0, ctx->stream>>>(down.part, splits, a);
     return cuda_status(cudaGetLastError());

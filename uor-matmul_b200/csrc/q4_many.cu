@@ -1,27 +1,29 @@
 // q4_many.cu -- products of many rows with 4-bit weights and group scales.
 //
 // Bound by the tensor cores: 2 m n k operations on 16-bit floats. A work item is a tile of 256
-// weight rows by up to 192 activation rows, on a pair of CTAs (tcgen05.mma.cta_group::2): each
+// weight rows by up to 256 activation rows, on a pair of CTAs (tcgen05.mma.cta_group::2): each
 // CTA holds 128 of the weight rows and brings half of the activation rows. The weights are the
 // instruction's M side, so that a thread of the epilogue owns one weight row and a group's scale
 // is one number per thread.
 //
 // The roles of a CTA: a warp brings 128-position stages of activations by TMA, another the codes;
-// two warpgroups turn each code into a 16-bit float, exactly (code - zero), and store it to tensor
+// a warpgroup turns each code into a 16-bit float, exactly (code - zero), and stores it to tensor
 // memory, where the instruction takes its A side from; one thread of the pair issues the
-// tcgen05.mma; two warpgroups hold the sums. A group's products are summed in tensor memory, and
-// at the group's end these warpgroups add scale x sum to their f32 registers, while the next group
-// runs in the other of two accumulators. So no weight is rounded: rounding scale x code to 16
-// bits would cost as much precision as rounding the output does.
+// tcgen05.mma, for one half of the tile's columns and then the other; a warpgroup for each half
+// holds its sums. A group's products are summed in tensor memory, and at the group's end the
+// warpgroup adds scale x sum to its f32 registers, while the instructions run on in the two
+// other accumulators. So no weight is rounded: rounding scale x code to 16 bits would cost as
+// much precision as rounding the output does.
 //
 // Why this shape. With the weights in shared memory and one CTA per 128 x 256 tile, the operands'
 // reads, the TMA's and the decoders' writes came to 104 KB per 64 positions, 830 cycles at 128
 // bytes a cycle, for 512 cycles of multiplication (2048 x 8192 x 8192: 366 us, 295 us without
-// decoding and scaling). Here 64 positions move 4 x 3 KB of operands, 12 KB of TMA and 8 KB of
-// codes for 384. Beside that it is instructions that count, and waiting ones among them: one
-// arrival and one commit per 128 positions, waits that sleep, and no release at cluster scope.
-// Tensor memory's 512 columns hold two accumulators of 192 and two stages of weights of 64, or
-// two of 128 and four where tiles have at most 128 columns.
+// decoding and scaling); here they are 40 KB. Beside that it is issue slots that count: decoding
+// takes 13 instructions per eight codes and a sum half a one per column, waits and bookkeeping as
+// much again, so a tile has as many columns as the sums' registers allow (192 of them, with
+// two decoding warpgroups: 287 us), there is one commit per 128 positions and half, waits sleep,
+// and no arrival carries a release at cluster scope, which held its warp for 2000 cycles.
+// Tensor memory's 512 columns hold three accumulators of 128 and two stages of weights of 64.
 //
 // Every wait is bounded; a role that gives up records it, and every other role leaves after it.
 #include "q4_many.cuh"
@@ -38,30 +40,36 @@ namespace {
 constexpr int BM = 128;        // weight rows of a CTA's half of a tile
 constexpr int BK = 128;        // reduction positions of a stage
 constexpr int ATOM = 64;       // positions in the 128 bytes that the activations' swizzle spans
-constexpr int MAX_COLS = 192;  // activation rows of a tile
+constexpr int MAX_COLS = 256;  // activation rows of a tile
+constexpr int HALF = 128;      // columns of an accumulator: half a tile's
 constexpr int X_BOX = 32;      // activation rows of one TMA copy
 constexpr int X_BOX_BYTES = X_BOX * ATOM * 2;
-constexpr int ATOM_BYTES = MAX_COLS / 2 * ATOM * 2;
+constexpr int HALF_BYTES = HALF / 2 * ATOM * 2;      // a CTA's rows of a half, per atom
+constexpr int ATOM_BYTES = 2 * HALF_BYTES;
 constexpr int X_BYTES = ATOM_BYTES * BK / ATOM;
 constexpr int C_BYTES = BM * BK / 2;
-constexpr int STAGES = 4, CSTAGES = 6, MOST_ASTAGES = 4;
+constexpr int STAGES = 4, CSTAGES = 4, ASTAGES = 2, ACCS = 3;
 constexpr int A_COLS = BK / 2;                       // tensor-memory columns of a stage of weights
-constexpr int DECODERS = 8, SUMMERS = 8;             // warps of a CTA
-constexpr int PART = MAX_COLS / 2;                   // columns of a summing warpgroup
+constexpr int A_FIRST = ACCS * HALF;
+constexpr int DECODERS = 4, SUMMERS = 4;             // warps of a CTA; of a CTA and a half
 constexpr int OUT_COLS = 32;                         // columns that leave at a time
-constexpr int EXCHANGE = BM * OUT_COLS * 4;          // bytes, per summing warpgroup
-constexpr int BARS = 2 * STAGES + 2 * CSTAGES + MOST_ASTAGES + 5;
+constexpr int EXCHANGE = BM * OUT_COLS * 4;          // bytes, per half
+// Signals of filled accumulators, per half: as many as can be filled before the first is read, and
+// one, since a warpgroup waits for its own half's alone and must not mistake a later filling.
+constexpr int FULLS = ACCS + 1;
+constexpr int BARS = 2 * STAGES + 2 * CSTAGES + ASTAGES + 2 * FULLS + ACCS + 1;
 constexpr int SMEM = STAGES * X_BYTES + CSTAGES * C_BYTES + 2 * EXCHANGE + (BARS + 1) * 8 + (MANY_MAX_EXPERTS + 1) * 4 + 1024;
 constexpr uint32_t NAP_NS = 1000;  // a wait's sleep between looks; an arrival ends it at once
-// Warpgroup 0: TMA, MMA; 1 and 2: decoders; 3 and 4: sums. Registers: 96 a thread at launch.
-constexpr int THREADS = 640;
-constexpr int REGS_CONTROL = 32, REGS_DECODE = 56, REGS_SUM = 168;
+// Warpgroup 0: TMA, MMA; 1: decoders; 2 and 3: sums. Registers: 128 a thread at launch.
+constexpr int THREADS = 512;
+constexpr int REGS_CONTROL = 32, REGS_DECODE = 80, REGS_SUM = 200;
 static_assert(SMEM <= 232448, "shared memory of a block");
-static_assert(2 * MAX_COLS + 2 * A_COLS <= 512 && 2 * 128 + 4 * A_COLS <= 512, "tensor memory");
-static_assert(REGS_CONTROL + 2 * REGS_DECODE + 2 * REGS_SUM <= 5 * 96, "registers of the launch");
+static_assert(A_FIRST + ASTAGES * A_COLS <= 512, "tensor memory");
+static_assert(REGS_CONTROL + REGS_DECODE + 2 * REGS_SUM <= 4 * 128, "registers of the launch");
 
 struct Item {
-    int expert, cols, n;      // cols: existing activation rows; n: the instruction's
+    int cols, half;           // existing activation rows; an instruction's columns
+    int halves;               // instructions' columns in the tile: one or two
     int64_t p0;               // first activation row
     int64_t row0;             // first weight row
     int j0;                   // first output
@@ -87,11 +95,11 @@ __device__ __forceinline__ bool item_at(int u, const ManyParams& p, const int* f
     const int begin = p.offsets ? p.offsets[lo] : 0;
     const int count = p.offsets ? p.offsets[lo + 1] - begin : p.m;
     const int parts = tiles_of(count, p.max_cols);
-    const int size = ((count + parts - 1) / parts + 31) & ~31;  // even shares, in whole instructions
+    const int size = ((count + parts - 1) / parts + 63) & ~63;  // even shares, in whole instructions
     const int i = tt - first_tile[lo];
-    it->expert = lo;
     it->cols = min(size, count - i * size);
-    it->n = (it->cols + 31) & ~31;
+    it->halves = it->cols > 32 ? 2 : 1;
+    it->half = it->halves == 2 ? (it->cols + 63) / 64 * 32 : 32;
     it->p0 = begin + static_cast<int64_t>(i) * size;
     const int outputs = p.mode == MANY_UP ? BM / 2 : BM;  // of a CTA
     it->j0 = (2 * rt + rank) * outputs;
@@ -133,13 +141,12 @@ __device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
 
 // Steps along a row's scales (or zero points) by a piece of a group at a time.
 struct GroupWalk {
-    int at, pos, group, last;
-    __device__ __forceinline__ GroupWalk(int k, int group, int cols)
-        : at(k / group), pos(k - k / group * group), group(group), last((cols + group - 1) / group - 1) {}
-    __device__ __forceinline__ int index() const { return min(at, last); }
-    __device__ __forceinline__ void step(int by) {
+    int at, pos;
+    __device__ __forceinline__ GroupWalk(int k, const ManyParams& p) : at(k / p.w.group), pos(k - k / p.w.group * p.w.group) {}
+    __device__ __forceinline__ int index(const ManyParams& p) const { return min(at, p.groups - 1); }
+    __device__ __forceinline__ void step(int by, const ManyParams& p) {
         pos += by;
-        while (pos >= group) pos -= group, ++at;
+        while (pos >= p.w.group) pos -= p.w.group, ++at;
     }
 };
 
@@ -226,12 +233,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
     int* first_tile = reinterpret_cast<int*>(bars + BARS + 1);
     // xfull, afull and tempty count on the leader, for both CTAs. done: a stage's products are
-    // complete, which frees its activations and its weights, and with one group to a stage is the
-    // sums' signal too (tfull otherwise).
+    // complete, which frees its activations and its weights. tfull: a group's are, of one half.
     const uint32_t xfull = smem_u32(bars), done = xfull + 8 * STAGES;
     const uint32_t cfull = done + 8 * STAGES, cempty = cfull + 8 * CSTAGES;
     const uint32_t afull = cempty + 8 * CSTAGES;
-    const uint32_t tfull = afull + 8 * MOST_ASTAGES, tempty = tfull + 16, drain = tempty + 16;
+    const uint32_t tfull = afull + 8 * ASTAGES, tempty = tfull + 8 * 2 * FULLS, drain = tempty + 8 * ACCS;
     constexpr int GROUPS = BK / SEG;  // of a stage
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
     const uint32_t rank = cluster_ctarank();
@@ -247,11 +253,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(cfull + 8 * s, 1);
             mbar_init(cempty + 8 * s, DECODERS);
         }
-        for (int s = 0; s < MOST_ASTAGES; ++s) mbar_init(afull + 8 * s, 2 * DECODERS);
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(tfull + 8 * b, 1);
-            mbar_init(tempty + 8 * b, 2 * SUMMERS);
-        }
+        for (int s = 0; s < ASTAGES; ++s) mbar_init(afull + 8 * s, 2 * DECODERS);
+        for (int b = 0; b < 2 * FULLS; ++b) mbar_init(tfull + 8 * b, 1);
+        for (int b = 0; b < ACCS; ++b) mbar_init(tempty + 8 * b, 2 * SUMMERS);
         mbar_init(drain, 1);
         fence_barrier_init();
         tma_prefetch_desc(&tm_codes);
@@ -279,8 +283,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int items = p.row_tiles * first_tile[p.experts] * p.splits;
-    const int acc_cols = p.max_cols > 128 ? MAX_COLS : 128;
-    const uint32_t a_stages = p.max_cols > 128 ? 2 : 4;
     Item it;
 
     if (wg == 0) {
@@ -292,8 +294,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 bool ok = true;
                 for (int u = pair; u < items && ok; u += pairs) {
                     if (!item_at(u, p, first_tile, rank, &it)) continue;
-                    const int boxes = (it.n / 2 + X_BOX - 1) / X_BOX;
-                    const int row = static_cast<int>(it.p0) + static_cast<int>(rank) * (it.n / 2);
+                    const int boxes = (it.half / 2 + X_BOX - 1) / X_BOX;  // of a half
+                    const int row = static_cast<int>(it.p0) + static_cast<int>(rank) * (it.half / 2);
                     for (int kb = 0; kb < it.kbs; ++kb, ++n) {
                         const uint32_t s = n % STAGES, phase = n / STAGES & 1;
                         if (!mbar_wait_hint(done + 8 * s, phase ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER, NAP_NS)) {
@@ -301,16 +303,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                             break;
                         }
                         if (leader) {
-                            mbar_expect_tx(xfull + 8 * s, 2 * (BK / ATOM) * boxes * X_BOX_BYTES);
+                            mbar_expect_tx(xfull + 8 * s, 2 * (BK / ATOM) * it.halves * boxes * X_BOX_BYTES);
                             armed |= 1u << s;
                             armed_phase = (armed_phase & ~(1u << s)) | phase << s;
                         }
                         const uint32_t full = mapa_shared(xfull + 8 * s, 0);
                         const uint32_t dst = smem_u32(smem + s * X_BYTES);
-                        for (int h = 0; h < BK / ATOM; ++h)
-                            for (int b = 0; b < boxes; ++b)
-                                tma_load_2d_pair(dst + h * ATOM_BYTES + b * X_BOX_BYTES, &tm_x, full,
-                                                 (it.kb0 + kb) * BK + h * ATOM, row + b * X_BOX, policy);
+                        for (int a = 0; a < BK / ATOM; ++a)
+                            for (int h = 0; h < it.halves; ++h)
+                                for (int b = 0; b < boxes; ++b)
+                                    tma_load_2d_pair(dst + a * ATOM_BYTES + h * HALF_BYTES + b * X_BOX_BYTES, &tm_x, full,
+                                                     (it.kb0 + kb) * BK + a * ATOM, row + h * it.half + b * X_BOX, policy);
                     }
                 }
                 if (!ok && leader)
@@ -351,51 +354,54 @@ __global__ void __launch_bounds__(THREADS, 1)
             __syncwarp();
         } else if (warp == 1 && leader) {  // the tensor cores of both CTAs
             if (elect_one()) {
-                uint32_t n = 0, g = 0;  // stages and groups so far
+                uint32_t n = 0, b = 0, turn = 0;  // stages so far; the next accumulator, its round's parity
+                uint32_t filled[2] = {0, 0};      // accumulators of each half so far
                 bool ok = true;
                 for (int u = pair; u < items && ok; u += pairs) {
                     if (!item_at(u, p, first_tile, rank, &it)) continue;
-                    const uint32_t idesc = idesc_f16(2 * BM, it.n, std::is_same<T, __nv_bfloat16>::value);
+                    const uint32_t idesc = idesc_f16(2 * BM, it.half, std::is_same<T, __nv_bfloat16>::value);
                     for (int kb = 0; kb < it.kbs && ok; ++kb, ++n) {
-                        const uint32_t s = n % STAGES, a = n % a_stages;
+                        const uint32_t s = n % STAGES, a = n % ASTAGES;
                         ok = mbar_wait(xfull + 8 * s, n / STAGES & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL) &&
-                             mbar_wait(afull + 8 * a, n / a_stages & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL);
-                        const uint32_t sx = smem_u32(smem + s * X_BYTES), sa = tmem + 2 * acc_cols + a * A_COLS;
+                             mbar_wait(afull + 8 * a, n / ASTAGES & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL);
+                        const uint32_t sx = smem_u32(smem + s * X_BYTES), sa = tmem + A_FIRST + a * A_COLS;
 #pragma unroll
-                        for (int h = 0; h < GROUPS; ++h) {
-                            if (!ok || (h && (it.kb0 + kb) * BK + h * SEG >= p.w.cols)) break;
-                            const uint32_t b = g & 1;
-                            ok = mbar_wait(tempty + 8 * b, (g >> 1 & 1) ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_ACC);
-                            if (!ok) break;
-                            tc_fence_after();
+                        for (int g = 0; g < GROUPS; ++g) {
+                            if (g && (it.kb0 + kb) * BK + g * SEG >= p.w.cols) break;
 #pragma unroll
-                            for (int i = 0; i < SEG / 16; ++i) {
-                                const int k16 = h * (SEG / 16) + i;
-                                mma_f16_pair_ts(tmem + b * acc_cols, sa + k16 * 8,
-                                                smem_desc_sw128(sx + k16 / 4 * ATOM_BYTES + k16 % 4 * 32, 16, 1024), idesc, i != 0);
+                            for (int h = 0; h < 2; ++h) {
+                                if (h >= it.halves || !ok) break;
+                                ok = mbar_wait(tempty + 8 * b, turn ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_ACC);
+                                if (!ok) break;
+                                tc_fence_after();
+#pragma unroll
+                                for (int i = 0; i < SEG / 16; ++i) {
+                                    const int k16 = g * (SEG / 16) + i;
+                                    mma_f16_pair_ts(tmem + b * HALF, sa + k16 * 8,
+                                                    smem_desc_sw128(sx + k16 / 4 * ATOM_BYTES + h * HALF_BYTES + k16 % 4 * 32, 16, 1024),
+                                                    idesc, i != 0);
+                                }
+                                mma_commit_pair(tfull + 8 * (h * FULLS + filled[h]++ % FULLS), 0x3);
+                                if (++b == ACCS) b = 0, turn ^= 1;
                             }
-                            if (GROUPS > 1) mma_commit_pair(tfull + 8 * b, 0x3);
-                            ++g;
                         }
                         if (ok) mma_commit_pair(done + 8 * s, 0x3);
                     }
                 }
-                if (!ok && g) {
+                if (!ok && (n || b || turn)) {
                     mma_commit_pair(drain, 0x1);
                     mbar_wait(drain, 0, p.budget_ns, p.status, KERR_TIMEOUT_DRAIN);
                 }
             }
             __syncwarp();
         }
-    } else if (wg <= 2) {
+    } else if (wg == 1) {
         regs_down<REGS_DECODE>();
-        // A thread turns its row's codes into the operand's row, lane r of tensor memory: one
-        // warpgroup the first half of a stage's positions, the other the second.
-        const int r = threadIdx.x & 127, part = wg - 1;
-        const uint32_t to = tmem + (static_cast<uint32_t>(r & ~31) << 16) + 2 * acc_cols + part * (A_COLS / 2);
-        const int turn = (r >> 1) & 3;  // the 64-byte swizzle's
+        // A thread turns its row's codes into the operand's row, lane r of tensor memory.
+        const int r = threadIdx.x & 127;
+        const uint32_t to = tmem + (static_cast<uint32_t>(r & ~31) << 16) + A_FIRST;
+        const int turn = ((r >> 1) & 3) << 4;  // the 64-byte swizzle's
         const uint8_t* from = codes_at + r * (BK / 2);
-        const int at0 = ((2 * part) ^ turn) << 4, at1 = ((2 * part + 1) ^ turn) << 4;
         int q = 0;
         uint32_t qphase = 0, n = 0;  // n: stages so far
         bool ok = true;
@@ -403,17 +409,17 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (!item_at(u, p, first_tile, rank, &it)) continue;
             const int64_t row = min(it.row0 + (r < 64 ? r : r - 64 + (p.mode == MANY_UP ? p.n : 64)), static_cast<int64_t>(p.w.rows) - 1);
             const uint8_t* zeros = p.w.zeros ? p.w.zeros + row * p.w.groups_rs : nullptr;
-            uint32_t next0 = 8, next1 = 8;  // the zero points of this half's two 32 positions
-            GroupWalk walk(it.kb0 * BK + part * (BK / 2), p.w.group, p.w.cols);
+            constexpr int PIECES = BK / SEG;  // zero points of a stage
+            uint32_t next[PIECES];
+#pragma unroll
+            for (int i = 0; i < PIECES; ++i) next[i] = 8;
+            GroupWalk walk(it.kb0 * BK, p);
             auto fetch = [&]() {
                 if (!zeros) return;
-                next0 = next1 = zeros[walk.index()];
-                if (SEG == 32) {
-                    walk.step(32);
-                    next1 = zeros[walk.index()];
-                    walk.step(BK - 32);
-                } else {
-                    walk.step(BK);
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    next[i] = zeros[walk.index(p)];
+                    walk.step(SEG, p);
                 }
             };
             fetch();
@@ -422,34 +428,35 @@ __global__ void __launch_bounds__(THREADS, 1)
                     ok = false;
                     break;
                 }
-                const uint4 c0 = *reinterpret_cast<const uint4*>(from + q * C_BYTES + at0);
-                const uint4 c1 = *reinterpret_cast<const uint4*>(from + q * C_BYTES + at1);
+                uint4 c[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) c[i] = *reinterpret_cast<const uint4*>(from + q * C_BYTES + ((i << 4) ^ turn));
                 __syncwarp();
                 if (lane == 0) mbar_arrive(cempty + 8 * q);
                 if (++q == CSTAGES) q = 0, qphase ^= 1;
-                const uint32_t z0 = zero_pair<T>(next0 & 15u), z1 = zero_pair<T>(next1 & 15u);
+                uint32_t z[PIECES];
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) z[i] = zero_pair<T>(next[i] & 15u);
                 fetch();
-                // the stage that used this one's columns is `a_stages` back
-                const uint32_t a = n % a_stages, before = n - a_stages;
-                if (n >= a_stages && !mbar_wait_warp_hint(done + 8 * (before % STAGES), before / STAGES & 1, p.budget_ns, p.status,
-                                                          KERR_TIMEOUT_PRODUCER, NAP_NS)) {
+                // the stage that used this one's columns is ASTAGES back
+                const uint32_t a = n % ASTAGES, before = n - ASTAGES;
+                if (n >= ASTAGES && !mbar_wait_warp_hint(done + 8 * (before % STAGES), before / STAGES & 1, p.budget_ns, p.status,
+                                                         KERR_TIMEOUT_PRODUCER, NAP_NS)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                uint32_t v[16];
-                auto put = [&](const uint4& c, uint32_t z, int at) {
-                    const uint32_t w[4] = {c.x, c.y, c.z, c.w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint4 d = decode8<T>(w[i], z);
-                        v[4 * i] = d.x, v[4 * i + 1] = d.y, v[4 * i + 2] = d.z, v[4 * i + 3] = d.w;
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t w[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+                    uint32_t v[16];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint4 d = decode8<T>(w[k], z[i * 32 / SEG]);
+                        v[4 * k] = d.x, v[4 * k + 1] = d.y, v[4 * k + 2] = d.z, v[4 * k + 3] = d.w;
                     }
-                    __syncwarp();
-                    tmem_st16(to + a * A_COLS + at, v);
-                };
-                put(c0, z0, 0);
-                put(c1, z1, 16);
+                    tmem_st16(to + a * A_COLS + i * 16, v);
+                }
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
@@ -458,78 +465,87 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     } else {
         regs_up<REGS_SUM>();
-        const int r = threadIdx.x & 127, part = wg - 3;
+        const int r = threadIdx.x & 127, part = wg - 2;  // part: which half of a tile's columns
         const uint32_t lanes = tmem + (static_cast<uint32_t>(r & ~31) << 16);
-        uint32_t g = 0;  // groups so far
+        const bool wide = p.w.scale_type == UOR_B200_F32, bf16 = p.w.scale_type == UOR_B200_BF16;
+        const int per_group = p.w.group / SEG;
+        uint32_t g = 0, filled = 0;  // accumulators filled before this item's; of this half so far
         bool ok = true;
         for (int u = pair; u < items && ok; u += pairs) {
             if (!item_at(u, p, first_tile, rank, &it)) continue;
             const int64_t row = min(it.row0 + (r < 64 ? r : r - 64 + (p.mode == MANY_UP ? p.n : 64)), static_cast<int64_t>(p.w.rows) - 1);
-            const int from = it.kb0 * BK, to = min(p.w.cols, from + it.kbs * BK);
-            GroupWalk walk(from, p.w.group, p.w.cols);
-            const bool wide = p.w.scale_type == UOR_B200_F32, bf16 = p.w.scale_type == UOR_B200_BF16;
-            const char* scales = static_cast<const char*>(p.w.scales) + row * p.w.groups_rs * (wide ? 4 : 2);
-            uint32_t next;
-            auto fetch = [&]() {
-                if (wide) next = reinterpret_cast<const uint32_t*>(scales)[walk.index()];
-                else next = reinterpret_cast<const uint16_t*>(scales)[walk.index()];
-                walk.step(SEG);
+            const int k0 = it.kb0 * BK, first = k0 / p.w.group;
+            const int steps = (min(p.w.cols - k0, it.kbs * BK) + SEG - 1) / SEG;
+            int repeat = per_group - (k0 - first * p.w.group) / SEG;  // steps with the scale at hand
+            const char* scale_at = static_cast<const char*>(p.w.scales) + (row * p.w.groups_rs + first) * (wide ? 4 : 2);
+            auto load = [&]() -> uint32_t {
+                return wide ? *reinterpret_cast<const uint32_t*>(scale_at) : *reinterpret_cast<const uint16_t*>(scale_at);
             };
-            uint64_t acc[PART / 2];
+            auto value = [&](uint32_t raw) {
+                return wide ? raw
+                       : bf16 ? raw << 16
+                              : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(raw))));
+            };
+            uint64_t acc[HALF / 2];
 #pragma unroll
-            for (int i = 0; i < PART / 2; ++i) acc[i] = 0;
-            const int mine = it.n / 2;  // this warpgroup's columns: sixteens
-            const uint32_t sums = lanes + part * mine;
-            fetch();
-            for (int k = from; k < to; k += SEG, ++g) {
-                const uint32_t b = g & 1;
-                const uint32_t sb = wide ? next
-                                    : bf16 ? next << 16
-                                           : __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(next))));
+            for (int i = 0; i < HALF / 2; ++i) acc[i] = 0;
+            const int mine = part < it.halves ? it.half : 0;  // this warpgroup's columns
+            uint32_t next = load();
+            // Accumulators are filled in turn, those of both halves: this one's are every
+            // `halves`-th from its own first on.
+            uint32_t at = g + part;
+            for (int i = 0; i < steps && mine; ++i, at += it.halves, ++filled) {
+                const uint32_t sb = value(next), b = at % ACCS;
                 const uint64_t scale = static_cast<uint64_t>(sb) << 32 | sb;
-                if (k + SEG < to) fetch();
-                const uint32_t bar = GROUPS == 1 ? done + 8 * (g % STAGES) : tfull + 8 * b;
-                const uint32_t phase = GROUPS == 1 ? g / STAGES & 1 : g >> 1 & 1;
-                if (!mbar_wait_warp_hint(bar, phase, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE, NAP_NS)) {
+                if (--repeat == 0 && i + 1 < steps) {
+                    repeat = per_group;
+                    scale_at += wide ? 4 : 2;
+                    next = load();
+                }
+                if (!mbar_wait_warp_hint(tfull + 8 * (part * FULLS + filled % FULLS), filled / FULLS & 1, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE, NAP_NS)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                // Half of the columns travel at a time: a read takes some 250 cycles, however many
-                // are under way.
+                // Columns travel 48 at a time: a read takes some 250 cycles, however many are under way.
                 __syncwarp();
 #pragma unroll
-                for (int h = 0; h < PART; h += 48) {
+                for (int h = 0; h < HALF; h += 48) {
                     uint32_t v[3][16];
 #pragma unroll
                     for (int c = 0; c < 3; ++c)
-                        if (h + c * 16 < mine) tmem_ld16(sums + b * acc_cols + h + c * 16, v[c]);
+                        if (h + c * 16 < HALF && h + c * 16 < mine) tmem_ld16(lanes + b * HALF + h + c * 16, v[c]);
                     tmem_ld_wait();
+                    if (h + 48 >= HALF || h + 48 >= mine) {  // the last: the accumulator is free
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0 && h < mine) mbar_arrive_pair(mapa_shared(tempty + 8 * b, 0));
+                    }
 #pragma unroll
                     for (int c = 0; c < 3; ++c)
-                        if (h + c * 16 < mine) {
+                        if (h + c * 16 < HALF && h + c * 16 < mine) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) fma2(acc[h / 2 + c * 8 + i], v[c][2 * i], v[c][2 * i + 1], scale);
+                            for (int k = 0; k < 8; ++k) fma2(acc[h / 2 + c * 8 + k], v[c][2 * k], v[c][2 * k + 1], scale);
                         }
+                    if (h + 48 >= mine) break;
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_pair(mapa_shared(tempty + 8 * b, 0));
             }
+            g += steps * it.halves;
             // The warpgroup stores together or not at all: a warp that gave up meets the others here.
             ok = bar_and_all(1 + part, 128, ok);
             if (!ok) break;
+            item_at(u, p, first_tile, rank, &it);  // again: nothing of it is kept above
             // Sums leave through shared memory 32 columns at a time, [column][row], so that a
             // thread stores neighbouring outputs of one column at once.
-            const int left = min(mine, it.cols - part * mine);  // this warpgroup's existing columns
+            const int left = min(mine, it.cols - part * it.half);  // this warpgroup's existing columns
             float* swap = exchange + part * (BM * OUT_COLS);
 #pragma unroll
-            for (int c = 0; c < PART; c += OUT_COLS)
+            for (int c = 0; c < HALF; c += OUT_COLS)
                 if (c < left) {
 #pragma unroll
                     for (int i = 0; i < OUT_COLS; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                    sums_out<T>(p, it, swap, it.p0 + part * mine + c, min(OUT_COLS, left - c), r);
+                    sums_out<T>(p, it, swap, it.p0 + part * it.half + c, min(OUT_COLS, left - c), r);
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
                 }
         }
@@ -558,12 +574,12 @@ void plan(const uor_b200_ctx* ctx, ManyParams* p) {
     int64_t tiles = p->experts;
     if (p->mode == MANY_DENSE) {
         double best = 0;
-        for (int width = MAX_COLS; width >= 96 && p->m > MAX_COLS; width -= 32) {
+        for (int width = MAX_COLS; width >= 128 && p->m > 128; width -= 64) {
             const int64_t tt = (p->m + width - 1) / width;
-            const int64_t each = ((p->m + tt - 1) / tt + 31) & ~31ll;
+            const int64_t each = ((p->m + tt - 1) / tt + 63) & ~63ll;
             const int64_t waves = (tt * p->row_tiles + clusters - 1) / clusters;
-            // a tile's fixed part, and decoding, which takes as long as 144 columns' products
-            const double cost = static_cast<double>(waves) * ((each > 144 ? each : 144) + 24);
+            // decoding and scaling take as long beside narrow tiles as beside wide ones
+            const double cost = static_cast<double>(waves) * (each + 128);
             if (best == 0 || cost < best) best = cost, p->max_cols = width;
         }
         tiles = (p->m + p->max_cols - 1) / p->max_cols;
@@ -652,6 +668,7 @@ int many_splits(const uor_b200_ctx* ctx, const ManyParams& p) {
 
 int many_launch(uor_b200_ctx* ctx, int elem, ManyParams p) {
     plan(ctx, &p);
+    p.groups = (p.w.cols + p.w.group - 1) / p.w.group;
     p.status = ctx->d_status;
     p.budget_ns = ctx->budget_ns;
     return elem == UOR_B200_BF16 ? by_segment<__nv_bfloat16>(ctx, p) : by_segment<__half>(ctx, p);

@@ -29,8 +29,8 @@ struct ManyParams {
     void* h;              // up: [sorted rows][h_rs]
     int64_t h_rs;
     // Set by the launch:
-    int max_cols;         // rows of x in a tile, a multiple of 32
-    int row_tiles, splits, kb_per_split;
+    int max_cols;         // rows of x in a tile, a multiple of 64
+    int row_tiles, splits, kb_per_split, groups;
     int* status;
     uint64_t budget_ns;
 };
