@@ -44,9 +44,20 @@ __global__ void codes_kernel(const uint8_t* codes, int64_t row_bytes, int64_t ro
     const int c = static_cast<int>(at - i * per_row) * 16;
     const uint8_t* from = codes + i * row_bytes + c;
     uint32_t w[4] = {0, 0, 0, 0};
+    if (c + 19 <= row_len) {  // five aligned words hold the sixteen bytes, and end within the row
+        const int past = static_cast<int>(reinterpret_cast<uint64_t>(from) & 3);
+        const uint32_t* a = reinterpret_cast<const uint32_t*>(from - past);
+        uint32_t v[5];
 #pragma unroll
-    for (int b = 0; b < 16; ++b)
-        if (c + b < row_len) w[b >> 2] |= static_cast<uint32_t>(from[b]) << (8 * (b & 3));
+        for (int b = 0; b < 4; ++b) v[b] = a[b];
+        v[4] = past ? a[4] : 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) w[b] = __funnelshift_r(v[b], v[b + 1], 8 * past);
+    } else {
+#pragma unroll
+        for (int b = 0; b < 16; ++b)
+            if (c + b < row_len) w[b >> 2] |= static_cast<uint32_t>(from[b]) << (8 * (b & 3));
+    }
     *reinterpret_cast<uint4*>(to + i * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
@@ -94,36 +105,76 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(Mat ids, int pairs, 
         if (id(i) == e) perm[at++] = i;
 }
 
-// y[i][j] = the parts' sum, in their order (no parts: 0).
+// Four neighbouring outputs of a row; one by one where they do not lie as a vector.
+__device__ __forceinline__ void store4(const MatOut& y, int64_t i, int j, int n, const float (&v)[4]) {
+    const int64_t at = i * y.rs + j * y.cs;
+    char* to = static_cast<char*>(y.p) + at * (y.type == UOR_B200_F32 ? 4 : 2);
+    if (j + 4 <= n && y.cs == 1 && reinterpret_cast<uint64_t>(to) % (y.type == UOR_B200_F32 ? 16 : 8) == 0) {
+        if (y.type == UOR_B200_F32) {
+            *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+        } else if (y.type == UOR_B200_BF16) {
+            const __nv_bfloat162 t[2] = {__floats2bfloat162_rn(v[0], v[1]), __floats2bfloat162_rn(v[2], v[3])};
+            memcpy(to, t, 8);
+        } else {
+            const __half2 t[2] = {__floats2half2_rn(v[0], v[1]), __floats2half2_rn(v[2], v[3])};
+            memcpy(to, t, 8);
+        }
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (j + k < n) store_f32(y.p, at + k * y.cs, y.type, v[k]);
+}
+// Four neighbouring f32 of a row of n, zeros past its end.
+__device__ __forceinline__ float4 load4(const float* row, int j, int n, bool vec) {
+    if (vec && j + 4 <= n) return *reinterpret_cast<const float4*>(row + j);
+    return make_float4(j < n ? row[j] : 0.0f, j + 1 < n ? row[j + 1] : 0.0f, j + 2 < n ? row[j + 2] : 0.0f,
+                       j + 3 < n ? row[j + 3] : 0.0f);
+}
+
+// y[i][j] = the parts' sum, in their order (no parts: 0). A block's x takes 1024 outputs of a
+// row, its y strides the rows.
 __global__ void add_parts_kernel(const float* part, int splits, int64_t rows, int n, MatOut y) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (at >= rows * n) return;
-    const int64_t i = at / n, j = at - i * n;
-    float v = 0;
-    for (int s = 0; s < splits; ++s) v += part[s * rows * n + at];
-    store_f32(y.p, i * y.rs + j * y.cs, y.type, v);
+    const int j = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
+    if (j >= n) return;
+    for (int64_t i = blockIdx.y; i < rows; i += gridDim.y) {
+        float v[4] = {0, 0, 0, 0};
+        for (int s = 0; s < splits; ++s) {
+            const float4 a = load4(part + (s * rows + i) * n, j, n, n % 4 == 0);
+            v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+        }
+        store4(y, i, j, n, v);
+    }
 }
 
 // y[t][j] = the token's choices' products, each times its weight, in the choices' order.
-__global__ void combine_kernel(const float* part, int splits, FfnArgs a) {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int64_t t = at / a.d, j = at - t * a.d;
-    if (t >= a.tokens) return;
-    const int64_t step = a.tokens * a.top_k * a.d;
-    float v = 0;
-    for (int s = 0; s < a.top_k; ++s) {
-        const int e = static_cast<const int32_t*>(a.ids.p)[t * a.ids.rs + s * a.ids.cs];
-        if (e < 0 || e >= a.experts) continue;
-        const float w = static_cast<const float*>(a.weights.p)[t * a.weights.rs + s * a.weights.cs];
-        const float* from = part + (t * a.top_k + s) * a.d + j;
-        float sum = from[0];
-        for (int c = 1; c < splits; ++c) sum += from[c * step];
-        v = fmaf(w, sum, v);
+__global__ void combine_kernel(const float* part, int splits, const __grid_constant__ FfnArgs a) {
+    const int j = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
+    if (j >= a.d) return;
+    const int64_t step = a.tokens * a.top_k;
+    for (int64_t t = blockIdx.y; t < a.tokens; t += gridDim.y) {
+        float v[4] = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int s = 0; s < a.top_k; ++s) {
+            const int e = static_cast<const int32_t*>(a.ids.p)[t * a.ids.rs + s * a.ids.cs];
+            if (e < 0 || e >= a.experts) continue;
+            const float w = static_cast<const float*>(a.weights.p)[t * a.weights.rs + s * a.weights.cs];
+            float4 sum = load4(part + (t * a.top_k + s) * a.d, j, a.d, a.d % 4 == 0);
+            for (int c = 1; c < splits; ++c) {
+                const float4 more = load4(part + (c * step + t * a.top_k + s) * a.d, j, a.d, a.d % 4 == 0);
+                sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
+            }
+            v[0] = fmaf(w, sum.x, v[0]), v[1] = fmaf(w, sum.y, v[1]), v[2] = fmaf(w, sum.z, v[2]), v[3] = fmaf(w, sum.w, v[3]);
+        }
+        store4(a.y, t, j, a.d, v);
     }
-    store_f32(a.y.p, t * a.y.rs + j * a.y.cs, a.y.type, v);
 }
 
 constexpr int THREADS = 256;
+// Four outputs to a thread, a row to a block's y.
+dim3 blocks_of_rows(int64_t rows, int n) {
+    return dim3((n + 4 * THREADS - 1) / (4 * THREADS), static_cast<unsigned>(rows < 65535 ? rows : 65535));
+}
 unsigned blocks_for(int64_t threads) { return static_cast<unsigned>((threads + THREADS - 1) / THREADS); }
 
 int up_to(int v, int by) { return (v + by - 1) / by * by; }
@@ -176,7 +227,7 @@ void few_align(FewParams* p) {
 }
 
 int zeros_out(uor_b200_ctx* ctx, int64_t rows, int n, const MatOut& y) {
-    add_parts_kernel<<<blocks_for(rows * n), THREADS, 0, ctx->stream>>>(nullptr, 0, rows, n, y);
+    add_parts_kernel<<<blocks_of_rows(rows, n), THREADS, 0, ctx->stream>>>(nullptr, 0, rows, n, y);
     return cuda_status(cudaGetLastError());
 }
 
@@ -231,7 +282,7 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     route->k_chunks = splits;
     if ((st = many_launch(ctx, elem, many))) return st;
     if (splits > 1) {
-        add_parts_kernel<<<blocks_for(m * w.rows), THREADS, 0, ctx->stream>>>(many.part, splits, m, w.rows, y);
+        add_parts_kernel<<<blocks_of_rows(m, w.rows), THREADS, 0, ctx->stream>>>(many.part, splits, m, w.rows, y);
         return cuda_status(cudaGetLastError());
     }
     return UOR_B200_OK;
@@ -313,7 +364,7 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     down.part = reinterpret_cast<float*>(ws + part_at);
     route->tile_m = 256, route->tile_n = 256, route->tile_k = 64;
     if ((st = many_launch(ctx, a.elem, up)) || (st = many_launch(ctx, a.elem, down))) return st;
-    combine_kernel<<<blocks_for(a.tokens * a.d), THREADS, 0, ctx->stream>>>(down.part, splits, a);
+    combine_kernel<<<blocks_of_rows(a.tokens, a.d), THREADS, 0, ctx->stream>>>(down.part, splits, a);
     return cuda_status(cudaGetLastError());
 }
 
