@@ -1,9 +1,15 @@
 // expert_route.cu -- the experts' router and the gradient of its logits.
 //
-// A warp per token. Lane l holds the experts l, l + 32, ...; a key is ordered as an unsigned
-// integer (the float's bits, negative ones complemented), so that the largest key is one
-// warp-wide integer maximum and the lowest index among its equals one minimum. What is closed
-// (a logit or key of -inf or NaN) is key 0, below every open one.
+// A warp per token, a run of neighbouring experts per lane: a row is read (and its gradient
+// written) as vectors, a group of experts is a run of lanes, and among equal keys the lowest lane
+// has the lowest expert. A key is ordered as an unsigned integer (the float's bits, negative
+// ones complemented), so that the largest of a warp is one integer reduction. What is closed (a
+// logit or key of -inf or NaN) is key 0, below every open one.
+//
+// Bound by instructions: a token's 256 logits are 1 KB, 0.16 us of one processor's share of the
+// memory, and some 500 instructions (scores 90, keys and groups 110, eight choices 270).
+#include <cstring>
+
 #include "q4.cuh"
 
 namespace uor {
@@ -30,7 +36,8 @@ __device__ __forceinline__ float warp_sum(float v) {
 // exp(l - top) with the infinities' differences as limits have them: equal ones give 1.
 __device__ __forceinline__ float exp_below(float l, float top) { return l == top ? 1.0f : expf(l - top); }
 
-__device__ __forceinline__ float sigmoid(float l) { return 1.0f / (1.0f + expf(-l)); }
+// Within 3 units: the reciprocal's and the exponential's own, and an addition's.
+__device__ __forceinline__ float sigmoid(float l) { return __fdividef(1.0f, 1.0f + expf(-l)); }
 
 // The chosen experts' shares of their scores' sum; lane s holds choice s (open: whether it is
 // one). They are taken relative to the largest chosen logit, so that scores which underflow
@@ -63,100 +70,158 @@ __device__ __forceinline__ void softmax_of(const float (&l)[VPL], float* top, fl
     *total = warp_sum(s);
 }
 
+// This lane's logits, experts lane * VPL on; -inf past the last.
 template <typename T, int VPL>
-__device__ __forceinline__ void load_row(float (&l)[VPL], const Mat& m, int64_t t, int experts, int lane) {
+__device__ __forceinline__ void load_row(float (&l)[VPL], const Mat& m, bool vec, int64_t t, int experts, int lane) {
     const T* p = static_cast<const T*>(m.p) + t * m.rs;
+    const int e0 = lane * VPL;
+    constexpr int BYTES = VPL * sizeof(T);
+    if (BYTES >= 4 && vec && e0 + VPL <= experts) {
+        constexpr int WORDS = BYTES >= 4 ? BYTES / 4 : 1;
+        uint32_t w[WORDS];
+        if constexpr (WORDS % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        const int e = lane + 32 * i;
-        l[i] = e < experts ? to_f32(p[e * m.cs]) : -INFINITY;
+            for (int i = 0; i < WORDS; i += 4) {
+                const uint4 v = reinterpret_cast<const uint4*>(p + e0)[i / 4];
+                w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
+            }
+        } else if constexpr (WORDS == 2) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p + e0);
+            w[0] = v.x, w[1] = v.y;
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p + e0);
+        }
+        T v[VPL];
+        memcpy(v, w, BYTES < WORDS * 4 ? BYTES : WORDS * 4);
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) l[i] = to_f32(v[i]);
+        return;
     }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) l[i] = e0 + i < experts ? to_f32(p[(e0 + i) * m.cs]) : -INFINITY;
 }
 
-// The largest of the warp's keys and the lowest expert that has it.
+// The two largest of two ordered pairs.
+__device__ __forceinline__ void merge2(uint32_t& a1, uint32_t& a2, uint32_t b1, uint32_t b2) {
+    a2 = max(min(a1, b1), max(a2, b2));
+    a1 = max(a1, b1);
+}
+
+// The groups that stay open, a bit each. A group's order is its score's key plus one: a group of
+// -inf is behind every other, and before none. Groups are runs of whole lanes, as many as a power
+// of two, or else looked at one after another.
 template <int VPL>
-__device__ __forceinline__ uint32_t warp_best(const uint32_t (&key)[VPL], int lane, int* expert) {
-    uint32_t k = 0;
-    int at = 0;
+__device__ __forceinline__ uint32_t open_groups(const uint32_t (&key)[VPL], const uor_b200_router& r, int lane) {
+    const int groups = r.groups, size = r.experts / r.groups, lanes = size / VPL;
+    uint32_t mine = 0;  // lane g: group g's
+    if (size % VPL == 0 && (lanes & (lanes - 1)) == 0) {
+        uint32_t k1 = 0, k2 = 0;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-        if (key[i] > k) k = key[i], at = lane + 32 * i;
-    const uint32_t best = __reduce_max_sync(FULL, k);
-    *expert = static_cast<int>(__reduce_min_sync(FULL, k == best ? static_cast<unsigned>(at) : FULL));
-    return best;
+        for (int i = 0; i < VPL; ++i) merge2(k1, k2, key[i], 0);
+        for (int o = 1; o < lanes; o <<= 1) {
+            const uint32_t b1 = __shfl_xor_sync(FULL, k1, o), b2 = __shfl_xor_sync(FULL, k2, o);
+            merge2(k1, k2, b1, b2);
+        }
+        const uint32_t sum = size == 1 ? k1 : k2 ? open_key(key_value(k1) + key_value(k2)) : 0u;
+        mine = __shfl_sync(FULL, sum, lane * lanes & 31) + 1;
+    } else {
+        for (int g = 0; g < groups; ++g) {
+            uint32_t k1 = 0, k2 = 0;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                const int e = lane * VPL + i;
+                if (e >= g * size && e < (g + 1) * size) merge2(k1, k2, key[i], 0);
+            }
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t b1 = __shfl_xor_sync(FULL, k1, o), b2 = __shfl_xor_sync(FULL, k2, o);
+                merge2(k1, k2, b1, b2);
+            }
+            const uint32_t sum = size == 1 ? k1 : k2 ? open_key(key_value(k1) + key_value(k2)) : 0u;
+            if (lane == g) mine = sum + 1;
+        }
+    }
+    int ahead = 0;  // groups before this lane's
+    for (int g = 0; g < groups; ++g) {
+        const uint32_t other = __shfl_sync(FULL, mine, g);
+        ahead += other > mine || (other == mine && g < lane);
+    }
+    return __ballot_sync(FULL, lane < groups && ahead < static_cast<int>(r.top_groups));
 }
 
 template <typename T, int VPL>
-__global__ void route_kernel(RouterArgs a) {
+__global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ RouterArgs a) {
     const int lane = threadIdx.x & 31;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (t >= a.tokens) return;
-    const int experts = a.r.experts, top_k = a.r.top_k;
+    const int experts = a.r.experts, top_k = a.r.top_k, e0 = lane * VPL;
+    const bool softmax = a.r.score == UOR_B200_SOFTMAX;
     float l[VPL];
-    load_row<T>(l, a.logits, t, experts, lane);
+    load_row<T>(l, a.logits, a.vec, t, experts, lane);
     float top = 0, total = 1;
-    if (a.r.score == UOR_B200_SOFTMAX) softmax_of(l, &top, &total);
     uint32_t key[VPL];
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        const int e = lane + 32 * i;
-        float s = a.r.score == UOR_B200_SOFTMAX ? exp_below(l[i], top) / total : sigmoid(l[i]);
-        if (a.bias && e < experts) s += a.bias[e];
-        key[i] = l[i] > -INFINITY ? open_key(s) : 0u;
-    }
-    if (a.r.top_groups < a.r.groups) {
-        // Lane g keeps group g's score; a group without two open experts has -inf's.
-        const int size = experts / a.r.groups;
-        uint32_t mine = 0;
-        for (int g = 0; g < static_cast<int>(a.r.groups); ++g) {
-            uint32_t in[VPL];
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                const int e = lane + 32 * i;
-                in[i] = e >= g * size && e < (g + 1) * size ? key[i] : 0u;
-            }
-            int e1, e2;
-            const uint32_t k1 = warp_best(in, lane, &e1);
-            uint32_t sum = k1;
-            if (size > 1) {
-#pragma unroll
-                for (int i = 0; i < VPL; ++i)
-                    if (lane + 32 * i == e1) in[i] = 0;
-                const uint32_t k2 = warp_best(in, lane, &e2);
-                sum = k1 && k2 ? open_key(key_value(k1) + key_value(k2)) : 0u;
-            }
-            if (lane == g) mine = sum + 1;  // 1: a group of -inf, which is behind every other
-        }
-        uint32_t keep = 0;
-        for (int s = 0; s < static_cast<int>(a.r.top_groups); ++s) {
-            const uint32_t best = __reduce_max_sync(FULL, mine);
-            const unsigned g = __reduce_min_sync(FULL, mine == best ? static_cast<unsigned>(lane) : FULL);
-            keep |= 1u << g;
-            if (lane == static_cast<int>(g)) mine = 0;
-        }
+    if (softmax) {
+        softmax_of(l, &top, &total);
+        const float share = 1.0f / total;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
-            const int e = lane + 32 * i;
-            if (e < experts && !(keep >> (e / size) & 1)) key[i] = 0;
+            float s = exp_below(l[i], top) * share;
+            if (a.bias && e0 + i < experts) s += a.bias[e0 + i];
+            key[i] = l[i] > -INFINITY ? open_key(s) : 0u;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            float s = sigmoid(l[i]);
+            if (a.bias && e0 + i < experts) s += a.bias[e0 + i];
+            key[i] = l[i] > -INFINITY ? open_key(s) : 0u;
         }
     }
-    // Lane s keeps choice s.
+    if (a.r.top_groups < a.r.groups) {
+        const uint32_t open = open_groups(key, a.r, lane);
+        const int size = experts / a.r.groups;
+        if (size % VPL == 0) {
+            if (e0 < experts && !(open >> (e0 / size) & 1)) {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) key[i] = 0;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i)
+                if (e0 + i < experts && !(open >> ((e0 + i) / size) & 1)) key[i] = 0;
+        }
+    }
+    // Lane s keeps choice s. A choice's lane takes out its key, the first among equals.
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) best = max(best, key[i]);
     int expert = -1;
     for (int s = 0; s < top_k; ++s) {
-        int e;
-        const uint32_t best = warp_best(key, lane, &e);
-        if (!best) break;
+        const uint32_t k = __reduce_max_sync(FULL, best);
+        if (!k) break;
+        const int from = __ffs(__ballot_sync(FULL, best == k)) - 1;
+        int at = 0;
+        if (lane == from) {
+            bool found = false;
+            best = 0;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-            if (lane + 32 * i == e) key[i] = 0;
-        if (lane == s) expert = e;
+            for (int i = 0; i < VPL; ++i) {
+                if (!found && key[i] == k) {
+                    found = true;
+                    key[i] = 0;
+                    at = e0 + i;
+                }
+                best = max(best, key[i]);
+            }
+        }
+        at = __shfl_sync(FULL, at, from);
+        if (lane == s) expert = at;
     }
     float v = -INFINITY, w = 0;
     if (expert >= 0) v = to_f32(static_cast<const T*>(a.logits.p)[t * a.logits.rs + expert * a.logits.cs]);
     if (a.r.renormalize)
-        w = chosen_share(v, expert >= 0, a.r.score == UOR_B200_SOFTMAX);
+        w = chosen_share(v, expert >= 0, softmax);
     else if (expert >= 0)
-        w = a.r.score == UOR_B200_SOFTMAX ? exp_below(v, top) / total : sigmoid(v);
+        w = softmax ? exp_below(v, top) / total : sigmoid(v);
     if (lane < top_k) {
         static_cast<int32_t*>(a.ids.p)[t * a.ids.rs + lane * a.ids.cs] = expert;
         static_cast<float*>(a.weights.p)[t * a.weights.rs + lane * a.weights.cs] = w * a.r.scale;
@@ -167,55 +232,91 @@ __global__ void route_kernel(RouterArgs a) {
 // experts' shares (0 for the others):
 //   renormalised: dl_j = w_j (g_j - sum_i g_i w_i), and that times (1 - s_j) for the sigmoid;
 //   otherwise:    softmax dl = s (g - sum_i g_i s_i), sigmoid dl = g s (1 - s).
-// Only the softmax without renormalisation has gradients beyond the chosen experts.
+// Only the softmax without renormalisation has gradients beyond the chosen experts; elsewhere
+// these alone are written, over a row of zeros.
 template <typename T, int VPL>
-__global__ void route_backward_kernel(RouterArgs a) {
+__global__ void __launch_bounds__(256) route_backward_kernel(const __grid_constant__ RouterArgs a) {
     const int lane = threadIdx.x & 31;
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (t >= a.tokens) return;
-    const int experts = a.r.experts, top_k = a.r.top_k;
+    const int experts = a.r.experts, top_k = a.r.top_k, e0 = lane * VPL;
     const bool softmax = a.r.score == UOR_B200_SOFTMAX, whole = softmax && !a.r.renormalize;
     int expert = -1;
     float g = 0, v = -INFINITY;
     if (lane < top_k) {
         expert = static_cast<const int32_t*>(a.in_ids.p)[t * a.in_ids.rs + lane * a.in_ids.cs];
+        g = static_cast<const float*>(a.dweights.p)[t * a.dweights.rs + lane * a.dweights.cs] * a.r.scale;
         if (expert < 0 || expert >= experts) expert = -1;
+    }
+    T* row = static_cast<T*>(a.dlogits.p) + t * a.dlogits.rs;
+    const int64_t cs = a.dlogits.cs;
+    constexpr int BYTES = VPL * sizeof(T);
+    const bool vec = BYTES % 16 == 0 && a.vec_out && e0 + VPL <= experts;
+    if (!whole) {  // while the chosen logits travel
+        if (vec) {
+#pragma unroll
+            for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(row + e0)[i] = make_uint4(0, 0, 0, 0);
+        } else {
+            for (int e = lane; e < experts; e += 32) row[e * cs] = from_f32<T>(0.0f);
+        }
     }
     if (expert >= 0) {
         v = to_f32(static_cast<const T*>(a.logits.p)[t * a.logits.rs + expert * a.logits.cs]);
         if (!(v > -INFINITY)) expert = -1;
     }
-    if (expert >= 0)
-        g = static_cast<const float*>(a.dweights.p)[t * a.dweights.rs + lane * a.dweights.cs] * a.r.scale;
-    float l[VPL], d[VPL];
-    float top = 0, total = 1, inner = 0;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) d[i] = 0;
-    if (whole) {
-        load_row<T>(l, a.logits, t, experts, lane);
-        softmax_of(l, &top, &total);
-        inner = warp_sum(expert >= 0 ? g * (exp_below(v, top) / total) : 0.0f);
-    } else if (a.r.renormalize) {
-        const float w = chosen_share(v, expert >= 0, softmax);
-        const float dot = warp_sum(g * w);
-        g = w * (g - dot);
-        if (!softmax && expert >= 0) g *= sigmoid(-v);
-    } else if (expert >= 0) {
-        g *= sigmoid(v) * sigmoid(-v);
+    if (expert < 0) g = 0;
+    if (!whole) {
+        if (a.r.renormalize) {
+            const float w = chosen_share(v, expert >= 0, softmax);
+            const float dot = warp_sum(g * w);
+            g = w * (g - dot);
+            if (!softmax && expert >= 0) g *= sigmoid(-v);
+        } else if (expert >= 0) {
+            g *= sigmoid(v) * sigmoid(-v);
+        }
+        // An expert chosen more than once gets the sum, in the choices' order.
+        const unsigned same = __match_any_sync(FULL, expert);
+        if (__any_sync(FULL, expert >= 0 && (same & (same - 1)))) {
+            float sum = 0;
+            for (int j = 0; j < top_k; ++j) {
+                const float other = __shfl_sync(FULL, g, j);
+                if (same >> j & 1) sum += other;
+            }
+            g = sum;
+        }
+        __syncwarp();  // the zeros are written
+        if (expert >= 0) row[expert * cs] = from_f32<T>(g);
+        return;
     }
+    float l[VPL], d[VPL];
+    float top = 0, total = 1;
+    load_row<T>(l, a.logits, a.vec, t, experts, lane);
+    softmax_of(l, &top, &total);
+    const float inner = warp_sum(expert >= 0 ? g * (exp_below(v, top) / total) : 0.0f);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) d[i] = -inner;
     for (int j = 0; j < top_k; ++j) {
         const int e = __shfl_sync(FULL, expert, j);
         const float add = __shfl_sync(FULL, g, j);
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
-            if (lane + 32 * i == e) d[i] += add;
+            if (e0 + i == e) d[i] += add;
     }
+    const float share = 1.0f / total;
+    T out[VPL];
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-        const int e = lane + 32 * i;
-        if (e >= experts) continue;
-        if (whole) d[i] = l[i] > -INFINITY ? exp_below(l[i], top) / total * (d[i] - inner) : 0.0f;
-        store_f32(a.dlogits.p, t * a.dlogits.rs + e * a.dlogits.cs, a.dlogits.type, d[i]);
+    for (int i = 0; i < VPL; ++i) out[i] = from_f32<T>(l[i] > -INFINITY ? exp_below(l[i], top) * share * d[i] : 0.0f);
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            uint4 w;
+            memcpy(&w, reinterpret_cast<const char*>(out) + i * 16, 16);
+            reinterpret_cast<uint4*>(row + e0)[i] = w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (e0 + i < experts) row[(e0 + i) * cs] = out[i];
     }
 }
 
@@ -239,8 +340,11 @@ int launch(uor_b200_ctx* ctx, const RouterArgs& a, bool backward) {
     return cuda_status(cudaGetLastError());
 }
 
-int run(uor_b200_ctx* ctx, const RouterArgs& a, bool backward, uor_b200_route* route) {
+int run(uor_b200_ctx* ctx, RouterArgs a, bool backward, uor_b200_route* route) {
     route->kernel = UOR_B200_KERNEL_ROUTER;
+    const uint64_t size = a.elem == UOR_B200_F32 ? 4 : 2;
+    a.vec = a.logits.cs == 1 && (reinterpret_cast<uint64_t>(a.logits.p) | static_cast<uint64_t>(a.logits.rs) * size) % 16 == 0;
+    a.vec_out = a.dlogits.cs == 1 && (reinterpret_cast<uint64_t>(a.dlogits.p) | static_cast<uint64_t>(a.dlogits.rs) * size) % 16 == 0;
     if (a.elem == UOR_B200_F32) return launch<float>(ctx, a, backward);
     if (a.elem == UOR_B200_BF16) return launch<__nv_bfloat16>(ctx, a, backward);
     return launch<__half>(ctx, a, backward);

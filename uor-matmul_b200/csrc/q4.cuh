@@ -84,6 +84,7 @@ struct RouterArgs {
     MatOut ids, weights;            // forward
     Mat in_ids, dweights;           // backward
     MatOut dlogits;
+    bool vec, vec_out;              // rows of logits (of dlogits) are whole vectors; set by the launch
 };
 int run_expert_route(uor_b200_ctx* ctx, const RouterArgs& a, uor_b200_route* route);
 int run_expert_route_backward(uor_b200_ctx* ctx, const RouterArgs& a, uor_b200_route* route);
