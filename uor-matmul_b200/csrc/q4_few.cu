@@ -1,14 +1,15 @@
 // q4_few.cu -- products of few rows with 4-bit weights and group scales.
 //
-// Bound by the weights' bytes, read once: 4 bits and a share of a scale each. A CTA takes 16 rows
-// of weights and its eight warps split the reduction into chunks of 256 positions (128 bytes of a
-// row), warp w taking chunks w, w + 8, ...: side by side they read 1 KB of each row. Each warp
-// keeps a ring of chunks of codes in flight with cp.async, in shared memory of its own, so no
-// warp waits for another until the sums are joined at the end. The scales and zero points of the
-// tile, and the activations, are laid out in shared memory while the first chunks travel.
+// Bound by the weights' bytes, read once: 4 bits and a share of a scale each. A CTA takes tiles of
+// 16 rows of weights, one after another, and its warps split a tile's reduction into chunks of 256
+// positions (128 bytes of a row), neighbouring warps taking neighbouring chunks. Each warp keeps a
+// ring of chunks of codes in flight with cp.async, in shared memory of its own and across the
+// tiles, so no warp waits for another but where a tile's sums are joined. A chunk's scales and
+// zero points travel in registers one chunk ahead; the activations are laid out in shared memory
+// once, while the first chunks travel.
 //
 // The products run on the tensor cores (mma.m16n8k16) with the weights as the 16 rows and up to 8
-// activation rows as the columns, since CUDA cores could not multiply at the rate the codes
+// or 16 activation rows as the columns, since CUDA cores could not multiply at the rate the codes
 // arrive at from four rows on. A code is exact as a 16-bit float: its bits under the exponent of
 // 128 (bfloat16) or 1024 (float16), less the same plus the zero point. So the sum of a group is
 // exact but for its f32 additions, and the group's scale multiplies it in f32: no weight is ever
@@ -20,6 +21,9 @@
 // What is left beside the memory is instructions: 11 to unpack eight weights of bfloat16 (three
 // shifts, four and-or, four subtractions), so addresses, scales and their types are kept out of
 // the loop.
+//
+// With experts a CTA finds the pairs (token, choice) of one of them by looking through all ids:
+// its columns are these pairs' activation rows.
 #include "q4_few.cuh"
 
 #include <type_traits>
@@ -30,7 +34,6 @@ namespace uor {
 
 namespace {
 
-constexpr int WARPS = 8;
 constexpr int STAGES = 2;
 constexpr int ROWS = 16;
 constexpr int SUB = 128;                       // positions of the reduction in 64 bytes of a row
@@ -38,7 +41,6 @@ constexpr int CHUNK = 2 * SUB;                 // positions per ring stage
 constexpr int HALF_BYTES = ROWS * SUB / 2;     // of a stage's codes, per SUB
 constexpr int PITCH_ANY = 144;                 // of a row's codes whose addresses are not aligned
 constexpr int X_BYTES = SUB * 2;               // of a SUB, per activation row
-constexpr int X_MOST = 64 * 1024;              // resident activations of a CTA
 
 template <bool ANY>
 constexpr int stage_bytes() {
@@ -176,10 +178,6 @@ __device__ __forceinline__ uint4 in_pairs(uint4 w) {
                       __byte_perm(w.y, w.w, 0x7632));
 }
 
-__device__ __forceinline__ int id_at(const FewParams& p, int pair) {
-    return static_cast<const int32_t*>(p.ids.p)[pair / p.top_k * p.ids.rs + pair % p.top_k * p.ids.cs];
-}
-
 // Reads of shared memory at its 32-bit addresses, as loads the compiler may order by itself.
 template <typename V>
 __device__ __forceinline__ V lds(uint32_t at) {
@@ -188,15 +186,6 @@ __device__ __forceinline__ V lds(uint32_t at) {
 
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-
-// A tile's joined sum: [warp][lane][4] in shared memory, added in the warps' order.
-__device__ __forceinline__ float joined(const float* red, int row, int col) {
-    const int at = ((row & 7) * 4 + (col >> 1)) * 4 + (row >> 3) * 2 + (col & 1);
-    float v = 0;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) v += red[w * 128 + at];
-    return v;
 }
 
 // The scales and zero points of a chunk for this lane's two rows (lane / 4 of each half of the
@@ -270,33 +259,37 @@ struct Quants {
     }
 };
 
+// A tile of weights: its rows r are row0 + r (half 8), or eight rows from row0 on and eight from
+// row0 + half on; `lo` and `hi` of the halves' rows are valid, and the last valid one stands in for
+// those past it.
+struct Tile {
+    int64_t row0, half;
+    int lo, hi;
+    __device__ __forceinline__ int64_t row(int r) const {
+        return r < 8 ? row0 + min(r, lo - 1) : row0 + half + min(r - 8, hi - 1);
+    }
+};
+
 // One warp's ring of chunks of codes.
 template <typename T, typename S, int SEG, bool ANY>
 struct Ring {
     static constexpr int NSEG = SUB / SEG;
     uint32_t base;               // shared address of stage 0
     const uint8_t* row[ANY ? 2 : 4];  // this lane's rows of codes: its pieces' (lane / 8 + 4 v), or g and g + 8
-    int64_t step;                // from one expert's codes to the next's, in bytes
     int row_len;
 
-    __device__ __forceinline__ void init(const FewParams& p, int lane, int64_t row0, int64_t half, int lo, int hi) {
-        auto at = [&](int r) {  // the last valid row stands in for those past it
-            const int64_t i = r < 8 ? row0 + min(r, lo - 1) : row0 + half + min(r - 8, hi - 1);
-            return p.w.codes + i * p.w.row_bytes;
-        };
+    __device__ __forceinline__ void set(const FewParams& p, int lane, const Tile& t) {
         if constexpr (ANY) {
-            row[0] = at(lane >> 2), row[1] = at((lane >> 2) + 8);
+            row[0] = p.w.codes + t.row(lane >> 2) * p.w.row_bytes, row[1] = p.w.codes + t.row((lane >> 2) + 8) * p.w.row_bytes;
         } else {
 #pragma unroll
-            for (int v = 0; v < 4; ++v) row[v] = at((lane >> 3) + 4 * v) + 16 * (lane & 7);
+            for (int v = 0; v < 4; ++v) row[v] = p.w.codes + t.row((lane >> 3) + 4 * v) * p.w.row_bytes + 16 * (lane & 7);
         }
-        step = static_cast<int64_t>(p.n) * p.w.row_bytes;
-        row_len = (p.w.cols + 1) / 2;
     }
 
-    __device__ __forceinline__ void load(int stage, int chunk, int expert, int lane) const {
+    __device__ __forceinline__ void load(int stage, int chunk, int lane) const {
         const uint32_t at = base + stage * stage_bytes<ANY>();
-        const int64_t from = expert * step + chunk * (CHUNK / 2);
+        const int from = chunk * (CHUNK / 2);
         const int left = row_len - chunk * (CHUNK / 2);  // bytes of the row from here
         if constexpr (!ANY) {
             const int c = lane & 7;
@@ -324,9 +317,11 @@ struct Ring {
     }
 
     // sum += the products of one half of the chunk (`sub`). xs: the half's activations of this
-    // lane's column of the instruction (row x_row of them); left: positions that exist.
-    __device__ __forceinline__ void compute(int stage, int sub, int expert, int lane, const Quants<T, S, SEG>& q, bool zeros,
-                                            uint32_t xs, int x_row, int left, float (&sum)[4]) const {
+    // lane's columns of the instructions (rows x_row of them); left: positions that exist;
+    // m0, m1: how far past a word the lane's two rows of codes begin, in bits.
+    template <int NT>
+    __device__ __forceinline__ void compute(int stage, int sub, int lane, const Quants<T, S, SEG>& q, bool zeros, int m0, int m1,
+                                            const uint32_t (&xs)[NT], const int (&x_row)[NT], int left, float (&sum)[NT][4]) const {
         const uint32_t codes = base + stage * stage_bytes<ANY>() + (ANY ? sub * 64 : sub * HALF_BYTES);
         const int g = lane >> 2, c = lane & 3;
 #pragma unroll
@@ -340,8 +335,6 @@ struct Ring {
             if constexpr (ANY) {
                 const int word = SEG == 128 ? 4 * c : SEG == 64 ? 8 * s + 2 * c : 4 * s + c;
                 const uint32_t a0 = codes + g * PITCH_ANY + 4 * word, a1 = a0 + 8 * PITCH_ANY;
-                const int m0 = 8 * static_cast<int>((reinterpret_cast<uint64_t>(row[0]) + expert * step) & 3);
-                const int m1 = 8 * static_cast<int>((reinterpret_cast<uint64_t>(row[1]) + expert * step) & 3);
                 uint32_t n0 = lds<uint32_t>(a0), n1 = lds<uint32_t>(a1);
 #pragma unroll
                 for (int j = 0; j < WORDS; ++j) {
@@ -362,21 +355,29 @@ struct Ring {
                 const uint32_t a = codes + code_at(g, s) + c * 4;
                 w0[0] = lds<uint32_t>(a), w1[0] = lds<uint32_t>(a + 8 * 64);
             }
-            float acc[4] = {0, 0, 0, 0};
+            float acc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
 #pragma unroll
             for (int j = 0; j < WORDS; ++j) {
                 uint32_t a0[4], a1[4];
                 Decode<T>::unpack(w0[j], zero0, a0[0], a0[2], a1[0], a1[2]);
                 Decode<T>::unpack(w1[j], zero1, a0[1], a0[3], a1[1], a1[3]);
                 const int piece = SEG == 128 ? 4 * c + j : SEG == 64 ? 8 * s + 2 * c + j : 4 * s + c;
-                const uint4 x = lds<uint4>(xs + x_piece<SEG>(x_row, piece));
-                Decode<T>::mma(acc, a0, x.x, x.y);
-                Decode<T>::mma(acc, a1, x.z, x.w);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const uint4 x = lds<uint4>(xs[n] + sub * X_BYTES + x_piece<SEG>(x_row[n], piece));
+                    Decode<T>::mma(acc[n], a0, x.x, x.y);
+                    Decode<T>::mma(acc[n], a1, x.z, x.w);
+                }
             }
-            sum[0] = fmaf(scale0, acc[0], sum[0]);
-            sum[1] = fmaf(scale0, acc[1], sum[1]);
-            sum[2] = fmaf(scale1, acc[2], sum[2]);
-            sum[3] = fmaf(scale1, acc[3], sum[3]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                sum[n][0] = fmaf(scale0, acc[n][0], sum[n][0]);
+                sum[n][1] = fmaf(scale0, acc[n][1], sum[n][1]);
+                sum[n][2] = fmaf(scale1, acc[n][2], sum[n][2]);
+                sum[n][3] = fmaf(scale1, acc[n][3], sum[n][3]);
+            }
         }
     }
 };
@@ -384,308 +385,325 @@ struct Ring {
 // An activation's place among its eight in the operands' order.
 __device__ __forceinline__ int paired(int r) { return r < 4 ? 2 * r : 2 * r - 7; }
 
-template <typename T, typename S, int SEG, int MODE, bool ANY>
-__global__ void __launch_bounds__(WARPS * 32, 3) few_kernel(const FewParams p) {
-    using R = Ring<T, S, SEG, ANY>;
-    constexpr bool DOWN = MODE == FEW_DOWN;
+// NT: columns in eights. A block has 8 warps a column eight.
+template <int NT>
+struct Block {
+    static constexpr int WARPS = 8 * NT, THREADS = 32 * WARPS;
+    static constexpr int RED = 2 * WARPS * NT * 128 * 4;  // joined sums, twice
+    static constexpr int X_MOST = NT == 1 ? 64 * 1024 : 112 * 1024;  // resident activations
+};
+
+template <typename T, typename S, int SEG, int NT, bool ANY>
+__global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kernel(const __grid_constant__ FewParams p) {
+    constexpr int WARPS = Block<NT>::WARPS, THREADS = Block<NT>::THREADS, COLS = 8 * NT;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int id_of[MODE == FEW_DENSE ? 1 : FEW_MAX_PAIRS];
-    __shared__ int expert_of[DOWN ? FEW_MAX_PAIRS : 1];        // the chosen experts, each once
-    __shared__ float weight_of[DOWN ? FEW_MAX_PAIRS * 8 : 1];  // by expert and token
-    __shared__ int pair_of[DOWN ? FEW_MAX_PAIRS * 8 : 1];
-    __shared__ unsigned chosen_by[DOWN ? FEW_MAX_PAIRS : 1];   // an expert's tokens, a bit each
-    __shared__ int rank_of[DOWN ? FEW_MAX_PAIRS : 1];
-    __shared__ int count[WARPS];
+    __shared__ uint32_t bits[FEW_MAX_EXPERTS / 32];  // the chosen experts
+    __shared__ uint16_t id_of[FEW_MAX_PAIRS], list[FEW_MAX_PAIRS];  // the pairs' experts; this one's pairs
+    __shared__ int counts[WARPS], chosen;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int chunks = (p.w.cols + CHUNK - 1) / CHUNK;
-    const int pairs = p.tokens * p.top_k;
+    const int kind = p.kind;
+    if (kind != FEW_DENSE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    int64_t row0 = 0, half = 8, x0 = 0;  // the tile's first row of weights; from it to its ninth
-    int lo, hi;                          // valid rows of the tile's two halves
-    int rows_x = p.tokens, units = chunks;
-    if (MODE == FEW_UP) {
-        // CTA y takes the expert of pair y, unless an earlier pair has the same one.
-        const int j0 = blockIdx.x * 8;
-        if (threadIdx.x < pairs) id_of[threadIdx.x] = id_at(p, threadIdx.x);
-        __syncthreads();
-        const int e = id_of[blockIdx.y];
-        if (e < 0 || e >= p.experts) return;
-        if (__syncthreads_or(threadIdx.x < blockIdx.y && id_of[threadIdx.x] == e)) return;
-        row0 = static_cast<int64_t>(e) * 2 * p.n + j0;
-        half = p.n;
-        lo = hi = min(8, p.n - j0);
+    // The columns: activation rows from x0 on, or of the listed pairs of expert e.
+    int e = 0, listed = 0;
+    int64_t x0 = 0;
+    if (kind == FEW_DENSE) {
+        x0 = static_cast<int64_t>(blockIdx.y) * COLS;
+        listed = static_cast<int>(min(static_cast<int64_t>(COLS), p.m - x0));
     } else {
-        row0 = static_cast<int64_t>(blockIdx.x) * ROWS;
-        lo = min(8, p.n - static_cast<int>(row0));
-        hi = max(1, min(8, p.n - static_cast<int>(row0) - 8));
-        if (p.n - row0 <= 8) half = 0;  // no second half: the first row stands in
-        if (MODE == FEW_DENSE) {
-            x0 = static_cast<int64_t>(blockIdx.y) * 8;
-            rows_x = static_cast<int>(min(static_cast<int64_t>(8), p.m - x0));
-        }
-    }
-    if (DOWN) {
-        // The experts in the order of their first choice, with their tokens' weights; an expert
-        // that a token chose twice has both weights.
-        const int i = threadIdx.x, t = i / p.top_k, slot = i % p.top_k;
-        float w = 0;
-        int e = -1;
-        if (i < pairs) {
-            e = id_at(p, i);
-            if (e < 0 || e >= p.experts) e = -1;
-            w = static_cast<const float*>(p.weights.p)[t * p.weights.rs + slot * p.weights.cs];
-            id_of[i] = e;
-            weight_of[i] = w;  // by pair until they are summed
-            chosen_by[i] = 0;
+        // CTA y takes the y-th of the chosen experts.
+        const int pairs = p.tokens * p.top_k;
+        if (threadIdx.x < FEW_MAX_EXPERTS / 32) bits[threadIdx.x] = 0;
+        if (threadIdx.x == 0) chosen = -1;
+        __syncthreads();
+        for (int i = threadIdx.x; i < pairs; i += THREADS) {
+            const int t = i / p.top_k;
+            const int id = static_cast<const int32_t*>(p.ids.p)[t * p.ids.rs + (i - t * p.top_k) * p.ids.cs];
+            const bool in = id >= 0 && id < p.experts;
+            id_of[i] = in ? static_cast<uint16_t>(id) : 0xFFFF;
+            if (in) atomicOr(&bits[id >> 5], 1u << (id & 31));
         }
         __syncthreads();
-        int first = i;  // the first pair of this pair's expert
-        if (e >= 0)
-            for (int o = i - 1; o >= 0; --o)
-                if (id_of[o] == e) first = o;
-        const bool head = e >= 0 && first == i;
-        const unsigned vote = __ballot_sync(0xffffffffu, head);
-        if (lane == 0) count[warp] = __popc(vote);
-        bool mine = e >= 0;  // the token's first choice of this expert sums its weights
-        for (int s = 0; s < p.top_k && i < pairs; ++s) {
-            const int o = t * p.top_k + s;
-            if (id_of[o] != e || o == i) continue;
-            if (o < i) mine = false;
-            if (mine) w += weight_of[o];
+        if (warp == 0) {
+            const uint32_t w = bits[lane];
+            int before = __popc(w);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += v;
+            }
+            before -= __popc(w);
+            const int nth = static_cast<int>(blockIdx.y) - before;
+            if (nth >= 0 && nth < __popc(w)) {
+                uint32_t left = w;
+                for (int b = 0; b < nth; ++b) left &= left - 1;
+                chosen = lane * 32 + __ffs(left) - 1;
+            }
         }
         __syncthreads();
-        int before = 0, listed = 0;
-        for (int v = 0; v < WARPS; ++v) {
-            if (v < warp) before += count[v];
-            listed += count[v];
+        e = chosen;
+        if (e < 0) return;
+        // its pairs, in order: a run of pairs to a thread. A token that chose it more than once is
+        // there with its first choice alone, so there are at most as many columns as tokens.
+        auto lists = [&](int i) {
+            if (id_of[i] != e) return false;
+            for (int o = i - i % p.top_k; o < i; ++o)
+                if (id_of[o] == e) return false;
+            return true;
+        };
+        const int run = (pairs + THREADS - 1) / THREADS, from = min(pairs, static_cast<int>(threadIdx.x) * run);
+        const int to = min(pairs, from + run);
+        int mine = 0;
+        for (int i = from; i < to; ++i) mine += lists(i);
+        int upto = mine;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
         }
-        if (head) {
-            const int a = before + __popc(vote & ((1u << lane) - 1));
-            rank_of[i] = a;
-            expert_of[a] = e;
-        }
+        if (lane == 31) counts[warp] = upto;
         __syncthreads();
-        if (mine) {
-            const int a = rank_of[first];
-            weight_of[a * 8 + t] = w;
-            pair_of[a * 8 + t] = i;
-            atomicOr(&chosen_by[a], 1u << t);
+        int at = upto - mine;
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) at += counts[w];
+            listed += counts[w];
         }
+        for (int i = from; i < to; ++i)
+            if (lists(i)) list[at++] = static_cast<uint16_t>(i);
         __syncthreads();
-        units = chunks * listed;
     }
 
-    R ring;
-    ring.init(p, lane, row0, half, lo, hi);
-    ring.base = smem_u32(smem) + warp * (STAGES * stage_bytes<ANY>());
-    // Behind the rings the activations: resident rows of a panel of the reduction, or a chunk of
-    // them with each stage.
-    const int panel = DOWN ? units : min(units, p.panel);
-    const uint32_t x_all = smem_u32(smem) + WARPS * STAGES * stage_bytes<ANY>();
-    const uint32_t x_ring = x_all + warp * (STAGES * rows_x * 2 * X_BYTES);
-    const int x_row = min(lane >> 2, rows_x - 1);
-    const int groups = (p.w.cols + p.w.group - 1) / p.w.group;
-    const int64_t quants0 = (row0 + min(lane >> 2, lo - 1)) * p.w.groups_rs;
-    const int64_t quants1 = (row0 + half + min(lane >> 2, hi - 1)) * p.w.groups_rs;
-    const int64_t quants_step = static_cast<int64_t>(p.n) * p.w.groups_rs;
-    const bool zeros = p.w.zeros != nullptr;
-    float total[4] = {0, 0, 0, 0};
-
-    if (MODE == FEW_UP) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (DOWN && units == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-    // This warp's units of a panel: first + warp, first + warp + 8, ... A unit is a chunk, or with
-    // several experts the chunks of one after those of another.
-    for (int first = 0; first < units; first += panel) {
-        const int here = min(panel, units - first);
-        const int mine = here > warp ? (here - warp + WARPS - 1) / WARPS : 0;
-        int lstage = 0, le = 0, lc = first + warp;  // the next unit to load
-        if constexpr (DOWN) le = lc / chunks, lc = lc % chunks;
-        auto load_codes = [&]() { ring.load(lstage, lc, DOWN ? expert_of[le] : 0, lane); };
-        auto load_x = [&]() {
-            if constexpr (DOWN) {
-                for (int v = lane; v < rows_x * 32; v += 32) {
-                    const int r = v >> 5, piece = v & 31, k = lc * CHUNK + piece * 8;
-                    if (!(chosen_by[le] >> r & 1)) continue;
-                    const bool in = k < p.x_rs;
-                    cp_async16(x_ring + ((lstage * rows_x + r) * 2 + (piece >> 4)) * X_BYTES + x_piece<SEG>(r, piece & 15),
-                               static_cast<const T*>(p.x) + pair_of[le * 8 + r] * p.x_rs + (in ? k : 0), in ? 16 : 0);
-                }
-            }
-        };
-        auto advance = [&]() {
-            lstage = lstage + 1 == STAGES ? 0 : lstage + 1;
-            lc += WARPS;
-            if constexpr (DOWN) {
-                while (lc >= chunks) lc -= chunks, ++le;
-            }
-        };
-        if (first) __syncthreads();  // every warp is done with the panel before this one
-        const int c0 = lc, e0 = le;
-        for (int s = 0; s < STAGES - 1; ++s) {
-            if (s < mine) load_codes(), advance();
-            if (!DOWN) cp_commit();
-        }
-        Quants<T, S, SEG> now, next;
-        if (mine) now.load(p, quants0 + (DOWN ? expert_of[e0] * quants_step : 0), quants1 + (DOWN ? expert_of[e0] * quants_step : 0), c0, groups);
-        if (DOWN) {
-            // The weights depend on nothing before this launch, the inner activations on the
-            // launch before it.
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            lc = c0, le = e0, lstage = 0;
-            for (int s = 0; s < STAGES - 1; ++s) {
-                if (s < mine) load_x(), advance();
-                cp_commit();
-            }
+    // `kw` warps share a tile's reduction, so WARPS / kw tiles are under way at once.
+    const int kw = p.k_warps, k_warp = warp & (kw - 1), t_warp = warp / kw, abreast = WARPS / kw;
+    const int rows = kind == FEW_UP ? 8 : ROWS;  // outputs of a tile
+    const int tiles = (p.n + rows - 1) / rows;
+    auto tile_at = [&](int t) {
+        t = min(t, tiles - 1);
+        Tile w;
+        if (kind == FEW_UP) {
+            w.row0 = static_cast<int64_t>(e) * 2 * p.n + t * 8;
+            w.half = p.n;
+            w.lo = w.hi = min(8, p.n - t * 8);
         } else {
-            const int pieces = here * 32;
-            for (int v0 = threadIdx.x; v0 < rows_x * pieces; v0 += 4 * blockDim.x) {
-                uint4 x8[4];
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int v = min(v0 + b * static_cast<int>(blockDim.x), rows_x * pieces - 1);
-                    const int r = rows_x == 1 ? 0 : v / pieces, k = first * CHUNK + (v - r * pieces) * 8;
-                    x8[b] = load_x8(static_cast<const T*>(p.x) + (x0 + r) * p.x_rs + k, p.w.cols - k, p.x_vec != 0);
-                }
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    const int v = v0 + b * static_cast<int>(blockDim.x);
-                    const int r = rows_x == 1 ? 0 : v / pieces, piece = v - r * pieces;
-                    if (v < rows_x * pieces)
-                        sts128(x_all + (r * panel * 2 + (piece >> 4)) * X_BYTES + x_piece<SEG>(r, piece & 15), in_pairs(x8[b]));
-                }
-            }
+            const int left = p.n - t * ROWS;
+            w.row0 = static_cast<int64_t>(e) * p.n + t * ROWS;
+            w.half = left > 8 ? 8 : 0;  // no second half: the first row stands in
+            w.lo = min(8, left);
+            w.hi = max(1, min(8, left - 8));
         }
-        __syncthreads();
-        int stage = 0, e = 0, c = first + warp;
-        if constexpr (DOWN) e = c / chunks, c = c % chunks;
-        uint32_t xs = x_all + (x_row * panel + warp) * (2 * X_BYTES);
-        for (int i = 0; i < mine; ++i) {
-            cp_wait<STAGES - 2>();
-            __syncwarp();
-            if (i + STAGES - 1 < mine) load_codes(), load_x(), advance();
+        return w;
+    };
+    Ring<T, S, SEG, ANY> ring;
+    ring.base = smem_u32(smem) + warp * (STAGES * stage_bytes<ANY>());
+    ring.row_len = (p.w.cols + 1) / 2;
+    float* red = reinterpret_cast<float*>(smem + WARPS * STAGES * stage_bytes<ANY>());
+    const uint32_t x_all = smem_u32(smem) + WARPS * STAGES * stage_bytes<ANY>() + Block<NT>::RED;
+    const int groups = (p.w.cols + p.w.group - 1) / p.w.group;
+    const bool zeros = p.w.zeros != nullptr;
+    const int panel = p.panel, panels = (chunks + panel - 1) / panel;  // chunks whose activations are resident
+    const int tile_step = gridDim.x * abreast;
+    bool waited = kind != FEW_PART;
+
+    for (int c0 = 0; c0 < listed; c0 += COLS) {
+        const int rows_x = min(COLS, listed - c0);
+        int x_row[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) x_row[n] = min(n * 8 + (lane >> 2), rows_x - 1);
+        int buffer = 0;
+        // A warp's units: of each of its tiles in turn, of each panel, chunks k_warp, k_warp + kw, ..
+        int lt = blockIdx.x * abreast + t_warp, lpanel = 0, lc = k_warp, lstage = 0;  // the next to load
+        auto settle = [&]() {  // past the end of a panel or a tile
+            while (lt < tiles && lc >= min(chunks, (lpanel + 1) * panel)) {
+                if (++lpanel == panels) {
+                    lpanel = 0;
+                    lt += tile_step;
+                    if (lt < tiles) ring.set(p, lane, tile_at(lt));
+                }
+                lc = lpanel * panel + k_warp;
+            }
+        };
+        auto load = [&]() {
+            if (lt < tiles) {
+                ring.load(lstage, lc, lane);
+                lc += kw;
+                settle();
+            }
+            lstage = lstage + 1 == STAGES ? 0 : lstage + 1;
             cp_commit();
-            int e2 = e, c2 = c + WARPS;  // the unit after this one
-            if constexpr (DOWN) {
-                while (c2 >= chunks) c2 -= chunks, ++e2;
+        };
+        if (lt < tiles) ring.set(p, lane, tile_at(lt));
+        settle();
+        // The weights depend on nothing before this launch; the inner activations do.
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) load();
+        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+        waited = true;
+        int stage = 0;
+        for (int t0 = blockIdx.x * abreast; t0 < tiles; t0 += tile_step) {
+            const int t = t0 + t_warp;
+            const Tile tile = tile_at(t);
+            const int64_t r0 = tile.row(lane >> 2), r1 = tile.row((lane >> 2) + 8);
+            const int64_t quants0 = r0 * p.w.groups_rs, quants1 = r1 * p.w.groups_rs;
+            int m0 = 0, m1 = 0;
+            if constexpr (ANY) {
+                m0 = 8 * static_cast<int>((reinterpret_cast<uint64_t>(p.w.codes) + r0 * p.w.row_bytes) & 3);
+                m1 = 8 * static_cast<int>((reinterpret_cast<uint64_t>(p.w.codes) + r1 * p.w.row_bytes) & 3);
             }
-            if (i + 1 < mine) {
-                const int64_t to = DOWN ? expert_of[e2] * quants_step : 0;
-                next.load(p, quants0 + to, quants1 + to, c2, groups);
+            float total[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) total[n][0] = total[n][1] = total[n][2] = total[n][3] = 0;
+            for (int pn = 0; pn < panels; ++pn) {
+                const int first = pn * panel, last = min(chunks, first + panel);
+                const int units = t < tiles && last - first > k_warp ? (last - first - k_warp + kw - 1) / kw : 0;
+                Quants<T, S, SEG> now, next;
+                if (units) now.load(p, quants0, quants1, first + k_warp, groups);
+                if (panels > 1 || t0 == static_cast<int>(blockIdx.x) * abreast) {
+                    __syncthreads();  // every warp is done with the activations before these
+                    const int pieces = (last - first) * 32;
+                    for (int v0 = threadIdx.x; v0 < rows_x * pieces; v0 += 4 * THREADS) {
+                        uint4 x8[4];
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const int v = min(v0 + b * THREADS, rows_x * pieces - 1);
+                            const int r = rows_x == 1 ? 0 : v / pieces, k = first * CHUNK + (v - r * pieces) * 8;
+                            const int64_t row = kind == FEW_DENSE ? x0 + r : kind == FEW_UP ? list[c0 + r] / p.top_k : list[c0 + r];
+                            // rows of inner activations end in whole eights
+                            const int left = kind == FEW_PART ? (k < p.x_rs ? 8 : 0) : p.w.cols - k;
+                            x8[b] = load_x8(static_cast<const T*>(p.x) + row * p.x_rs + (left > 0 ? k : 0), left, p.x_vec != 0);
+                        }
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) {
+                            const int v = v0 + b * THREADS;
+                            const int r = rows_x == 1 ? 0 : v / pieces, piece = v - r * pieces;
+                            if (v < rows_x * pieces)
+                                sts128(x_all + (r * panel * 2 + (piece >> 4)) * X_BYTES + x_piece<SEG>(r, piece & 15),
+                                       kind == FEW_PART ? x8[b] : in_pairs(x8[b]));
+                        }
+                    }
+                    __syncthreads();
+                }
+                uint32_t xs[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) xs[n] = x_all + (x_row[n] * panel + k_warp) * (2 * X_BYTES);
+                int c = first + k_warp;
+                for (int i = 0; i < units; ++i, c += kw) {
+                    cp_wait<STAGES - 2>();
+                    __syncwarp();
+                    load();
+                    if (i + 1 < units) next.load(p, quants0, quants1, c + kw, groups);
+                    const int left = p.w.cols - c * CHUNK;
+                    ring.compute(stage, 0, lane, now, zeros, m0, m1, xs, x_row, left, total);
+                    if (left > SUB) ring.compute(stage, 1, lane, now, zeros, m0, m1, xs, x_row, left - SUB, total);
+                    stage = stage + 1 == STAGES ? 0 : stage + 1;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) xs[n] += kw * (2 * X_BYTES);
+                    now = next;
+                }
             }
-            const int left = p.w.cols - c * CHUNK;
-            if constexpr (DOWN) {
-                float part[4] = {0, 0, 0, 0};
-                const uint32_t x2 = x_ring + (stage * rows_x + x_row) * (2 * X_BYTES);
-                ring.compute(stage, 0, expert_of[e], lane, now, zeros, x2, x_row, left, part);
-                if (left > SUB) ring.compute(stage, 1, expert_of[e], lane, now, zeros, x2 + X_BYTES, x_row, left - SUB, part);
-                const int t = (lane & 3) * 2;
-                const unsigned chosen = chosen_by[e] >> t;
-                const float2 w = *reinterpret_cast<const float2*>(&weight_of[e * 8 + t]);
-                if (chosen & 1) total[0] = fmaf(w.x, part[0], total[0]), total[2] = fmaf(w.x, part[2], total[2]);
-                if (chosen & 2) total[1] = fmaf(w.y, part[1], total[1]), total[3] = fmaf(w.y, part[3], total[3]);
-            } else {
-                ring.compute(stage, 0, 0, lane, now, zeros, xs, x_row, left, total);
-                if (left > SUB) ring.compute(stage, 1, 0, lane, now, zeros, xs + X_BYTES, x_row, left - SUB, total);
+            // Join the warps' sums, [warp][column eight][lane][4], in the warps' order.
+            float* joined = red + buffer * (WARPS * NT * 128);
+            buffer ^= 1;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                reinterpret_cast<float4*>(joined)[(warp * NT + n) * 32 + lane] = make_float4(total[n][0], total[n][1], total[n][2], total[n][3]);
+            __syncthreads();
+            for (int v = threadIdx.x; v < abreast * rows * rows_x; v += THREADS) {
+                const int r = v & (rows - 1), rest = v / rows, ab = rest % abreast, col = rest / abreast;
+                const int out = (t0 + ab) * rows + r;
+                auto sum = [&](int row) {
+                    const float* at = joined + (ab * kw * NT + (col >> 3)) * 128 + ((row & 7) * 4 + ((col & 7) >> 1)) * 4 + (row >> 3) * 2 + (col & 1);
+                    float s = 0;
+                    for (int w = 0; w < kw; ++w) s += at[w * NT * 128];
+                    return s;
+                };
+                if (kind == FEW_UP) {
+                    // eight inner activations in the operands' order, zeros behind the last
+                    if (t0 + ab < tiles)
+                        static_cast<T*>(p.h)[static_cast<int64_t>(list[c0 + col]) * p.h_rs + (t0 + ab) * 8 + paired(r)] =
+                            from_f32<T>(out < p.n ? silu(sum(r)) * sum(r + 8) : 0.0f);
+                } else if (out < p.n) {
+                    if (kind == FEW_PART)
+                        p.part[static_cast<int64_t>(list[c0 + col]) * p.n + out] = sum(r);
+                    else
+                        store_f32(p.y.p, (x0 + col) * p.y.rs + out * p.y.cs, p.y.type, sum(r));
+                }
             }
-            stage = stage + 1 == STAGES ? 0 : stage + 1;
-            xs += WARPS * (2 * X_BYTES);
-            c = c2, e = e2;
-            now = next;
         }
         cp_wait<0>();
-    }
-    __syncthreads();
-    float* red = reinterpret_cast<float*>(smem);
-    reinterpret_cast<float4*>(red)[warp * 32 + lane] = make_float4(total[0], total[1], total[2], total[3]);
-    __syncthreads();
-    if (MODE == FEW_UP) {
-        // Eight inner activations in the operands' order, zeros behind the last.
-        const int e = id_of[blockIdx.y];
-        for (int v = threadIdx.x; v < 8 * pairs; v += blockDim.x) {
-            const int r = v & 7, i = v >> 3, t = i / p.top_k;
-            if (id_of[i] == e)
-                static_cast<T*>(p.h)[static_cast<int64_t>(i) * p.h_rs + blockIdx.x * 8 + paired(r)] =
-                    from_f32<T>(r < lo ? silu(joined(red, r, t)) * joined(red, r + 8, t) : 0.0f);
-        }
-    } else {
-        const int v = threadIdx.x, r = v & 15, t = v >> 4;
-        if (t < rows_x && row0 + r < p.n)
-            store_f32(p.y.p, (x0 + t) * p.y.rs + (row0 + r) * p.y.cs, p.y.type, joined(red, r, t));
+        __syncthreads();
     }
 }
 
-template <typename T, typename S, int SEG, int MODE, bool ANY>
-int launch_few(uor_b200_ctx* ctx, FewParams& p, bool after_up) {
+template <typename T, typename S, int SEG, int NT, bool ANY>
+int launch_few(uor_b200_ctx* ctx, FewParams& p, bool early) {
+    using B = Block<NT>;
     const int chunks = (p.w.cols + CHUNK - 1) / CHUNK;
-    const int rows_x = MODE == FEW_DENSE ? static_cast<int>(p.m < 8 ? p.m : 8) : p.tokens;
+    int64_t cols = p.kind == FEW_DENSE ? p.m : p.tokens;  // of a block, at most
+    if (cols > 8 * NT) cols = 8 * NT;
     p.group_shift = (p.w.group & (p.w.group - 1)) == 0 ? __builtin_ctz(p.w.group) : -1;
     constexpr int N = CHUNK / SEG;
     constexpr int VEC = N * sizeof(S) < 16 ? N * sizeof(S) : 16;
     p.quants_vec = p.w.group == SEG && (sizeof(S) == 2 || p.w.scale_type == UOR_B200_F32) &&
                    (reinterpret_cast<uint64_t>(p.w.scales) | static_cast<uint64_t>(p.w.groups_rs) * sizeof(S)) % VEC == 0 &&
                    (reinterpret_cast<uint64_t>(p.w.zeros) | (p.w.zeros ? static_cast<uint64_t>(p.w.groups_rs) : 0)) % N == 0;
-    int x_bytes = WARPS * STAGES * rows_x * 2 * X_BYTES;
-    if (MODE != FEW_DOWN) {
-        p.panel = X_MOST / (rows_x * 2 * X_BYTES);
-        if (p.panel > chunks) p.panel = chunks;
-        x_bytes = rows_x * p.panel * 2 * X_BYTES;
-    }
-    auto* kernel = few_kernel<T, S, SEG, MODE, ANY>;
-    constexpr int RINGS = WARPS * STAGES * stage_bytes<ANY>();
+    p.panel = static_cast<int>(B::X_MOST / (cols * 2 * X_BYTES));
+    if (p.panel > chunks) p.panel = chunks;
+    p.k_warps = B::WARPS;
+    while (p.k_warps > 1 && p.k_warps / 2 >= p.panel) p.k_warps /= 2;
+    constexpr int FIXED = B::WARPS * STAGES * stage_bytes<ANY>() + B::RED;
+    auto* kernel = few_kernel<T, S, SEG, NT, ANY>;
     static bool ready[64] = {};
     if (!ready[ctx->device & 63]) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, RINGS + X_MOST) != cudaSuccess)
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FIXED + B::X_MOST) != cudaSuccess)
             return UOR_B200_DEVICE_ERROR;
         ready[ctx->device & 63] = true;
     }
+    // Tiles are dealt to about as many blocks as run at one time.
+    const int rows = p.kind == FEW_UP ? 8 : ROWS, abreast = B::WARPS / p.k_warps;
+    const int64_t bundles = ((p.n + rows - 1) / rows + abreast - 1) / abreast;
+    int64_t across = p.kind == FEW_DENSE ? (p.m + 8 * NT - 1) / (8 * NT) : static_cast<int64_t>(p.tokens) * p.top_k;
+    if (p.kind != FEW_DENSE && across > p.experts) across = p.experts;
+    const int64_t resident = static_cast<int64_t>(ctx->sm_count) * (NT == 1 ? 3 : 1);
+    const int64_t each = (bundles * across + resident - 1) / resident;
     cudaLaunchConfig_t c = {};
-    c.blockDim = dim3(WARPS * 32);
-    c.dynamicSmemBytes = RINGS + x_bytes;
+    c.gridDim = dim3(static_cast<unsigned>((bundles + each - 1) / each), static_cast<unsigned>(across));
+    c.blockDim = dim3(B::THREADS);
+    c.dynamicSmemBytes = FIXED + cols * p.panel * 2 * X_BYTES;
     c.stream = ctx->stream;
-    if (MODE == FEW_DENSE)
-        c.gridDim = dim3((p.n + ROWS - 1) / ROWS, static_cast<unsigned>((p.m + 7) / 8));
-    else if (MODE == FEW_UP)
-        c.gridDim = dim3((p.n + 7) / 8, p.tokens * p.top_k);
-    else
-        c.gridDim = dim3((p.n + ROWS - 1) / ROWS);
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = &early;
-    c.numAttrs = after_up ? 1 : 0;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &attr;
+    c.numAttrs = early ? 1 : 0;
     return cuda_status(cudaLaunchKernelEx(&c, kernel, p));
-}
-
-template <typename T, typename S, int SEG, bool ANY>
-int by_mode(uor_b200_ctx* ctx, FewMode mode, FewParams& p, bool after_up) {
-    if (mode == FEW_UP) return launch_few<T, S, SEG, FEW_UP, ANY>(ctx, p, after_up);
-    if (mode == FEW_DOWN) return launch_few<T, S, SEG, FEW_DOWN, ANY>(ctx, p, after_up);
-    return launch_few<T, S, SEG, FEW_DENSE, ANY>(ctx, p, after_up);
 }
 
 // The segment is what one scale covers within 128 positions: the largest of 128, 64 and 32 that
 // divides the group.
-template <typename T, typename S, bool ANY>
-int by_segment(uor_b200_ctx* ctx, FewMode mode, FewParams& p, bool after_up) {
-    if (p.w.group % 128 == 0) return by_mode<T, S, 128, ANY>(ctx, mode, p, after_up);
-    if (p.w.group % 64 == 0) return by_mode<T, S, 64, ANY>(ctx, mode, p, after_up);
-    return by_mode<T, S, 32, ANY>(ctx, mode, p, after_up);
+template <typename T, typename S, int NT, bool ANY>
+int by_segment(uor_b200_ctx* ctx, FewParams& p, bool early) {
+    if (p.w.group % 128 == 0) return launch_few<T, S, 128, NT, ANY>(ctx, p, early);
+    if (p.w.group % 64 == 0) return launch_few<T, S, 64, NT, ANY>(ctx, p, early);
+    return launch_few<T, S, 32, NT, ANY>(ctx, p, early);
 }
 
-// Rows of codes that do not all begin at multiples of 16 bytes are copied by words and shifted
-// into place; scales that are neither float nor of the activations' type are converted as they
-// are read.
+// Eight columns, or sixteen where there are more rows than eight. Rows of codes that do not all
+// begin at multiples of 16 bytes are copied by words and shifted into place; scales that are
+// neither float nor of the activations' type are converted as they are read.
+template <typename T, typename S, bool ANY>
+int by_columns(uor_b200_ctx* ctx, FewParams& p, bool early) {
+    return (p.kind == FEW_DENSE ? p.m : p.tokens) > 8 ? by_segment<T, S, 2, ANY>(ctx, p, early) : by_segment<T, S, 1, ANY>(ctx, p, early);
+}
 template <typename T>
-int by_codes(uor_b200_ctx* ctx, int elem, FewMode mode, FewParams& p, bool after_up) {
-    if (p.codes_align != 16) return by_segment<T, float, true>(ctx, mode, p, after_up);
-    if (p.w.scale_type == elem) return by_segment<T, T, false>(ctx, mode, p, after_up);
-    return by_segment<T, float, false>(ctx, mode, p, after_up);
+int by_codes(uor_b200_ctx* ctx, int elem, FewParams& p, bool early) {
+    if (p.codes_align != 16) return by_columns<T, float, true>(ctx, p, early);
+    if (p.w.scale_type == elem) return by_columns<T, T, false>(ctx, p, early);
+    return by_columns<T, float, false>(ctx, p, early);
 }
 
 }  // namespace
 
-int few_launch(uor_b200_ctx* ctx, int elem, FewMode mode, FewParams p, bool after_up) {
-    return elem == UOR_B200_BF16 ? by_codes<__nv_bfloat16>(ctx, elem, mode, p, after_up) : by_codes<__half>(ctx, elem, mode, p, after_up);
+int few_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early) {
+    return elem == UOR_B200_BF16 ? by_codes<__nv_bfloat16>(ctx, elem, p, early) : by_codes<__half>(ctx, elem, p, early);
 }
 
 }  // namespace uor

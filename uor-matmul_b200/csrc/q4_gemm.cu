@@ -147,11 +147,13 @@ __global__ void add_parts_kernel(const float* part, int splits, int64_t rows, in
     }
 }
 
-// y[t][j] = the token's choices' products, each times its weight, in the choices' order.
-__global__ void combine_kernel(const float* part, int splits, const __grid_constant__ FfnArgs a) {
+// y[t][j] = the token's choices' products, each times its weight, in the choices' order. once: a
+// token's second choice of an expert has no product of its own, it is the first's.
+__global__ void combine_kernel(const float* part, int splits, bool once, const __grid_constant__ FfnArgs a) {
     const int j = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
     if (j >= a.d) return;
     const int64_t step = a.tokens * a.top_k;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     for (int64_t t = blockIdx.y; t < a.tokens; t += gridDim.y) {
         float v[4] = {0, 0, 0, 0};
 #pragma unroll 4
@@ -159,9 +161,13 @@ __global__ void combine_kernel(const float* part, int splits, const __grid_const
             const int e = static_cast<const int32_t*>(a.ids.p)[t * a.ids.rs + s * a.ids.cs];
             if (e < 0 || e >= a.experts) continue;
             const float w = static_cast<const float*>(a.weights.p)[t * a.weights.rs + s * a.weights.cs];
-            float4 sum = load4(part + (t * a.top_k + s) * a.d, j, a.d, a.d % 4 == 0);
+            int from = s;
+            if (once)
+                for (int o = s - 1; o >= 0; --o)
+                    if (static_cast<const int32_t*>(a.ids.p)[t * a.ids.rs + o * a.ids.cs] == e) from = o;
+            float4 sum = load4(part + (t * a.top_k + from) * a.d, j, a.d, a.d % 4 == 0);
             for (int c = 1; c < splits; ++c) {
-                const float4 more = load4(part + (c * step + t * a.top_k + s) * a.d, j, a.d, a.d % 4 == 0);
+                const float4 more = load4(part + (c * step + t * a.top_k + from) * a.d, j, a.d, a.d % 4 == 0);
                 sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
             }
             v[0] = fmaf(w, sum.x, v[0]), v[1] = fmaf(w, sum.y, v[1]), v[2] = fmaf(w, sum.z, v[2]), v[3] = fmaf(w, sum.w, v[3]);
@@ -226,6 +232,27 @@ void few_align(FewParams* p) {
     p->x_vec = rows_aligned(p->x, p->x_rs * 2);
 }
 
+// few: after the few-rows kernel, which wrote a token's products with an expert once; the launch may
+// begin while that one still runs.
+int launch_combine(uor_b200_ctx* ctx, const float* part, int splits, const FfnArgs& a, bool few) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = blocks_of_rows(a.tokens, a.d);
+    c.blockDim = dim3(THREADS);
+    c.stream = ctx->stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &attr;
+    c.numAttrs = few ? 1 : 0;
+    return cuda_status(cudaLaunchKernelEx(&c, combine_kernel, part, splits, few, a));
+}
+
+// Few pairs to an expert: reading every chosen expert's weights is then most of the work, and the
+// few-rows kernel reads them as they lie, without sorting rows and laying codes out first.
+bool few_experts(const FfnArgs& a) {
+    return a.tokens <= 16 || a.tokens * a.top_k <= 12 * static_cast<int64_t>(a.experts);
+}
+
 int zeros_out(uor_b200_ctx* ctx, int64_t rows, int n, const MatOut& y) {
     add_parts_kernel<<<blocks_of_rows(rows, n), THREADS, 0, ctx->stream>>>(nullptr, 0, rows, n, y);
     return cuda_status(cudaGetLastError());
@@ -238,7 +265,7 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     route->kernel = UOR_B200_KERNEL_Q4;
     if (w.cols == 0) return zeros_out(ctx, m, w.rows, y);
     int st = UOR_B200_OK;
-    const bool few = m <= FEW_MAX_TOKENS;
+    const bool few = m <= 16;
     Pieces pieces;
     // The few-rows kernel reads any row whose elements follow one another.
     const bool own_rows = few ? x.cs != 1 : !x_in_place(x, w.cols);
@@ -263,6 +290,7 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     }
     if (few) {
         FewParams p{};
+        p.kind = FEW_DENSE;
         p.w = w;
         p.x = rows.p;
         p.x_rs = rows.rs;
@@ -270,8 +298,8 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
         p.n = w.rows;
         p.y = y;
         few_align(&p);
-        route->tile_m = 16, route->tile_n = 8, route->tile_k = 256;
-        return few_launch(ctx, elem, FEW_DENSE, p, false);
+        route->tile_m = 16, route->tile_n = m > 8 ? 16 : 8, route->tile_k = 256;
+        return few_launch(ctx, elem, p, false);
     }
     copy_codes(ctx, &many.w, ws + codes_at);
     many.x = rows.p;
@@ -296,11 +324,13 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     const int h_rs = up_to(a.f, 8), x_rs = up_to(a.d, 8);
     Pieces pieces;
     const size_t h_at = pieces.add(static_cast<size_t>(pairs) * h_rs * 2);
-    if (a.tokens <= FEW_MAX_TOKENS && pairs <= FEW_MAX_PAIRS) {
+    if (pairs <= FEW_MAX_PAIRS && few_experts(a)) {
         const size_t x_at = pieces.add(a.x.cs == 1 ? 0 : static_cast<size_t>(a.tokens) * x_rs * 2);
+        const size_t part_at = pieces.add(static_cast<size_t>(pairs) * a.d * 4);
         uint8_t* ws = pieces.get(ctx, &st);
         if (!ws) return st;
         FewParams p{};
+        p.kind = FEW_UP;
         p.h = ws + h_at;
         p.h_rs = h_rs;
         p.w = a.up;
@@ -313,20 +343,21 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
         }
         p.n = a.f;
         p.ids = a.ids;
-        p.weights = a.weights;
         p.tokens = static_cast<int>(a.tokens);
         p.top_k = a.top_k;
         p.experts = a.experts;
         few_align(&p);
-        route->tile_m = 16, route->tile_n = 8, route->tile_k = 256;
-        if ((st = few_launch(ctx, a.elem, FEW_UP, p, false))) return st;
+        route->tile_m = 16, route->tile_n = a.tokens > 8 ? 16 : 8, route->tile_k = 256;
+        if ((st = few_launch(ctx, a.elem, p, false))) return st;
+        p.kind = FEW_PART;
         p.w = a.down;
         p.x = p.h;
         p.x_rs = h_rs;
         p.n = a.d;
-        p.y = a.y;
+        p.part = reinterpret_cast<float*>(ws + part_at);
         few_align(&p);
-        return few_launch(ctx, a.elem, FEW_DOWN, p, true);
+        if ((st = few_launch(ctx, a.elem, p, true))) return st;
+        return launch_combine(ctx, p.part, 1, a, true);
     }
 
     ManyParams up{};
@@ -364,8 +395,7 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     down.part = reinterpret_cast<float*>(ws + part_at);
     route->tile_m = 256, route->tile_n = 256, route->tile_k = 64;
     if ((st = many_launch(ctx, a.elem, up)) || (st = many_launch(ctx, a.elem, down))) return st;
-    combine_kernel<<<blocks_of_rows(a.tokens, a.d), THREADS, 0, ctx->stream>>>(down.part, splits, a);
-    return cuda_status(cudaGetLastError());
+    return launch_combine(ctx, down.part, splits, a, false);
 }
 
 }  // namespace uor
