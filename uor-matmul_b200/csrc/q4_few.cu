@@ -26,21 +26,16 @@
 // its columns are these pairs' activation rows.
 #include "q4_few.cuh"
 
-#include <type_traits>
-
 #include "ptx.cuh"
+#include "q4_mma.cuh"
 
 namespace uor {
 
 namespace {
 
 constexpr int STAGES = 2;
-constexpr int ROWS = 16;
-constexpr int SUB = 128;                       // positions of the reduction in 64 bytes of a row
-constexpr int CHUNK = 2 * SUB;                 // positions per ring stage
 constexpr int HALF_BYTES = ROWS * SUB / 2;     // of a stage's codes, per SUB
 constexpr int PITCH_ANY = 144;                 // of a row's codes whose addresses are not aligned
-constexpr int X_BYTES = SUB * 2;               // of a SUB, per activation row
 
 template <bool ANY>
 constexpr int stage_bytes() {
@@ -59,217 +54,11 @@ __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
-    return r;
-}
-
-// A word's eight codes less their zero point, as pairs of 16-bit floats: positions (0, 4),
-// (1, 5), (2, 6), (3, 7).
-template <typename T>
-struct Decode;
-template <>
-struct Decode<__nv_bfloat16> {
-    // 128 + code, less 128 + zero.
-    struct Zero {
-        __nv_bfloat162 v;
-    };
-    static constexpr uint32_t ZERO_8 = 0x43084308u;
-    // Of byte i of a word of zero points.
-    __device__ static __forceinline__ uint32_t zero_bits(uint32_t w, int i) { return __byte_perm(w, 0x43, 0x4040 + 0x101 * i); }
-    __device__ static __forceinline__ Zero zero(uint32_t b) {
-        Zero r;
-        memcpy(&r.v, &b, 4);
-        return r;
-    }
-    __device__ static __forceinline__ uint32_t one(uint32_t w, const Zero& z) {
-        const uint32_t b = and_or(w, 0x000F000Fu, 0x43004300u);
-        __nv_bfloat162 v;
-        memcpy(&v, &b, 4);
-        v = __hsub2(v, z.v);
-        uint32_t r;
-        memcpy(&r, &v, 4);
-        return r;
-    }
-    __device__ static __forceinline__ void unpack(uint32_t w, const Zero& z, uint32_t& p0, uint32_t& p1, uint32_t& p2,
-                                                  uint32_t& p3) {
-        p0 = one(w, z), p1 = one(w >> 4, z), p2 = one(w >> 8, z), p3 = one(w >> 12, z);
-    }
-    __device__ static __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-template <>
-struct Decode<__half> {
-    // 1024 + code, less 1024 + zero; and, of the nibble above it, (1024 + 16 code) / 16 less
-    // 64 + zero, which spares the shift.
-    struct Zero {
-        __half2 low, high;
-    };
-    static constexpr uint32_t ZERO_8 = 0x64086408u;
-    __device__ static __forceinline__ uint32_t zero_bits(uint32_t w, int i) { return __byte_perm(w, 0x64, 0x4040 + 0x101 * i); }
-    __device__ static __forceinline__ Zero zero(uint32_t b) {
-        Zero r;
-        memcpy(&r.low, &b, 4);
-        r.high = __hsub2(__float2half2_rn(960.0f), r.low);  // -(64 + zero)
-        return r;
-    }
-    __device__ static __forceinline__ uint32_t low(uint32_t w, const Zero& z) {
-        const uint32_t b = and_or(w, 0x000F000Fu, 0x64006400u);
-        __half2 v;
-        memcpy(&v, &b, 4);
-        v = __hsub2(v, z.low);
-        uint32_t r;
-        memcpy(&r, &v, 4);
-        return r;
-    }
-    __device__ static __forceinline__ uint32_t high(uint32_t w, const Zero& z) {
-        const uint32_t b = and_or(w, 0x00F000F0u, 0x64006400u);
-        __half2 v;
-        memcpy(&v, &b, 4);
-        v = __hfma2(v, __float2half2_rn(0.0625f), z.high);
-        uint32_t r;
-        memcpy(&r, &v, 4);
-        return r;
-    }
-    __device__ static __forceinline__ void unpack(uint32_t w, const Zero& z, uint32_t& p0, uint32_t& p1, uint32_t& p2,
-                                                  uint32_t& p3) {
-        p0 = low(w, z), p1 = high(w, z), p2 = low(w >> 8, z), p3 = high(w >> 8, z);
-    }
-    __device__ static __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    }
-};
-
 // Where 16-byte piece c of a row's 64 bytes of codes lies: eight rows' reads of any width meet no
 // bank twice.
 __device__ __forceinline__ int code_at(int row, int c) {
     return row * 64 + ((c ^ ((row & 2) | ((row >> 2) & 1))) << 4);
 }
-// The same for 16-byte piece p of an activation row's 256 bytes of a chunk, read by lane c of
-// segment s as piece 4 c + j (SEG 128), 8 s + 2 c + j (64) or 4 s + c (32).
-template <int SEG>
-__device__ __forceinline__ int x_piece(int row, int p) {
-    const int odd = row & 1;
-    return (SEG == 128 ? p ^ ((p >> 2) & 2) ^ odd : SEG == 64 ? p ^ odd : p ^ (odd << 2)) << 4;
-}
-
-// Eight activations from positions k .. k + 7 of a row, `left` of them existing.
-template <typename T>
-__device__ __forceinline__ uint4 load_x8(const T* p, int left, bool vec) {
-    if (vec && left >= 8) return *reinterpret_cast<const uint4*>(p);
-    uint32_t w[4] = {0, 0, 0, 0};
-    const uint16_t* s = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-    for (int b = 0; b < 8; ++b)
-        if (b < left) w[b >> 1] |= static_cast<uint32_t>(s[b]) << (16 * (b & 1));
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-// The same in the order of the operands.
-__device__ __forceinline__ uint4 in_pairs(uint4 w) {
-    return make_uint4(__byte_perm(w.x, w.z, 0x5410), __byte_perm(w.x, w.z, 0x7632), __byte_perm(w.y, w.w, 0x5410),
-                      __byte_perm(w.y, w.w, 0x7632));
-}
-
-// Reads of shared memory at its 32-bit addresses, as loads the compiler may order by itself.
-template <typename V>
-__device__ __forceinline__ V lds(uint32_t at) {
-    return *static_cast<const V*>(__cvta_shared_to_generic(at));
-}
-
-__device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-
-// The scales and zero points of a chunk for this lane's two rows (lane / 4 of each half of the
-// tile), as they lie in memory. S: T where the scales are of that type, float otherwise.
-template <typename T, typename S, int SEG>
-struct Quants {
-    static constexpr int N = CHUNK / SEG;
-    static constexpr int SW = N * sizeof(S) / 4, ZW = (N + 3) / 4;
-    uint32_t s[2][SW], z[2][ZW];
-
-    template <int WORDS>
-    __device__ static __forceinline__ void copy(uint32_t (&to)[WORDS], const void* from) {
-        if constexpr (WORDS % 4 == 0) {
-#pragma unroll
-            for (int i = 0; i < WORDS; i += 4) {
-                const uint4 v = static_cast<const uint4*>(from)[i / 4];
-                to[i] = v.x, to[i + 1] = v.y, to[i + 2] = v.z, to[i + 3] = v.w;
-            }
-        } else if constexpr (WORDS == 2) {
-            const uint2 v = *static_cast<const uint2*>(from);
-            to[0] = v.x, to[1] = v.y;
-        } else {
-            to[0] = *static_cast<const uint32_t*>(from);
-        }
-    }
-
-    // row0, row1: scale indexes of the rows' first groups. Where every row's scales begin at a
-    // multiple of a chunk's and a group is a segment, a chunk's are one vector.
-    __device__ __forceinline__ void load(const FewParams& p, int64_t row0, int64_t row1, int chunk, int groups) {
-        if (p.quants_vec && (chunk + 1) * N <= groups) {
-            copy(s[0], static_cast<const S*>(p.w.scales) + row0 + chunk * N);
-            copy(s[1], static_cast<const S*>(p.w.scales) + row1 + chunk * N);
-            if (p.w.zeros) {
-                if constexpr (N == 2) {
-                    z[0][0] = *reinterpret_cast<const uint16_t*>(p.w.zeros + row0 + chunk * N);
-                    z[1][0] = *reinterpret_cast<const uint16_t*>(p.w.zeros + row1 + chunk * N);
-                } else {
-                    copy(z[0], p.w.zeros + row0 + chunk * N);
-                    copy(z[1], p.w.zeros + row1 + chunk * N);
-                }
-            }
-            return;
-        }
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-#pragma unroll
-            for (int i = 0; i < ZW; ++i) z[v][i] = 0;
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int at = chunk * CHUNK + i * SEG;
-                const int64_t q = (v ? row1 : row0) + min(p.group_shift >= 0 ? at >> p.group_shift : at / p.w.group, groups - 1);
-                if constexpr (sizeof(S) == 4) {
-                    s[v][i] = __float_as_uint(load_f32(p.w.scales, q, p.w.scale_type));
-                } else {
-                    const uint32_t raw = static_cast<const uint16_t*>(p.w.scales)[q];
-                    s[v][i / 2] = i & 1 ? s[v][i / 2] | raw << 16 : raw;
-                }
-                if (p.w.zeros) z[v][i / 4] |= static_cast<uint32_t>(p.w.zeros[q]) << (8 * (i & 3));
-            }
-        }
-    }
-    __device__ __forceinline__ float scale(int v, int i) const {
-        if constexpr (sizeof(S) == 4) return __uint_as_float(s[v][i]);
-        if constexpr (std::is_same<S, __nv_bfloat16>::value)
-            return __uint_as_float(i & 1 ? s[v][i / 2] & 0xFFFF0000u : s[v][i / 2] << 16);
-        else
-            return __half2float(__ushort_as_half(static_cast<unsigned short>(i & 1 ? s[v][i / 2] >> 16 : s[v][i / 2])));
-    }
-    __device__ __forceinline__ uint32_t zero(int v, int i, bool given) const {
-        return given ? Decode<T>::zero_bits(z[v][i / 4] & 0x0F0F0F0Fu, i & 3) : Decode<T>::ZERO_8;
-    }
-};
-
-// A tile of weights: its rows r are row0 + r (half 8), or eight rows from row0 on and eight from
-// row0 + half on; `lo` and `hi` of the halves' rows are valid, and the last valid one stands in for
-// those past it.
-struct Tile {
-    int64_t row0, half;
-    int lo, hi;
-    __device__ __forceinline__ int64_t row(int r) const {
-        return r < 8 ? row0 + min(r, lo - 1) : row0 + half + min(r - 8, hi - 1);
-    }
-};
-
 // One warp's ring of chunks of codes.
 template <typename T, typename S, int SEG, bool ANY>
 struct Ring {
@@ -382,27 +171,13 @@ struct Ring {
     }
 };
 
-// An activation's place among its eight in the operands' order.
-__device__ __forceinline__ int paired(int r) { return r < 4 ? 2 * r : 2 * r - 7; }
-
-// NT: columns in eights. A block has 8 warps a column eight.
-template <int NT>
-struct Block {
-    static constexpr int WARPS = 8 * NT, THREADS = 32 * WARPS;
-    static constexpr int RED = 2 * WARPS * NT * 128 * 4;  // joined sums, twice
-    static constexpr int X_MOST = NT == 1 ? 64 * 1024 : 112 * 1024;  // resident activations
-};
-
 template <typename T, typename S, int SEG, int NT, bool ANY>
 __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kernel(const __grid_constant__ FewParams p) {
     constexpr int WARPS = Block<NT>::WARPS, THREADS = Block<NT>::THREADS, COLS = 8 * NT;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint32_t bits[FEW_MAX_EXPERTS / 32];  // the chosen experts
-    __shared__ uint16_t id_of[FEW_MAX_PAIRS], list[FEW_MAX_PAIRS];  // the pairs' experts; this one's pairs
-    __shared__ int counts[WARPS], chosen;
+    __shared__ Found found;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int chunks = (p.w.cols + CHUNK - 1) / CHUNK;
-    const int kind = p.kind;
+    const int chunks = p.chunks, kind = p.kind;
     if (kind != FEW_DENSE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // The columns: activation rows from x0 on, or of the listed pairs of expert e.
@@ -412,94 +187,22 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
         x0 = static_cast<int64_t>(blockIdx.y) * COLS;
         listed = static_cast<int>(min(static_cast<int64_t>(COLS), p.m - x0));
     } else {
-        // CTA y takes the y-th of the chosen experts.
-        const int pairs = p.tokens * p.top_k;
-        if (threadIdx.x < FEW_MAX_EXPERTS / 32) bits[threadIdx.x] = 0;
-        if (threadIdx.x == 0) chosen = -1;
-        __syncthreads();
-        for (int i = threadIdx.x; i < pairs; i += THREADS) {
-            const int t = i / p.top_k;
-            const int id = static_cast<const int32_t*>(p.ids.p)[t * p.ids.rs + (i - t * p.top_k) * p.ids.cs];
-            const bool in = id >= 0 && id < p.experts;
-            id_of[i] = in ? static_cast<uint16_t>(id) : 0xFFFF;
-            if (in) atomicOr(&bits[id >> 5], 1u << (id & 31));
-        }
-        __syncthreads();
-        if (warp == 0) {
-            const uint32_t w = bits[lane];
-            int before = __popc(w);
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, before, o);
-                if (lane >= o) before += v;
-            }
-            before -= __popc(w);
-            const int nth = static_cast<int>(blockIdx.y) - before;
-            if (nth >= 0 && nth < __popc(w)) {
-                uint32_t left = w;
-                for (int b = 0; b < nth; ++b) left &= left - 1;
-                chosen = lane * 32 + __ffs(left) - 1;
-            }
-        }
-        __syncthreads();
-        e = chosen;
-        if (e < 0) return;
-        // its pairs, in order: a run of pairs to a thread. A token that chose it more than once is
-        // there with its first choice alone, so there are at most as many columns as tokens.
-        auto lists = [&](int i) {
-            if (id_of[i] != e) return false;
-            for (int o = i - i % p.top_k; o < i; ++o)
-                if (id_of[o] == e) return false;
-            return true;
-        };
-        const int run = (pairs + THREADS - 1) / THREADS, from = min(pairs, static_cast<int>(threadIdx.x) * run);
-        const int to = min(pairs, from + run);
-        int mine = 0;
-        for (int i = from; i < to; ++i) mine += lists(i);
-        int upto = mine;
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += v;
-        }
-        if (lane == 31) counts[warp] = upto;
-        __syncthreads();
-        int at = upto - mine;
-        for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) at += counts[w];
-            listed += counts[w];
-        }
-        for (int i = from; i < to; ++i)
-            if (lists(i)) list[at++] = static_cast<uint16_t>(i);
-        __syncthreads();
+        listed = find_pairs<WARPS>(p, found);
+        if (listed < 0) return;
+        e = found.chosen;
     }
 
     // `kw` warps share a tile's reduction, so WARPS / kw tiles are under way at once.
-    const int kw = p.k_warps, k_warp = warp & (kw - 1), t_warp = warp / kw, abreast = WARPS / kw;
-    const int rows = kind == FEW_UP ? 8 : ROWS;  // outputs of a tile
-    const int tiles = (p.n + rows - 1) / rows;
-    auto tile_at = [&](int t) {
-        t = min(t, tiles - 1);
-        Tile w;
-        if (kind == FEW_UP) {
-            w.row0 = static_cast<int64_t>(e) * 2 * p.n + t * 8;
-            w.half = p.n;
-            w.lo = w.hi = min(8, p.n - t * 8);
-        } else {
-            const int left = p.n - t * ROWS;
-            w.row0 = static_cast<int64_t>(e) * p.n + t * ROWS;
-            w.half = left > 8 ? 8 : 0;  // no second half: the first row stands in
-            w.lo = min(8, left);
-            w.hi = max(1, min(8, left - 8));
-        }
-        return w;
-    };
+    const int kw = 1 << p.k_shift, k_warp = warp & (kw - 1), t_warp = warp >> p.k_shift, abreast = WARPS >> p.k_shift;
+    const int tiles = p.tiles;
     Ring<T, S, SEG, ANY> ring;
     ring.base = smem_u32(smem) + warp * (STAGES * stage_bytes<ANY>());
     ring.row_len = (p.w.cols + 1) / 2;
     float* red = reinterpret_cast<float*>(smem + WARPS * STAGES * stage_bytes<ANY>());
     const uint32_t x_all = smem_u32(smem) + WARPS * STAGES * stage_bytes<ANY>() + Block<NT>::RED;
-    const int groups = (p.w.cols + p.w.group - 1) / p.w.group;
+    const int groups = p.groups;
     const bool zeros = p.w.zeros != nullptr;
-    const int panel = p.panel, panels = (chunks + panel - 1) / panel;  // chunks whose activations are resident
+    const int panel = p.panel, panels = p.panels;  // chunks whose activations are resident
     const int tile_step = gridDim.x * abreast;
     bool waited = kind != FEW_PART;
 
@@ -516,7 +219,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
                 if (++lpanel == panels) {
                     lpanel = 0;
                     lt += tile_step;
-                    if (lt < tiles) ring.set(p, lane, tile_at(lt));
+                    if (lt < tiles) ring.set(p, lane, tile_at(p, e, lt));
                 }
                 lc = lpanel * panel + k_warp;
             }
@@ -530,7 +233,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
             lstage = lstage + 1 == STAGES ? 0 : lstage + 1;
             cp_commit();
         };
-        if (lt < tiles) ring.set(p, lane, tile_at(lt));
+        if (lt < tiles) ring.set(p, lane, tile_at(p, e, lt));
         settle();
         // The weights depend on nothing before this launch; the inner activations do.
 #pragma unroll
@@ -540,7 +243,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
         int stage = 0;
         for (int t0 = blockIdx.x * abreast; t0 < tiles; t0 += tile_step) {
             const int t = t0 + t_warp;
-            const Tile tile = tile_at(t);
+            const Tile tile = tile_at(p, e, t);
             const int64_t r0 = tile.row(lane >> 2), r1 = tile.row((lane >> 2) + 8);
             const int64_t quants0 = r0 * p.w.groups_rs, quants1 = r1 * p.w.groups_rs;
             int m0 = 0, m1 = 0;
@@ -553,7 +256,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
             for (int n = 0; n < NT; ++n) total[n][0] = total[n][1] = total[n][2] = total[n][3] = 0;
             for (int pn = 0; pn < panels; ++pn) {
                 const int first = pn * panel, last = min(chunks, first + panel);
-                const int units = t < tiles && last - first > k_warp ? (last - first - k_warp + kw - 1) / kw : 0;
+                const int units = t < tiles && last - first > k_warp ? (last - first - k_warp + kw - 1) >> p.k_shift : 0;
                 Quants<T, S, SEG> now, next;
                 if (units) now.load(p, quants0, quants1, first + k_warp, groups);
                 if (panels > 1 || t0 == static_cast<int>(blockIdx.x) * abreast) {
@@ -565,7 +268,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
                         for (int b = 0; b < 4; ++b) {
                             const int v = min(v0 + b * THREADS, rows_x * pieces - 1);
                             const int r = rows_x == 1 ? 0 : v / pieces, k = first * CHUNK + (v - r * pieces) * 8;
-                            const int64_t row = kind == FEW_DENSE ? x0 + r : kind == FEW_UP ? list[c0 + r] / p.top_k : list[c0 + r];
+                            const int64_t row = kind == FEW_DENSE ? x0 + r : kind == FEW_UP ? found.list[c0 + r] / p.top_k : found.list[c0 + r];
                             // rows of inner activations end in whole eights
                             const int left = kind == FEW_PART ? (k < p.x_rs ? 8 : 0) : p.w.cols - k;
                             x8[b] = load_x8(static_cast<const T*>(p.x) + row * p.x_rs + (left > 0 ? k : 0), left, p.x_vec != 0);
@@ -591,6 +294,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
                     load();
                     if (i + 1 < units) next.load(p, quants0, quants1, c + kw, groups);
                     const int left = p.w.cols - c * CHUNK;
+                    now.mask();
                     ring.compute(stage, 0, lane, now, zeros, m0, m1, xs, x_row, left, total);
                     if (left > SUB) ring.compute(stage, 1, lane, now, zeros, m0, m1, xs, x_row, left - SUB, total);
                     stage = stage + 1 == STAGES ? 0 : stage + 1;
@@ -606,27 +310,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
             for (int n = 0; n < NT; ++n)
                 reinterpret_cast<float4*>(joined)[(warp * NT + n) * 32 + lane] = make_float4(total[n][0], total[n][1], total[n][2], total[n][3]);
             __syncthreads();
-            for (int v = threadIdx.x; v < abreast * rows * rows_x; v += THREADS) {
-                const int r = v & (rows - 1), rest = v / rows, ab = rest % abreast, col = rest / abreast;
-                const int out = (t0 + ab) * rows + r;
-                auto sum = [&](int row) {
-                    const float* at = joined + (ab * kw * NT + (col >> 3)) * 128 + ((row & 7) * 4 + ((col & 7) >> 1)) * 4 + (row >> 3) * 2 + (col & 1);
-                    float s = 0;
-                    for (int w = 0; w < kw; ++w) s += at[w * NT * 128];
-                    return s;
-                };
-                if (kind == FEW_UP) {
-                    // eight inner activations in the operands' order, zeros behind the last
-                    if (t0 + ab < tiles)
-                        static_cast<T*>(p.h)[static_cast<int64_t>(list[c0 + col]) * p.h_rs + (t0 + ab) * 8 + paired(r)] =
-                            from_f32<T>(out < p.n ? silu(sum(r)) * sum(r + 8) : 0.0f);
-                } else if (out < p.n) {
-                    if (kind == FEW_PART)
-                        p.part[static_cast<int64_t>(list[c0 + col]) * p.n + out] = sum(r);
-                    else
-                        store_f32(p.y.p, (x0 + col) * p.y.rs + out * p.y.cs, p.y.type, sum(r));
-                }
-            }
+            tiles_out<T, NT>(p, found, joined, e, t0, c0, rows_x, x0);
         }
         cp_wait<0>();
         __syncthreads();
@@ -636,7 +320,8 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
 template <typename T, typename S, int SEG, int NT, bool ANY>
 int launch_few(uor_b200_ctx* ctx, FewParams& p, bool early) {
     using B = Block<NT>;
-    const int chunks = (p.w.cols + CHUNK - 1) / CHUNK;
+    const int chunks = p.chunks = (p.w.cols + CHUNK - 1) / CHUNK;
+    p.groups = (p.w.cols + p.w.group - 1) / p.w.group;
     int64_t cols = p.kind == FEW_DENSE ? p.m : p.tokens;  // of a block, at most
     if (cols > 8 * NT) cols = 8 * NT;
     p.group_shift = (p.w.group & (p.w.group - 1)) == 0 ? __builtin_ctz(p.w.group) : -1;
@@ -647,8 +332,9 @@ int launch_few(uor_b200_ctx* ctx, FewParams& p, bool early) {
                    (reinterpret_cast<uint64_t>(p.w.zeros) | (p.w.zeros ? static_cast<uint64_t>(p.w.groups_rs) : 0)) % N == 0;
     p.panel = static_cast<int>(B::X_MOST / (cols * 2 * X_BYTES));
     if (p.panel > chunks) p.panel = chunks;
-    p.k_warps = B::WARPS;
-    while (p.k_warps > 1 && p.k_warps / 2 >= p.panel) p.k_warps /= 2;
+    p.panels = (chunks + p.panel - 1) / p.panel;
+    p.k_shift = __builtin_ctz(B::WARPS);
+    while (p.k_shift > 0 && 1 << (p.k_shift - 1) >= p.panel) --p.k_shift;
     constexpr int FIXED = B::WARPS * STAGES * stage_bytes<ANY>() + B::RED;
     auto* kernel = few_kernel<T, S, SEG, NT, ANY>;
     static bool ready[64] = {};
@@ -658,8 +344,9 @@ int launch_few(uor_b200_ctx* ctx, FewParams& p, bool early) {
         ready[ctx->device & 63] = true;
     }
     // Tiles are dealt to about as many blocks as run at one time.
-    const int rows = p.kind == FEW_UP ? 8 : ROWS, abreast = B::WARPS / p.k_warps;
-    const int64_t bundles = ((p.n + rows - 1) / rows + abreast - 1) / abreast;
+    const int rows = p.kind == FEW_UP ? 8 : ROWS, abreast = B::WARPS >> p.k_shift;
+    p.tiles = (p.n + rows - 1) / rows;
+    const int64_t bundles = (p.tiles + abreast - 1) / abreast;
     int64_t across = p.kind == FEW_DENSE ? (p.m + 8 * NT - 1) / (8 * NT) : static_cast<int64_t>(p.tokens) * p.top_k;
     if (p.kind != FEW_DENSE && across > p.experts) across = p.experts;
     const int64_t resident = static_cast<int64_t>(ctx->sm_count) * (NT == 1 ? 3 : 1);
@@ -703,6 +390,8 @@ int by_codes(uor_b200_ctx* ctx, int elem, FewParams& p, bool early) {
 }  // namespace
 
 int few_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early) {
+    int st = UOR_B200_OK;
+    if (lean_launch(ctx, elem, p, early, &st)) return st;
     return elem == UOR_B200_BF16 ? by_codes<__nv_bfloat16>(ctx, elem, p, early) : by_codes<__half>(ctx, elem, p, early);
 }
 

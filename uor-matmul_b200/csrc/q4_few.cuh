@@ -31,7 +31,8 @@ struct FewParams {
     int x_vec;           // rows of x begin at multiples of 16 bytes
     // Set by the launch:
     int panel;           // chunks whose activations are resident
-    int k_warps;         // warps that share a tile's reduction, a power of two
+    int k_shift;         // log2 of the warps that share a tile's reduction
+    int chunks, panels, groups, tiles;
     int group_shift;     // log2 of the group, or -1
     int quants_vec;      // a chunk's scales, and its zero points, are one vector each
 };
@@ -39,5 +40,8 @@ struct FewParams {
 // early: the launch may begin while the one before it runs; it reads what that wrote (the inner
 // activations) only after its end.
 int few_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early);
+
+// The same for what lies well (q4_lean.cu): whether it does, and then the launch's status.
+bool lean_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early, int* status);
 
 }  // namespace uor

@@ -1,0 +1,294 @@
+// q4_lean.cu -- products of few rows with 4-bit weights that lie well: rows of codes at multiples of
+// 16 bytes, a group of 32, 64 or 128 positions, scales that are read as vectors, activations that
+// fit in a block's shared memory.
+//
+// q4_few.cu's product and its split, but for the way of the codes: each lane reads its operands'
+// words straight from memory into registers, one chunk ahead, so that there are no copies to
+// place, to wait for and to read back. Instructions are what bounds these products beside the
+// memory (an operand's word takes 11 to unpack), and so are the few microseconds of a launch:
+// activations are asked for first, and nothing is divided on the device.
+#include "ptx.cuh"
+#include "q4_mma.cuh"
+
+namespace uor {
+
+namespace {
+
+// A chunk's codes of this lane's two rows: word SEG / 32 s + j is the j-th of segment s.
+template <int SEG>
+struct Codes {
+    static constexpr int WORDS = SEG / 32, SEGS = CHUNK / SEG;
+    uint32_t w[2][8];
+
+    // at0, at1: the chunk's rows at this lane's first word; bytes: what is left of a row from there.
+    __device__ __forceinline__ void load(const uint8_t* at0, const uint8_t* at1, int bytes, int c) {
+        if (bytes >= CHUNK / 2) {
+            read<false>(w[0], at0, bytes, c);
+            read<false>(w[1], at1, bytes, c);
+        } else {
+            read<true>(w[0], at0, bytes, c);
+            read<true>(w[1], at1, bytes, c);
+        }
+    }
+    template <bool TAIL>
+    __device__ static __forceinline__ void read(uint32_t (&w)[8], const uint8_t* at, int bytes, int c) {
+#pragma unroll
+        for (int s = 0; s < SEGS; ++s) {
+            const uint8_t* from = at + s * (SEG / 2);
+            uint32_t* to = w + s * WORDS;
+            if (TAIL && s * (SEG / 2) + c * 4 * WORDS >= bytes) {
+#pragma unroll
+                for (int j = 0; j < WORDS; ++j) to[j] = 0;
+            } else if constexpr (WORDS == 4) {
+                const uint4 x = __ldg(reinterpret_cast<const uint4*>(from));
+                to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
+            } else if constexpr (WORDS == 2) {
+                const uint2 x = __ldg(reinterpret_cast<const uint2*>(from));
+                to[0] = x.x, to[1] = x.y;
+            } else {
+                to[0] = __ldg(reinterpret_cast<const uint32_t*>(from));
+            }
+        }
+    }
+};
+
+template <typename T, typename S, int SEG, int NT>
+__global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kernel(const __grid_constant__ FewParams p) {
+    constexpr int WARPS = Block<NT>::WARPS, THREADS = Block<NT>::THREADS, COLS = 8 * NT;
+    constexpr int WORDS = SEG / 32, SEGS = CHUNK / SEG;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Found found;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int kind = p.kind, chunks = p.chunks;
+    if (kind != FEW_DENSE) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    int e = 0, listed;
+    int64_t x0 = 0;
+    if (kind == FEW_DENSE) {
+        x0 = static_cast<int64_t>(blockIdx.y) * COLS;
+        listed = static_cast<int>(min(static_cast<int64_t>(COLS), p.m - x0));
+    } else {
+        listed = find_pairs<WARPS>(p, found);
+        if (listed < 0) return;
+        e = found.chosen;
+    }
+    const int kw = 1 << p.k_shift, k_warp = warp & (kw - 1), t_warp = warp >> p.k_shift, abreast = WARPS >> p.k_shift;
+    float* red = reinterpret_cast<float*>(smem);
+    const uint32_t x_all = smem_u32(smem) + Block<NT>::RED;
+    const bool zeros = p.w.zeros != nullptr;
+    const int row_len = p.w.cols / 2, tile_step = gridDim.x * abreast;
+    const int units = chunks > k_warp ? (chunks - k_warp + kw - 1) >> p.k_shift : 0;  // chunks of a tile for this warp
+    bool waited = kind != FEW_PART;
+
+    for (int c0 = 0; c0 < listed; c0 += COLS) {
+        const int rows_x = min(COLS, listed - c0), pieces = chunks * 32;
+        auto x_at = [&](int v) {  // 16-byte piece v of the activations
+            const int r = rows_x == 1 ? 0 : v / pieces, k = (v - r * pieces) * 8;
+            const int64_t row = kind == FEW_DENSE ? x0 + r : kind == FEW_UP ? found.list[c0 + r] / p.top_k : found.list[c0 + r];
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (k < p.w.cols) x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row * p.x_rs + k);
+            return x;
+        };
+        auto x_put = [&](int v, uint4 x) {
+            const int r = rows_x == 1 ? 0 : v / pieces, piece = v - r * pieces;
+            sts128(x_all + (r * chunks * 2 + (piece >> 4)) * X_BYTES + x_piece<SEG>(r, piece & 15), kind == FEW_PART ? x : in_pairs(x));
+        };
+        const int total_x = rows_x * pieces;
+        uint4 x8[2];
+        if (waited) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b) x8[b] = x_at(min(static_cast<int>(threadIdx.x) + b * THREADS, total_x - 1));
+        }
+        // The next unit to read: its tile and chunk, its rows of codes at this lane's words, and
+        // its rows' first scales.
+        int lt = blockIdx.x * abreast + t_warp, lu = 0;
+        const uint8_t *at0 = nullptr, *at1 = nullptr, *z0 = nullptr, *z1 = nullptr;
+        const S *s0 = nullptr, *s1 = nullptr;
+        auto settle = [&]() {
+            const Tile tile = tile_at(p, e, lt);
+            const int64_t r0 = tile.row(g), r1 = tile.row(g + 8);
+            const int k = k_warp * (CHUNK / 2) + c * 4 * WORDS;
+            at0 = p.w.codes + r0 * p.w.row_bytes + k;
+            at1 = p.w.codes + r1 * p.w.row_bytes + k;
+            s0 = static_cast<const S*>(p.w.scales) + r0 * p.w.groups_rs + k_warp * SEGS;
+            s1 = static_cast<const S*>(p.w.scales) + r1 * p.w.groups_rs + k_warp * SEGS;
+            if (zeros) {
+                z0 = p.w.zeros + r0 * p.w.groups_rs + k_warp * SEGS;
+                z1 = p.w.zeros + r1 * p.w.groups_rs + k_warp * SEGS;
+            }
+        };
+        Codes<SEG> now, next;
+        Quants<T, S, SEG> q_now, q_next;
+        auto read = [&](Codes<SEG>& codes, Quants<T, S, SEG>& q) {
+            const int chunk = k_warp + (lu << p.k_shift), step = lu << p.k_shift;
+            codes.load(at0 + step * (CHUNK / 2), at1 + step * (CHUNK / 2), row_len - chunk * (CHUNK / 2), c);
+            q.load_at(s0 + step * SEGS, s1 + step * SEGS, z0 + step * SEGS, z1 + step * SEGS, zeros, p.groups - chunk * SEGS);
+            if (++lu == units) {
+                lu = 0;
+                lt += tile_step;
+                if (lt < p.tiles) settle();
+            }
+        };
+        if (units && lt < p.tiles) {
+            settle();
+            read(next, q_next);
+        }
+        if (!waited) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+#pragma unroll
+            for (int b = 0; b < 2; ++b) x8[b] = x_at(min(static_cast<int>(threadIdx.x) + b * THREADS, total_x - 1));
+        }
+        waited = true;
+        for (int v = threadIdx.x + 2 * THREADS; v < total_x; v += 2 * THREADS) {
+            uint4 more[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) more[b] = x_at(min(v + b * THREADS, total_x - 1));
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+                if (v + b * THREADS < total_x) x_put(v + b * THREADS, more[b]);
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+            if (static_cast<int>(threadIdx.x) + b * THREADS < total_x) x_put(threadIdx.x + b * THREADS, x8[b]);
+        __syncthreads();
+
+        int x_row[NT];
+        uint32_t x_base[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            x_row[n] = min(n * 8 + g, rows_x - 1);
+            x_base[n] = x_all + (x_row[n] * chunks + k_warp) * (2 * X_BYTES);
+        }
+        int buffer = 0;
+        for (int t0 = blockIdx.x * abreast; t0 < p.tiles; t0 += tile_step) {
+            float total[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) total[n][0] = total[n][1] = total[n][2] = total[n][3] = 0;
+            if (t0 + t_warp < p.tiles) {
+                uint32_t xs[NT];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) xs[n] = x_base[n];
+                for (int u = 0; u < units; ++u) {
+                    now = next;
+                    q_now = q_next;
+                    if (lt < p.tiles) read(next, q_next);
+                    q_now.mask();
+                    const int left = p.w.cols - (k_warp + (u << p.k_shift)) * CHUNK;
+#pragma unroll
+                    for (int s = 0; s < SEGS; ++s) {
+                        if (s && s * SEG >= left) break;
+                        const float scale0 = q_now.scale(0, s), scale1 = q_now.scale(1, s);
+                        const auto zero0 = Decode<T>::zero(q_now.zero(0, s, zeros)), zero1 = Decode<T>::zero(q_now.zero(1, s, zeros));
+                        float acc[NT][4];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0;
+#pragma unroll
+                        for (int j = 0; j < WORDS; ++j) {
+                            uint32_t a0[4], a1[4];
+                            Decode<T>::unpack(now.w[0][s * WORDS + j], zero0, a0[0], a0[2], a1[0], a1[2]);
+                            Decode<T>::unpack(now.w[1][s * WORDS + j], zero1, a0[1], a0[3], a1[1], a1[3]);
+                            const int in_sub = s % (SUB / SEG);  // the segment within its 128 positions
+                            const int piece = SEG == 128 ? 4 * c + j : SEG == 64 ? 8 * in_sub + 2 * c + j : 4 * in_sub + c;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const uint4 x = lds<uint4>(xs[n] + s * SEG / SUB * X_BYTES + x_piece<SEG>(x_row[n], piece));
+                                Decode<T>::mma(acc[n], a0, x.x, x.y);
+                                Decode<T>::mma(acc[n], a1, x.z, x.w);
+                            }
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            total[n][0] = fmaf(scale0, acc[n][0], total[n][0]);
+                            total[n][1] = fmaf(scale0, acc[n][1], total[n][1]);
+                            total[n][2] = fmaf(scale1, acc[n][2], total[n][2]);
+                            total[n][3] = fmaf(scale1, acc[n][3], total[n][3]);
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) xs[n] += (2 * X_BYTES) << p.k_shift;
+                }
+            }
+            float* joined = red + buffer * (WARPS * NT * 128);
+            buffer ^= 1;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+                reinterpret_cast<float4*>(joined)[(warp * NT + n) * 32 + lane] = make_float4(total[n][0], total[n][1], total[n][2], total[n][3]);
+            __syncthreads();
+            tiles_out<T, NT>(p, found, joined, e, t0, c0, rows_x, x0);
+        }
+        __syncthreads();
+    }
+}
+
+template <typename T, typename S, int SEG, int NT>
+int launch_lean(uor_b200_ctx* ctx, FewParams& p, int cols, bool early) {
+    using B = Block<NT>;
+    p.k_shift = __builtin_ctz(B::WARPS);
+    while (p.k_shift > 0 && 1 << (p.k_shift - 1) >= p.chunks) --p.k_shift;
+    const int rows = p.kind == FEW_UP ? 8 : ROWS, abreast = B::WARPS >> p.k_shift;
+    p.tiles = (p.n + rows - 1) / rows;
+    const int64_t bundles = (p.tiles + abreast - 1) / abreast;
+    int64_t across = p.kind == FEW_DENSE ? (p.m + 8 * NT - 1) / (8 * NT) : static_cast<int64_t>(p.tokens) * p.top_k;
+    if (p.kind != FEW_DENSE && across > p.experts) across = p.experts;
+    // Tiles are dealt to about as many blocks as run at one time.
+    const int64_t resident = static_cast<int64_t>(ctx->sm_count) * (NT == 1 ? 2 : 1);
+    const int64_t each = bundles * across * 2 < resident * 3 ? 1 : (bundles * across + resident - 1) / resident;
+    auto* kernel = lean_kernel<T, S, SEG, NT>;
+    static bool ready[64] = {};
+    if (!ready[ctx->device & 63]) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, B::RED + B::X_MOST) != cudaSuccess)
+            return UOR_B200_DEVICE_ERROR;
+        ready[ctx->device & 63] = true;
+    }
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(static_cast<unsigned>((bundles + each - 1) / each), static_cast<unsigned>(across));
+    c.blockDim = dim3(B::THREADS);
+    c.dynamicSmemBytes = B::RED + static_cast<size_t>(cols) * p.chunks * 2 * X_BYTES;
+    c.stream = ctx->stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &attr;
+    c.numAttrs = early ? 1 : 0;
+    return cuda_status(cudaLaunchKernelEx(&c, kernel, p));
+}
+
+template <typename T, typename S, int SEG>
+bool try_lean(uor_b200_ctx* ctx, FewParams& p, bool early, int* status) {
+    constexpr int N = CHUNK / SEG;
+    constexpr int VEC = N * sizeof(S) < 16 ? N * sizeof(S) : 16;
+    const uint64_t scales = reinterpret_cast<uint64_t>(p.w.scales) | static_cast<uint64_t>(p.w.groups_rs) * sizeof(S);
+    const uint64_t zeros = p.w.zeros ? reinterpret_cast<uint64_t>(p.w.zeros) | static_cast<uint64_t>(p.w.groups_rs) : 0;
+    if (scales % VEC || zeros % N) return false;
+    p.quants_vec = 1;
+    p.group_shift = __builtin_ctz(SEG);
+    p.chunks = (p.w.cols + CHUNK - 1) / CHUNK;
+    p.groups = (p.w.cols + SEG - 1) / SEG;
+    const int64_t most = p.kind == FEW_DENSE ? p.m : p.tokens;
+    const bool two = most > 8;
+    const int cols = static_cast<int>(two ? (most < 16 ? most : 16) : most);
+    if (static_cast<int64_t>(cols) * p.chunks * 2 * X_BYTES > (two ? Block<2>::X_MOST : Block<1>::X_MOST)) return false;
+    *status = two ? launch_lean<T, S, SEG, 2>(ctx, p, cols, early) : launch_lean<T, S, SEG, 1>(ctx, p, cols, early);
+    return true;
+}
+
+template <typename T, typename S>
+bool by_group(uor_b200_ctx* ctx, FewParams& p, bool early, int* status) {
+    if (p.w.group == 128) return try_lean<T, S, 128>(ctx, p, early, status);
+    if (p.w.group == 64) return try_lean<T, S, 64>(ctx, p, early, status);
+    return p.w.group == 32 && try_lean<T, S, 32>(ctx, p, early, status);
+}
+
+template <typename T>
+bool by_scales(uor_b200_ctx* ctx, int elem, FewParams& p, bool early, int* status) {
+    if (p.w.scale_type == elem) return by_group<T, T>(ctx, p, early, status);
+    return p.w.scale_type == UOR_B200_F32 && by_group<T, float>(ctx, p, early, status);
+}
+
+}  // namespace
+
+bool lean_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early, int* status) {
+    if (p.codes_align != 16 || !p.x_vec || p.w.cols % 32) return false;
+    return elem == UOR_B200_BF16 ? by_scales<__nv_bfloat16>(ctx, elem, p, early, status) : by_scales<__half>(ctx, elem, p, early, status);
+}
+
+}  // namespace uor
