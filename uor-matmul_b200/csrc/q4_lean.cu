@@ -224,13 +224,16 @@ int launch_lean(uor_b200_ctx* ctx, FewParams& p, int cols, bool early) {
     using B = Block<NT>;
     p.k_shift = __builtin_ctz(B::WARPS);
     while (p.k_shift > 0 && 1 << (p.k_shift - 1) >= p.chunks) --p.k_shift;
-    const int rows = p.kind == FEW_UP ? 8 : ROWS, abreast = B::WARPS >> p.k_shift;
+    const int rows = p.kind == FEW_UP ? 8 : ROWS;
     p.tiles = (p.n + rows - 1) / rows;
-    const int64_t bundles = (p.tiles + abreast - 1) / abreast;
     int64_t across = p.kind == FEW_DENSE ? (p.m + 8 * NT - 1) / (8 * NT) : static_cast<int64_t>(p.tokens) * p.top_k;
     if (p.kind != FEW_DENSE && across > p.experts) across = p.experts;
     // Tiles are dealt to about as many blocks as run at one time.
     const int64_t resident = static_cast<int64_t>(ctx->sm_count) * (NT == 1 ? 2 : 1);
+    auto bundles_at = [&](int shift) { return (p.tiles + (B::WARPS >> shift) - 1) / (B::WARPS >> shift); };
+    // A warp with one chunk of a tile spends as long on joining it: two, where tiles abound.
+    while (p.k_shift > 0 && p.chunks >> p.k_shift < 2 && bundles_at(p.k_shift - 1) * across >= resident) --p.k_shift;
+    const int64_t bundles = bundles_at(p.k_shift);
     const int64_t each = bundles * across * 2 < resident * 3 ? 1 : (bundles * across + resident - 1) / resident;
     auto* kernel = lean_kernel<T, S, SEG, NT>;
     static bool ready[64] = {};

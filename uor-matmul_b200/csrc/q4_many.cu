@@ -53,7 +53,7 @@ constexpr int A_COLS = BK / 2;                       // tensor-memory columns of
 constexpr int A_FIRST = ACCS * HALF;
 constexpr int DECODERS = 4, SUMMERS = 4;             // warps of a CTA; of a CTA and a half
 constexpr int OUT_COLS = 32;                         // columns that leave at a time
-constexpr int EXCHANGE = BM * OUT_COLS * 4;          // bytes, per half
+constexpr int EXCHANGE = BM * OUT_COLS * 4 + HALF * 4;  // bytes, per half: sums, and their rows' pairs
 // Signals of filled accumulators, per half: as many as can be filled before the first is read, and
 // one, since a warpgroup waits for its own half's alone and must not mistake a later filling.
 constexpr int FULLS = ACCS + 1;
@@ -159,10 +159,11 @@ __device__ __forceinline__ float half_of(uint64_t v, int i) {
 }
 
 // The sums of `cols` activation rows from row i0 on, [column][row] in shared memory, to where
-// this launch's outputs go; 128 threads, `r` this one. Each stores eight neighbouring outputs of a
+// this launch's outputs go (pairs: the ones behind them); 128 threads, `r` this one. Each stores eight neighbouring outputs of a
 // column (four with gates and ups), as one vector where they lie so.
 template <typename T>
-__device__ __noinline__ void sums_out(const ManyParams& p, const Item& it, const float* swap, int64_t i0, int cols, int r) {
+__device__ __noinline__ void sums_out(const ManyParams& p, const Item& it, const float* swap, const int* pairs, int64_t i0, int cols,
+                                      int r) {
     if (p.mode == MANY_UP) {
         // Rows 0 .. 63 are gates, 64 .. 127 the same outputs' ups.
         const int j = (r & 15) * 4, valid = min(4, p.n - it.j0 - j);
@@ -190,7 +191,7 @@ __device__ __noinline__ void sums_out(const ManyParams& p, const Item& it, const
     for (int c = r >> 4; c < cols && valid > 0; c += 8) {
         const float4 a = *reinterpret_cast<const float4*>(swap + c * BM + j);
         const float4 b = *reinterpret_cast<const float4*>(swap + c * BM + j + 4);
-        const int64_t i = p.mode == MANY_DOWN ? p.perm[i0 + c] : i0 + c;
+        const int64_t i = p.mode == MANY_DOWN ? pairs[c] : i0 + c;
         const int64_t at = i * rs + (it.j0 + j) * step;
         char* first = static_cast<char*>(to) + at * (type == UOR_B200_F32 ? 4 : 2);
         if (valid == 8 && step == 1 && reinterpret_cast<uint64_t>(first) % 16 == 0) {
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* codes_at = smem + STAGES * X_BYTES;
     float* exchange = reinterpret_cast<float*>(codes_at + CSTAGES * C_BYTES);
-    uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + 2 * BM * OUT_COLS);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(exchange + 2 * (EXCHANGE / 4));
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
     int* first_tile = reinterpret_cast<int*>(bars + BARS + 1);
     // xfull, afull and tempty count on the leader, for both CTAs. done: a stage's products are
@@ -490,6 +491,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
             for (int i = 0; i < HALF / 2; ++i) acc[i] = 0;
             const int mine = part < it.halves ? it.half : 0;  // this warpgroup's columns
+            // asked for long before it is needed: the pair behind this half's column r
+            const int row_pair = p.mode == MANY_DOWN && r < mine && part * it.half + r < it.cols ? p.perm[it.p0 + part * it.half + r] : 0;
             uint32_t next = load();
             // Accumulators are filled in turn, those of both halves: this one's are every
             // `halves`-th from its own first on.
@@ -538,14 +541,16 @@ __global__ void __launch_bounds__(THREADS, 1)
             // Sums leave through shared memory 32 columns at a time, [column][row], so that a
             // thread stores neighbouring outputs of one column at once.
             const int left = min(mine, it.cols - part * it.half);  // this warpgroup's existing columns
-            float* swap = exchange + part * (BM * OUT_COLS);
+            float* swap = exchange + part * (EXCHANGE / 4);
+            int* pairs_at = reinterpret_cast<int*>(swap + BM * OUT_COLS);
+            pairs_at[r] = row_pair;
 #pragma unroll
             for (int c = 0; c < HALF; c += OUT_COLS)
                 if (c < left) {
 #pragma unroll
                     for (int i = 0; i < OUT_COLS; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
-                    sums_out<T>(p, it, swap, it.p0 + part * it.half + c, min(OUT_COLS, left - c), r);
+                    sums_out<T>(p, it, swap, pairs_at + c, it.p0 + part * it.half + c, min(OUT_COLS, left - c), r);
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
                 }
         }
