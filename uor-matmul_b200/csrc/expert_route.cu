@@ -6,8 +6,7 @@
 // ones complemented), so that the largest of a warp is one integer reduction. What is closed (a
 // logit or key of -inf or NaN) is key 0, below every open one.
 //
-// Bound by instructions: a token's 256 logits are 1 KB, 0.16 us of one processor's share of the
-// memory, and some 500 instructions (scores 90, keys and groups 110, eight choices 270).
+// Bound by instructions: a token's 256 logits are 1 KB, and some 700 instructions.
 #include <cstring>
 
 #include "q4.cuh"
@@ -148,9 +147,90 @@ __device__ __forceinline__ uint32_t open_groups(const uint32_t (&key)[VPL], cons
     return __ballot_sync(FULL, lane < groups && ahead < static_cast<int>(r.top_groups));
 }
 
+// The expert of this lane's choice (lane s: the s-th largest key's), or -1. The top_k-th of the
+// lanes' own largest keys bounds the choices from below, so few keys are left to order, a lane to
+// each: by how many are ahead of it. Where equal keys leave more than that, the choices are taken
+// one after another.
+template <int VPL>
+__device__ __forceinline__ int choose(uint32_t (&key)[VPL], int top_k, int lane, uint2* candidates) {
+    const int e0 = lane * VPL;
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) mine = max(mine, key[i]);
+    uint32_t bound = 1;
+    if (VPL > 1) {
+        uint32_t left = mine;
+        for (int s = 0; s < top_k; ++s) {
+            const uint32_t k = __reduce_max_sync(FULL, left);
+            bound = max(k, 1u);
+            if (k == 0) break;
+            const unsigned at = __ballot_sync(FULL, left == k);
+            if (lane == __ffs(at) - 1) left = 0;
+        }
+    }
+    int count = 0, my_at = 0;  // candidates; where this lane's begin
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) count += key[i] >= bound;
+    int upto = count;
+    if (VPL > 1) {
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(FULL, upto, o);
+            if (lane >= o) upto += v;
+        }
+    } else {
+        upto = __popc(__ballot_sync(FULL, count) & (0xFFFFFFFFu >> (31 - lane)));
+    }
+    my_at = upto - count;
+    const int all = __shfl_sync(FULL, upto, 31);
+    int expert = -1;
+    if (all <= 32) {
+        if (count) {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i)
+                if (key[i] >= bound) candidates[my_at++] = make_uint2(key[i], e0 + i);
+        }
+        __syncwarp();
+        // In the experts' order, so that of equal ones those before this one are ahead of it.
+        const uint2 c = lane < all ? candidates[lane] : make_uint2(0, 0);
+        int ahead = 0;
+        for (int o = 0; o < all; ++o) {
+            const uint32_t other = __shfl_sync(FULL, c.x, o);
+            ahead += other > c.x || (other == c.x && o < lane);
+        }
+        __syncwarp();
+        if (lane < all && ahead < top_k) candidates[ahead].y = c.y;
+        __syncwarp();
+        if (lane < min(top_k, all)) expert = static_cast<int>(candidates[lane].y);
+        return expert;
+    }
+    for (int s = 0; s < top_k; ++s) {  // a choice's lane takes out its key, the first among equals
+        const uint32_t k = __reduce_max_sync(FULL, mine);
+        if (!k) break;
+        const int from = __ffs(__ballot_sync(FULL, mine == k)) - 1;
+        int at = 0;
+        if (lane == from) {
+            bool found = false;
+            mine = 0;
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) {
+                if (!found && key[i] == k) {
+                    found = true;
+                    key[i] = 0;
+                    at = e0 + i;
+                }
+                mine = max(mine, key[i]);
+            }
+        }
+        at = __shfl_sync(FULL, at, from);
+        if (lane == s) expert = at;
+    }
+    return expert;
+}
+
 template <typename T, int VPL>
 __global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ RouterArgs a) {
     const int lane = threadIdx.x & 31;
+    __shared__ uint2 candidates[8][32];
     const int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (t >= a.tokens) return;
     const int experts = a.r.experts, top_k = a.r.top_k, e0 = lane * VPL;
@@ -190,32 +270,8 @@ __global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ Rout
                 if (e0 + i < experts && !(open >> ((e0 + i) / size) & 1)) key[i] = 0;
         }
     }
-    // Lane s keeps choice s. A choice's lane takes out its key, the first among equals.
-    uint32_t best = 0;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) best = max(best, key[i]);
-    int expert = -1;
-    for (int s = 0; s < top_k; ++s) {
-        const uint32_t k = __reduce_max_sync(FULL, best);
-        if (!k) break;
-        const int from = __ffs(__ballot_sync(FULL, best == k)) - 1;
-        int at = 0;
-        if (lane == from) {
-            bool found = false;
-            best = 0;
-#pragma unroll
-            for (int i = 0; i < VPL; ++i) {
-                if (!found && key[i] == k) {
-                    found = true;
-                    key[i] = 0;
-                    at = e0 + i;
-                }
-                best = max(best, key[i]);
-            }
-        }
-        at = __shfl_sync(FULL, at, from);
-        if (lane == s) expert = at;
-    }
+    // Lane s keeps choice s.
+    const int expert = choose(key, top_k, lane, candidates[threadIdx.x >> 5]);
     float v = -INFINITY, w = 0;
     if (expert >= 0) v = to_f32(static_cast<const T*>(a.logits.p)[t * a.logits.rs + expert * a.logits.cs]);
     if (a.r.renormalize)

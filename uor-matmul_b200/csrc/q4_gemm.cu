@@ -151,26 +151,49 @@ __global__ void add_parts_kernel(const float* part, int splits, int64_t rows, in
 // token's second choice of an expert has no product of its own, it is the first's.
 __global__ void combine_kernel(const float* part, int splits, bool once, const __grid_constant__ FfnArgs a) {
     const int j = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
-    if (j >= a.d) return;
+    if (j >= a.d) return;  // with nothing read or written, there is nothing to wait for
     const int64_t step = a.tokens * a.top_k;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const auto* ids = static_cast<const int32_t*>(a.ids.p);
+    const auto* weights = static_cast<const float*>(a.weights.p);
+    bool waited = false;
     for (int64_t t = blockIdx.y; t < a.tokens; t += gridDim.y) {
         float v[4] = {0, 0, 0, 0};
-#pragma unroll 4
-        for (int s = 0; s < a.top_k; ++s) {
-            const int e = static_cast<const int32_t*>(a.ids.p)[t * a.ids.rs + s * a.ids.cs];
-            if (e < 0 || e >= a.experts) continue;
-            const float w = static_cast<const float*>(a.weights.p)[t * a.weights.rs + s * a.weights.cs];
-            int from = s;
-            if (once)
-                for (int o = s - 1; o >= 0; --o)
-                    if (static_cast<const int32_t*>(a.ids.p)[t * a.ids.rs + o * a.ids.cs] == e) from = o;
-            float4 sum = load4(part + (t * a.top_k + from) * a.d, j, a.d, a.d % 4 == 0);
-            for (int c = 1; c < splits; ++c) {
-                const float4 more = load4(part + (c * step + t * a.top_k + from) * a.d, j, a.d, a.d % 4 == 0);
-                sum.x += more.x, sum.y += more.y, sum.z += more.z, sum.w += more.w;
+        for (int s0 = 0; s0 < a.top_k; s0 += 8) {  // eight choices' reads at a time
+            int e[8], from[8];
+            float w[8];
+            float4 sum[8];
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                e[b] = s0 + b < a.top_k ? ids[t * a.ids.rs + (s0 + b) * a.ids.cs] : -1;
+                w[b] = s0 + b < a.top_k ? weights[t * a.weights.rs + (s0 + b) * a.weights.cs] : 0.0f;
+                if (e[b] >= a.experts) e[b] = -1;
             }
-            v[0] = fmaf(w, sum.x, v[0]), v[1] = fmaf(w, sum.y, v[1]), v[2] = fmaf(w, sum.z, v[2]), v[3] = fmaf(w, sum.w, v[3]);
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                from[b] = s0 + b;
+                if (once && e[b] >= 0) {
+#pragma unroll
+                    for (int o = b - 1; o >= 0; --o)
+                        if (e[o] == e[b]) from[b] = s0 + o;
+                    for (int o = s0 - 1; o >= 0; --o)
+                        if (ids[t * a.ids.rs + o * a.ids.cs] == e[b]) from[b] = o;
+                }
+            }
+            if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+            waited = true;
+#pragma unroll
+            for (int b = 0; b < 8; ++b)
+                if (e[b] >= 0) sum[b] = load4(part + (t * a.top_k + from[b]) * a.d, j, a.d, a.d % 4 == 0);
+#pragma unroll
+            for (int b = 0; b < 8; ++b) {
+                if (e[b] < 0) continue;
+                for (int c = 1; c < splits; ++c) {
+                    const float4 more = load4(part + (c * step + t * a.top_k + from[b]) * a.d, j, a.d, a.d % 4 == 0);
+                    sum[b].x += more.x, sum[b].y += more.y, sum[b].z += more.z, sum[b].w += more.w;
+                }
+                v[0] = fmaf(w[b], sum[b].x, v[0]), v[1] = fmaf(w[b], sum[b].y, v[1]);
+                v[2] = fmaf(w[b], sum[b].z, v[2]), v[3] = fmaf(w[b], sum[b].w, v[3]);
+            }
         }
         store4(a.y, t, j, a.d, v);
     }
