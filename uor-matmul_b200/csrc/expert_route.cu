@@ -110,10 +110,11 @@ __device__ __forceinline__ void merge2(uint32_t& a1, uint32_t& a2, uint32_t b1, 
 // -inf is behind every other, and before none. Groups are runs of whole lanes, as many as a power
 // of two, or else looked at one after another.
 template <int VPL>
-__device__ __forceinline__ uint32_t open_groups(const uint32_t (&key)[VPL], const uor_b200_router& r, int lane) {
-    const int groups = r.groups, size = r.experts / r.groups, lanes = size / VPL;
+__device__ __forceinline__ uint32_t open_groups(const uint32_t (&key)[VPL], const RouterArgs& a, int lane) {
+    const int groups = a.r.groups, size = a.group_size;
     uint32_t mine = 0;  // lane g: group g's
-    if (size % VPL == 0 && (lanes & (lanes - 1)) == 0) {
+    if (a.lane_shift >= 0) {
+        const int lanes = 1 << a.lane_shift;
         uint32_t k1 = 0, k2 = 0;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) merge2(k1, k2, key[i], 0);
@@ -144,7 +145,7 @@ __device__ __forceinline__ uint32_t open_groups(const uint32_t (&key)[VPL], cons
         const uint32_t other = __shfl_sync(FULL, mine, g);
         ahead += other > mine || (other == mine && g < lane);
     }
-    return __ballot_sync(FULL, lane < groups && ahead < static_cast<int>(r.top_groups));
+    return __ballot_sync(FULL, lane < groups && ahead < static_cast<int>(a.r.top_groups));
 }
 
 // The expert of this lane's choice (lane s: the s-th largest key's), or -1. The top_k-th of the
@@ -245,22 +246,22 @@ __global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ Rout
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             float s = exp_below(l[i], top) * share;
-            if (a.bias && e0 + i < experts) s += a.bias[e0 + i];
+            if (a.bias) s += a.bias[min(e0 + i, experts - 1)];
             key[i] = l[i] > -INFINITY ? open_key(s) : 0u;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             float s = sigmoid(l[i]);
-            if (a.bias && e0 + i < experts) s += a.bias[e0 + i];
+            if (a.bias) s += a.bias[min(e0 + i, experts - 1)];
             key[i] = l[i] > -INFINITY ? open_key(s) : 0u;
         }
     }
     if (a.r.top_groups < a.r.groups) {
-        const uint32_t open = open_groups(key, a.r, lane);
-        const int size = experts / a.r.groups;
-        if (size % VPL == 0) {
-            if (e0 < experts && !(open >> (e0 / size) & 1)) {
+        const uint32_t open = open_groups(key, a, lane);
+        const int size = a.group_size;
+        if (a.lane_shift >= 0) {
+            if (!(open >> (lane >> a.lane_shift) & 1)) {
 #pragma unroll
                 for (int i = 0; i < VPL; ++i) key[i] = 0;
             }
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const __grid_consta
 }
 
 template <typename T>
-int launch(uor_b200_ctx* ctx, const RouterArgs& a, bool backward) {
+int launch(uor_b200_ctx* ctx, RouterArgs& a, bool backward) {
     const unsigned grid = static_cast<unsigned>((a.tokens + 7) / 8);
     auto go = [&](auto vpl) {
         constexpr int V = decltype(vpl)::value;
@@ -387,6 +388,10 @@ int launch(uor_b200_ctx* ctx, const RouterArgs& a, bool backward) {
             route_kernel<T, V><<<grid, 256, 0, ctx->stream>>>(a);
     };
     const int v = (static_cast<int>(a.r.experts) + 31) / 32;
+    const int vpl = v <= 1 ? 1 : v <= 2 ? 2 : v <= 4 ? 4 : v <= 8 ? 8 : v <= 16 ? 16 : 32;
+    a.group_size = static_cast<int>(a.r.experts / a.r.groups);
+    const int lanes = a.group_size / vpl;
+    a.lane_shift = a.group_size % vpl == 0 && (lanes & (lanes - 1)) == 0 ? __builtin_ctz(lanes) : -1;
     if (v <= 1) go(std::integral_constant<int, 1>());
     else if (v <= 2) go(std::integral_constant<int, 2>());
     else if (v <= 4) go(std::integral_constant<int, 4>());

@@ -84,7 +84,10 @@ struct RouterArgs {
     MatOut ids, weights;            // forward
     Mat in_ids, dweights;           // backward
     MatOut dlogits;
-    bool vec, vec_out;              // rows of logits (of dlogits) are whole vectors; set by the launch
+    // Set by the launch:
+    bool vec, vec_out;              // rows of logits (of dlogits) are whole vectors
+    int group_size;
+    int lane_shift;                 // log2 of the lanes that hold a group, or -1 where they do not hold one alone
 };
 int run_expert_route(uor_b200_ctx* ctx, const RouterArgs& a, uor_b200_route* route);
 int run_expert_route_backward(uor_b200_ctx* ctx, const RouterArgs& a, uor_b200_route* route);
