@@ -529,41 +529,44 @@ def arena_canonicalize(values):
 
 # ------------------------------------------------------------------ 4-bit weights, experts
 
+def _placed(buf, v):
+    """A view of a buffer from its (rows, cols[, rs[, cs]]), and whether it is on the device."""
+    ptr, n, dev = _buffer(buf)
+    return View(ptr, n, v[0], v[1], v[2] if len(v) > 2 and v[2] is not None else v[1],
+                v[3] if len(v) > 3 else 1), dev
+
+
+def _same_place(first, *others):
+    if any(o != first for o in others):
+        raise ValueError("operands must all be host arrays or all be CUDA tensors")
+    return first
+
+
 def q4_gemm(elem, out, a, av, w, c, cv, ctx=None, route=None, asynchronous=False):
     """C := A dequant(W)^T for a Q4 descriptor w: elem BF16 or F16, out elem or F32; f32 sums,
     rounded once. NumPy has no bfloat16: its bits pass as uint16 arrays."""
-    dev = _on_device(a, c)
-    if dev != w.on_device:
-        raise ValueError("operands must all be host arrays or all be CUDA tensors")
-    A, C = view(a, *av), view(c, *cv)
-    call = make_call(NEAREST, dev, ctx, route, asynchronous)
-    _check(lib().uor_b200_q4_gemm(elem, out, ctypes.byref(A), ctypes.byref(w), ctypes.byref(C),
-                                  ctypes.byref(call)), "q4_gemm")
+    (A, da), (C, dc) = _placed(a, av), _placed(c, cv)
+    call = make_call(NEAREST, _same_place(w.on_device, da, dc), ctx, route, asynchronous)
+    _check(lib().uor_b200_q4_gemm(elem, out, A, w, C, call), "q4_gemm")
 
 
 def expert_route(elem, router, logits, lv, bias, ids, iv, weights, wv, ctx=None, route=None,
                  asynchronous=False):
     """Each row's top_k experts (int32, -1 where none is left) and their f32 weights; bias is
     None or one float per expert, added for the choice alone."""
-    dev = _on_device(logits, ids, weights) if bias is None else \
-        _on_device(logits, ids, weights, bias)
-    L, IDS, W = view(logits, *lv), view(ids, *iv), view(weights, *wv)
-    pb, lb = _buffer(bias)[:2] if bias is not None else (None, 0)
-    call = make_call(NEAREST, dev, ctx, route, asynchronous)
-    _check(lib().uor_b200_expert_route(elem, ctypes.byref(router), ctypes.byref(L), pb, lb,
-                                       ctypes.byref(IDS), ctypes.byref(W), ctypes.byref(call)),
-           "expert_route")
+    (L, dl), (I, di), (W, dw) = _placed(logits, lv), _placed(ids, iv), _placed(weights, wv)
+    pb, lb, db = _buffer(bias) if bias is not None else (None, 0, dl)
+    call = make_call(NEAREST, _same_place(dl, di, dw, db), ctx, route, asynchronous)
+    _check(lib().uor_b200_expert_route(elem, router, L, pb, lb, I, W, call), "expert_route")
 
 
 def expert_route_backward(elem, router, logits, lv, ids, iv, dweights, gv, dlogits, dv, ctx=None,
                           route=None, asynchronous=False):
     """The logits' gradient from the weights', the choice ids held fixed."""
-    dev = _on_device(logits, ids, dweights, dlogits)
-    L, IDS, G, D = view(logits, *lv), view(ids, *iv), view(dweights, *gv), view(dlogits, *dv)
-    call = make_call(NEAREST, dev, ctx, route, asynchronous)
-    _check(lib().uor_b200_expert_route_backward(elem, ctypes.byref(router), ctypes.byref(L),
-                                                ctypes.byref(IDS), ctypes.byref(G),
-                                                ctypes.byref(D), ctypes.byref(call)),
+    (L, dl), (I, di) = _placed(logits, lv), _placed(ids, iv)
+    (G, dg), (D, dd) = _placed(dweights, gv), _placed(dlogits, dv)
+    call = make_call(NEAREST, _same_place(dl, di, dg, dd), ctx, route, asynchronous)
+    _check(lib().uor_b200_expert_route_backward(elem, router, L, I, G, D, call),
            "expert_route_backward")
 
 
@@ -571,14 +574,12 @@ def expert_q4_ffn(elem, out, experts, x, xv, ids, iv, weights, wv, up, down, y, 
                   route=None, asynchronous=False):
     """y[t] = sum_s weights[t][s] down_e (silu(gate_e x[t]) * (up_e x[t])), e = ids[t][s], over
     Q4 descriptors: up holds experts * 2 f rows (each expert's gate rows, then its up rows)."""
-    dev = _on_device(x, ids, weights, y)
-    if dev != up.on_device or dev != down.on_device:
-        raise ValueError("operands must all be host arrays or all be CUDA tensors")
-    X, IDS, W, Y = view(x, *xv), view(ids, *iv), view(weights, *wv), view(y, *yv)
+    (X, dx), (I, di) = _placed(x, xv), _placed(ids, iv)
+    (W, dw), (Y, dy) = _placed(weights, wv), _placed(y, yv)
+    dev = _same_place(up.on_device, down.on_device, dx, di, dw, dy)
     call = make_call(NEAREST, dev, ctx, route, asynchronous)
-    _check(lib().uor_b200_expert_q4_ffn(elem, out, experts, ctypes.byref(X), ctypes.byref(IDS),
-                                        ctypes.byref(W), ctypes.byref(up), ctypes.byref(down),
-                                        ctypes.byref(Y), ctypes.byref(call)), "expert_q4_ffn")
+    _check(lib().uor_b200_expert_q4_ffn(elem, out, experts, X, I, W, up, down, Y, call),
+           "expert_q4_ffn")
 
 
 # ------------------------------------------------------------------ split-K exchange
