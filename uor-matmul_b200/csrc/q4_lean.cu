@@ -1,6 +1,6 @@
 // q4_lean.cu -- products of few rows with 4-bit weights that lie well: rows of codes at multiples of
-// 16 bytes, a group of 32, 64 or 128 positions, scales that are read as vectors, activations that
-// fit in a block's shared memory.
+// four bytes, in whole eights, groups of 32, 64 or 128 positions, activations that fit in a block's
+// shared memory.
 //
 // q4_few.cu's product and its split, but for the way of the codes: each lane reads its operands'
 // words straight from memory into registers, one chunk ahead, so that there are no copies to
@@ -14,8 +14,9 @@ namespace uor {
 
 namespace {
 
-// A chunk's codes of this lane's two rows: word SEG / 32 s + j is the j-th of segment s.
-template <int SEG>
+// A chunk's codes of this lane's two rows: word SEG / 32 s + j is the j-th of segment s. WIDE: a
+// segment's words are one vector, else rows begin at multiples of four bytes only.
+template <int SEG, bool WIDE>
 struct Codes {
     static constexpr int WORDS = SEG / 32, SEGS = CHUNK / SEG;
     uint32_t w[2][8];
@@ -36,9 +37,13 @@ struct Codes {
         for (int s = 0; s < SEGS; ++s) {
             const uint8_t* from = at + s * (SEG / 2);
             uint32_t* to = w + s * WORDS;
-            if (TAIL && s * (SEG / 2) + c * 4 * WORDS >= bytes) {
+            const int left = bytes - s * (SEG / 2) - c * 4 * WORDS;
+            if (TAIL && left < 4 * WORDS) {
 #pragma unroll
-                for (int j = 0; j < WORDS; ++j) to[j] = 0;
+                for (int j = 0; j < WORDS; ++j) to[j] = 4 * j < left ? __ldg(reinterpret_cast<const uint32_t*>(from) + j) : 0;
+            } else if constexpr (!WIDE) {
+#pragma unroll
+                for (int j = 0; j < WORDS; ++j) to[j] = __ldg(reinterpret_cast<const uint32_t*>(from) + j);
             } else if constexpr (WORDS == 4) {
                 const uint4 x = __ldg(reinterpret_cast<const uint4*>(from));
                 to[0] = x.x, to[1] = x.y, to[2] = x.z, to[3] = x.w;
@@ -52,7 +57,7 @@ struct Codes {
     }
 };
 
-template <typename T, typename S, int SEG, int NT>
+template <typename T, typename S, int SEG, int NT, bool WIDE>
 __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kernel(const __grid_constant__ FewParams p) {
     constexpr int WARPS = Block<NT>::WARPS, THREADS = Block<NT>::THREADS, COLS = 8 * NT;
     constexpr int WORDS = SEG / 32, SEGS = CHUNK / SEG;
@@ -116,12 +121,12 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kern
                 z1 = p.w.zeros + r1 * p.w.groups_rs + k_warp * SEGS;
             }
         };
-        Codes<SEG> now, next;
+        Codes<SEG, WIDE> now, next;
         Quants<T, S, SEG> q_now, q_next;
-        auto read = [&](Codes<SEG>& codes, Quants<T, S, SEG>& q) {
+        auto read = [&](Codes<SEG, WIDE>& codes, Quants<T, S, SEG>& q) {
             const int chunk = k_warp + (lu << p.k_shift), step = lu << p.k_shift;
             codes.load(at0 + step * (CHUNK / 2), at1 + step * (CHUNK / 2), row_len - chunk * (CHUNK / 2), c);
-            q.load_at(s0 + step * SEGS, s1 + step * SEGS, z0 + step * SEGS, z1 + step * SEGS, zeros, p.groups - chunk * SEGS);
+            q.load_at(s0 + step * SEGS, s1 + step * SEGS, z0 + step * SEGS, z1 + step * SEGS, zeros, p.quants_vec != 0, p.groups - chunk * SEGS);
             if (++lu == units) {
                 lu = 0;
                 lt += tile_step;
@@ -219,7 +224,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kern
     }
 }
 
-template <typename T, typename S, int SEG, int NT>
+template <typename T, typename S, int SEG, int NT, bool WIDE>
 int launch_lean(uor_b200_ctx* ctx, FewParams& p, int cols, bool early) {
     using B = Block<NT>;
     p.k_shift = __builtin_ctz(B::WARPS);
@@ -235,7 +240,7 @@ int launch_lean(uor_b200_ctx* ctx, FewParams& p, int cols, bool early) {
     while (p.k_shift > 0 && p.chunks >> p.k_shift < 2 && bundles_at(p.k_shift - 1) * across >= resident) --p.k_shift;
     const int64_t bundles = bundles_at(p.k_shift);
     const int64_t each = bundles * across * 2 < resident * 3 ? 1 : (bundles * across + resident - 1) / resident;
-    auto* kernel = lean_kernel<T, S, SEG, NT>;
+    auto* kernel = lean_kernel<T, S, SEG, NT, WIDE>;
     static bool ready[64] = {};
     if (!ready[ctx->device & 63]) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, B::RED + B::X_MOST) != cudaSuccess)
@@ -255,14 +260,13 @@ int launch_lean(uor_b200_ctx* ctx, FewParams& p, int cols, bool early) {
     return cuda_status(cudaLaunchKernelEx(&c, kernel, p));
 }
 
-template <typename T, typename S, int SEG>
+template <typename T, typename S, int SEG, bool WIDE>
 bool try_lean(uor_b200_ctx* ctx, FewParams& p, bool early, int* status) {
     constexpr int N = CHUNK / SEG;
     constexpr int VEC = N * sizeof(S) < 16 ? N * sizeof(S) : 16;
     const uint64_t scales = reinterpret_cast<uint64_t>(p.w.scales) | static_cast<uint64_t>(p.w.groups_rs) * sizeof(S);
     const uint64_t zeros = p.w.zeros ? reinterpret_cast<uint64_t>(p.w.zeros) | static_cast<uint64_t>(p.w.groups_rs) : 0;
-    if (scales % VEC || zeros % N) return false;
-    p.quants_vec = 1;
+    p.quants_vec = scales % VEC == 0 && zeros % N == 0;
     p.group_shift = __builtin_ctz(SEG);
     p.chunks = (p.w.cols + CHUNK - 1) / CHUNK;
     p.groups = (p.w.cols + SEG - 1) / SEG;
@@ -270,15 +274,19 @@ bool try_lean(uor_b200_ctx* ctx, FewParams& p, bool early, int* status) {
     const bool two = most > 8;
     const int cols = static_cast<int>(two ? (most < 16 ? most : 16) : most);
     if (static_cast<int64_t>(cols) * p.chunks * 2 * X_BYTES > (two ? Block<2>::X_MOST : Block<1>::X_MOST)) return false;
-    *status = two ? launch_lean<T, S, SEG, 2>(ctx, p, cols, early) : launch_lean<T, S, SEG, 1>(ctx, p, cols, early);
+    *status = two ? launch_lean<T, S, SEG, 2, WIDE>(ctx, p, cols, early) : launch_lean<T, S, SEG, 1, WIDE>(ctx, p, cols, early);
     return true;
 }
 
 template <typename T, typename S>
 bool by_group(uor_b200_ctx* ctx, FewParams& p, bool early, int* status) {
-    if (p.w.group == 128) return try_lean<T, S, 128>(ctx, p, early, status);
-    if (p.w.group == 64) return try_lean<T, S, 64>(ctx, p, early, status);
-    return p.w.group == 32 && try_lean<T, S, 32>(ctx, p, early, status);
+    const uint64_t rows = reinterpret_cast<uint64_t>(p.w.codes) | static_cast<uint64_t>(p.w.row_bytes);
+    if (rows % 4) return false;
+    if (p.w.group == 128)
+        return rows % 16 ? try_lean<T, S, 128, false>(ctx, p, early, status) : try_lean<T, S, 128, true>(ctx, p, early, status);
+    if (p.w.group == 64)
+        return rows % 8 ? try_lean<T, S, 64, false>(ctx, p, early, status) : try_lean<T, S, 64, true>(ctx, p, early, status);
+    return p.w.group == 32 && try_lean<T, S, 32, true>(ctx, p, early, status);
 }
 
 template <typename T>
@@ -290,7 +298,7 @@ bool by_scales(uor_b200_ctx* ctx, int elem, FewParams& p, bool early, int* statu
 }  // namespace
 
 bool lean_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early, int* status) {
-    if (p.codes_align != 16 || !p.x_vec || p.w.cols % 32) return false;
+    if (!p.x_vec || p.w.cols % 8) return false;
     return elem == UOR_B200_BF16 ? by_scales<__nv_bfloat16>(ctx, elem, p, early, status) : by_scales<__half>(ctx, elem, p, early, status);
 }
 

@@ -200,9 +200,9 @@ struct Quants {
         }
     }
     // The same from the rows' addresses of the chunk's first scale and zero point, of which `left`
-    // exist, where they are vectors.
-    __device__ __forceinline__ void load_at(const S* s0, const S* s1, const uint8_t* z0, const uint8_t* z1, bool zeros, int left) {
-        if (left >= N) {
+    // exist; vec: they are vectors.
+    __device__ __forceinline__ void load_at(const S* s0, const S* s1, const uint8_t* z0, const uint8_t* z1, bool zeros, bool vec, int left) {
+        if (vec && left >= N) {
             copy(s[0], s0);
             copy(s[1], s1);
             if (zeros) {
