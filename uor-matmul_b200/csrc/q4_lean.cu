@@ -86,22 +86,24 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kern
 
     for (int c0 = 0; c0 < listed; c0 += COLS) {
         const int rows_x = min(COLS, listed - c0), pieces = chunks * 32;
-        auto x_at = [&](int v) {  // 16-byte piece v of the activations
-            const int r = rows_x == 1 ? 0 : v / pieces, k = (v - r * pieces) * 8;
+        auto x_row_at = [&](int r) {
             const int64_t row = kind == FEW_DENSE ? x0 + r : kind == FEW_UP ? found.list[c0 + r] / p.top_k : found.list[c0 + r];
+            return static_cast<const T*>(p.x) + row * p.x_rs;
+        };
+        auto x_get = [&](const T* row, int piece) {  // 16-byte piece of an activation row
             uint4 x = make_uint4(0, 0, 0, 0);
-            if (k < p.w.cols) x = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.x) + row * p.x_rs + k);
+            if (piece * 8 < p.w.cols) x = *reinterpret_cast<const uint4*>(row + piece * 8);
             return x;
         };
-        auto x_put = [&](int v, uint4 x) {
-            const int r = rows_x == 1 ? 0 : v / pieces, piece = v - r * pieces;
+        auto x_put = [&](int r, int piece, uint4 x) {
             sts128(x_all + (r * chunks * 2 + (piece >> 4)) * X_BYTES + x_piece<SEG>(r, piece & 15), kind == FEW_PART ? x : in_pairs(x));
         };
-        const int total_x = rows_x * pieces;
-        uint4 x8[2];
-        if (waited) {
+        uint4 x8[2];  // of a single row
+        const bool asked = waited && rows_x == 1;
+        if (asked) {
+            const T* row = x_row_at(0);
 #pragma unroll
-            for (int b = 0; b < 2; ++b) x8[b] = x_at(min(static_cast<int>(threadIdx.x) + b * THREADS, total_x - 1));
+            for (int b = 0; b < 2; ++b) x8[b] = x_get(row, threadIdx.x + b * THREADS);
         }
         // The next unit to read: its tile and chunk, its rows of codes at this lane's words, and
         // its rows' first scales.
@@ -137,23 +139,30 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kern
             settle();
             read(next, q_next);
         }
-        if (!waited) {
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-#pragma unroll
-            for (int b = 0; b < 2; ++b) x8[b] = x_at(min(static_cast<int>(threadIdx.x) + b * THREADS, total_x - 1));
-        }
+        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
         waited = true;
-        for (int v = threadIdx.x + 2 * THREADS; v < total_x; v += 2 * THREADS) {
-            uint4 more[2];
-#pragma unroll
-            for (int b = 0; b < 2; ++b) more[b] = x_at(min(v + b * THREADS, total_x - 1));
+        if (asked) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
-                if (v + b * THREADS < total_x) x_put(v + b * THREADS, more[b]);
+                if (static_cast<int>(threadIdx.x) + b * THREADS < pieces) x_put(0, threadIdx.x + b * THREADS, x8[b]);
         }
+        // Three rows' reads at a time; where a row has fewer pieces than the block threads, other
+        // threads take other rows.
+        const int beside = pieces < THREADS ? THREADS / pieces : 1, turn = pieces < THREADS ? threadIdx.x / pieces : 0;
+        for (int r0 = 3 * turn; r0 < rows_x && turn < beside; r0 += 3 * beside) {
+            const T* row[3];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-            if (static_cast<int>(threadIdx.x) + b * THREADS < total_x) x_put(threadIdx.x + b * THREADS, x8[b]);
+            for (int b = 0; b < 3; ++b) row[b] = x_row_at(min(r0 + b, rows_x - 1));
+            for (int piece = threadIdx.x - turn * pieces + (asked ? 2 * THREADS : 0); piece < pieces; piece += THREADS) {
+                uint4 x[3];
+#pragma unroll
+                for (int b = 0; b < 3; ++b)
+                    if (r0 + b < rows_x) x[b] = x_get(row[b], piece);
+#pragma unroll
+                for (int b = 0; b < 3; ++b)
+                    if (r0 + b < rows_x) x_put(r0 + b, piece, x[b]);
+            }
+        }
         __syncthreads();
 
         int x_row[NT];
@@ -237,9 +246,9 @@ int launch_lean(uor_b200_ctx* ctx, FewParams& p, int cols, bool early) {
     const int64_t resident = static_cast<int64_t>(ctx->sm_count) * (NT == 1 ? 2 : 1);
     auto bundles_at = [&](int shift) { return (p.tiles + (B::WARPS >> shift) - 1) / (B::WARPS >> shift); };
     // A warp with one chunk of a tile spends as long on joining it: two, where tiles abound.
-    while (p.k_shift > 0 && p.chunks >> p.k_shift < 2 && bundles_at(p.k_shift - 1) * across >= resident) --p.k_shift;
+    while (p.k_shift > 0 && p.chunks >> p.k_shift < 2 && bundles_at(p.k_shift - 1) * across >= resident * (NT == 1 ? 1 : 4)) --p.k_shift;
     const int64_t bundles = bundles_at(p.k_shift);
-    const int64_t each = bundles * across * 2 < resident * 3 ? 1 : (bundles * across + resident - 1) / resident;
+    const int64_t each = NT == 1 && bundles * across * 2 < resident * 3 ? 1 : (bundles * across + resident - 1) / resident;
     auto* kernel = lean_kernel<T, S, SEG, NT, WIDE>;
     static bool ready[64] = {};
     if (!ready[ctx->device & 63]) {

@@ -216,6 +216,31 @@ struct Quants {
             }
             return;
         }
+        if (left >= N) {
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const S* from = v ? s1 : s0;
+                const uint8_t* zfrom = v ? z1 : z0;
+#pragma unroll
+                for (int i = 0; i < SW; ++i) {
+                    if constexpr (sizeof(S) == 4) {
+                        s[v][i] = reinterpret_cast<const uint32_t*>(from)[i];
+                    } else {
+                        const uint32_t lo = reinterpret_cast<const uint16_t*>(from)[2 * i], hi = reinterpret_cast<const uint16_t*>(from)[2 * i + 1];
+                        s[v][i] = lo | hi << 16;
+                    }
+                }
+                if (zeros) {
+#pragma unroll
+                    for (int i = 0; i < ZW; ++i) {
+                        z[v][i] = 0;
+#pragma unroll
+                        for (int b = 0; b < 4 && 4 * i + b < N; ++b) z[v][i] |= static_cast<uint32_t>(zfrom[4 * i + b]) << (8 * b);
+                    }
+                }
+            }
+            return;
+        }
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
 #pragma unroll
