@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
         listed = find_pairs<WARPS>(p, found);
         if (listed < 0) return;
         e = found.chosen;
+        if (kind == FEW_PART) listed <<= p.twice;
     }
 
     // `kw` warps share a tile's reduction, so WARPS / kw tiles are under way at once.
@@ -268,7 +269,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
                         for (int b = 0; b < 4; ++b) {
                             const int v = min(v0 + b * THREADS, rows_x * pieces - 1);
                             const int r = rows_x == 1 ? 0 : v / pieces, k = first * CHUNK + (v - r * pieces) * 8;
-                            const int64_t row = kind == FEW_DENSE ? x0 + r : kind == FEW_UP ? found.list[c0 + r] / p.top_k : found.list[c0 + r];
+                            const int64_t row = x_row_of(p, found, x0, c0 + r);
                             // rows of inner activations end in whole eights
                             const int left = kind == FEW_PART ? (k < p.x_rs ? 8 : 0) : p.w.cols - k;
                             x8[b] = load_x8(static_cast<const T*>(p.x) + row * p.x_rs + (left > 0 ? k : 0), left, p.x_vec != 0);
@@ -322,7 +323,7 @@ int launch_few(uor_b200_ctx* ctx, FewParams& p, bool early) {
     using B = Block<NT>;
     const int chunks = p.chunks = (p.w.cols + CHUNK - 1) / CHUNK;
     p.groups = (p.w.cols + p.w.group - 1) / p.w.group;
-    int64_t cols = p.kind == FEW_DENSE ? p.m : p.tokens;  // of a block, at most
+    int64_t cols = few_columns(p);  // of a block, at most
     if (cols > 8 * NT) cols = 8 * NT;
     p.group_shift = (p.w.group & (p.w.group - 1)) == 0 ? __builtin_ctz(p.w.group) : -1;
     constexpr int N = CHUNK / SEG;
@@ -378,7 +379,7 @@ int by_segment(uor_b200_ctx* ctx, FewParams& p, bool early) {
 // neither float nor of the activations' type are converted as they are read.
 template <typename T, typename S, bool ANY>
 int by_columns(uor_b200_ctx* ctx, FewParams& p, bool early) {
-    return (p.kind == FEW_DENSE ? p.m : p.tokens) > 8 ? by_segment<T, S, 2, ANY>(ctx, p, early) : by_segment<T, S, 1, ANY>(ctx, p, early);
+    return few_columns(p) > 8 ? by_segment<T, S, 2, ANY>(ctx, p, early) : by_segment<T, S, 1, ANY>(ctx, p, early);
 }
 template <typename T>
 int by_codes(uor_b200_ctx* ctx, int elem, FewParams& p, bool early) {

@@ -11,6 +11,13 @@ enum FewKind {
     FEW_PART = 2    // part[pair][j] = h[pair] . w[j]
 };
 
+// Of up to 4 tokens an inner activation is kept as two of the 16-bit type, a rounded one and what
+// that left, in two columns of the down product: the tensor instruction's eight have room for both,
+// so the result lacks h's rounding for little (8 of 64 experts of 2048x1024: 1 token 19.9 -> 20.2
+// us, 4 41.8 -> 42.5). More tokens take more eights of columns (5: 48.2 -> 52.6, 8: 68.9 -> 75.7)
+// and average the rounding over more outputs; there h is rounded once.
+inline int few_twice(int64_t tokens) { return tokens <= 4 ? 1 : 0; }
+
 constexpr int FEW_MAX_PAIRS = 1024;    // tokens * top_k with experts
 constexpr int FEW_MAX_EXPERTS = 1024;  // a word of bits to a lane
 
@@ -24,7 +31,8 @@ struct FewParams {
     MatOut y;            // dense
     Mat ids;             // experts
     int tokens, top_k, experts;
-    void* h;             // up: [tokens * top_k][h_rs], every eight in the operands' order
+    void* h;             // up: [tokens * top_k][1 + twice][h_rs], every eight in the operands' order
+    int twice;           // experts: 1 if an inner activation is two of the 16-bit type, see few_twice
     int64_t h_rs;        // n rounded up to 8
     float* part;         // part: [tokens * top_k][n]
     int codes_align;     // 16 if every row of codes begins at a multiple of 16 bytes

@@ -346,8 +346,9 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     const int64_t pairs = a.tokens * a.top_k;
     const int h_rs = up_to(a.f, 8), x_rs = up_to(a.d, 8);
     Pieces pieces;
-    const size_t h_at = pieces.add(static_cast<size_t>(pairs) * h_rs * 2);
-    if (pairs <= FEW_MAX_PAIRS && few_experts(a)) {
+    const bool few = pairs <= FEW_MAX_PAIRS && few_experts(a);
+    const size_t h_at = pieces.add(static_cast<size_t>(pairs) * h_rs * (few && few_twice(a.tokens) ? 4 : 2));
+    if (few) {
         const size_t x_at = pieces.add(a.x.cs == 1 ? 0 : static_cast<size_t>(a.tokens) * x_rs * 2);
         const size_t part_at = pieces.add(static_cast<size_t>(pairs) * a.d * 4);
         uint8_t* ws = pieces.get(ctx, &st);
@@ -356,6 +357,7 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
         p.kind = FEW_UP;
         p.h = ws + h_at;
         p.h_rs = h_rs;
+        p.twice = few_twice(a.tokens);
         p.w = a.up;
         p.x = a.x.p;
         p.x_rs = a.x.rs;

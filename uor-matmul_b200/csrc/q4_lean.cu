@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kern
         listed = find_pairs<WARPS>(p, found);
         if (listed < 0) return;
         e = found.chosen;
+        if (kind == FEW_PART) listed <<= p.twice;
     }
     const int kw = 1 << p.k_shift, k_warp = warp & (kw - 1), t_warp = warp >> p.k_shift, abreast = WARPS >> p.k_shift;
     float* red = reinterpret_cast<float*>(smem);
@@ -87,8 +88,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kern
     for (int c0 = 0; c0 < listed; c0 += COLS) {
         const int rows_x = min(COLS, listed - c0), pieces = chunks * 32;
         auto x_row_at = [&](int r) {
-            const int64_t row = kind == FEW_DENSE ? x0 + r : kind == FEW_UP ? found.list[c0 + r] / p.top_k : found.list[c0 + r];
-            return static_cast<const T*>(p.x) + row * p.x_rs;
+            return static_cast<const T*>(p.x) + x_row_of(p, found, x0, c0 + r) * p.x_rs;
         };
         auto x_get = [&](const T* row, int piece) {  // 16-byte piece of an activation row
             uint4 x = make_uint4(0, 0, 0, 0);
@@ -279,7 +279,7 @@ bool try_lean(uor_b200_ctx* ctx, FewParams& p, bool early, int* status) {
     p.group_shift = __builtin_ctz(SEG);
     p.chunks = (p.w.cols + CHUNK - 1) / CHUNK;
     p.groups = (p.w.cols + SEG - 1) / SEG;
-    const int64_t most = p.kind == FEW_DENSE ? p.m : p.tokens;
+    const int64_t most = few_columns(p);
     const bool two = most > 8;
     const int cols = static_cast<int>(two ? (most < 16 ? most : 16) : most);
     if (static_cast<int64_t>(cols) * p.chunks * 2 * X_BYTES > (two ? Block<2>::X_MOST : Block<1>::X_MOST)) return false;

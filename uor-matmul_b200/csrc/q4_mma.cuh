@@ -393,6 +393,17 @@ __device__ __forceinline__ int find_pairs(const FewParams& p, Found& found) {
     return listed;
 }
 
+// The activation row behind column c: of a dense block's first x0, the token's of a listed pair, or
+// a pair's inner activations.
+__device__ __forceinline__ int64_t x_row_of(const FewParams& p, const Found& found, int64_t x0, int c) {
+    if (p.kind == FEW_DENSE) return x0 + c;
+    if (p.kind == FEW_UP) return found.list[c] / p.top_k;
+    return (static_cast<int64_t>(found.list[c >> p.twice]) << p.twice) + (c & p.twice);
+}
+
+// The columns that a launch's largest block may have.
+inline int64_t few_columns(const FewParams& p) { return p.kind == FEW_DENSE ? p.m : p.kind == FEW_UP ? p.tokens : p.tokens << p.twice; }
+
 // The tiles t0, t0 + 1, .. that a block's warps hold side by side: their sums, [warp][column
 // eight][lane][4] in shared memory, added in the warps' order and put where the launch's go.
 // Columns c0 .. c0 + cols - 1 of the block's.
@@ -401,24 +412,30 @@ __device__ __forceinline__ void tiles_out(const FewParams& p, const Found& found
                                           int cols, int64_t x0) {
     const int kw = 1 << p.k_shift, abreast = Block<NT>::WARPS >> p.k_shift;
     const int row_bits = p.kind == FEW_UP ? 3 : 4, rows = 1 << row_bits;  // outputs of a tile
-    for (int v = threadIdx.x; v < abreast * rows * cols; v += Block<NT>::THREADS) {
+    const int twice = p.kind == FEW_PART ? p.twice : 0;  // a pair's two columns are one output
+    for (int v = threadIdx.x; v < (abreast * rows * cols) >> twice; v += Block<NT>::THREADS) {
         const int r = v & (rows - 1), rest = v >> row_bits;
-        const int col = abreast == 1 ? rest : rest / abreast, ab = rest - col * abreast;
+        const int out_col = abreast == 1 ? rest : rest / abreast, ab = rest - out_col * abreast, col = out_col << twice;
         const int out = (t0 + ab) * rows + r;
-        auto sum = [&](int row) {
-            const float* at = joined + (ab * kw * NT + (col >> 3)) * 128 + ((row & 7) * 4 + ((col & 7) >> 1)) * 4 + (row >> 3) * 2 + (col & 1);
+        auto sum = [&](int row, int c = 0) {
+            const float* at = joined + (ab * kw * NT + (col >> 3)) * 128 + ((row & 7) * 4 + ((col & 7) >> 1)) * 4 + (row >> 3) * 2 + ((col + c) & 1);
             float s = 0;
             for (int w = 0; w < kw; ++w) s += at[w * NT * 128];
             return s;
         };
         if (p.kind == FEW_UP) {
-            // eight inner activations in the operands' order, zeros behind the last
-            if (t0 + ab < p.tiles)
-                static_cast<T*>(p.h)[static_cast<int64_t>(found.list[c0 + col]) * p.h_rs + (t0 + ab) * 8 + paired(r)] =
-                    from_f32<T>(out < p.n ? silu(sum(r)) * sum(r + 8) : 0.0f);
+            // eight inner activations in the operands' order, zeros behind the last; in a second
+            // row what the first one's rounding left
+            if (t0 + ab < p.tiles) {
+                const float h = out < p.n ? silu(sum(r)) * sum(r + 8) : 0.0f;
+                const T high = from_f32<T>(h);
+                T* to = static_cast<T*>(p.h) + (static_cast<int64_t>(found.list[c0 + col]) << p.twice) * p.h_rs + (t0 + ab) * 8 + paired(r);
+                to[0] = high;
+                if (p.twice) to[p.h_rs] = from_f32<T>(fabsf(to_f32(high)) < INFINITY ? h - to_f32(high) : 0.0f);
+            }
         } else if (out < p.n) {
             if (p.kind == FEW_PART)
-                p.part[static_cast<int64_t>(found.list[c0 + col]) * p.n + out] = sum(r);
+                p.part[static_cast<int64_t>(found.list[(c0 + col) >> twice]) * p.n + out] = twice ? sum(r) + sum(r, 1) : sum(r);
             else
                 store_f32(p.y.p, (x0 + col) * p.y.rs + out * p.y.cs, p.y.type, sum(r));
         }
