@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
     const int tile_step = gridDim.x * abreast;
     bool waited = kind != FEW_PART;
 
-    for (int c0 = 0; c0 < listed; c0 += COLS) {
+    for (int c0 = blockIdx.z * COLS; c0 < listed; c0 += gridDim.z * COLS) {
         const int rows_x = min(COLS, listed - c0);
         int x_row[NT];
 #pragma unroll
@@ -350,10 +350,15 @@ int launch_few(uor_b200_ctx* ctx, FewParams& p, bool early) {
     const int64_t bundles = (p.tiles + abreast - 1) / abreast;
     int64_t across = p.kind == FEW_DENSE ? (p.m + 8 * NT - 1) / (8 * NT) : static_cast<int64_t>(p.tokens) * p.top_k;
     if (p.kind != FEW_DENSE && across > p.experts) across = p.experts;
+    const auto blocks_y = static_cast<unsigned>(across);
+    // An expert of twice the mean has a block for each of its column tiles (8 experts of 512 x 768,
+    // 16 pairs each: 27 -> 21 us), and the dealing below counts those that the mean fills.
+    const int shares = few_shares(p, 8 * NT, 2);
+    across *= few_shares(p, 8 * NT, 1);
     const int64_t resident = static_cast<int64_t>(ctx->sm_count) * (NT == 1 ? 3 : 1);
     const int64_t each = (bundles * across + resident - 1) / resident;
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(static_cast<unsigned>((bundles + each - 1) / each), static_cast<unsigned>(across));
+    c.gridDim = dim3(static_cast<unsigned>((bundles + each - 1) / each), blocks_y, shares);
     c.blockDim = dim3(B::THREADS);
     c.dynamicSmemBytes = FIXED + cols * p.panel * 2 * X_BYTES;
     c.stream = ctx->stream;
@@ -379,7 +384,11 @@ int by_segment(uor_b200_ctx* ctx, FewParams& p, bool early) {
 // neither float nor of the activations' type are converted as they are read.
 template <typename T, typename S, bool ANY>
 int by_columns(uor_b200_ctx* ctx, FewParams& p, bool early) {
-    return few_columns(p) > 8 ? by_segment<T, S, 2, ANY>(ctx, p, early) : by_segment<T, S, 1, ANY>(ctx, p, early);
+    // Where the activations leave room for one or two blocks of eight warps, one of sixteen hides
+    // more (5003 x 4008 with 8 rows 47 -> 27 us, 300 x 12000 with 4 31 -> 13); one row would pay for
+    // fifteen others' columns.
+    const int64_t bytes = few_columns(p) * ((p.w.cols + CHUNK - 1) / CHUNK) * 2 * X_BYTES;
+    return few_columns(p) > 8 || (few_columns(p) > 1 && bytes > Block<1>::X_MOST / 4) ? by_segment<T, S, 2, ANY>(ctx, p, early) : by_segment<T, S, 1, ANY>(ctx, p, early);
 }
 template <typename T>
 int by_codes(uor_b200_ctx* ctx, int elem, FewParams& p, bool early) {

@@ -10,29 +10,52 @@ namespace uor {
 
 namespace {
 
+// A kernel that begins while the one before it in the call still runs: it waits for that one's
+// results here, and lets the next begin as its blocks leave.
+__device__ __forceinline__ void follow() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+constexpr int THREADS = 256;
+constexpr int ROWS_EACH = 4;
+
 // Rows of x, strided anyhow, as contiguous ones of `pitch` elements; row i is x's row
 // perm[i] / top_k where there is a permutation, and then only offsets[experts] rows exist.
-// Eight elements to a thread.
-__global__ void rows_kernel(Mat x, int cols, int pitch, int64_t rows, const int* perm, int top_k, const int* total, bool vec,
-                            uint16_t* to) {
+// Eight elements to a thread, four times side by side.
+__global__ void __launch_bounds__(THREADS) rows_kernel(Mat x, int cols, int pitch, int64_t rows, const int* perm, int top_k,
+                                                       const int* total, bool vec, uint16_t* to) {
+    follow();
     const int per_row = pitch / 8;
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int64_t i = at / per_row;
-    if (i >= (total ? min(static_cast<int64_t>(*total), rows) : rows)) return;
-    const int c = static_cast<int>(at - i * per_row) * 8;
-    const int64_t row = perm ? perm[i] / top_k : i;
-    const auto* from = static_cast<const uint16_t*>(x.p) + row * x.rs;
-    uint4 v;
-    if (vec && c + 8 <= cols) {
-        v = *reinterpret_cast<const uint4*>(from + c);
-    } else {
-        uint32_t w[4] = {0, 0, 0, 0};
+    const int64_t exist = total ? min(static_cast<int64_t>(*total), rows) : rows;
+    int64_t i[ROWS_EACH];
+    int c[ROWS_EACH];
+    const uint16_t* from[ROWS_EACH];
 #pragma unroll
-        for (int b = 0; b < 8; ++b)
-            if (c + b < cols) w[b >> 1] |= static_cast<uint32_t>(from[(c + b) * x.cs]) << (16 * (b & 1));
-        v = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int b = 0; b < ROWS_EACH; ++b) {
+        const int64_t at = (static_cast<int64_t>(blockIdx.x) * ROWS_EACH + b) * THREADS + threadIdx.x;
+        i[b] = at / per_row;
+        c[b] = static_cast<int>(at - i[b] * per_row) * 8;
+        const int64_t row = i[b] >= exist ? 0 : perm ? perm[i[b]] / top_k : i[b];
+        from[b] = static_cast<const uint16_t*>(x.p) + row * x.rs;
     }
-    *reinterpret_cast<uint4*>(to + i * pitch + c) = v;
+    uint4 v[ROWS_EACH];
+#pragma unroll
+    for (int b = 0; b < ROWS_EACH; ++b) {
+        if (i[b] >= exist) continue;
+        if (vec && c[b] + 8 <= cols) {
+            v[b] = *reinterpret_cast<const uint4*>(from[b] + c[b]);
+        } else {
+            uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (c[b] + e < cols) w[e >> 1] |= static_cast<uint32_t>(from[b][(c[b] + e) * x.cs]) << (16 * (e & 1));
+            v[b] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < ROWS_EACH; ++b)
+        if (i[b] < exist) *reinterpret_cast<uint4*>(to + i[b] * pitch + c[b]) = v[b];
 }
 
 // Rows of codes at any address and distance as rows of `pitch` bytes, a multiple of 16.
@@ -61,49 +84,57 @@ __global__ void codes_kernel(const uint8_t* codes, int64_t row_bytes, int64_t ro
     *reinterpret_cast<uint4*>(to + i * pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-constexpr int SORT_THREADS = 256;
+constexpr int SORT_THREADS = 1024, SORT_BATCH = 8;
 
 // The pairs (token, choice) of one expert per block, in their own order, behind those of the
 // experts before it: offsets[e] counts the pairs of lower experts. Ids outside the experts have
-// no place. Every thread counts and then places a run of pairs of its own.
+// no place. Every warp counts and then places a run of pairs of its own, 32 abreast and eight
+// times 32 under way (8192 pairs among 32 experts: 5.8 us).
 __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(Mat ids, int pairs, int top_k, int experts, int* offsets, int* perm) {
-    __shared__ int warp_less[SORT_THREADS / 32], warp_same[SORT_THREADS / 32];
+    constexpr int WARPS = SORT_THREADS / 32;
+    __shared__ int warp_less[WARPS], warp_same[WARPS];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int run = (pairs + SORT_THREADS - 1) / SORT_THREADS;
-    const int first = min(pairs, static_cast<int>(threadIdx.x) * run), last = min(pairs, first + run);
-    auto id = [&](int i) {
-        const int t = i / top_k;
-        return static_cast<const int32_t*>(ids.p)[t * ids.rs + (i - t * top_k) * ids.cs];
+    const int run = (pairs + SORT_THREADS - 1) / SORT_THREADS * 32;
+    const int first = min(pairs, warp * run), last = min(pairs, first + run);
+    auto read = [&](int at, int (&v)[SORT_BATCH]) {
+#pragma unroll
+        for (int b = 0; b < SORT_BATCH; ++b) {
+            const int i = at + b * 32 + lane, t = i / top_k;
+            v[b] = i < last ? static_cast<const int32_t*>(ids.p)[t * ids.rs + (i - t * top_k) * ids.cs] : -1;
+        }
     };
-    int less = 0, same = 0;
-#pragma unroll 8
-    for (int i = first; i < last; ++i) {
-        const int v = id(i);
-        less += v >= 0 && v < e;
-        same += v == e;
-    }
-    int before = same;  // pairs of this expert in the runs up to this one's end
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
+    int less = 0, same = 0, v[SORT_BATCH];
+    for (int at = first; at < last; at += 32 * SORT_BATCH) {
+        read(at, v);
+#pragma unroll
+        for (int b = 0; b < SORT_BATCH; ++b) {
+            less += v[b] >= 0 && v[b] < e;
+            same += v[b] == e;
+        }
     }
     less = __reduce_add_sync(0xffffffffu, less);
-    if (lane == 31) warp_less[warp] = less, warp_same[warp] = before;
+    same = __reduce_add_sync(0xffffffffu, same);
+    if (lane == 0) warp_less[warp] = less, warp_same[warp] = same;
     __syncthreads();
-    int begin = 0, here = 0, all = 0;
-    for (int w = 0; w < SORT_THREADS / 32; ++w) {
-        begin += warp_less[w];
-        if (w < warp) here += warp_same[w];
-        all += warp_same[w];
-    }
+    const int begin = __reduce_add_sync(0xffffffffu, warp_less[lane]), all = __reduce_add_sync(0xffffffffu, warp_same[lane]);
+    int to = begin + __reduce_add_sync(0xffffffffu, lane < warp ? warp_same[lane] : 0);
     if (threadIdx.x == 0) {
         offsets[e] = begin;
         if (e == experts - 1) offsets[experts] = begin + all;
     }
-    int at = begin + here + before - same;
-    for (int i = first; i < last; ++i)
-        if (id(i) == e) perm[at++] = i;
+    if (!same) return;
+    for (int at = first; at < last; at += 32 * SORT_BATCH) {
+        if (last - first > 32 * SORT_BATCH) read(at, v);  // else they are at hand
+#pragma unroll
+        for (int b = 0; b < SORT_BATCH; ++b) {
+            const uint32_t mine = __ballot_sync(0xffffffffu, v[b] == e);
+            if (v[b] == e) perm[to + __popc(mine & ((1u << lane) - 1))] = at + b * 32 + lane;
+            to += __popc(mine);
+        }
+    }
 }
+static_assert(SORT_THREADS == 1024, "a lane for each warp's counts");
 
 // Four neighbouring outputs of a row; one by one where they do not lie as a vector.
 __device__ __forceinline__ void store4(const MatOut& y, int64_t i, int j, int n, const float (&v)[4]) {
@@ -135,6 +166,7 @@ __device__ __forceinline__ float4 load4(const float* row, int j, int n, bool vec
 // y[i][j] = the parts' sum, in their order (no parts: 0). A block's x takes 1024 outputs of a
 // row, its y strides the rows.
 __global__ void add_parts_kernel(const float* part, int splits, int64_t rows, int n, MatOut y) {
+    follow();
     const int j = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
     if (j >= n) return;
     for (int64_t i = blockIdx.y; i < rows; i += gridDim.y) {
@@ -199,10 +231,24 @@ __global__ void combine_kernel(const float* part, int splits, bool once, const _
     }
 }
 
-constexpr int THREADS = 256;
 // Four outputs to a thread, a row to a block's y.
 dim3 blocks_of_rows(int64_t rows, int n) {
     return dim3((n + 4 * THREADS - 1) / (4 * THREADS), static_cast<unsigned>(rows < 65535 ? rows : 65535));
+}
+// A launch of THREADS to a block; early: it may begin while the kernel before it still runs, whose
+// results it waits for itself.
+template <typename... P, typename... A>
+int launch(uor_b200_ctx* ctx, dim3 grid, bool early, void (*kernel)(P...), const A&... args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3(THREADS);
+    c.stream = ctx->stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &attr;
+    c.numAttrs = early ? 1 : 0;
+    return cuda_status(cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...));
 }
 unsigned blocks_for(int64_t threads) { return static_cast<unsigned>((threads + THREADS - 1) / THREADS); }
 
@@ -243,10 +289,12 @@ void copy_codes(uor_b200_ctx* ctx, Q4Dev* w, uint8_t* to) {
     w->codes = to;
     w->row_bytes = pitch;
 }
-void copy_rows(uor_b200_ctx* ctx, const Mat& x, int cols, int64_t rows, const int* perm, int top_k, const int* total, void* to) {
+// early: after a kernel of the same call, and may begin while that one still runs.
+void copy_rows(uor_b200_ctx* ctx, const Mat& x, int cols, int64_t rows, const int* perm, int top_k, const int* total, void* to,
+               bool early) {
     const int pitch = up_to(cols, 8);
-    rows_kernel<<<blocks_for(rows * (pitch / 8)), THREADS, 0, ctx->stream>>>(
-        x, cols, pitch, rows, perm, top_k, total, x.cs == 1 && rows_aligned(x.p, x.rs * 2), static_cast<uint16_t*>(to));
+    launch(ctx, dim3(blocks_for((rows * (pitch / 8) + ROWS_EACH - 1) / ROWS_EACH)), early, rows_kernel, x, cols, pitch, rows, perm,
+           top_k, total, x.cs == 1 && rows_aligned(x.p, x.rs * 2), static_cast<uint16_t*>(to));
 }
 
 // What the few-rows kernel's vector loads may rely on.
@@ -255,30 +303,39 @@ void few_align(FewParams* p) {
     p->x_vec = rows_aligned(p->x, p->x_rs * 2);
 }
 
-// few: after the few-rows kernel, which wrote a token's products with an expert once; the launch may
-// begin while that one still runs.
+// few: after the few-rows kernel, which wrote a token's products with an expert once.
 int launch_combine(uor_b200_ctx* ctx, const float* part, int splits, const FfnArgs& a, bool few) {
-    cudaLaunchConfig_t c = {};
-    c.gridDim = blocks_of_rows(a.tokens, a.d);
-    c.blockDim = dim3(THREADS);
-    c.stream = ctx->stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = &attr;
-    c.numAttrs = few ? 1 : 0;
-    return cuda_status(cudaLaunchKernelEx(&c, combine_kernel, part, splits, few, a));
+    return launch(ctx, blocks_of_rows(a.tokens, a.d), true, combine_kernel, part, splits, few, a);
 }
 
-// Few pairs to an expert: reading every chosen expert's weights is then most of the work, and the
-// few-rows kernel reads them as they lie, without sorting rows and laying codes out first.
+// The few-rows kernel's 16 columns at a time against the tensor-memory kernel's 256 (which starts
+// slower, takes rows as TMA can read them, and with experts has them sorted and copied first).
+// Times in us, few : many.
+//
+// Dense: while the activations of a pass stay in shared memory, few rows are the weights' reading
+// (8192 x 8192 with 6 rows 20 : 30, 4096 x 4096 with 12 9 : 16, 5003 x 4008 at odd addresses with 8
+// 27 : 34), and else not (8192 x 8192 with 8 53 : 30, 4096 x 4096 with 16 25 : 17). Small products
+// fit the processors many passes abreast: 2048 x 2048 with 64 rows 9.4 : 15.0, 128 14.6 : 17.8,
+// 256 40 : 18.5; 768 x 768 with 512 rows 12 : 17, 1024 20 : 17; 1000 x 1001 with 128 rows 11.5 : 34,
+// 512 30 : 35. That is up to 2^25 weights and passes together.
+bool few_rows(int64_t m, const Q4Dev& w) {
+    const int64_t passes = (m + 15) / 16, cols = m < 16 ? m : 16;
+    return m <= 2 || (cols * w.cols <= 57344 && (passes == 1 || (passes <= 65535 && passes * w.rows * w.cols <= int64_t(1) << 25)));
+}
+
+// Experts: their weights times the passes over them, half a pass empty on average, against a start
+// of some 36 us and then the same weights once. 8 experts of 2048 x 1024 with 8 pairs each
+// 30 : 40, 12 43 : 41; 16 of 1024 x 512 with 12 35 : 37, 24 53 : 40; 8 of 512 x 768 with 48
+// 38 : 53, 96 71 : 61; 4 of 512 x 128 with 128 23 : 48. With 4 pairs an expert, 32 of 2048 x 1024
+// still run 75 : 100, with 8 121 : 105.
 bool few_experts(const FfnArgs& a) {
-    return a.tokens <= 16 || a.tokens * a.top_k <= 12 * static_cast<int64_t>(a.experts);
+    const int64_t pairs = a.tokens * a.top_k;
+    return pairs <= FEW_MAX_PAIRS && (a.tokens <= 16 || pairs <= 4 * static_cast<int64_t>(a.experts) ||
+                                      static_cast<int64_t>(a.d) * a.f <= 192000000 / (pairs + a.experts));
 }
 
 int zeros_out(uor_b200_ctx* ctx, int64_t rows, int n, const MatOut& y) {
-    add_parts_kernel<<<blocks_of_rows(rows, n), THREADS, 0, ctx->stream>>>(nullptr, 0, rows, n, y);
-    return cuda_status(cudaGetLastError());
+    return launch(ctx, blocks_of_rows(rows, n), false, add_parts_kernel, nullptr, 0, rows, n, y);
 }
 
 }  // namespace
@@ -288,7 +345,7 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     route->kernel = UOR_B200_KERNEL_Q4;
     if (w.cols == 0) return zeros_out(ctx, m, w.rows, y);
     int st = UOR_B200_OK;
-    const bool few = m <= 16;
+    const bool few = few_rows(m, w);
     Pieces pieces;
     // The few-rows kernel reads any row whose elements follow one another.
     const bool own_rows = few ? x.cs != 1 : !x_in_place(x, w.cols);
@@ -308,7 +365,7 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     if (!ws) return st;
     Mat rows = x;
     if (own_rows) {
-        copy_rows(ctx, x, w.cols, m, nullptr, 1, nullptr, ws + x_at);
+        copy_rows(ctx, x, w.cols, m, nullptr, 1, nullptr, ws + x_at, false);
         rows = Mat{ws + x_at, up_to(w.cols, 8), 1};
     }
     if (few) {
@@ -329,12 +386,11 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     many.x_rs = rows.rs;
     many.x_rows = m;
     many.part = reinterpret_cast<float*>(ws + part_at);
-    route->tile_m = 256, route->tile_n = 256, route->tile_k = 64;
+    route->tile_m = 256, route->tile_n = 256, route->tile_k = 128;
     route->k_chunks = splits;
-    if ((st = many_launch(ctx, elem, many))) return st;
+    if ((st = many_launch(ctx, elem, many, own_rows || codes_copy_bytes(w) > 0))) return st;
     if (splits > 1) {
-        add_parts_kernel<<<blocks_of_rows(m, w.rows), THREADS, 0, ctx->stream>>>(many.part, splits, m, w.rows, y);
-        return cuda_status(cudaGetLastError());
+        return launch(ctx, blocks_of_rows(m, w.rows), true, add_parts_kernel, many.part, splits, m, w.rows, y);
     }
     return UOR_B200_OK;
 }
@@ -346,7 +402,7 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     const int64_t pairs = a.tokens * a.top_k;
     const int h_rs = up_to(a.f, 8), x_rs = up_to(a.d, 8);
     Pieces pieces;
-    const bool few = pairs <= FEW_MAX_PAIRS && few_experts(a);
+    const bool few = few_experts(a);
     const size_t h_at = pieces.add(static_cast<size_t>(pairs) * h_rs * (few && few_twice(a.tokens) ? 4 : 2));
     if (few) {
         const size_t x_at = pieces.add(a.x.cs == 1 ? 0 : static_cast<size_t>(a.tokens) * x_rs * 2);
@@ -362,7 +418,7 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
         p.x = a.x.p;
         p.x_rs = a.x.rs;
         if (a.x.cs != 1) {
-            copy_rows(ctx, a.x, a.d, a.tokens, nullptr, 1, nullptr, ws + x_at);
+            copy_rows(ctx, a.x, a.d, a.tokens, nullptr, 1, nullptr, ws + x_at, false);
             p.x = ws + x_at;
             p.x_rs = x_rs;
         }
@@ -409,7 +465,7 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     int* offsets = reinterpret_cast<int*>(ws + offsets_at);
     int* perm = reinterpret_cast<int*>(ws + perm_at);
     sort_kernel<<<a.experts, SORT_THREADS, 0, ctx->stream>>>(a.ids, static_cast<int>(pairs), a.top_k, a.experts, offsets, perm);
-    copy_rows(ctx, a.x, a.d, pairs, perm, a.top_k, offsets + a.experts, ws + x_at);
+    copy_rows(ctx, a.x, a.d, pairs, perm, a.top_k, offsets + a.experts, ws + x_at, true);
     copy_codes(ctx, &up.w, ws + up_at);
     copy_codes(ctx, &down.w, ws + down_at);
     up.offsets = down.offsets = offsets;
@@ -418,8 +474,8 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     up.h = ws + h_at;
     down.x = ws + h_at;
     down.part = reinterpret_cast<float*>(ws + part_at);
-    route->tile_m = 256, route->tile_n = 256, route->tile_k = 64;
-    if ((st = many_launch(ctx, a.elem, up)) || (st = many_launch(ctx, a.elem, down))) return st;
+    route->tile_m = 256, route->tile_n = 256, route->tile_k = 128;
+    if ((st = many_launch(ctx, a.elem, up, true)) || (st = many_launch(ctx, a.elem, down, true))) return st;
     return launch_combine(ctx, down.part, splits, a, false);
 }
 

@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kern
     const int units = chunks > k_warp ? (chunks - k_warp + kw - 1) >> p.k_shift : 0;  // chunks of a tile for this warp
     bool waited = kind != FEW_PART;
 
-    for (int c0 = 0; c0 < listed; c0 += COLS) {
+    for (int c0 = blockIdx.z * COLS; c0 < listed; c0 += gridDim.z * COLS) {
         const int rows_x = min(COLS, listed - c0), pieces = chunks * 32;
         auto x_row_at = [&](int r) {
             return static_cast<const T*>(p.x) + x_row_of(p, found, x0, c0 + r) * p.x_rs;
@@ -242,6 +242,11 @@ int launch_lean(uor_b200_ctx* ctx, FewParams& p, int cols, bool early) {
     p.tiles = (p.n + rows - 1) / rows;
     int64_t across = p.kind == FEW_DENSE ? (p.m + 8 * NT - 1) / (8 * NT) : static_cast<int64_t>(p.tokens) * p.top_k;
     if (p.kind != FEW_DENSE && across > p.experts) across = p.experts;
+    const auto blocks_y = static_cast<unsigned>(across);
+    // An expert of twice the mean has a block for each of its column tiles (8 experts of 512 x 768,
+    // 16 pairs each: 27 -> 21 us), and the dealing below counts those that the mean fills.
+    const int shares = few_shares(p, 8 * NT, 2);
+    across *= few_shares(p, 8 * NT, 1);
     // Tiles are dealt to about as many blocks as run at one time.
     const int64_t resident = static_cast<int64_t>(ctx->sm_count) * (NT == 1 ? 2 : 1);
     auto bundles_at = [&](int shift) { return (p.tiles + (B::WARPS >> shift) - 1) / (B::WARPS >> shift); };
@@ -257,7 +262,7 @@ int launch_lean(uor_b200_ctx* ctx, FewParams& p, int cols, bool early) {
         ready[ctx->device & 63] = true;
     }
     cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(static_cast<unsigned>((bundles + each - 1) / each), static_cast<unsigned>(across));
+    c.gridDim = dim3(static_cast<unsigned>((bundles + each - 1) / each), blocks_y, shares);
     c.blockDim = dim3(B::THREADS);
     c.dynamicSmemBytes = B::RED + static_cast<size_t>(cols) * p.chunks * 2 * X_BYTES;
     c.stream = ctx->stream;
@@ -280,7 +285,9 @@ bool try_lean(uor_b200_ctx* ctx, FewParams& p, bool early, int* status) {
     p.chunks = (p.w.cols + CHUNK - 1) / CHUNK;
     p.groups = (p.w.cols + SEG - 1) / SEG;
     const int64_t most = few_columns(p);
-    const bool two = most > 8;
+    // Activations too many for two blocks of eight warps may fit one of sixteen (8192 x 8192 with 6
+    // rows 41 -> 20 us, 2048 x 7168 with 8 17 -> 8.3).
+    const bool two = most > 8 || most * p.chunks * 2 * X_BYTES > Block<1>::X_MOST;
     const int cols = static_cast<int>(two ? (most < 16 ? most : 16) : most);
     if (static_cast<int64_t>(cols) * p.chunks * 2 * X_BYTES > (two ? Block<2>::X_MOST : Block<1>::X_MOST)) return false;
     *status = two ? launch_lean<T, S, SEG, 2, WIDE>(ctx, p, cols, early) : launch_lean<T, S, SEG, 1, WIDE>(ctx, p, cols, early);

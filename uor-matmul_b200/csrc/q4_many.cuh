@@ -38,7 +38,7 @@ struct ManyParams {
 // The reduction is cut `splits` ways when a launch would otherwise leave processors idle; the
 // caller provides `part` for many_splits' answer and adds the parts.
 int many_splits(const uor_b200_ctx* ctx, const ManyParams& p);
-// Status; codes and x have to be TMA-readable (16-byte aligned rows).
-int many_launch(uor_b200_ctx* ctx, int elem, ManyParams p);
+// Status; early: after a kernel of the same call, and may begin while that one still runs. Codes and x have to be TMA-readable (16-byte aligned rows).
+int many_launch(uor_b200_ctx* ctx, int elem, ManyParams p, bool early);
 
 }  // namespace uor

@@ -404,6 +404,15 @@ __device__ __forceinline__ int64_t x_row_of(const FewParams& p, const Found& fou
 // The columns that a launch's largest block may have.
 inline int64_t few_columns(const FewParams& p) { return p.kind == FEW_DENSE ? p.m : p.kind == FEW_UP ? p.tokens : p.tokens << p.twice; }
 
+// The blocks that share an expert's columns, `width` at a time: as many as `spread` times the mean
+// of them needs, where the largest expert may have that many.
+inline int few_shares(const FewParams& p, int width, int spread) {
+    if (p.kind == FEW_DENSE) return 1;
+    const int64_t most = (few_columns(p) + width - 1) / width, all = static_cast<int64_t>(p.experts) * width;
+    const int64_t mean = (spread * few_columns(p) * p.top_k + all - 1) / all;
+    return static_cast<int>(mean < 1 ? 1 : mean < most ? mean : most);
+}
+
 // The tiles t0, t0 + 1, .. that a block's warps hold side by side: their sums, [warp][column
 // eight][lane][4] in shared memory, added in the warps' order and put where the launch's go.
 // Columns c0 .. c0 + cols - 1 of the block's.
