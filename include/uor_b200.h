@@ -509,12 +509,12 @@ int uor_b200_expert_route_backward(uor_b200_dtype elem, const uor_b200_router *r
 
 /* The chosen experts' gated feed-forward layer over 4-bit weights:
  *   y[t] = sum_s weights[t][s] * down_e (silu(gate_e x[t]) * (up_e x[t])),  e = ids[t][s],
- * silu(v) = v / (1 + exp(-v)), with 1 .. 1024 experts. x is tokens x d of elem (BF16 or F16), y tokens x d of out (elem
- * or F32). `up` holds every expert's gate rows and then its up rows: experts * 2 f rows of d;
- * `down` experts * d rows of f. ids (int32) and weights (f32) are tokens x top_k; an id outside
- * [0, experts) is skipped, whatever its weight, and a token without any gets zeros. The inner
- * activations are rounded once to elem between the two products; of up to 4 tokens a second elem
- * keeps what that left. */
+ * silu(v) = v / (1 + exp(-v)), with 1 .. 1024 experts. x is tokens x d of elem (BF16 or F16),
+ * y tokens x d of out (elem or F32). `up` holds every expert's gate rows and then its up rows:
+ * experts * 2 f rows of d; `down` experts * d rows of f. ids (int32) and weights (f32) are tokens
+ * x top_k; an id outside [0, experts) is skipped, whatever its weight, and a token without any
+ * gets zeros. The inner activations are rounded once to elem between the two products; of up to 4
+ * tokens a second elem keeps what that left. */
 int uor_b200_expert_q4_ffn(uor_b200_dtype elem, uor_b200_dtype out, size_t experts,
                            const uor_b200_view *x, const uor_b200_view *ids,
                            const uor_b200_view *weights, const uor_b200_q4 *up,
