@@ -6,7 +6,8 @@
 // words straight from memory into registers, one chunk ahead, so that there are no copies to
 // place, to wait for and to read back. Instructions are what bounds these products beside the
 // memory (an operand's word takes 11 to unpack), and so are the few microseconds of a launch:
-// activations are asked for first, and nothing is divided on the device.
+// activations are asked for first, and nothing is divided on the device. One row: 4096 x 4096 in
+// 6.3 us, 8192 x 8192 with zero points in 15.6 (2.4 TB/s), 17.0 by way of shared memory.
 #include "ptx.cuh"
 #include "q4_mma.cuh"
 
