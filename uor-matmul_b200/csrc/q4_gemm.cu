@@ -31,11 +31,14 @@ __global__ void __launch_bounds__(THREADS) rows_kernel(Mat x, int cols, int pitc
     int64_t i[ROWS_EACH];
     int c[ROWS_EACH];
     const uint16_t* from[ROWS_EACH];
+    // one long division a block: the rest is within 32 bits
+    const int64_t begin = static_cast<int64_t>(blockIdx.x) * (ROWS_EACH * THREADS), i0 = begin / per_row;
+    const uint32_t c0 = static_cast<uint32_t>(begin - i0 * per_row) + threadIdx.x;
 #pragma unroll
     for (int b = 0; b < ROWS_EACH; ++b) {
-        const int64_t at = (static_cast<int64_t>(blockIdx.x) * ROWS_EACH + b) * THREADS + threadIdx.x;
-        i[b] = at / per_row;
-        c[b] = static_cast<int>(at - i[b] * per_row) * 8;
+        const uint32_t at = c0 + b * THREADS, down = at / static_cast<uint32_t>(per_row);
+        i[b] = i0 + down;
+        c[b] = static_cast<int>(at - down * per_row) * 8;
         const int64_t row = i[b] >= exist ? 0 : perm ? perm[i[b]] / top_k : i[b];
         from[b] = static_cast<const uint16_t*>(x.p) + row * x.rs;
     }
@@ -180,8 +183,11 @@ __global__ void add_parts_kernel(const float* part, int splits, int64_t rows, in
 }
 
 // y[t][j] = the token's choices' products, each times its weight, in the choices' order. once: a
-// token's second choice of an expert has no product of its own, it is the first's.
-__global__ void combine_kernel(const float* part, int splits, bool once, const __grid_constant__ FfnArgs a) {
+// token's second choice of an expert has no product of its own, it is the first's. AT: choices that
+// are read at a time; four where there are no more, which halves the registers (2048 tokens, 4
+// choices of 2048: 35 -> 21 us).
+template <int AT>
+__global__ void __launch_bounds__(256) combine_kernel(const float* part, int splits, bool once, const __grid_constant__ FfnArgs a) {
     const int j = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
     if (j >= a.d) return;  // with nothing read or written, there is nothing to wait for
     const int64_t step = a.tokens * a.top_k;
@@ -190,18 +196,18 @@ __global__ void combine_kernel(const float* part, int splits, bool once, const _
     bool waited = false;
     for (int64_t t = blockIdx.y; t < a.tokens; t += gridDim.y) {
         float v[4] = {0, 0, 0, 0};
-        for (int s0 = 0; s0 < a.top_k; s0 += 8) {  // eight choices' reads at a time
-            int e[8], from[8];
-            float w[8];
-            float4 sum[8];
+        for (int s0 = 0; s0 < a.top_k; s0 += AT) {
+            int e[AT], from[AT];
+            float w[AT];
+            float4 sum[AT];
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
+            for (int b = 0; b < AT; ++b) {
                 e[b] = s0 + b < a.top_k ? ids[t * a.ids.rs + (s0 + b) * a.ids.cs] : -1;
                 w[b] = s0 + b < a.top_k ? weights[t * a.weights.rs + (s0 + b) * a.weights.cs] : 0.0f;
                 if (e[b] >= a.experts) e[b] = -1;
             }
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
+            for (int b = 0; b < AT; ++b) {
                 from[b] = s0 + b;
                 if (once && e[b] >= 0) {
 #pragma unroll
@@ -214,10 +220,10 @@ __global__ void combine_kernel(const float* part, int splits, bool once, const _
             if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
             waited = true;
 #pragma unroll
-            for (int b = 0; b < 8; ++b)
+            for (int b = 0; b < AT; ++b)
                 if (e[b] >= 0) sum[b] = load4(part + (t * a.top_k + from[b]) * a.d, j, a.d, a.d % 4 == 0);
 #pragma unroll
-            for (int b = 0; b < 8; ++b) {
+            for (int b = 0; b < AT; ++b) {
                 if (e[b] < 0) continue;
                 for (int c = 1; c < splits; ++c) {
                     const float4 more = load4(part + (c * step + t * a.top_k + from[b]) * a.d, j, a.d, a.d % 4 == 0);
@@ -305,7 +311,8 @@ void few_align(FewParams* p) {
 
 // few: after the few-rows kernel, which wrote a token's products with an expert once.
 int launch_combine(uor_b200_ctx* ctx, const float* part, int splits, const FfnArgs& a, bool few) {
-    return launch(ctx, blocks_of_rows(a.tokens, a.d), true, combine_kernel, part, splits, few, a);
+    return launch(ctx, blocks_of_rows(a.tokens, a.d), true, a.top_k <= 4 ? combine_kernel<4> : combine_kernel<8>, part, splits, few,
+                  a);
 }
 
 // The few-rows kernel's 16 columns at a time against the tensor-memory kernel's 256 (which starts

@@ -7,7 +7,8 @@
 // place, to wait for and to read back. Instructions are what bounds these products beside the
 // memory (an operand's word takes 11 to unpack), and so are the few microseconds of a launch:
 // activations are asked for first, and nothing is divided on the device. One row: 4096 x 4096 in
-// 6.3 us, 8192 x 8192 with zero points in 15.6 (2.4 TB/s), 17.0 by way of shared memory.
+// 6.3 us, 8192 x 8192 with zero points in 15.6 (2.4 TB/s), 17.0 by way of shared memory. 13 x 5003
+// x 4008 with a scale and a zero point per 32 positions: 21.9, of which the bytes are 2.1.
 #include "ptx.cuh"
 #include "q4_mma.cuh"
 
