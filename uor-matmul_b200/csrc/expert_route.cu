@@ -311,13 +311,15 @@ __global__ void __launch_bounds__(256) route_backward_kernel(const __grid_consta
     T* row = static_cast<T*>(a.dlogits.p) + t * a.dlogits.rs;
     const int64_t cs = a.dlogits.cs;
     constexpr int BYTES = VPL * sizeof(T);
-    const bool vec = BYTES % 16 == 0 && a.vec_out && e0 + VPL <= experts;
+    const bool vec_row = BYTES % 16 == 0 && a.vec_out, vec = vec_row && e0 + VPL <= experts;
     if (!whole) {  // while the chosen logits travel
-        if (vec) {
+        if (!vec_row) {  // the lanes side by side, all of them
+            for (int e = lane; e < experts; e += 32) row[e * cs] = from_f32<T>(0.0f);
+        } else if (vec) {
 #pragma unroll
             for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(row + e0)[i] = make_uint4(0, 0, 0, 0);
-        } else {
-            for (int e = lane; e < experts; e += 32) row[e * cs] = from_f32<T>(0.0f);
+        } else {  // the lane whose run the row ends in
+            for (int e = e0; e < experts; ++e) row[e * cs] = from_f32<T>(0.0f);
         }
     }
     if (expert >= 0) {
