@@ -76,6 +76,39 @@ class Codec(ctypes.Structure):
 TIER_GRID, TIER_SIGN, TIER_TERNARY, TIER_BOOK = range(4)
 
 
+_ARRAYS = {I8: "bytes", I32: "32-bit integers", F32: "float32", BF16: "bfloat16", F16: "float16"}
+_NUMPY, _TORCH = 1, 2
+_FITS = {}  # (an array's dtype, an operand's type): whose array it is, or 0 where it does not fit
+
+
+def _fits(dtype, t):
+    if dtype is None:
+        return 0
+    if type(dtype).__module__.startswith("torch"):
+        whose, name = _TORCH, str(dtype).rpartition(".")[2]
+        whole = name in ("uint8", "int8", "uint16", "int16", "uint32", "int32", "uint64", "int64")
+    else:
+        whose, name, whole = _NUMPY, dtype.name, dtype.kind in "iu"
+    return whose if name == _ARRAYS[t] or (whole and t != F32 and dtype.itemsize == DTYPE_SIZE[t]) else 0
+
+
+def _typed(buf, t):
+    """_buffer of an array whose elements are of type t (integers of their size, for bytes, ids and
+    the bits of 16-bit floats), and of no other. None, a type that the library itself refuses,
+    takes anything."""
+    if t is None:
+        return _buffer(buf)
+    dtype = getattr(buf, "dtype", None)
+    whose = _FITS.get((dtype, t))
+    if whose is None:
+        whose = _FITS[dtype, t] = _fits(dtype, t)
+    if whose == _TORCH:
+        return buf.data_ptr(), buf.numel(), buf.is_cuda
+    if whose == _NUMPY:
+        return _buffer(buf)
+    raise TypeError(f"an operand of {_ARRAYS[t]} as {type(buf).__name__} of {dtype}")
+
+
 class Q4(ctypes.Structure):
     """uor_b200_q4: rows x cols weights in 4 bits, codes two per byte, low nibble first, with a
     scale (and a zero point, else 8) per row and `group` positions of the reduction. Holds the
@@ -89,11 +122,10 @@ class Q4(ctypes.Structure):
 
     def __init__(self, codes, scales, scale_type, rows, cols, group, zeros=None, row_bytes=None,
                  groups_rs=None):
-        pc, lc, dev = _buffer(codes)
-        ps, ls, _ = _buffer(scales)
-        pz, lz = _buffer(zeros)[:2] if zeros is not None else (None, 0)
-        if (_on_device(codes, scales) if zeros is None else _on_device(codes, scales, zeros)) != dev:
-            raise ValueError("operands must all be host arrays or all be CUDA tensors")
+        pc, lc, dev = _typed(codes, I8)
+        ps, ls, ds = _typed(scales, scale_type if scale_type in (F32, BF16, F16) else None)
+        pz, lz, dz = _typed(zeros, I8) if zeros is not None else (None, 0, dev)
+        _same_place(dev, ds, dz)
         super().__init__(pc, lc, rows, cols, (cols + 1) // 2 if row_bytes is None else row_bytes,
                          ps, ls, scale_type, group,
                          -(-cols // max(group, 1)) if groups_rs is None else groups_rs, pz, lz)
@@ -529,9 +561,10 @@ def arena_canonicalize(values):
 
 # ------------------------------------------------------------------ 4-bit weights, experts
 
-def _placed(buf, v):
-    """A view of a buffer from its (rows, cols[, rs[, cs]]), and whether it is on the device."""
-    ptr, n, dev = _buffer(buf)
+def _placed(buf, v, t):
+    """A view of a buffer of elements of type t from its (rows, cols[, rs[, cs]]), and whether it is
+    on the device."""
+    ptr, n, dev = _typed(buf, t)
     return View(ptr, n, v[0], v[1], v[2] if len(v) > 2 and v[2] is not None else v[1],
                 v[3] if len(v) > 3 else 1), dev
 
@@ -542,10 +575,16 @@ def _same_place(first, *others):
     return first
 
 
+def _out_type(elem, out):
+    """The output's type where the library takes it beside elem, a 16-bit float."""
+    return out if elem in (BF16, F16) and out in (elem, F32) else None
+
+
 def q4_gemm(elem, out, a, av, w, c, cv, ctx=None, route=None, asynchronous=False):
     """C := A dequant(W)^T for a Q4 descriptor w: elem BF16 or F16, out elem or F32; f32 sums,
     rounded once. NumPy has no bfloat16: its bits pass as uint16 arrays."""
-    (A, da), (C, dc) = _placed(a, av), _placed(c, cv)
+    (A, da) = _placed(a, av, elem if elem in (BF16, F16) else None)
+    (C, dc) = _placed(c, cv, _out_type(elem, out))
     call = make_call(NEAREST, _same_place(w.on_device, da, dc), ctx, route, asynchronous)
     _check(lib().uor_b200_q4_gemm(elem, out, A, w, C, call), "q4_gemm")
 
@@ -554,8 +593,9 @@ def expert_route(elem, router, logits, lv, bias, ids, iv, weights, wv, ctx=None,
                  asynchronous=False):
     """Each row's top_k experts (int32, -1 where none is left) and their f32 weights; bias is
     None or one float per expert, added for the choice alone."""
-    (L, dl), (I, di), (W, dw) = _placed(logits, lv), _placed(ids, iv), _placed(weights, wv)
-    pb, lb, db = _buffer(bias) if bias is not None else (None, 0, dl)
+    (L, dl) = _placed(logits, lv, elem if elem in (F32, BF16, F16) else None)
+    (I, di), (W, dw) = _placed(ids, iv, I32), _placed(weights, wv, F32)
+    pb, lb, db = _typed(bias, F32) if bias is not None else (None, 0, dl)
     call = make_call(NEAREST, _same_place(dl, di, dw, db), ctx, route, asynchronous)
     _check(lib().uor_b200_expert_route(elem, router, L, pb, lb, I, W, call), "expert_route")
 
@@ -563,8 +603,9 @@ def expert_route(elem, router, logits, lv, bias, ids, iv, weights, wv, ctx=None,
 def expert_route_backward(elem, router, logits, lv, ids, iv, dweights, gv, dlogits, dv, ctx=None,
                           route=None, asynchronous=False):
     """The logits' gradient from the weights', the choice ids held fixed."""
-    (L, dl), (I, di) = _placed(logits, lv), _placed(ids, iv)
-    (G, dg), (D, dd) = _placed(dweights, gv), _placed(dlogits, dv)
+    of = elem if elem in (F32, BF16, F16) else None
+    (L, dl), (I, di) = _placed(logits, lv, of), _placed(ids, iv, I32)
+    (G, dg), (D, dd) = _placed(dweights, gv, F32), _placed(dlogits, dv, of)
     call = make_call(NEAREST, _same_place(dl, di, dg, dd), ctx, route, asynchronous)
     _check(lib().uor_b200_expert_route_backward(elem, router, L, I, G, D, call),
            "expert_route_backward")
@@ -574,8 +615,8 @@ def expert_q4_ffn(elem, out, experts, x, xv, ids, iv, weights, wv, up, down, y, 
                   route=None, asynchronous=False):
     """y[t] = sum_s weights[t][s] down_e (silu(gate_e x[t]) * (up_e x[t])), e = ids[t][s], over
     Q4 descriptors: up holds experts * 2 f rows (each expert's gate rows, then its up rows)."""
-    (X, dx), (I, di) = _placed(x, xv), _placed(ids, iv)
-    (W, dw), (Y, dy) = _placed(weights, wv), _placed(y, yv)
+    (X, dx), (I, di) = _placed(x, xv, elem if elem in (BF16, F16) else None), _placed(ids, iv, I32)
+    (W, dw), (Y, dy) = _placed(weights, wv, F32), _placed(y, yv, _out_type(elem, out))
     dev = _same_place(up.on_device, down.on_device, dx, di, dw, dy)
     call = make_call(NEAREST, dev, ctx, route, asynchronous)
     _check(lib().uor_b200_expert_q4_ffn(elem, out, experts, X, I, W, up, down, Y, call),
