@@ -442,6 +442,8 @@ int uor_b200_arena_canonicalize(uor_b200_dtype elem, void *values, size_t len, s
  * like the rest of the library: the products are of 16-bit floats, sums are held in f32 in an
  * order that depends on the shapes alone (the same call gives the same bytes), and the result
  * is rounded once to `out`. Non-finite activations and scales spread as the formula has them.
+ * Device pointers of this family and the router are multiples of their element's size (codes lie
+ * at any byte): INVALID_ARGUMENT otherwise.
  * No reference counterpart: the reference's codecs carry no scales. */
 typedef struct uor_b200_q4 {
     const uint8_t *codes;

@@ -13,13 +13,22 @@ constexpr size_t MOST = static_cast<size_t>(INT_MAX) / 2;
 
 bool half_type(uor_b200_dtype t) { return t == UOR_B200_BF16 || t == UOR_B200_F16; }
 
-int place(const uor_b200_view* v, size_t es, Operand* o) {
-    return place_view(v->data, v->len, v->rows, v->cols, v->rs, v->cs, es, o);
+// Kernels read and write whole elements: a device address that is no multiple of their size faults
+// there. Host arrays are copied, from any address.
+bool at_element(const void* p, size_t rows, size_t cols, size_t es, bool device) {
+    return !device || rows == 0 || cols == 0 || reinterpret_cast<uintptr_t>(p) % es == 0;
 }
-int place(const uor_b200_view_mut* v, size_t es, Operand* o) {
+
+int place(const uor_b200_view* v, size_t es, bool device, Operand* o) {
     const int st = place_view(v->data, v->len, v->rows, v->cols, v->rs, v->cs, es, o);
     if (st) return st;
-    return self_aliases(v->rows, v->cols, v->rs, v->cs) ? UOR_B200_OUTPUT_ALIASES : UOR_B200_OK;
+    return at_element(v->data, v->rows, v->cols, es, device) ? UOR_B200_OK : UOR_B200_INVALID_ARGUMENT;
+}
+int place(const uor_b200_view_mut* v, size_t es, bool device, Operand* o) {
+    const int st = place_view(v->data, v->len, v->rows, v->cols, v->rs, v->cs, es, o);
+    if (st) return st;
+    if (self_aliases(v->rows, v->cols, v->rs, v->cs)) return UOR_B200_OUTPUT_ALIASES;
+    return at_element(v->data, v->rows, v->cols, es, device) ? UOR_B200_OK : UOR_B200_INVALID_ARGUMENT;
 }
 
 // Whether (rows - 1) * stride + row elements are within len.
@@ -31,7 +40,7 @@ bool reaches(size_t rows, size_t stride, size_t row, size_t len) {
     return last <= len;
 }
 
-int check_q4(const uor_b200_q4* w) {
+int check_q4(const uor_b200_q4* w, bool device) {
     if (!w) return UOR_B200_INVALID_ARGUMENT;
     if (w->group == 0 || w->group % 32 || w->group > MOST) return UOR_B200_INVALID_ARGUMENT;
     const auto type = static_cast<uor_b200_dtype>(w->scale_type);
@@ -45,7 +54,7 @@ int check_q4(const uor_b200_q4* w) {
     if (w->row_bytes > static_cast<size_t>(PTRDIFF_MAX) || w->groups_rs > static_cast<size_t>(PTRDIFF_MAX))
         return UOR_B200_DOES_NOT_FIT;
     if (w->rows && w->cols && (!w->codes || !w->scales)) return UOR_B200_INVALID_ARGUMENT;
-    return UOR_B200_OK;
+    return at_element(w->scales, w->rows, w->cols, dtype_size(type), device) ? UOR_B200_OK : UOR_B200_INVALID_ARGUMENT;
 }
 
 // Host operands travel to one device buffer together, each at a 256-byte boundary.
@@ -146,9 +155,9 @@ int uor_b200_q4_gemm(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_vie
     bool dev = false;
     Operand A, C;
     int st;
-    if ((st = check_call(call, &dev)) || (st = check_q4(w)) || (st = place(a, 2, &A))) return st;
+    if ((st = check_call(call, &dev)) || (st = check_q4(w, dev)) || (st = place(a, 2, dev, &A))) return st;
     if (a->cols != w->cols || c->rows != a->rows || c->cols != w->rows) return UOR_B200_NONCONFORMANT;
-    if ((st = place(c, dtype_size(out), &C))) return st;
+    if ((st = place(c, dtype_size(out), dev, &C))) return st;
     uor_b200_route local;
     uor_b200_route* route = clear_route(call, &local);
     if (a->rows == 0 || w->rows == 0) return UOR_B200_OK;
@@ -180,14 +189,15 @@ int uor_b200_expert_route(uor_b200_dtype elem, const uor_b200_router* router, co
     bool dev = false;
     Operand L, I, W;
     int st;
-    if ((st = check_call(call, &dev)) || (st = check_router(router)) || (st = place(logits, dtype_size(elem), &L)))
+    if ((st = check_call(call, &dev)) || (st = check_router(router)) || (st = place(logits, dtype_size(elem), dev, &L)))
         return st;
     const size_t t = logits->rows;
     if (logits->cols != router->experts || ids->rows != t || ids->cols != router->top_k || weights->rows != t ||
         weights->cols != router->top_k)
         return UOR_B200_NONCONFORMANT;
-    if ((st = place(ids, 4, &I)) || (st = place(weights, 4, &W))) return st;
+    if ((st = place(ids, 4, dev, &I)) || (st = place(weights, 4, dev, &W))) return st;
     if (bias && bias_len < router->experts) return UOR_B200_DOES_NOT_FIT;
+    if (!at_element(bias, t, router->experts, sizeof(float), dev)) return UOR_B200_INVALID_ARGUMENT;
     uor_b200_route local;
     uor_b200_route* route = clear_route(call, &local);
     if (t == 0) return UOR_B200_OK;
@@ -225,13 +235,13 @@ int uor_b200_expert_route_backward(uor_b200_dtype elem, const uor_b200_router* r
     bool dev = false;
     Operand L, I, G, D;
     int st;
-    if ((st = check_call(call, &dev)) || (st = check_router(router)) || (st = place(logits, dtype_size(elem), &L)))
+    if ((st = check_call(call, &dev)) || (st = check_router(router)) || (st = place(logits, dtype_size(elem), dev, &L)))
         return st;
     const size_t t = logits->rows;
     if (logits->cols != router->experts || ids->rows != t || ids->cols != router->top_k || dweights->rows != t ||
         dweights->cols != router->top_k || dlogits->rows != t || dlogits->cols != router->experts)
         return UOR_B200_NONCONFORMANT;
-    if ((st = place(ids, 4, &I)) || (st = place(dweights, 4, &G)) || (st = place(dlogits, dtype_size(elem), &D)))
+    if ((st = place(ids, 4, dev, &I)) || (st = place(dweights, 4, dev, &G)) || (st = place(dlogits, dtype_size(elem), dev, &D)))
         return st;
     uor_b200_route local;
     uor_b200_route* route = clear_route(call, &local);
@@ -269,15 +279,15 @@ int uor_b200_expert_q4_ffn(uor_b200_dtype elem, uor_b200_dtype out, size_t exper
     bool dev = false;
     Operand X, I, W, Y;
     int st;
-    if ((st = check_call(call, &dev)) || (st = check_q4(up)) || (st = check_q4(down)) || (st = place(x, 2, &X)) ||
-        (st = place(ids, 4, &I)) || (st = place(weights, 4, &W)))
+    if ((st = check_call(call, &dev)) || (st = check_q4(up, dev)) || (st = check_q4(down, dev)) || (st = place(x, 2, dev, &X)) ||
+        (st = place(ids, 4, dev, &I)) || (st = place(weights, 4, dev, &W)))
         return st;
     const size_t t = x->rows, d = x->cols, f = down->cols, k = ids->cols;
     if (experts > 1024) return UOR_B200_UNSUPPORTED;
     if (up->cols != d || up->rows != experts * 2 * f || down->rows != experts * d || ids->rows != t ||
         weights->rows != t || weights->cols != k || y->rows != t || y->cols != d)
         return UOR_B200_NONCONFORMANT;
-    if ((st = place(y, dtype_size(out), &Y))) return st;
+    if ((st = place(y, dtype_size(out), dev, &Y))) return st;
     uor_b200_route local;
     uor_b200_route* route = clear_route(call, &local);
     if (t == 0 || d == 0) return UOR_B200_OK;
