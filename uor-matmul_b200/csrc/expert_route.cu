@@ -38,8 +38,10 @@ __device__ __forceinline__ float warp_sum(float v) {
 // exp(l - top) with the infinities' differences as limits have them: equal ones give 1.
 __device__ __forceinline__ float exp_below(float l, float top) { return l == top ? 1.0f : expf(l - top); }
 
-// Within 3 units: the reciprocal's and the exponential's own, and an addition's.
-__device__ __forceinline__ float sigmoid(float l) { return __fdividef(1.0f, 1.0f + expf(-l)); }
+// 1 / (1 + exp(-l)) within 3 units: the reciprocal's and the exponential's own, and an addition's.
+// The divisor is taken as a fourth, exactly: past 2^126 (logits below -87.3) the quick division
+// gives 0, where the score is a denormal still.
+__device__ __forceinline__ float sigmoid(float l) { return 0.25f * __fdividef(1.0f, fmaf(0.25f, expf(-l), 0.25f)); }
 
 // The chosen experts' shares of their scores' sum; lane s holds choice s (open: whether it is
 // one). They are taken relative to the largest chosen logit, so that scores which underflow
