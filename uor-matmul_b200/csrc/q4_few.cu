@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 3 : 1) few_kerne
 template <typename T, typename S, int SEG, int NT, bool ANY>
 int launch_few(uor_b200_ctx* ctx, FewParams& p, bool early) {
     using B = Block<NT>;
+    p.columns = 8 * NT;
     const int chunks = p.chunks = (p.w.cols + CHUNK - 1) / CHUNK;
     p.groups = (p.w.cols + p.w.group - 1) / p.w.group;
     int64_t cols = few_columns(p);  // of a block, at most
@@ -399,7 +400,7 @@ int by_codes(uor_b200_ctx* ctx, int elem, FewParams& p, bool early) {
 
 }  // namespace
 
-int few_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early) {
+int few_launch(uor_b200_ctx* ctx, int elem, FewParams& p, bool early) {
     int st = UOR_B200_OK;
     if (lean_launch(ctx, elem, p, early, &st)) return st;
     return elem == UOR_B200_BF16 ? by_codes<__nv_bfloat16>(ctx, elem, p, early) : by_codes<__half>(ctx, elem, p, early);

@@ -38,6 +38,7 @@ struct FewParams {
     int codes_align;     // 16 if every row of codes begins at a multiple of 16 bytes
     int x_vec;           // rows of x begin at multiples of 16 bytes
     // Set by the launch:
+    int columns;         // of a pass: 8 or 16
     int panel;           // chunks whose activations are resident
     int k_shift;         // log2 of the warps that share a tile's reduction
     int chunks, panels, groups, tiles;
@@ -47,9 +48,9 @@ struct FewParams {
 
 // early: the launch may begin while the one before it runs; it reads what that wrote (the inner
 // activations) only after its end.
-int few_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early);
+int few_launch(uor_b200_ctx* ctx, int elem, FewParams& p, bool early);
 
 // The same for what lies well (q4_lean.cu): whether it does, and then the launch's status.
-bool lean_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early, int* status);
+bool lean_launch(uor_b200_ctx* ctx, int elem, FewParams& p, bool early, int* status);
 
 }  // namespace uor

@@ -385,8 +385,9 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
         p.n = w.rows;
         p.y = y;
         few_align(&p);
-        route->tile_m = 16, route->tile_n = m > 8 ? 16 : 8, route->tile_k = 256;
-        return few_launch(ctx, elem, p, false);
+        st = few_launch(ctx, elem, p, false);
+        route->tile_m = 16, route->tile_n = p.columns, route->tile_k = 256;
+        return st;
     }
     copy_codes(ctx, &many.w, ws + codes_at);
     many.x = rows.p;
@@ -435,8 +436,8 @@ int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
         p.top_k = a.top_k;
         p.experts = a.experts;
         few_align(&p);
-        route->tile_m = 16, route->tile_n = a.tokens > 8 ? 16 : 8, route->tile_k = 256;
         if ((st = few_launch(ctx, a.elem, p, false))) return st;
+        route->tile_m = 16, route->tile_n = p.columns, route->tile_k = 256;  // the up product's
         p.kind = FEW_PART;
         p.w = a.down;
         p.x = p.h;

@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(Block<NT>::THREADS, NT == 1 ? 2 : 1) lean_kern
 template <typename T, typename S, int SEG, int NT, bool WIDE>
 int launch_lean(uor_b200_ctx* ctx, FewParams& p, int cols, bool early) {
     using B = Block<NT>;
+    p.columns = 8 * NT;
     p.k_shift = __builtin_ctz(B::WARPS);
     while (p.k_shift > 0 && 1 << (p.k_shift - 1) >= p.chunks) --p.k_shift;
     const int rows = p.kind == FEW_UP ? 8 : ROWS;
@@ -315,7 +316,7 @@ bool by_scales(uor_b200_ctx* ctx, int elem, FewParams& p, bool early, int* statu
 
 }  // namespace
 
-bool lean_launch(uor_b200_ctx* ctx, int elem, FewParams p, bool early, int* status) {
+bool lean_launch(uor_b200_ctx* ctx, int elem, FewParams& p, bool early, int* status) {
     if (!p.x_vec || p.w.cols % 8) return false;
     return elem == UOR_B200_BF16 ? by_scales<__nv_bfloat16>(ctx, elem, p, early, status) : by_scales<__half>(ctx, elem, p, early, status);
 }
