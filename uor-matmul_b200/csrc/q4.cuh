@@ -57,6 +57,20 @@ __device__ __forceinline__ void store_f32(void* p, int64_t i, int type, float v)
         static_cast<__half*>(p)[i] = __float2half_rn(v);
 }
 
+// What a sum of codes' products is multiplied by in the end. bfloat16 activations reach f32's own
+// range, and a group's codes, before the scale that makes weights of them, would carry their sum
+// past it: there a code is held as 2^-12 of itself, exactly, so that 128 positions of 15 times the
+// largest activation still fit. Powers of two change no rounding but among f32's denormals: results
+// below 2^-114 keep 2^-137 absolute. Multiplied in the end, it costs nothing that was measured.
+template <typename T>
+struct CodeUnit {
+    static constexpr float VALUE = 1.0f;
+};
+template <>
+struct CodeUnit<__nv_bfloat16> {
+    static constexpr float VALUE = 4096.0f;
+};
+
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 
 // y (m x n) = x (m x k of elem) dequant(w)^T.

@@ -11,7 +11,8 @@
 // The products run on the tensor cores (mma.m16n8k16) with the weights as the 16 rows and up to 8
 // or 16 activation rows as the columns, since CUDA cores could not multiply at the rate the codes
 // arrive at from four rows on. A code is exact as a 16-bit float: its bits under the exponent of
-// 128 (bfloat16) or 1024 (float16), less the same plus the zero point. So the sum of a group is
+// 128 (bfloat16, in units of 2^-12) or 1024 (float16), less the same plus the zero point: the old
+// conversion of small integers by a float whose unit they are. So the sum of a group is
 // exact but for its f32 additions, and the group's scale multiplies it in f32: no weight is ever
 // rounded. The reduction's order within a group is free, so a lane's 16 bytes are taken as they
 // lie: word j of lane c holds positions 32 c + 8 j .. + 7, and the instruction's operands are its

@@ -112,10 +112,10 @@ __device__ __forceinline__ bool item_at(int u, const ManyParams& p, const int* f
     return it->cols > 0 && it->kbs > 0;
 }
 
-// Eight codes of a word, in order, less their zero point, as 16-bit floats.
+// Eight codes of a word, in order, less their zero point, in CodeUnits, as 16-bit floats.
 template <typename T>
 __device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t zero) {
-    constexpr uint32_t HIGH = std::is_same<T, __half>::value ? 0x64u : 0x43u;  // 1024 or 128
+    constexpr uint32_t HIGH = std::is_same<T, __half>::value ? 0x64u : 0x3Du;  // 1024, or 128 of 2^-12
     const uint32_t lo = w & 0x0F0F0F0Fu, hi = (w >> 4) & 0x0F0F0F0Fu;
     const uint32_t a = __byte_perm(lo, hi, 0x5140), b = __byte_perm(lo, hi, 0x7362);
     auto less = [&](uint32_t v) {
@@ -139,7 +139,7 @@ __device__ __forceinline__ uint4 decode8(uint32_t w, uint32_t zero) {
 }
 template <typename T>
 __device__ __forceinline__ uint32_t zero_pair(uint32_t z) {
-    return (std::is_same<T, __half>::value ? 0x64006400u : 0x43004300u) | (z << 16) | z;
+    return (std::is_same<T, __half>::value ? 0x64006400u : 0x3D003D00u) | (z << 16) | z;
 }
 
 // Steps along a row's scales (or zero points) by a piece of a group at a time.
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int c = 0; c < HALF; c += OUT_COLS)
                 if (c < left) {
 #pragma unroll
-                    for (int i = 0; i < OUT_COLS; ++i) swap[i * BM + r] = half_of(acc[(c + i) / 2], i & 1);
+                    for (int i = 0; i < OUT_COLS; ++i) swap[i * BM + r] = CodeUnit<T>::VALUE * half_of(acc[(c + i) / 2], i & 1);
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");
                     sums_out<T>(p, it, swap, pairs_at + c, it.p0 + part * it.half + c, min(OUT_COLS, left - c), r);
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + part) : "memory");

@@ -21,26 +21,26 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t b
     return r;
 }
 
-// A word's eight codes less their zero point, as pairs of 16-bit floats: positions (0, 4),
-// (1, 5), (2, 6), (3, 7).
+// A word's eight codes less their zero point, in CodeUnits, as pairs of 16-bit floats: positions
+// (0, 4), (1, 5), (2, 6), (3, 7).
 template <typename T>
 struct Decode;
 template <>
 struct Decode<__nv_bfloat16> {
-    // 128 + code, less 128 + zero.
+    // 128 + code, less 128 + zero, both of 2^-12.
     struct Zero {
         __nv_bfloat162 v;
     };
-    static constexpr uint32_t ZERO_8 = 0x43084308u;
+    static constexpr uint32_t ZERO_8 = 0x3D083D08u;
     // Of byte i of a word of zero points.
-    __device__ static __forceinline__ uint32_t zero_bits(uint32_t w, int i) { return __byte_perm(w, 0x43, 0x4040 + 0x101 * i); }
+    __device__ static __forceinline__ uint32_t zero_bits(uint32_t w, int i) { return __byte_perm(w, 0x3D, 0x4040 + 0x101 * i); }
     __device__ static __forceinline__ Zero zero(uint32_t b) {
         Zero r;
         memcpy(&r.v, &b, 4);
         return r;
     }
     __device__ static __forceinline__ uint32_t one(uint32_t w, const Zero& z) {
-        const uint32_t b = and_or(w, 0x000F000Fu, 0x43004300u);
+        const uint32_t b = and_or(w, 0x000F000Fu, 0x3D003D00u);
         __nv_bfloat162 v;
         memcpy(&v, &b, 4);
         v = __hsub2(v, z.v);
@@ -430,7 +430,7 @@ __device__ __forceinline__ void tiles_out(const FewParams& p, const Found& found
             const float* at = joined + (ab * kw * NT + (col >> 3)) * 128 + ((row & 7) * 4 + ((col & 7) >> 1)) * 4 + (row >> 3) * 2 + ((col + c) & 1);
             float s = 0;
             for (int w = 0; w < kw; ++w) s += at[w * NT * 128];
-            return s;
+            return CodeUnit<T>::VALUE * s;
         };
         if (p.kind == FEW_UP) {
             // eight inner activations in the operands' order, zeros behind the last; in a second
