@@ -440,9 +440,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 uint4 c[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) c[i] = *reinterpret_cast<const uint4*>(from + q * C_BYTES + ((i << 4) ^ turn));
-                __syncwarp();
-                if (lane == 0) mbar_arrive(cempty + 8 * q);
-                if (++q == CSTAGES) q = 0, qphase ^= 1;
                 uint32_t z[PIECES];
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) z[i] = zero_pair<T>(next[i] & 15u);
@@ -469,7 +466,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive_pair(mapa_shared(afull + 8 * a, 0));
+                // The codes are given back only now that they have been used. Given back behind their
+                // reads alone, which a global access that misses can hold up for microseconds, the next
+                // copy overtook those: its first rows stood in for this stage's, some passes in a
+                // hundred over weights just laid out.
+                if (lane == 0) {
+                    mbar_arrive(cempty + 8 * q);
+                    mbar_arrive_pair(mapa_shared(afull + 8 * a, 0));
+                }
+                if (++q == CSTAGES) q = 0, qphase ^= 1;
             }
         }
     } else {
