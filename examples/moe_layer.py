@@ -30,9 +30,7 @@ def quantize(w, group):
     scales = ((high - low) / 15).clamp(min=1e-8)
     zeros = (-low / scales).round().clamp(0, 15)
     codes = (padded / scales[..., None] + zeros[..., None]).round().clamp(0, 15).to(torch.uint8).view(rows, -1)
-    codes = codes[:, :cols + cols % 2]
-    if codes.shape[1] % 2:  # an odd last column that ends a group
-        codes = torch.nn.functional.pad(codes, (0, 1))
+    codes = codes[:, :cols + cols % 2]  # groups are even: the last byte's other half is there
     packed = (codes[:, 0::2] | codes[:, 1::2] << 4).contiguous()
     return U.Q4(packed.view(-1), scales.view(-1), U.F32, rows, cols, group, zeros=zeros.to(torch.uint8).view(-1))
 

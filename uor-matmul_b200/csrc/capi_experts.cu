@@ -110,7 +110,6 @@ void add_q4(Inputs* in, const uor_b200_q4* w, Q4Dev* q) {
     const size_t scales = w->rows && w->cols ? (w->rows - 1) * w->groups_rs + groups : 0;
     q->row_bytes = static_cast<int64_t>(w->row_bytes);
     q->groups_rs = static_cast<int64_t>(w->groups_rs);
-    q->codes_len = static_cast<int64_t>(codes);
     q->rows = static_cast<int>(w->rows);
     q->cols = static_cast<int>(w->cols);
     q->group = static_cast<int>(w->group);

@@ -14,7 +14,6 @@ struct Q4Dev {
     const void* scales;
     const uint8_t* zeros;  // null: every zero point is 8
     int64_t row_bytes, groups_rs;
-    int64_t codes_len;     // bytes from `codes` that may be read
     int rows, cols, group;
     int scale_type;        // uor_b200_dtype: F32, BF16 or F16
 };

@@ -284,7 +284,6 @@ bool try_lean(uor_b200_ctx* ctx, FewParams& p, bool early, int* status) {
     const uint64_t scales = reinterpret_cast<uint64_t>(p.w.scales) | static_cast<uint64_t>(p.w.groups_rs) * sizeof(S);
     const uint64_t zeros = p.w.zeros ? reinterpret_cast<uint64_t>(p.w.zeros) | static_cast<uint64_t>(p.w.groups_rs) : 0;
     p.quants_vec = scales % VEC == 0 && zeros % N == 0;
-    p.group_shift = __builtin_ctz(SEG);
     p.chunks = (p.w.cols + CHUNK - 1) / CHUNK;
     p.groups = (p.w.cols + SEG - 1) / SEG;
     const int64_t most = few_columns(p);
