@@ -440,8 +440,10 @@ int uor_b200_arena_canonicalize(uor_b200_dtype elem, void *values, size_t len, s
  * codes 0..15 two per byte, low nibble first (the order of Packed<Grid<16>, 2>), a row
  * beginning on a byte of its own; without zero points the zero is 8. This family is not exact
  * like the rest of the library: the products are of 16-bit floats, sums are held in f32 in an
- * order that depends on the shapes alone (the same call gives the same bytes), and the result
- * is rounded once to `out`. Non-finite activations and scales spread as the formula has them.
+ * order that the shapes, strides and alignment of the operands fix (the same call gives the same
+ * bytes), and the result is rounded once to `out`. Non-finite activations and scales spread as the
+ * formula has them; finite ones overflow only where f32 sums of weight times activation do. No
+ * output of this family or the router overlaps an input.
  * Device pointers of this family and the router are multiples of their element's size (codes lie
  * at any byte): INVALID_ARGUMENT otherwise.
  * No reference counterpart: the reference's codecs carry no scales. */
@@ -503,7 +505,8 @@ int uor_b200_expert_route(uor_b200_dtype elem, const uor_b200_router *router,
 
 /* The gradient of the logits (tokens x experts, of elem) from that of the weights (tokens x
  * top_k, f32), with the choice `ids` held fixed: the choice, and so the bias, has no gradient.
- * ids outside [0, experts) take no part; every element of dlogits is written. */
+ * ids outside [0, experts) take no part; every element of dlogits is written. Not in place:
+ * dlogits is no part of logits. */
 int uor_b200_expert_route_backward(uor_b200_dtype elem, const uor_b200_router *router,
                                    const uor_b200_view *logits, const uor_b200_view *ids,
                                    const uor_b200_view *dweights, const uor_b200_view_mut *dlogits,
@@ -515,8 +518,9 @@ int uor_b200_expert_route_backward(uor_b200_dtype elem, const uor_b200_router *r
  * y tokens x d of out (elem or F32). `up` holds every expert's gate rows and then its up rows:
  * experts * 2 f rows of d; `down` experts * d rows of f. ids (int32) and weights (f32) are tokens
  * x top_k; an id outside [0, experts) is skipped, whatever its weight, and a token without any
- * gets zeros. The inner activations are rounded once to elem between the two products; of up to 4
- * tokens a second elem keeps what that left. */
+ * gets zeros. The inner activations are rounded once to elem between the two products, whatever
+ * `out` is, so in float16 what passes 65504 there is infinite (bfloat16 has f32's range); of up to 4
+ * tokens, with up to 1024 choices, a second elem keeps what a finite one's rounding left. */
 int uor_b200_expert_q4_ffn(uor_b200_dtype elem, uor_b200_dtype out, size_t experts,
                            const uor_b200_view *x, const uor_b200_view *ids,
                            const uor_b200_view *weights, const uor_b200_q4 *up,
