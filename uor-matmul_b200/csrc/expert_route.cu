@@ -7,7 +7,7 @@
 // logit or key of -inf or NaN) is key 0, below every open one.
 //
 // Bound by instructions: a token's 256 logits are 1 KB, and some 900 instructions of its warp.
-// 16384 x 256 with groups and a bias: 18.1 us (0.98 TB/s); with a lane's experts 32 apart and every
+// 16384 x 256 with groups and a bias: 18.0 us (0.99 TB/s); with a lane's experts 32 apart and every
 // choice a reduction over them, 52. Its gradient, two rows of memory and eight values: 10.6 us
 // (3.3 TB/s); with every element computed rather than scattered over zeros, 14.6.
 #include <cstring>

@@ -4,11 +4,13 @@
 //
 // q4_few.cu's product and its split, but for the way of the codes: each lane reads its operands'
 // words straight from memory into registers, one chunk ahead, so that there are no copies to
-// place, to wait for and to read back. Instructions are what bounds these products beside the
-// memory (an operand's word takes 11 to unpack), and so are the few microseconds of a launch:
+// place, to wait for and to read back. What bounds these products is latency: four warps a
+// scheduler, 128 registers of each under way, keep a third to half of the issue slots busy (an
+// operand's word takes 11 instructions to unpack), and a launch has its few microseconds of start:
 // activations are asked for first, and nothing is divided on the device. One row: 4096 x 4096 in
-// 6.3 us, 8192 x 8192 with zero points in 15.6 (2.4 TB/s), 17.0 by way of shared memory. 13 x 5003
-// x 4008 with a scale and a zero point per 32 positions: 21.9, of which the bytes are 2.1.
+// 6.3 us, 8192 x 8192 with zero points in 15.7 (2.3 TB/s), 17.0 by way of shared memory. 13 x 5003
+// x 4008 with a scale and a zero point per 32 positions: 21.9, of which the bytes are 2.1; two
+// chunks of 16 scales do not fit the registers beside 16 columns, and 220 bytes a thread are spilled.
 #include "ptx.cuh"
 #include "q4_mma.cuh"
 
