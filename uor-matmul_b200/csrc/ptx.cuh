@@ -379,11 +379,11 @@ __device__ __forceinline__ void mma_f16_pair_ts(uint32_t d_tmem, uint32_t a_tmem
         : "memory");
 }
 
-// The same arrival without a release at cluster scope, for what passes through tensor memory
-// alone: there tcgen05.wait and tcgen05.fence order it, and the release's fence would hold the
-// arriving warp for some 2000 cycles.
+// The same arrival without the release, for what passes through tensor memory alone: there
+// tcgen05.wait and tcgen05.fence order it, and the release's fence would hold the arriving warp for
+// some 2000 cycles.
 __device__ __forceinline__ void mbar_arrive_pair(uint32_t cluster_addr) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // Arrive once on the barrier at the same offset in every CTA of `mask` when the pair's
