@@ -113,7 +113,8 @@ typedef enum uor_b200_kernel {
     UOR_B200_KERNEL_EPILOGUE_ONLY = 6, /* k == 0: C := encode(beta * C) */
     UOR_B200_KERNEL_SKINNY = 7,        /* <= 16 rows or columns: dp4a reduce / column kernels */
     UOR_B200_KERNEL_Q4 = 8,            /* 4-bit weights with group scales */
-    UOR_B200_KERNEL_ROUTER = 9         /* the experts' router and its gradient */
+    UOR_B200_KERNEL_ROUTER = 9,        /* the experts' router and its gradient */
+    UOR_B200_KERNEL_KV4 = 10           /* a 4-bit cache of keys and values, and its attention */
 } uor_b200_kernel;
 
 typedef struct uor_b200_route {
@@ -467,6 +468,123 @@ typedef struct uor_b200_q4 {
  * encode NEAREST is supported. */
 int uor_b200_q4_gemm(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_view *a,
                      const uor_b200_q4 *w, const uor_b200_view_mut *c, const uor_b200_call *call);
+
+typedef enum uor_b200_activation {
+    UOR_B200_IDENTITY = 0,
+    UOR_B200_RELU = 1,      /* max(v, 0); NaN stays NaN */
+    UOR_B200_GELU = 2,      /* v / 2 (1 + erf(v / sqrt 2)) */
+    UOR_B200_GELU_TANH = 3, /* v / 2 (1 + tanh(sqrt(2 / pi) (v + 0.044715 v^3))) */
+    UOR_B200_SILU = 4       /* v / (1 + exp(-v)) */
+} uor_b200_activation;
+
+/* q4_gemm with what follows a product in a layer, in f32 before the one rounding:
+ *   C := act(A dequant(W)^T + bias) + residual.
+ * bias: n elements of bias_type (elem or F32) one after another, or NULL. residual: m x n of `out`,
+ * or NULL; it may be C itself (the same elements in the same order: the stream that a projection is
+ * added to) and is otherwise no part of C. k == 0 gives act(bias) + residual. */
+int uor_b200_q4_linear(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_view *a,
+                       const uor_b200_q4 *w, const void *bias, size_t bias_len,
+                       uor_b200_dtype bias_type, uint32_t activation,
+                       const uor_b200_view *residual, const uor_b200_view_mut *c,
+                       const uor_b200_call *call);
+
+/* ---------------------------------- keys and values in 4 bits, and attention */
+
+/* A cache of keys and values in 4 bits, in pages of page_size tokens. Every token and head has, of
+ * its key and of its value, a code (0 .. 15) per channel, and per `group` channels a scale and a
+ * middle of elem:
+ *   x = mid + scale (code - 7.5).
+ * The pool holds `pages` pages of uor_b200_kv4_page_bytes bytes. Its order is the library's own: per
+ * page and head blocks of 16 tokens, in each the keys' codes, their scales and middles, then the
+ * values' (kv4.cuh); uor_b200_kv4_append writes it and uor_b200_kv4_read gives it back. Device memory,
+ * at a multiple of 16 bytes. What it held before a token was appended does not matter. */
+typedef struct uor_b200_kv4 {
+    uint8_t *pool;
+    size_t pool_len;     /* bytes */
+    size_t pages;        /* at most 2^31 - 1 */
+    uint32_t page_size;  /* a power of two, 16 .. 4096 */
+    uint32_t heads;      /* of keys and values, 1 .. 1024 */
+    uint32_t dim;        /* channels of a head: 64, 96, 128, 192 or 256 */
+    uint32_t group;      /* 32, 64, 128 or 256, a divisor of dim */
+    uint32_t elem;       /* BF16 or F16 */
+} uor_b200_kv4;
+
+/* Bytes of a page; 0 for a shape outside the limits above. */
+size_t uor_b200_kv4_page_bytes(const uor_b200_kv4 *cache);
+
+/* The sequences of a call. Sequence s has the rows starts[s] .. starts[s + 1] - 1 of the call's
+ * matrices: its newest tokens. lengths[s] counts its tokens in the cache, those rows among them, so
+ * its first row is at position lengths[s] - (starts[s + 1] - starts[s]). table[s * table_rs + i] is the
+ * page with its positions i page_size and on. All are device memory, read when the work runs: a
+ * captured call follows what they hold at its replay. Rows outside every sequence are not read, and
+ * of outputs left as they were.
+ * What a call cannot know beforehand is safe all the same: of starts that do not rise or pass the
+ * rows, rows outside take no part; a position below 0, past the table or on a page outside the pool
+ * holds no token. Where two tokens of one call fall on one place (two sequences with one page), it
+ * holds either's codes and scales, in any mixture. */
+typedef struct uor_b200_batch {
+    size_t seqs;            /* at most 4096 */
+    const int32_t *starts;  /* seqs + 1 */
+    size_t starts_len;
+    const int32_t *lengths; /* seqs */
+    size_t lengths_len;
+    const int32_t *table;   /* seqs x table_cols */
+    size_t table_len;
+    size_t table_cols;      /* pages: table_cols * page_size is at most 2^30 - 1 */
+    size_t table_rs;
+} uor_b200_batch;
+
+/* The rotation of positions: of the first `dims` channels of a head (an even number, at most dim) the
+ * pairs (x_i, x_{i + dims / 2}), or where interleaved (x_{2 i}, x_{2 i + 1}), become
+ *   (x cos[p][i] - y sin[p][i],  y cos[p][i] + x sin[p][i])
+ * at position p, from tables of f32 of dims / 2 columns, row p at p * rs. */
+typedef struct uor_b200_rotation {
+    const float *cos, *sin;
+    size_t len;          /* elements of each table */
+    size_t positions;    /* rows: at least table_cols * page_size of the call's batch */
+    size_t rs;
+    uint32_t dims;
+    uint32_t interleaved; /* 0 or 1 */
+} uor_b200_rotation;
+
+/* Rotates the rows' keys, brings keys and values to 4 bits and puts them into the cache at their
+ * positions; where q is given, q_out receives the rows' queries, rotated (it may be q itself: the same
+ * elements in the same order). k and v are rows x (heads * dim) of elem, q and q_out rows x
+ * (q_heads * dim); rows of any stride with their elements side by side (UNSUPPORTED else), so a fused
+ * projection's output serves for all three. rotation NULL: none.
+ * A rotated value is rounded to f32 and then to elem. Of every group of channels of a head, with its
+ * greatest value h and its least l, in f32 steps each rounded once:
+ *   mid = elem(h / 2 + l / 2), scale = elem((h / 2 - l / 2) / 7.5),
+ *   code = the integer nearest to (x - mid) / scale + 7.5 (half to even) within 0 .. 15; 0 where the
+ *   scale is 0.
+ * A key or value that is not finite has no place in a range of 15 steps: an infinity counts as elem's
+ * largest value of its sign, NaN as 0, so that no row's attention depends on a token it does not see.
+ * Device pointers only (call->flags DEVICE_POINTERS). */
+int uor_b200_kv4_append(uor_b200_dtype elem, const uor_b200_kv4 *cache, const uor_b200_batch *batch,
+                        const uor_b200_view *k, const uor_b200_view *v, const uor_b200_view *q,
+                        const uor_b200_view_mut *q_out, const uor_b200_rotation *rotation,
+                        const uor_b200_call *call);
+
+/* What the cache holds of the batch's rows' tokens, rounded to f32 and then to out (the cache's elem,
+ * or F32): with starts that count whole sequences, all of them. Rows of tokens that it does not hold
+ * are left as they were. Device pointers only. */
+int uor_b200_kv4_read(uor_b200_dtype out, const uor_b200_kv4 *cache, const uor_b200_batch *batch,
+                      const uor_b200_view_mut *k, const uor_b200_view_mut *v,
+                      const uor_b200_call *call);
+
+/* Causal attention of the batch's rows over the cache:
+ *   y = sum_j softmax_j(scale q . k_j) v_j
+ * for each of the q_heads heads of q (rows x (q_heads * dim) of elem), query head a reading the keys
+ * and values of head a / (q_heads / heads), over the positions j of its sequence that its row, at
+ * position p, sees: j <= p, and with window > 0 only j > p - window or j < sinks. y is rows x
+ * (q_heads * dim) of out (elem or F32); lse, rows x q_heads of F32 or NULL, the natural logarithm of the
+ * row's sum of exponentials. A row that sees nothing has zeros and an lse of -inf. Rows of any
+ * stride with their elements side by side. No output overlaps an input. Scores, sums and statistics
+ * are f32. Queries are taken as they are (kv4_append rotates them). Device pointers only. */
+int uor_b200_kv4_attention(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_kv4 *cache,
+                           const uor_b200_batch *batch, const uor_b200_view *q, float scale,
+                           uint32_t window, uint32_t sinks, const uor_b200_view_mut *y,
+                           const uor_b200_view_mut *lse, const uor_b200_call *call);
 
 /* ------------------------------------------------ mixture of experts */
 

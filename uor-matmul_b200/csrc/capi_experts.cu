@@ -149,7 +149,14 @@ extern "C" {
 
 int uor_b200_q4_gemm(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_view* a, const uor_b200_q4* w,
                      const uor_b200_view_mut* c, const uor_b200_call* call) {
-    if (!a || !c) return UOR_B200_INVALID_ARGUMENT;
+    return uor_b200_q4_linear(elem, out, a, w, nullptr, 0, UOR_B200_F32, UOR_B200_IDENTITY, nullptr, c, call);
+}
+
+int uor_b200_q4_linear(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_view* a, const uor_b200_q4* w, const void* bias,
+                       size_t bias_len, uor_b200_dtype bias_type, uint32_t activation, const uor_b200_view* residual,
+                       const uor_b200_view_mut* c, const uor_b200_call* call) {
+    if (!a || !c || activation > UOR_B200_SILU) return UOR_B200_INVALID_ARGUMENT;
+    if (bias && bias_type != elem && bias_type != UOR_B200_F32) return UOR_B200_UNSUPPORTED;
     if (!half_type(elem) || (out != elem && out != UOR_B200_F32)) return UOR_B200_UNSUPPORTED;
     bool dev = false;
     Operand A, C;
@@ -157,6 +164,15 @@ int uor_b200_q4_gemm(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_vie
     if ((st = check_call(call, &dev)) || (st = check_q4(w, dev)) || (st = place(a, 2, dev, &A))) return st;
     if (a->cols != w->cols || c->rows != a->rows || c->cols != w->rows) return UOR_B200_NONCONFORMANT;
     if ((st = place(c, dtype_size(out), dev, &C))) return st;
+    Operand R;
+    if (residual) {
+        if (residual->rows != c->rows || residual->cols != c->cols) return UOR_B200_NONCONFORMANT;
+        if ((st = place(residual, dtype_size(out), dev, &R))) return st;
+        // C itself, element by element, or no part of it
+        if (R.origin == C.origin && ((R.rows > 1 && R.rs != C.rs) || (R.cols > 1 && R.cs != C.cs))) return UOR_B200_INVALID_ARGUMENT;
+    }
+    if (bias && bias_len < w->rows) return UOR_B200_DOES_NOT_FIT;
+    if (bias && !at_element(bias, a->rows, w->rows, dtype_size(bias_type), dev)) return UOR_B200_INVALID_ARGUMENT;
     uor_b200_route local;
     uor_b200_route* route = clear_route(call, &local);
     if (a->rows == 0 || w->rows == 0) return UOR_B200_OK;
@@ -171,9 +187,18 @@ int uor_b200_q4_gemm(uor_b200_dtype elem, uor_b200_dtype out, const uor_b200_vie
     Q4Dev q{};
     in.add(A, &x.p);
     add_q4(&in, w, &q);
+    Epilogue e{};
+    e.act = static_cast<int>(activation);
+    e.bias_type = bias_type;
+    if (bias) in.add(bias, w->rows * dtype_size(bias_type), &e.bias);
+    if (residual) {
+        e.residual = Mat{nullptr, R.rs, R.cs};
+        in.add(R, &e.residual.p);
+    }
+    e.on = bias || residual || activation != UOR_B200_IDENTITY;
     OutStage cs;
     if ((st = in.copy()) || (st = stage_out_begin(ctx, C, dev, false, &cs))) return st;
-    if ((st = run_q4_gemm(ctx, elem, x, static_cast<int64_t>(a->rows), q, MatOut{cs.dev_origin, C.rs, C.cs, out},
+    if ((st = run_q4_gemm(ctx, elem, x, static_cast<int64_t>(a->rows), q, e, MatOut{cs.dev_origin, C.rs, C.cs, out},
                           route)))
         return st;
     if ((st = stage_out_end(ctx, cs))) return st;

@@ -72,8 +72,35 @@ struct CodeUnit<__nv_bfloat16> {
 
 __device__ __forceinline__ float silu(float v) { return v / (1.0f + expf(-v)); }
 
-// y (m x n) = x (m x k of elem) dequant(w)^T.
-int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4Dev& w, const MatOut& y,
+// What follows a product before its rounding (uor_b200_q4_linear): act(v + bias[j]) + residual[i][j].
+// Where `on` is 0 there is none of it.
+struct Epilogue {
+    int on;
+    int act;             // uor_b200_activation
+    const void* bias;    // null: none
+    int bias_type;
+    Mat residual;        // of the output's type; p null: none
+};
+__device__ __forceinline__ float activate(float v, int act) {
+    switch (act) {
+    case UOR_B200_RELU: return v < 0.0f ? 0.0f : v;
+    case UOR_B200_GELU: return 0.5f * v * erfcf(-0.70710678118654752f * v);  // 1 + erf, its tail included
+    case UOR_B200_GELU_TANH:  // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z))
+        return v / (1.0f + expf(-1.5957691216057308f * fmaf(0.044715f * v * v, v, v)));
+    case UOR_B200_SILU: return silu(v);
+    default: return v;
+    }
+}
+// The output at (i, j) from its product.
+__device__ __forceinline__ float follow_up(const Epilogue& e, int type, int64_t i, int64_t j, float v) {
+    if (e.bias) v += load_f32(e.bias, j, e.bias_type);
+    v = activate(v, e.act);
+    if (e.residual.p) v += load_f32(e.residual.p, i * e.residual.rs + j * e.residual.cs, type);
+    return v;
+}
+
+// y (m x n) = x (m x k of elem) dequant(w)^T, and what follows it.
+int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4Dev& w, const Epilogue& e, const MatOut& y,
                 uor_b200_route* route);
 
 // The experts' gated feed-forward layer (uor_b200_expert_q4_ffn).

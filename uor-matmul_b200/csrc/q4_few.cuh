@@ -29,6 +29,7 @@ struct FewParams {
     int64_t m;           // dense: rows of x
     int n;               // outputs of a matrix: w.rows, f or d
     MatOut y;            // dense
+    Epilogue e;          // dense
     Mat ids;             // experts
     int tokens, top_k, experts;
     void* h;             // up: [tokens * top_k][1 + twice][h_rs], every eight in the operands' order

@@ -168,7 +168,7 @@ __device__ __forceinline__ float4 load4(const float* row, int j, int n, bool vec
 
 // y[i][j] = the parts' sum, in their order (no parts: 0). A block's x takes 1024 outputs of a
 // row, its y strides the rows.
-__global__ void add_parts_kernel(const float* part, int splits, int64_t rows, int n, MatOut y) {
+__global__ void add_parts_kernel(const float* part, int splits, int64_t rows, int n, const __grid_constant__ Epilogue e, MatOut y) {
     follow();
     const int j = (blockIdx.x * blockDim.x + threadIdx.x) * 4;
     if (j >= n) return;
@@ -177,6 +177,11 @@ __global__ void add_parts_kernel(const float* part, int splits, int64_t rows, in
         for (int s = 0; s < splits; ++s) {
             const float4 a = load4(part + (s * rows + i) * n, j, n, n % 4 == 0);
             v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+        }
+        if (e.on) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (j + k < n) v[k] = follow_up(e, y.type, i, j + k, v[k]);
         }
         store4(y, i, j, n, v);
     }
@@ -341,16 +346,16 @@ bool few_experts(const FfnArgs& a) {
                                       static_cast<int64_t>(a.d) * a.f <= 192000000 / (pairs + a.experts));
 }
 
-int zeros_out(uor_b200_ctx* ctx, int64_t rows, int n, const MatOut& y) {
-    return launch(ctx, blocks_of_rows(rows, n), false, add_parts_kernel, nullptr, 0, rows, n, y);
+int zeros_out(uor_b200_ctx* ctx, int64_t rows, int n, const Epilogue& e, const MatOut& y) {
+    return launch(ctx, blocks_of_rows(rows, n), false, add_parts_kernel, nullptr, 0, rows, n, e, y);
 }
 
 }  // namespace
 
-int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4Dev& w, const MatOut& y,
+int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4Dev& w, const Epilogue& e, const MatOut& y,
                 uor_b200_route* route) {
     route->kernel = UOR_B200_KERNEL_Q4;
-    if (w.cols == 0) return zeros_out(ctx, m, w.rows, y);
+    if (w.cols == 0) return zeros_out(ctx, m, w.rows, e, y);
     int st = UOR_B200_OK;
     const bool few = few_rows(m, w);
     Pieces pieces;
@@ -364,6 +369,7 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     many.experts = 1;
     many.m = static_cast<int>(m);
     many.y = y;
+    many.e = e;
     many.part_rows = m;
     const int splits = few ? 1 : many_splits(ctx, many);
     const size_t codes_at = pieces.add(few ? 0 : codes_copy_bytes(w));
@@ -384,6 +390,7 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
         p.m = m;
         p.n = w.rows;
         p.y = y;
+        p.e = e;
         few_align(&p);
         st = few_launch(ctx, elem, p, false);
         route->tile_m = 16, route->tile_n = p.columns, route->tile_k = 256;
@@ -398,14 +405,14 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     route->k_chunks = splits;
     if ((st = many_launch(ctx, elem, many, own_rows || codes_copy_bytes(w) > 0))) return st;
     if (splits > 1) {
-        return launch(ctx, blocks_of_rows(m, w.rows), true, add_parts_kernel, many.part, splits, m, w.rows, y);
+        return launch(ctx, blocks_of_rows(m, w.rows), true, add_parts_kernel, many.part, splits, m, w.rows, e, y);
     }
     return UOR_B200_OK;
 }
 
 int run_expert_ffn(uor_b200_ctx* ctx, const FfnArgs& a, uor_b200_route* route) {
     route->kernel = UOR_B200_KERNEL_Q4;
-    if (a.top_k == 0 || a.f == 0) return zeros_out(ctx, a.tokens, a.d, a.y);
+    if (a.top_k == 0 || a.f == 0) return zeros_out(ctx, a.tokens, a.d, Epilogue{}, a.y);
     int st = UOR_B200_OK;
     const int64_t pairs = a.tokens * a.top_k;
     const int h_rs = up_to(a.f, 8), x_rs = up_to(a.d, 8);

@@ -193,9 +193,16 @@ __device__ __noinline__ void sums_out(const ManyParams& p, const Item& it, const
     const int64_t rs = parts ? p.n : p.y.rs, step = parts ? 1 : p.y.cs;
     void* to = parts ? p.part + it.split * p.part_rows * p.n : p.y.p;
     for (int c = r >> 4; c < cols && valid > 0; c += 8) {
-        const float4 a = *reinterpret_cast<const float4*>(swap + c * BM + j);
-        const float4 b = *reinterpret_cast<const float4*>(swap + c * BM + j + 4);
+        float4 a = *reinterpret_cast<const float4*>(swap + c * BM + j);
+        float4 b = *reinterpret_cast<const float4*>(swap + c * BM + j + 4);
         const int64_t i = p.mode == MANY_DOWN ? pairs[c] : i0 + c;
+        if (p.e.on && !parts) {
+            float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < valid) v[k] = follow_up(p.e, type, i, it.j0 + j + k, v[k]);
+            a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]);
+        }
         const int64_t at = i * rs + (it.j0 + j) * step;
         char* first = static_cast<char*>(to) + at * (type == UOR_B200_F32 ? 4 : 2);
         if (valid == 8 && step == 1 && reinterpret_cast<uint64_t>(first) % 16 == 0) {
@@ -216,7 +223,10 @@ __device__ __noinline__ void sums_out(const ManyParams& p, const Item& it, const
                 *reinterpret_cast<uint4*>(first) = w;
             }
         } else {
-            for (int k = 0; k < valid; ++k) store_f32(to, at + k * step, type, swap[c * BM + j + k]);
+            const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < valid) store_f32(to, at + k * step, type, v[k]);
         }
     }
 }

@@ -24,6 +24,7 @@ struct ManyParams {
     const int* perm;      // the pair behind each sorted row
     int m;                // dense: rows of x
     MatOut y;             // dense, without splits
+    Epilogue e;           // dense, without splits
     float* part;          // dense with splits: [splits][m][n]; down: [splits][pairs][n]
     int64_t part_rows;    // m or pairs
     void* h;              // up: [sorted rows][h_rs]

@@ -446,7 +446,8 @@ __device__ __forceinline__ void tiles_out(const FewParams& p, const Found& found
             if (p.kind == FEW_PART)
                 p.part[static_cast<int64_t>(found.list[(c0 + col) >> twice]) * p.n + out] = twice ? sum(r) + sum(r, 1) : sum(r);
             else
-                store_f32(p.y.p, (x0 + col) * p.y.rs + out * p.y.cs, p.y.type, sum(r));
+                store_f32(p.y.p, (x0 + col) * p.y.rs + out * p.y.cs, p.y.type,
+                          p.e.on ? follow_up(p.e, p.y.type, x0 + col, out, sum(r)) : sum(r));
         }
     }
 }

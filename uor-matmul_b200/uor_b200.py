@@ -26,7 +26,7 @@ I8, I16, I32, I64, I128, F32, F64, TROP_I8, TROP_I16, TROP_I32, TROP_I64, BF16, 
 DEVICE_POINTERS, ASYNC, DIGIT_SLICES, MODULAR, CODEC_ON_CHIP = 1, 2, 4, 8, 16
 KERNEL_NAMES = {0: "none", 1: "i8_tcgen05", 2: "limb_tcgen05", 3: "tropical",
                 4: "coded_tcgen05", 5: "float_exact", 6: "epilogue_only", 7: "skinny_dp4a",
-                8: "q4", 9: "router"}
+                8: "q4", 9: "router", 10: "kv4"}
 
 DTYPE_SIZE = {I8: 1, I16: 2, I32: 4, I64: 8, I128: 16, F32: 4, F64: 8,
               TROP_I8: 2, TROP_I16: 4, TROP_I32: 8, TROP_I64: 16, BF16: 2, F16: 2}
@@ -132,6 +132,68 @@ class Q4(ctypes.Structure):
         self.arrays, self.on_device = (codes, scales, zeros), dev
 
 
+IDENTITY, RELU, GELU, GELU_TANH, SILU = range(5)
+
+
+class KV4(ctypes.Structure):
+    """uor_b200_kv4: a cache of keys and values in 4 bits, pages of page_size tokens in `pool`, CUDA
+    bytes. Holds the pool, so one descriptor serves as long as its program keeps it."""
+    _fields_ = [("pool", ctypes.c_void_p), ("pool_len", ctypes.c_size_t), ("pages", ctypes.c_size_t),
+                ("page_size", ctypes.c_uint32), ("heads", ctypes.c_uint32), ("dim", ctypes.c_uint32),
+                ("group", ctypes.c_uint32), ("elem", ctypes.c_uint32)]
+
+    def __init__(self, pool, pages, page_size, heads, dim, group, elem):
+        p, n, dev = _typed(pool, I8)
+        _all_on_device(dev)
+        super().__init__(p, n, pages, page_size, heads, dim, group, elem)
+        self.arrays = pool
+
+
+def kv4_page_bytes(page_size, heads, dim, group, elem):
+    """Bytes that a page of such a cache takes in its pool; 0 for a shape outside its limits."""
+    return lib().uor_b200_kv4_page_bytes(ctypes.byref(_kv4_shape(page_size, heads, dim, group, elem)))
+
+
+def _kv4_shape(page_size, heads, dim, group, elem):
+    c = KV4.__new__(KV4)
+    ctypes.Structure.__init__(c, None, 0, 0, page_size, heads, dim, group, elem)
+    return c
+
+
+class Batch(ctypes.Structure):
+    """uor_b200_batch: the sequences of a call. starts (seqs + 1), lengths (seqs) and table (seqs x
+    table_cols pages) are int32 CUDA tensors that the work reads when it runs."""
+    _fields_ = [("seqs", ctypes.c_size_t), ("starts", ctypes.c_void_p), ("starts_len", ctypes.c_size_t),
+                ("lengths", ctypes.c_void_p), ("lengths_len", ctypes.c_size_t),
+                ("table", ctypes.c_void_p), ("table_len", ctypes.c_size_t),
+                ("table_cols", ctypes.c_size_t), ("table_rs", ctypes.c_size_t)]
+
+    def __init__(self, starts, lengths, table, seqs, table_cols, table_rs=None):
+        (ps, ls, ds), (pl, ll, dl), (pt, lt, dt) = (_typed(x, I32) for x in (starts, lengths, table))
+        _all_on_device(ds, dl, dt)
+        super().__init__(seqs, ps, ls, pl, ll, pt, lt, table_cols, table_cols if table_rs is None else table_rs)
+        self.arrays = starts, lengths, table
+
+
+class Rotation(ctypes.Structure):
+    """uor_b200_rotation: cosines and sines (positions x dims / 2, float32 CUDA tensors) of the
+    rotation of the first `dims` channels of a head."""
+    _fields_ = [("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("len", ctypes.c_size_t),
+                ("positions", ctypes.c_size_t), ("rs", ctypes.c_size_t), ("dims", ctypes.c_uint32),
+                ("interleaved", ctypes.c_uint32)]
+
+    def __init__(self, cos, sin, positions, dims, interleaved=False, rs=None):
+        (pc, lc, dc), (ps, ls, ds) = _typed(cos, F32), _typed(sin, F32)
+        _all_on_device(dc, ds)
+        super().__init__(pc, ps, min(lc, ls), positions, dims // 2 if rs is None else rs, dims, int(interleaved))
+        self.arrays = cos, sin
+
+
+def _all_on_device(*devs):
+    if not all(devs):
+        raise UorError(INVALID_ARGUMENT, "a cache and what goes in and out of it are CUDA tensors")
+
+
 SOFTMAX, SIGMOID = range(2)
 
 
@@ -213,6 +275,13 @@ def lib():
             "uor_b200_nccl_comm_init": ([P, I, P, Z, I, ctypes.POINTER(P)], I),
             "uor_b200_nccl_comm_destroy": ([P], I),
             "uor_b200_q4_gemm": ([I, I, VP, ctypes.POINTER(Q4), VP, CP], I),
+            "uor_b200_q4_linear": ([I, I, VP, ctypes.POINTER(Q4), P, Z, I, U32, VP, VP, CP], I),
+            "uor_b200_kv4_page_bytes": ([ctypes.POINTER(KV4)], Z),
+            "uor_b200_kv4_append": ([I, ctypes.POINTER(KV4), ctypes.POINTER(Batch), VP, VP, VP, VP,
+                                     ctypes.POINTER(Rotation), CP], I),
+            "uor_b200_kv4_read": ([I, ctypes.POINTER(KV4), ctypes.POINTER(Batch), VP, VP, CP], I),
+            "uor_b200_kv4_attention": ([I, I, ctypes.POINTER(KV4), ctypes.POINTER(Batch), VP,
+                                        ctypes.c_float, U32, U32, VP, VP, CP], I),
             "uor_b200_expert_route": ([I, ctypes.POINTER(Router), VP, P, Z, VP, VP, CP], I),
             "uor_b200_expert_route_backward": ([I, ctypes.POINTER(Router), VP, VP, VP, VP, CP], I),
             "uor_b200_expert_q4_ffn": ([I, I, Z, VP, VP, VP, ctypes.POINTER(Q4),
@@ -587,6 +656,60 @@ def q4_gemm(elem, out, a, av, w, c, cv, ctx=None, route=None, asynchronous=False
     (C, dc) = _placed(c, cv, _out_type(elem, out))
     call = make_call(NEAREST, _same_place(w.on_device, da, dc), ctx, route, asynchronous)
     _check(lib().uor_b200_q4_gemm(elem, out, A, w, C, call), "q4_gemm")
+
+
+def q4_linear(elem, out, a, av, w, c, cv, bias=None, activation=IDENTITY, residual=None, rv=None,
+              ctx=None, route=None, asynchronous=False):
+    """C := act(A dequant(W)^T + bias) + residual: bias one value per row of W, of elem or float32,
+    residual like C (it may be C itself), each None for none."""
+    (A, da) = _placed(a, av, elem if elem in (BF16, F16) else None)
+    of = _out_type(elem, out)
+    (C, dc) = _placed(c, cv, of)
+    (R, dr) = _placed(residual, cv if rv is None else rv, of) if residual is not None else (None, dc)
+    bias_type = F32 if bias is None or _fits(getattr(bias, "dtype", None), F32) else elem
+    pb, lb, db = _typed(bias, bias_type if bias_type in (F32, BF16, F16) else None) if bias is not None else (None, 0, dc)
+    call = make_call(NEAREST, _same_place(w.on_device, da, dc, dr, db), ctx, route, asynchronous)
+    _check(lib().uor_b200_q4_linear(elem, out, A, w, pb, lb, bias_type, activation, R, C, call), "q4_linear")
+
+
+# ------------------------------------------------------------------ 4-bit keys and values
+
+def _rows_of(buf, v, t):
+    """_placed of a CUDA tensor."""
+    placed, dev = _placed(buf, v, t)
+    _all_on_device(dev)
+    return placed
+
+
+def kv4_append(elem, cache, batch, k, kv, v, vv, q=None, qv=None, q_out=None, ov=None, rotation=None,
+               ctx=None, route=None, asynchronous=False):
+    """The batch's rows of k and v (rows x heads * dim) into the cache, keys rotated by their
+    positions, and q (rows x query heads * dim), where given, rotated into q_out (or in place)."""
+    of = elem if elem in (BF16, F16) else None
+    K, V = _rows_of(k, kv, of), _rows_of(v, vv, of)
+    Q, O = (None if x is None else _rows_of(x, xv, of) for x, xv in ((q, qv), (q_out, ov)))
+    call = make_call(NEAREST, True, ctx, route, asynchronous)
+    _check(lib().uor_b200_kv4_append(elem, cache, batch, K, V, Q, O, rotation, call), "kv4_append")
+
+
+def kv4_read(out, cache, batch, k, kv, v, vv, ctx=None, route=None, asynchronous=False):
+    """What the cache holds of the batch's rows' tokens, as its own type or float32."""
+    of = out if out in (cache.elem, F32) else None
+    K, V = _rows_of(k, kv, of), _rows_of(v, vv, of)
+    call = make_call(NEAREST, True, ctx, route, asynchronous)
+    _check(lib().uor_b200_kv4_read(out, cache, batch, K, V, call), "kv4_read")
+
+
+def kv4_attention(elem, out, cache, batch, q, qv, y, yv, scale=None, window=0, sinks=0, lse=None, lv=None,
+                  ctx=None, route=None, asynchronous=False):
+    """Causal attention of the batch's rows q (rows x query heads * dim) over the cache, within a
+    window of positions (0: all) and the first `sinks`; scale None: dim ** -0.5. lse (float32, rows x
+    query heads), where given, receives the logarithms of the rows' sums of exponentials."""
+    Q, Y = _rows_of(q, qv, elem if elem in (BF16, F16) else None), _rows_of(y, yv, _out_type(elem, out))
+    L = None if lse is None else _rows_of(lse, lv, F32)
+    call = make_call(NEAREST, True, ctx, route, asynchronous)
+    _check(lib().uor_b200_kv4_attention(elem, out, cache, batch, Q, cache.dim ** -0.5 if scale is None else scale,
+                                        window, sinks, Y, L, call), "kv4_attention")
 
 
 def expert_route(elem, router, logits, lv, bias, ids, iv, weights, wv, ctx=None, route=None,
