@@ -7,9 +7,16 @@ largest is M in size, |mid| <= M and scale <= 2 M / 14, so every term that the k
 Scores: sums of dim products in f32, none chained more than dim / 8 + 16 times: off by at most
 (dim / 8 + 16) 2^-23 scale sum |q| 6 M. Weights carry that and 2^-20 for the exponential, twice (their
 sum divides them). Values: weights times scales travel as two bfloat16, 2^-17 together, and f32 sums
-chain at most a block of 16 tokens at a time: (n / 16 + 64) 2^-23. Where keys, values and weights are
-rounded to 16 bits (many rows), half a unit of that type is added to each: to the scores of |q| |k|, to
-the weights and to the values. The output's own rounding is half a unit more."""
+chain at most a block of 16 tokens at a time: (n / 16 + 64) 2^-23.
+
+For a 16-bit result the products of codes run with offsets of up to 64 |q| until a group's end: terms
+of 16 * 65 scale |q| <= 150 M |q|, in sums of 32 channels that are added four times at most, 4 2^-23
+of them more. Queries are float16 then, of 2^-25 of a row's largest where they are less than 2^-14 of
+it. And weights times scales are rounded twice to bfloat16, 2 2^-8 of scale |code - 7.5| <= 1.1 M, and
+once, half a unit, beside the middles.
+
+Where keys, values and weights are rounded to 16 bits (many rows), half a unit of that type is added to
+each: to the scores of |q| |k|, to the weights and to the values. The output's own rounding is half a unit more."""
 import math
 
 import numpy as np
@@ -137,12 +144,17 @@ def attention(cache, q, share, scale, out, window=0, sinks=0, rounded=False, key
             y[start:start + n, h] = share_of @ v
             lse[start:start + n, h] = (top + torch.log(total))[:, 0]
             off = (dim / 8 + 16) * 2.0 ** -23 * abs(scale) * (x.abs() @ biggest(k).T)
+            if out != U.F32:
+                off = off + abs(scale) * (4 * 2.0 ** -23 * (x.abs() @ (25 * biggest(k)).T)
+                                          + 2.0 ** -25 * x.abs().amax(1, keepdim=True) * biggest(k).sum(1)[None])
             if rounded:
                 off = off + unit * abs(scale) * (x.abs() @ k.abs().T)
             off = off.masked_fill(~ok, 0.0) + s.abs().masked_fill(~ok, 0.0) * 2.0 ** -22
             worst = off.amax(1, keepdim=True) if there else torch.zeros(n, 1, device="cuda").double()
             by = 2 * torch.expm1(worst) + 2.0 ** -19 + 2.0 ** -16 + (there / 16 + 64) * 2.0 ** -23 + (3 * unit if rounded else 0.0)
             y_off[start:start + n, h] = by * (share_of @ biggest(v))
+            if out != U.F32 and not rounded:
+                y_off[start:start + n, h] += (2.2 * 2.0 ** -8 + unit) * (share_of @ (biggest(v) / 6))
             if rounded:  # a score's own error is as a rule far below the worst; values and weights 3 units of what they hold
                 y_off[start:start + n, h] = ((2 * torch.expm1(worst) + 3 * unit) * (share_of @ v.abs())
                                              + (2.0 ** -16 + (there / 16 + 64) * 2.0 ** -23) * (share_of @ biggest(v)))

@@ -33,6 +33,7 @@ int check_cache(const uor_b200_kv4* c, KvDev* kv) {
     size_t all;
     if (__builtin_mul_overflow(c->pages, static_cast<size_t>(kv->page_bytes), &all) || all > c->pool_len)
         return UOR_B200_DOES_NOT_FIT;
+    if (c->pages * c->heads * (c->page_size / KV_BLOCK) > INT_MAX) return UOR_B200_UNSUPPORTED;  // blocks are numbered in 31 bits
     if (all && (!c->pool || !multiple_of(c->pool, 16))) return UOR_B200_INVALID_ARGUMENT;
     kv->pool = c->pool;
     kv->pages = static_cast<int64_t>(c->pages);

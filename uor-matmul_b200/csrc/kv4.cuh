@@ -108,6 +108,12 @@ struct AttendArgs {
     float scale;
     int window, sinks;
 };
+// Few rows (kv4_few.cuh). EXACT: for f32 results.
+template <typename T, bool EXACT>
+int kv4_few(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route);
+// Many rows, 16-bit results (kv4_many.cuh).
+template <typename T>
+int kv4_many(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route);
 int run_kv4_attention(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route);
 
 }  // namespace uor

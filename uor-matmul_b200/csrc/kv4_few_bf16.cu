@@ -1,0 +1,4 @@
+// bf16 caches, 16-bit results.
+#include "kv4_few.cuh"
+
+template int uor::kv4_few<__nv_bfloat16, false>(uor_b200_ctx*, const uor::AttendArgs&, uor_b200_route*);

@@ -231,11 +231,6 @@ __device__ __noinline__ void sums_out(const ManyParams& p, const Item& it, const
     }
 }
 
-template <int N>
-__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
-template <int N>
-__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-
 template <typename T, int SEG>
 __global__ void __launch_bounds__(THREADS, 1)
     many_kernel(const __grid_constant__ CUtensorMap tm_codes, const __grid_constant__ CUtensorMap tm_x,
