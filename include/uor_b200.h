@@ -554,7 +554,8 @@ typedef struct uor_b200_rotation {
  * projection's output serves for all three. rotation NULL: none.
  * A rotated value is rounded to f32 and then to elem. Of every group of channels of a head, with its
  * greatest value h and its least l, in f32 steps each rounded once:
- *   mid = elem(h / 2 + l / 2), scale = elem((h / 2 - l / 2) / 7.5),
+ *   mid = elem(h / 2 + l / 2), scale = elem((h / 2 - l / 2) / 7.5), or where 7.5 scale + |mid| passes
+ *   elem's largest value the next smaller scale,
  *   code = the integer nearest to (x - mid) / scale + 7.5 (half to even) within 0 .. 15; 0 where the
  *   scale is 0.
  * A key or value that is not finite has no place in a range of 15 steps: an infinity counts as elem's

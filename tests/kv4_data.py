@@ -40,7 +40,9 @@ def held(x, group):
     v = torch.nan_to_num(x.float(), nan=0.0, posinf=most, neginf=-most).unflatten(-1, (-1, group))
     high, low = v.amax(-1, keepdim=True), v.amin(-1, keepdim=True)
     mid = (high * 0.5 + low * 0.5).to(kind).float()
-    scale = ((high * 0.5 - low * 0.5) / 7.5).to(kind).float()
+    scale = ((high * 0.5 - low * 0.5) / 7.5).to(kind)
+    past = 7.5 * scale.double() + mid.abs().double() > most
+    scale = torch.where(past, (scale.view(torch.int16) - 1).view(kind), scale).float()
     code = ((v - mid) / scale + 7.5).round().clamp(0, 15)
     code = torch.where(scale > 0, code, torch.zeros_like(code))
     return (mid.double() + scale.double() * (code.double() - 7.5)).flatten(-2)

@@ -44,12 +44,15 @@ struct Half<__nv_bfloat16> {
         memcpy(&r, &v, 4);
         return r;
     }
+    // The next smaller one of a positive value.
+    __device__ static __forceinline__ float below(float v) { return __uint_as_float(__float_as_uint(v) - 0x10000u); }
     __device__ static __forceinline__ float first(uint32_t w) { return __uint_as_float(w << 16); }
     __device__ static __forceinline__ float second(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 };
 template <>
 struct Half<__half> {
     static constexpr float MOST = 65504.0f;
+    __device__ static __forceinline__ float below(float v) { return __half2float(__ushort_as_half(__half_as_ushort(__float2half_rn(v)) - 1)); }
     __device__ static __forceinline__ uint32_t pair(float a, float b) {
         const __half2 v = __floats2half2_rn(a, b);
         uint32_t r;
@@ -247,7 +250,9 @@ __global__ void __launch_bounds__(WARPS * 32) append_kernel(const __grid_constan
             }
             if (!live || query) continue;
             const float mid = to_f32(from_f32<T>(__fadd_rn(high * 0.5f, low * 0.5f)));
-            const float scale = to_f32(from_f32<T>(__fdiv_rn(__fsub_rn(high * 0.5f, low * 0.5f), 7.5f)));
+            float scale = to_f32(from_f32<T>(__fdiv_rn(__fsub_rn(high * 0.5f, low * 0.5f), 7.5f)));
+            // half of the largest float and 7.5 halves of the scale: what is held stays within the type
+            if (fmaf(3.75f, scale, 0.5f * fabsf(mid)) > 0.5f * Half<T>::MOST) scale = Half<T>::below(scale);
             const float inverse = scale > 0x1p-120f ? __frcp_rn(scale) : 0.0f;
             uint32_t codes = 0;
             if (scale > 0.0f) {
