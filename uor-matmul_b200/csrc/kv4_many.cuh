@@ -26,11 +26,10 @@ namespace uor {
 
 namespace {
 
-constexpr int THREADS = 512;
-constexpr int REGS_SOFTMAX = 200, REGS_DECODE = 80, REGS_CONTROL = 32;
-static_assert(2 * REGS_SOFTMAX + REGS_DECODE + REGS_CONTROL <= 4 * 128, "registers of the launch");
-constexpr int DECODERS = 4;       // warps
-constexpr uint32_t NAP_NS = 1000;  // a wait's sleep between looks; an arrival ends it at once
+constexpr int THREADS = 640;
+constexpr int REGS_SOFTMAX = 136, REGS_DECODE = 80, REGS_CONTROL = 40;
+static_assert(2 * REGS_SOFTMAX + 2 * REGS_DECODE + REGS_CONTROL <= 5 * 96, "registers of the launch");
+constexpr int DECODERS = 4;  // warps for the keys, and for the values
 
 struct ManyAttend {
     AttendArgs a;
@@ -43,17 +42,20 @@ struct ManyAttend {
 template <int D>
 struct Shape {
     static constexpr int HALVES = D <= 128 ? 2 : 1;      // of 128 rows
-    static constexpr int TOKENS = D <= 128 ? 128 : 64;   // of a step
+    static constexpr int TOKENS = 64;                    // of a step
     static constexpr int BLOCKS = TOKENS / KV_BLOCK;
     static constexpr int ATOMS = (D + 63) / 64;          // of 64 channels, the 128 bytes that a swizzle spans
-    static constexpr int KSTAGES = 2, VSTAGES = D <= 192 ? 2 : 1, RING = 3;
+    static constexpr int KSTAGES = D <= 128 ? 4 : 2, VSTAGES = D <= 128 ? 4 : D <= 192 ? 2 : 1;
+    static constexpr int RING = 3;                       // blocks' keys, or values, under way of each decoding warp
+    static constexpr int THERE = 8;                      // steps that the decoders' notes are kept for
     static constexpr int Q_ATOM = 128 * 128, Q_HALF = ATOMS * Q_ATOM;
     static constexpr int T_ATOM = TOKENS * 128, T_BYTES = ATOMS * T_ATOM;  // a step's keys, or values
-    static constexpr int S_AT = 0, O_AT = HALVES * TOKENS;  // tensor-memory columns: scores, sums
-    static constexpr int BARS = 1 + 2 * KSTAGES + 2 * VSTAGES + 3 * HALVES + 1;
+    static constexpr int S_AT = 0, O_AT = 2 * HALVES * TOKENS;  // tensor-memory columns: scores, sums
+    static constexpr int BARS = HALVES + 3 + 2 * KSTAGES + 2 * VSTAGES + 6 * HALVES + 2 + 2 * DECODERS * RING;
     static constexpr int FIXED = HALVES * Q_HALF + KSTAGES * T_BYTES + VSTAGES * T_BYTES;
+    static_assert(BLOCKS == DECODERS, "a block of a step to each decoding warp");
     static_assert(O_AT + HALVES * D <= 512, "tensor memory");
-    static int smem(int groups) { return 1024 + FIXED + DECODERS * RING * kv_block_bytes(D, groups) + BARS * 8 + 4 * BLOCKS + 64; }
+    static int smem(int groups) { return 1024 + FIXED + DECODERS * RING * kv_block_bytes(D, groups) + BARS * 8 + THERE * BLOCKS; }
 };
 
 // What one item is; the same for all roles.
@@ -86,8 +88,64 @@ __device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c
         asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
 }
+// Into the tensor cores' operands, which no thread reads: reads of the rings may pass it.
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d));
+}
+
+// mbar_wait whose looks are few instructions: the roles wait for one another most of the time, and looks
+// take issue slots from those that work. The status is looked at every 512th time.
+__device__ __forceinline__ bool wait_on(uint32_t bar, uint32_t parity, uint64_t budget_ns, int* status, int code) {
+    uint64_t t0 = 0;  // the timer is slow to read: only by those who wait long
+    while (true) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p, q;\n .reg .u32 n;\n mov.u32 n, 512;\nAGAIN:\n"
+            " mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+            " sub.u32 n, n, 1;\n setp.ne.u32 q, n, 0;\n @q bra AGAIN;\nDONE:\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (*(volatile int*)status != 0) return false;
+        const uint64_t now = globaltimer();
+        if (t0 == 0) t0 = now;
+        if (now - t0 > budget_ns) {
+            atomicCAS(status, 0, code);
+            return false;
+        }
+    }
+}
+__device__ __forceinline__ bool wait_on_warp(uint32_t bar, uint32_t parity, uint64_t budget_ns, int* status, int code) {
+    uint64_t t0 = 0;
+    for (uint32_t looks = 1;; ++looks) {
+        uint32_t done = 0;
+        asm volatile(
+            "{\n .reg .pred p, first;\n setp.eq.u32 first, %3, 0;\n setp.ne.u32 p, 0, 0;\n"
+            " @first mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(bar), "r"(parity), "r"(threadIdx.x & 31)
+            : "memory");
+        if (__any_sync(0xffffffffu, done)) return true;
+        if ((looks & 511) == 0) {
+            const uint64_t now = globaltimer();
+            if (t0 == 0) t0 = now;
+            const bool late = now - t0 > budget_ns;
+            if (late) atomicCAS(status, 0, code);
+            if (__any_sync(0xffffffffu, late || *(volatile int*)status != 0)) return false;
+        }
+    }
+}
+// A wait of the way out, when a role has given up: for what is under way, whatever the status.
+__device__ __forceinline__ void wait_out(uint32_t bar, uint32_t parity, uint64_t budget_ns) {
+    const uint64_t t0 = globaltimer();
+    while (!mbar_try_wait(bar, parity) && globaltimer() - t0 <= budget_ns) {
+    }
+}
+// Contiguous bytes (a multiple of 16, at multiples of 16) into shared memory, counted on a barrier.
+__device__ __forceinline__ void bulk_load(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(to), "l"(from), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
 // The items before each sequence's, and the first to be taken.
@@ -133,22 +191,26 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
     uint8_t* values_at = keys_at + Z::KSTAGES * Z::T_BYTES;
     uint8_t* rings = values_at + Z::VSTAGES * Z::T_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(rings + DECODERS * Z::RING * a.kv.block_bytes);
-    uint8_t* there = reinterpret_cast<uint8_t*>(bars + Z::BARS);  // [4][BLOCKS]: whether a step's blocks are
-    const uint32_t qfull = smem_u32(bars), kfull = qfull + 8, kempty = kfull + 8 * Z::KSTAGES;
+    uint8_t* there = reinterpret_cast<uint8_t*>(bars + Z::BARS);  // [THERE][BLOCKS]: whether a step's blocks are
+    const uint32_t qfull = smem_u32(bars), ifull = qfull + 8 * Z::HALVES, iempty = ifull + 16, kfull = iempty + 8, kempty = kfull + 8 * Z::KSTAGES;
     const uint32_t vfull = kempty + 8 * Z::KSTAGES, vempty = vfull + 8 * Z::VSTAGES;
-    const uint32_t sfull = vempty + 8 * Z::VSTAGES, pfull = sfull + 8 * Z::HALVES, ofull = pfull + 8 * Z::HALVES;
-    const uint32_t drain = ofull + 8 * Z::HALVES;
+    // Scores, weights and sums of odd and even steps have signals of their own: a role may be two steps ahead
+    // of another, and a signal's parity tells one filling from the next alone.
+    const uint32_t sfull = vempty + 8 * Z::VSTAGES, pfull = sfull + 16 * Z::HALVES, ofull = pfull + 16 * Z::HALVES;
+    const uint32_t drain = ofull + 16 * Z::HALVES;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wg = warp >> 2;
 
     if (threadIdx.x == 0) {
-        mbar_init(qfull, 4 * Z::HALVES);
-        for (int i = 0; i < Z::KSTAGES; ++i) mbar_init(kfull + 8 * i, DECODERS), mbar_init(kempty + 8 * i, 1);
-        for (int i = 0; i < Z::VSTAGES; ++i) mbar_init(vfull + 8 * i, DECODERS), mbar_init(vempty + 8 * i, 1);
-        for (int i = 0; i < Z::HALVES; ++i) mbar_init(sfull + 8 * i, 1), mbar_init(pfull + 8 * i, 4), mbar_init(ofull + 8 * i, 1);
-        mbar_init(drain, 1);
+        for (int i = 0; i < Z::HALVES; ++i) mbar_init(qfull + 8 * i, 4);
+        for (int i = 0; i < 2; ++i) mbar_init(ifull + 8 * i, 1);
+        mbar_init(iempty, 5 * Z::HALVES + 2 * DECODERS);
+        for (int i = 0; i < Z::KSTAGES; ++i) mbar_init(kfull + 8 * i, DECODERS), mbar_init(kempty + 8 * i, Z::HALVES);
+        for (int i = 0; i < Z::VSTAGES; ++i) mbar_init(vfull + 8 * i, DECODERS), mbar_init(vempty + 8 * i, Z::HALVES);
+        for (int i = 0; i < 2 * Z::HALVES; ++i) mbar_init(sfull + 8 * i, 1), mbar_init(pfull + 8 * i, 4), mbar_init(ofull + 8 * i, 1);
+        for (int i = 0; i < 2 + 2 * DECODERS * Z::RING; ++i) mbar_init(drain + 8 * i, 1);
         fence_barrier_init();
     }
-    if (warp == 13) tmem_alloc(smem_u32(&tmem_slot), 512);
+    if (warp == 17) tmem_alloc(smem_u32(&tmem_slot), 512);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // Takes an item; none left: seq is -1.
     auto take = [&](int slot) {
@@ -166,36 +228,42 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
             it.seq = lo, it.tile = tiles - 1 - rel / a.kv.heads, it.head = rel % a.kv.heads;
         }
         items[slot] = it;
+        return it.seq >= 0;
     };
-    if (warp == 14 && lane == 0) take(0);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_slot;
-    // A role's items, one after another: all leave an item together.
+    // A role's items, one after another; every role goes on to the next as soon as it can. The lanes that
+    // ask agree.
     bool ok = true;
     uint32_t steps_done = 0;  // of the items before this one
-    auto end = [&](int steps) {
-        steps_done += steps;
-        tc_fence_before();
-        __syncwarp();
-        const bool on = bar_and_all(1, THREADS, ok);
-        tc_fence_after();
-        return on;
+    auto item_at = [&](int n, Item* it) {
+        if (!ok || !wait_on(ifull + 8 * (n & 1), n >> 1 & 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) return false;
+        *it = items[n & 1];
+        return it->seq >= 0;
     };
-    auto steps_of = [&](const Share& share) { return (share.blocks + Z::BLOCKS - 1) / Z::BLOCKS; };
+    auto next_item = [&](int n, Item* it) {
+        return static_cast<bool>(__all_sync(0xffffffffu, item_at(n, it)));
+    };
+    // The next item is taken when all know theirs and the decoders, who are ahead, are through with it: taken
+    // sooner, the last and shortest items would lie in line behind long ones.
+    auto wants_next = [&]() {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(iempty);
+    };
     if (wg < Z::HALVES) {
         regs_up<REGS_SOFTMAX>();
-        for (int n = 0;; ++n) {
-            const Item it = items[n & 1];
-            if (it.seq < 0) break;
+        Item it;
+        for (int n = 0; next_item(n, &it); ++n) {
             const Sequence seq(a.batch, it.seq);
-            const Share share(seq, a, 128 * Z::HALVES, Z::BLOCKS);
-            const int steps = steps_of(share);
+            const Share share(seq, a, 128 * Z::HALVES, Z::BLOCKS, it.tile);
+            const int steps = share.tiles;
+            wants_next();
             // A row to a thread.
             const int half = wg, t = threadIdx.x & 127;
             const uint32_t lanes = static_cast<uint32_t>(t & ~31) << 16;
-            const uint32_t scores = tmem + lanes + Z::S_AT + half * Z::TOKENS, sums = tmem + lanes + Z::O_AT + half * D;
+            const uint32_t scores_at = tmem + lanes + Z::S_AT + half * 2 * Z::TOKENS, sums = tmem + lanes + Z::O_AT + half * D;
             const int r = it.tile * 128 * Z::HALVES + half * 128 + t;
             const bool live = r < share.rows;
             const int at = live ? seq.at + r / a.share : -1;
@@ -205,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
             {
                 const uint16_t* from = static_cast<const uint16_t*>(a.q.p) + row * a.q.rs + static_cast<int64_t>(col) * D;
                 const uint32_t to = smem_u32(smem) + half * Z::Q_HALF + t * 128, flip = a.scale < 0 ? 0x80008000u : 0u;
-#pragma unroll 4
+#pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
                     uint32_t w[4] = {0, 0, 0, 0};
                     if (live) {
@@ -224,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(qfull);
+                if (lane == 0) mbar_arrive(qfull + 8 * half);
             }
             // Positions of this half's rows.
             const int first_row = it.tile * 128 * Z::HALVES + half * 128, last_row = min(first_row + 127, share.rows - 1);
@@ -236,7 +304,8 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
             uint64_t l = 0;
             for (int j = 0; j < steps; ++j) {
                 const uint32_t g = steps_done + j;
-                if (!mbar_wait_warp_hint(sfull + 8 * half, g & 1, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE, NAP_NS)) {
+                const uint32_t side = 2 * half + (g & 1), scores = scores_at + (g & 1) * Z::TOKENS;  // scores of odd and even steps
+                if (!wait_on_warp(sfull + 8 * side, g >> 1 & 1, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE)) {
                     ok = false;
                     break;
                 }
@@ -247,37 +316,29 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
                 if (!hidden) {
                     const int low = share.block_at(b0) * KV_BLOCK, high = share.block_at(b1) * KV_BLOCK + KV_BLOCK - 1;
                     hidden = high > nearest || (a.window && low <= behind && !(b1 < share.sink_blocks && high < a.sinks));
-                    if constexpr (Z::BLOCKS == 8) hidden |= *reinterpret_cast<const uint64_t*>(there + (g & 3) * 8) != 0x0101010101010101ull;
-                    else hidden |= *reinterpret_cast<const uint32_t*>(there + (g & 3) * 4) != 0x01010101u;
+                    hidden |= *reinterpret_cast<const uint32_t*>(there + g % Z::THERE * Z::BLOCKS) != 0x01010101u;
                 }
-                // 32 tokens' scores travel at a time, the next while these are used. They are read twice, for
-                // their maximum and for their weights: 128 of them do not fit the registers.
-                uint32_t s[2][32];
-                auto hide = [&](uint32_t (&v)[32], int c) {
+                uint32_t s[Z::TOKENS];
+                tmem_ld32(scores, *reinterpret_cast<uint32_t(*)[32]>(s));
+                tmem_ld32(scores + 32, *reinterpret_cast<uint32_t(*)[32]>(s + 32));
+                tmem_ld_wait();
+                if (hidden) {
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int b = b0 + c / KV_BLOCK + e, token = share.block_at(b) * KV_BLOCK;
-                        const bool block = b < share.blocks && there[(g & 3) * Z::BLOCKS + c / KV_BLOCK + e];
+                    for (int e = 0; e < Z::BLOCKS; ++e) {
+                        const int b = b0 + e, token = share.block_at(b) * KV_BLOCK;
+                        const bool block = b < share.blocks && there[g % Z::THERE * Z::BLOCKS + e];
                         const int upto = block ? min(at, seq.keys - 1) : -1;
                         const int window = a.window ? at - a.window : -1;
 #pragma unroll
                         for (int i = 0; i < KV_BLOCK; ++i) {
                             const int position = token + i;
-                            if (!(position <= upto && (position > window || position < a.sinks))) v[e * KV_BLOCK + i] = __float_as_uint(-INFINITY);
+                            if (!(position <= upto && (position > window || position < a.sinks))) s[e * KV_BLOCK + i] = __float_as_uint(-INFINITY);
                         }
                     }
-                };
-                tmem_ld32(scores, s[0]);
+                }
                 float part[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int c = 0; c < Z::TOKENS; c += 32) {
-                    auto& v = s[c / 32 & 1];
-                    tmem_ld_wait();
-                    tmem_ld32(scores + (c + 32) % Z::TOKENS, s[c / 32 + 1 & 1]);
-                    if (hidden) hide(v, c);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(v[i]));
-                }
+                for (int i = 0; i < Z::TOKENS; ++i) part[i & 3] = fmaxf(part[i & 3], __uint_as_float(s[i]));
                 const float top = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])) * k;
                 const bool higher = top > m + 8.0f;
                 if (__any_sync(0xffffffffu, higher)) {
@@ -286,7 +347,7 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
                     m = next;
                     l = mul2(l, pair_of(by, by));
                     if (j) {  // the sums so far, once the product before this one is in them
-                        if (!mbar_wait_warp_hint(ofull + 8 * half, (g - 1) & 1, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE, NAP_NS)) {
+                        if (!wait_on_warp(ofull + 8 * (side ^ 1), (g - 1) >> 1 & 1, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE)) {
                             ok = false;
                             break;
                         }
@@ -307,15 +368,11 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
                 uint64_t l2 = 0;
 #pragma unroll
                 for (int c = 0; c < Z::TOKENS; c += 32) {
-                    auto& v = s[c / 32 & 1];
-                    tmem_ld_wait();
-                    if (c + 32 < Z::TOKENS) tmem_ld32(scores + c + 32, s[c / 32 + 1 & 1]);
-                    if (hidden) hide(v, c);
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 32; i += 2) {
                         float x, y;
-                        parts_of(fma2(pair_of(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), kk, mm), x, y);
+                        parts_of(fma2(pair_of(__uint_as_float(s[c + i]), __uint_as_float(s[c + i + 1])), kk, mm), x, y);
                         x = ex2(x), y = ex2(y);
                         if (i & 2) l2 = add2(l2, pair_of(x, y));
                         else l = add2(l, pair_of(x, y));
@@ -327,10 +384,10 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
                 tmem_st_wait();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(pfull + 8 * half);
+                if (lane == 0) mbar_arrive(pfull + 8 * side);
             }
             if (ok && steps &&
-                !mbar_wait_warp_hint(ofull + 8 * half, (steps_done + steps - 1) & 1, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE, NAP_NS))
+                !wait_on_warp(ofull + 8 * (2 * half + ((steps_done + steps - 1) & 1)), (steps_done + steps - 1) >> 1 & 1, p.budget_ns, p.status, KERR_TIMEOUT_EPILOGUE))
                 ok = false;
             if (ok) {
                 tc_fence_after();
@@ -362,203 +419,215 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
                 if (live && a.lse.p) static_cast<float*>(a.lse.p)[row * a.lse.rs + col] = (m + log2f(all)) * LN2;
                 tc_fence_before();
             }
-            if (!end(steps)) break;
+            steps_done += steps;
+            if (!ok) break;
         }
-    } else if (wg == 2) {
+    } else if (wg == 2 || wg == 3) {
         regs_down<REGS_DECODE>();
-        for (int n = 0;; ++n) {
-            const Item it = items[n & 1];
-            if (it.seq < 0) break;
+        uint32_t turn = 0;  // the parity of each of the ring's signals
+        Item it;
+        for (int n = 0; next_item(n, &it); ++n) {
             const Sequence seq(a.batch, it.seq);
-            const Share share(seq, a, 128 * Z::HALVES, Z::BLOCKS);
-            const int steps = steps_of(share);
-            // Blocks w, w + 4 of each step, through a ring of this warp's own.
-            constexpr int EACH = Z::BLOCKS / DECODERS;
-            const int w = warp & 3, block_bytes = a.kv.block_bytes, groups = a.kv.groups, to_group = a.kv.group_shift - 5;
-            uint8_t* ring = rings + w * Z::RING * block_bytes;
-            const uint32_t ring_at = smem_u32(ring);
-            const int count = steps * EACH;  // of blocks; some behind the last
-            int places = -1;
-            auto index = [&](int i) { return i / EACH * Z::BLOCKS + w + i % EACH * DECODERS; };
-            auto place_of = [&](int i) { return __shfl_sync(0xffffffffu, places, i & 31); };
-            uint32_t gone = 0;  // of the ring's blocks
-            auto load = [&](int i) {
-                if (i < count) {
-                    if ((i & 31) == 0) {
-                        places = -1;
-                        const int b = index(i + lane);
-                        if (i + lane < count && b < share.blocks) {
-                            const int block = share.block_at(b), in_page = a.kv.page_shift - 4;
-                            const int page = a.batch.table[it.seq * a.batch.table_rs + (block >> in_page)];
-                            if (static_cast<uint32_t>(page) < a.kv.pages)
-                                places = ((page * a.kv.heads + it.head) << in_page) + (block & ((1 << in_page) - 1));
-                        }
-                    }
-                    const int place = place_of(i), slot = i % Z::RING;
-                    gone = place < 0 ? gone | 1u << slot : gone & ~(1u << slot);
-                    if (place >= 0) {
-                        const uint8_t* from = a.kv.pool + static_cast<int64_t>(place) * block_bytes;
-                        for (int b = lane * 16; b < block_bytes; b += 512) cp_async(ring_at + slot * block_bytes + b, from + b);
+            const Share share(seq, a, 128 * Z::HALVES, Z::BLOCKS, it.tile);
+            const int steps = share.tiles;
+            // The keys, or the values, of block w of each step, through a ring of this warp's own.
+            const bool keys = wg == 2;
+            const uint32_t raw = drain + 16 + (warp - 8) * 8 * Z::RING;  // signals of the ring's copies
+            const int w = warp & 3, block_bytes = a.kv.block_bytes, part_bytes = block_bytes / 2, groups = a.kv.groups;
+            const int to_group = a.kv.group_shift - 5;
+            uint8_t* ring = rings + (warp - 8) * Z::RING * part_bytes;
+            const uint8_t* pool = a.kv.pool + (keys ? 0 : part_bytes);
+            auto index = [&](int i) { return i * Z::BLOCKS + w; };
+            int places = -1;                 // where in the pool 32 of them lie, one to a lane; -1: nowhere
+            uint32_t gone = 0, asked = 0;    // of the ring's: those that are nowhere; those under way
+            auto load = [&](int i, int slot) {
+                if (i >= steps) return;
+                if ((i & 31) == 0) {
+                    places = -1;
+                    const int b = index(i + lane);
+                    if (b < share.blocks) {
+                        const int block = share.block_at(b), in_page = a.kv.page_shift - 4;
+                        const int page = a.batch.table[it.seq * a.batch.table_rs + (block >> in_page)];
+                        if (static_cast<uint32_t>(page) < a.kv.pages)
+                            places = ((page * a.kv.heads + it.head) << in_page) + (block & ((1 << in_page) - 1));
                     }
                 }
-                cp_commit();
+                const int place = __shfl_sync(0xffffffffu, places, i & 31);
+                gone = place < 0 ? gone | 1u << slot : gone & ~(1u << slot);
+                asked |= 1u << slot;
+                if (lane == 0) {
+                    mbar_expect_tx(raw + 8 * slot, place < 0 ? 0 : part_bytes);
+                    if (place >= 0) bulk_load(smem_u32(ring + slot * part_bytes), pool + static_cast<int64_t>(place) * block_bytes, part_bytes, raw + 8 * slot);
+                }
             };
-#pragma unroll
-            for (int i = 0; i < Z::RING - 1; ++i) load(i);
+            for (int i = 0; i < Z::RING; ++i) load(i, i);
             const int t = lane >> 2, c = lane & 3;
-            for (int j = 0; j < steps && ok; ++j) {
-                const uint32_t g = steps_done + j, ks = g % Z::KSTAGES, vs = g % Z::VSTAGES;
-                if (!mbar_wait_warp_hint(kempty + 8 * ks, (g / Z::KSTAGES & 1) ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER, NAP_NS)) {
+            const uint32_t full = keys ? kfull : vfull, empty = keys ? kempty : vempty, stages = keys ? Z::KSTAGES : Z::VSTAGES;
+            uint32_t stage = steps_done % stages, filled = steps_done / stages & 1, g = steps_done;
+            int slot = 0;
+#pragma unroll 1
+            for (int i = 0; i < steps; ++i) {
+                if (!wait_on_warp(empty + 8 * stage, filled ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER)) {
                     ok = false;
                     break;
                 }
-                // keys: all of the step's blocks of this warp, then its values
-#pragma unroll
-                for (int e = 0; e < EACH; ++e) {
-                    const int i = j * EACH + e, slot = i % Z::RING, in_step = w + e * DECODERS;
-                    cp_wait<Z::RING - 2>();
+                if (!wait_on_warp(raw + 8 * slot, turn >> slot & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL)) {
+                    ok = false;
+                    break;
+                }
+                turn ^= 1u << slot;
+                asked &= ~(1u << slot);
+                uint8_t* part = ring + slot * part_bytes;
+                const bool missing = gone >> slot & 1;
+                const int token = missing ? seq.keys : share.block_at(index(i)) * KV_BLOCK;
+                if (token + KV_BLOCK > seq.keys) {
+                    // What lies behind the last token may be anything: by a scale and a middle of 0 it is 0.
+                    for (int b = lane; b < 8 * groups; b += 32) {
+                        auto* q = reinterpret_cast<uint32_t*>(part + 8 * D + b * 8);
+                        const int first = token + b / groups * 2;
+                        const uint32_t keep = (first < seq.keys ? 0xFFFFu : 0u) | (first + 1 < seq.keys ? 0xFFFF0000u : 0u);
+                        q[0] &= keep, q[1] &= keep;
+                    }
                     __syncwarp();
-                    // With two blocks a step the first one's values are decoded before its slot is wanted
-                    // again; see below.
-                    const uint8_t* block = ring + slot * block_bytes;
-                    const bool missing = gone >> slot & 1;
-                    if (lane == 0) there[(g & 3) * Z::BLOCKS + in_step] = !missing;
-                    const int token = missing ? 0 : share.block_at(index(i)) * KV_BLOCK;
-                    const uint32_t to = smem_u32(keys_at) + ks * Z::T_BYTES;
-#pragma unroll
+                }
+                const int row = w * KV_BLOCK;
+                if (keys) {
+                    // Tokens t and 8 + t, channels 8 c .. 8 c + 7 of every 32.
+                    if (lane == 0) there[g % Z::THERE * Z::BLOCKS + w] = !missing;
+                    const uint32_t odd = (t & 1) ? 0x3232 : 0x1010;
+#pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
-                        const int tok = h * 8 + t, row = in_step * KV_BLOCK + tok;
+                        const uint32_t to = smem_u32(keys_at) + stage * Z::T_BYTES + (row + h * 8 + t) * 128;
                         uint32_t v[N32];
-                        words<N32>(block + (tok * 4 + c) * N32 * 4, v);
-                        const uint32_t odd = (tok & 1) ? 0x3232 : 0x1010;
-                        const bool none = missing || token + tok >= seq.keys;  // what lies there may be anything
-                        uint32_t scale = 0, mid = 0;
+                        uint2 q[N32];
+                        words<N32>(part + ((h * 8 + t) * 4 + c) * N32 * 4, v);
 #pragma unroll
-                        for (int n32 = 0; n32 < N32; ++n32) {
-                            if ((n32 & ((1 << to_group) - 1)) == 0) {
-                                const uint2 q = *reinterpret_cast<const uint2*>(block + 8 * D + ((tok >> 1) * groups + (n32 >> to_group)) * 8);
-                                scale = none ? 0u : __byte_perm(q.x, 0, odd), mid = none ? 0u : __byte_perm(q.y, 0, odd);
-                            }
+                        for (int n = 0; n < N32; ++n) q[n] = *reinterpret_cast<const uint2*>(part + 8 * D + ((h * 4 + (t >> 1)) * groups + (n >> to_group)) * 8);
+#pragma unroll
+                        for (int n = 0; n < N32; ++n) {
+                            const uint32_t scale = __byte_perm(q[n].x, 0, odd), mid = __byte_perm(q[n].y, 0, odd);
                             uint32_t x[4];
-                            centred<T>(v[n32], x);
+                            centred<T>(v[n], x);
 #pragma unroll
                             for (int b = 0; b < 4; ++b) x[b] = fma_half2<T>(scale, x[b], mid);
-                            sts128(to + (n32 >> 1) * Z::T_ATOM + row * 128 + ((((n32 & 1) * 4 + c) ^ (row & 7)) << 4), x[0], x[1], x[2], x[3]);
+                            sts128(to + (n >> 1) * Z::T_ATOM + ((((n & 1) * 4 + c) ^ t) << 4), x[0], x[1], x[2], x[3]);
                         }
                     }
-                    if (e == 0 && EACH == 2) load(i + Z::RING - 1);
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(kfull + 8 * ks);
-                if (!mbar_wait_warp_hint(vempty + 8 * vs, (g / Z::VSTAGES & 1) ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER, NAP_NS)) {
-                    ok = false;
-                    break;
-                }
-#pragma unroll
-                for (int e = 0; e < EACH; ++e) {
-                    const int i = j * EACH + e, slot = i % Z::RING, in_step = w + e * DECODERS;
-                    const uint8_t* block = ring + slot * block_bytes;
-                    const bool missing = gone >> slot & 1;
-                    const int token = missing ? 0 : share.block_at(index(i)) * KV_BLOCK;
-                    const uint32_t to = smem_u32(values_at) + vs * Z::T_BYTES;
+                } else {
                     // Two tokens, 8 h + 2 c and the next, by eight channels of every 32.
-                    const int h = lane >> 4, eight = lane >> 2 & 3;
-                    const int tok = 8 * h + 2 * c, row = in_step * KV_BLOCK + tok;
-                    const uint8_t* codes = block + 8 * D + 64 * groups + ((h * 8 + 2 * eight) * 4 + c) * N32 * 4;
+                    const int h = lane >> 4, eight = lane >> 2 & 3, tok = 8 * h + 2 * c;
+                    const uint32_t to = smem_u32(values_at) + stage * Z::T_BYTES + (row + tok) * 128;
                     uint32_t v[2][N32];
-                    words<N32>(codes, v[0]);
-                    words<N32>(codes + 4 * N32 * 4, v[1]);
-                    const uint32_t keep = missing ? 0u : (token + tok < seq.keys ? 0xFFFFu : 0u) | (token + tok + 1 < seq.keys ? 0xFFFF0000u : 0u);
-                    uint32_t scale = 0, mid = 0;
+                    uint2 q[N32];
+                    words<N32>(part + ((h * 8 + 2 * eight) * 4 + c) * N32 * 4, v[0]);
+                    words<N32>(part + ((h * 8 + 2 * eight + 1) * 4 + c) * N32 * 4, v[1]);
 #pragma unroll
-                    for (int n32 = 0; n32 < N32; ++n32) {
-                        if ((n32 & ((1 << to_group) - 1)) == 0) {
-                            const uint2 q = *reinterpret_cast<const uint2*>(block + 16 * D + 64 * groups + ((tok >> 1) * groups + (n32 >> to_group)) * 8);
-                            scale = q.x & keep, mid = q.y & keep;
-                        }
+                    for (int n = 0; n < N32; ++n) q[n] = *reinterpret_cast<const uint2*>(part + 8 * D + ((tok >> 1) * groups + (n >> to_group)) * 8);
+#pragma unroll
+                    for (int n = 0; n < N32; ++n) {
                         uint32_t x[2][4];
 #pragma unroll
                         for (int b = 0; b < 2; ++b) {
-                            centred<T>(v[b][n32], x[b]);
+                            centred<T>(v[b][n], x[b]);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) x[b][k] = fma_half2<T>(scale, x[b][k], mid);
+                            for (int k = 0; k < 4; ++k) x[b][k] = fma_half2<T>(q[n].x, x[b][k], q[n].y);
                         }
-                        const uint32_t dst = to + (n32 >> 1) * Z::T_ATOM + row * 128;
-                        const uint32_t chunk = (n32 & 1) * 4 + eight;
-                        sts128(dst + ((chunk ^ (row & 7)) << 4), __byte_perm(x[0][0], x[0][1], 0x5410), __byte_perm(x[0][2], x[0][3], 0x5410),
-                               __byte_perm(x[1][0], x[1][1], 0x5410), __byte_perm(x[1][2], x[1][3], 0x5410));
-                        sts128(dst + 128 + ((chunk ^ ((row + 1) & 7)) << 4), __byte_perm(x[0][0], x[0][1], 0x7632), __byte_perm(x[0][2], x[0][3], 0x7632),
-                               __byte_perm(x[1][0], x[1][1], 0x7632), __byte_perm(x[1][2], x[1][3], 0x7632));
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const uint32_t half = k ? 0x7632 : 0x5410;
+                            sts128(to + (n >> 1) * Z::T_ATOM + k * 128 + ((((n & 1) * 4 + eight) ^ ((2 * c + k) & 7)) << 4), __byte_perm(x[0][0], x[0][1], half),
+                                   __byte_perm(x[0][2], x[0][3], half), __byte_perm(x[1][0], x[1][1], half), __byte_perm(x[1][2], x[1][3], half));
+                        }
                     }
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(vfull + 8 * vs);
-                load((j + 1) * EACH - 1 + Z::RING - 1);
+                if (lane == 0) mbar_arrive(full + 8 * stage);
+                if (++stage == stages) stage = 0, filled ^= 1;
+                ++g;
+                load(i + Z::RING, slot);
+                if (++slot == Z::RING) slot = 0;
             }
-            cp_wait<0>();
-            if (!end(steps)) break;
+            if (!ok)  // copies under way end before the memory goes
+                for (int i = 0; i < Z::RING; ++i)
+                    if (asked >> i & 1) wait_out(raw + 8 * i, turn >> i & 1, p.budget_ns);
+            steps_done += steps;
+            if (!ok) break;
+            wants_next();
         }
     } else {
         regs_down<REGS_CONTROL>();
-        for (int n = 0;; ++n) {
-            const Item it = items[n & 1];
-            if (it.seq < 0) break;
-            int steps = 0;
-            if (warp == 12) {
-                const Sequence seq(a.batch, it.seq);
-                steps = steps_of(Share(seq, a, 128 * Z::HALVES, Z::BLOCKS));
-                if (lane == 0) {
-                    constexpr uint32_t QK = idesc_f16(128, Z::TOKENS, BF16), PV = idesc_f16(128, D, BF16, true);
-                    auto values = [&](int half, uint32_t g, bool first) {  // sums += weights values of step g
-                        const uint32_t v = smem_u32(values_at) + g % Z::VSTAGES * Z::T_BYTES;
+        if (warp >= 20 - Z::HALVES) {
+            // A thread for each half's products: one for both spent more time on its waits than they took.
+            const int half = warp - (20 - Z::HALVES);
+            if (elect_one()) {
+                Item it;
+                constexpr uint32_t QK = idesc_f16(128, Z::TOKENS, BF16), PV = idesc_f16(128, D, BF16, true);
+                const uint64_t q_at = smem_desc_sw128(smem_u32(smem), 16, 1024), k_at = smem_desc_sw128(smem_u32(keys_at), 16, 1024);
+                const uint64_t v_at = smem_desc_sw128(smem_u32(values_at), Z::T_ATOM, 1024);
+                auto scores = [&](uint32_t g) {
+                    const uint32_t side = 2 * half + (g & 1), ks = g % Z::KSTAGES;
 #pragma unroll
-                        for (int i = 0; i < Z::TOKENS / 16; ++i)
-                            mma_f16_ts(tmem + Z::O_AT + half * D, tmem + Z::S_AT + half * Z::TOKENS + i * 8, smem_desc_sw128(v + i * 2048, Z::T_ATOM, 1024), PV,
-                                       !(first && i == 0));
-                        mma_commit(ofull + 8 * half);
-                        if (half == Z::HALVES - 1) mma_commit(vempty + 8 * (g % Z::VSTAGES));
-                    };
-                    if (steps) ok = mbar_wait(qfull, n & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL);
-                    for (int j = 0; j <= steps && ok && steps; ++j) {
-                        const uint32_t g = steps_done + j;
-                        if (j < steps) ok = mbar_wait(kfull + 8 * (g % Z::KSTAGES), g / Z::KSTAGES & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL);
-                        for (int half = 0; half < Z::HALVES && ok; ++half) {
-                            if (j) {
-                                ok = mbar_wait(pfull + 8 * half, (g - 1) & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_ACC) &&
-                                     mbar_wait(vfull + 8 * ((g - 1) % Z::VSTAGES), (g - 1) / Z::VSTAGES & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL);
-                                if (!ok) break;
-                                tc_fence_after();
-                                values(half, g - 1, j == 1);
-                            }
-                            if (j < steps) {
-                                tc_fence_after();
-                                const uint32_t q = smem_u32(smem) + half * Z::Q_HALF, k = smem_u32(keys_at) + g % Z::KSTAGES * Z::T_BYTES;
+                    for (int i = 0; i < D / 16; ++i)
+                        mma_f16(tmem + Z::S_AT + side * Z::TOKENS, q_at + ((half * Z::Q_HALF + i / 4 * Z::Q_ATOM + i % 4 * 32) >> 4),
+                                k_at + (ks * Z::T_BYTES + i / 4 * Z::T_ATOM + i % 4 * 32) / 16, QK, i != 0);
+                    mma_commit(sfull + 8 * side);
+                };
+                auto values = [&](uint32_t g, bool first) {  // sums (+)= weights values
+                    const uint32_t side = 2 * half + (g & 1), vs = g % Z::VSTAGES;
 #pragma unroll
-                                for (int i = 0; i < D / 16; ++i)
-                                    mma_f16(tmem + Z::S_AT + half * Z::TOKENS, smem_desc_sw128(q + i / 4 * Z::Q_ATOM + i % 4 * 32, 16, 1024),
-                                            smem_desc_sw128(k + i / 4 * Z::T_ATOM + i % 4 * 32, 16, 1024), QK, i != 0);
-                                mma_commit(sfull + 8 * half);
-                                if (half == Z::HALVES - 1) mma_commit(kempty + 8 * (g % Z::KSTAGES));
-                            }
+                    for (int i = 0; i < Z::TOKENS / 16; ++i)
+                        mma_f16_ts(tmem + Z::O_AT + half * D, tmem + Z::S_AT + side * Z::TOKENS + i * 8, v_at + (vs * Z::T_BYTES + i * 2048) / 16, PV,
+                                   i != 0 || !first);
+                    mma_commit(ofull + 8 * side);
+                };
+                for (int n = 0; item_at(n, &it); ++n) {
+                    mbar_arrive(iempty);
+                    const Sequence seq(a.batch, it.seq);
+                    const int steps = Share(seq, a, 128 * Z::HALVES, Z::BLOCKS, it.tile).tiles;
+                    ok = wait_on(qfull + 8 * half, n & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL);
+                    // Scores are a step ahead of the weights: while a half's weights of one step are made, the
+                    // next step's scores are at hand.
+                    for (int j = -1; j <= steps && ok && steps; ++j) {
+                        const uint32_t g = steps_done + j;  // scores of step j + 1 after values of step j - 1
+                        if (j >= 1) {
+                            const uint32_t vs = (g - 1) % Z::VSTAGES;
+                            ok = wait_on(vfull + 8 * vs, (g - 1) / Z::VSTAGES & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL) &&
+                                 wait_on(pfull + 8 * (2 * half + ((g - 1) & 1)), (g - 1) >> 1 & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_ACC);
+                            if (!ok) break;
+                            tc_fence_after();
+                            values(g - 1, j == 1);
+                            mma_commit(vempty + 8 * vs);
+                        }
+                        if (j + 1 < steps) {
+                            const uint32_t ks = (g + 1) % Z::KSTAGES;
+                            ok = wait_on(kfull + 8 * ks, (g + 1) / Z::KSTAGES & 1, p.budget_ns, p.status, KERR_TIMEOUT_MMA_FULL);
+                            if (!ok) break;
+                            tc_fence_after();
+                            scores(g + 1);
+                            mma_commit(kempty + 8 * ks);
                         }
                     }
-                    if (!ok) {  // what was issued ends before the memory goes
-                        mma_commit(drain);
-                        mbar_wait(drain, 0, p.budget_ns, p.status, KERR_TIMEOUT_DRAIN);
-                    }
+                    steps_done += steps;
                 }
-                __syncwarp();
-            } else if (warp == 14 && lane == 0) {
-                take((n + 1) & 1);
+                if (!ok) {  // what was issued ends before the memory goes
+                    mma_commit(drain + 8 * half);
+                    wait_out(drain + 8 * half, 0, p.budget_ns);
+                }
             }
-            if (!end(steps)) break;
+        } else if (warp == 16 && elect_one()) {
+            // Behind the last item is one that says so.
+            for (int n = 0; !n || wait_on(iempty, n & 1 ^ 1, p.budget_ns, p.status, KERR_TIMEOUT_PRODUCER); ++n) {
+                const bool more = take(n & 1);
+                mbar_arrive(ifull + 8 * (n & 1));
+                if (!more) break;
+            }
         }
     }
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 13) {
+    if (warp == 17) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }

@@ -107,11 +107,23 @@ struct Share {
     __device__ __forceinline__ Share(const Sequence& s, const AttendArgs& a, int tile_rows, int tile_blocks) {
         rows = s.count * a.share;
         row_tiles = (rows + tile_rows - 1) / tile_rows;
-        const int low = a.window ? max(0, s.at - a.window + 1) : 0, ends = (s.keys + 15) >> 4;
-        first_block = low < s.keys ? low >> 4 : ends;
-        sink_blocks = a.window ? min((min(a.sinks, s.keys) + 15) >> 4, first_block) : 0;
-        blocks = sink_blocks + ends - first_block;
+        blocks_of(s.at, s.keys, a);
         tiles = max(1, (blocks + tile_blocks - 1) / tile_blocks);  // of one head and row tile
+    }
+    // Of one row tile alone.
+    __device__ __forceinline__ Share(const Sequence& s, const AttendArgs& a, int tile_rows, int tile_blocks, int tile) {
+        rows = s.count * a.share;
+        row_tiles = (rows + tile_rows - 1) / tile_rows;
+        const int last = s.at + min((tile + 1) * tile_rows - 1, rows - 1) / a.share;
+        blocks_of(s.at + tile * tile_rows / a.share, max(0, min(s.keys, last + 1)), a);
+        tiles = (blocks + tile_blocks - 1) / tile_blocks;
+    }
+    // From the first row's position on, keys 0 .. keys - 1.
+    __device__ __forceinline__ void blocks_of(int at, int keys, const AttendArgs& a) {
+        const int low = a.window ? max(0, at - a.window + 1) : 0, ends = (keys + 15) >> 4;
+        first_block = low < keys ? low >> 4 : ends;
+        sink_blocks = a.window ? min((min(a.sinks, keys) + 15) >> 4, first_block) : 0;
+        blocks = sink_blocks + ends - first_block;
     }
     __device__ __forceinline__ int block_at(int i) const { return i < sink_blocks ? i : first_block + i - sink_blocks; }
     __device__ __forceinline__ int64_t work(int heads) const { return static_cast<int64_t>(row_tiles) * heads * tiles; }
