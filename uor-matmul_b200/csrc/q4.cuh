@@ -81,22 +81,26 @@ struct Epilogue {
     int bias_type;
     Mat residual;        // of the output's type; p null: none
 };
+// v / (1 + e), e = exp(-u), without the exact quotient's branch, at which a thread's elements would
+// wait for one another; both sides are a quarter, since the fast quotient is 0 beyond 2^126.
+__device__ __forceinline__ float over_one_and(float v, float e) { return __fdividef(0.25f * v, fmaf(0.25f, e, 0.25f)); }
 __device__ __forceinline__ float activate(float v, int act) {
     switch (act) {
     case UOR_B200_RELU: return v < 0.0f ? 0.0f : v;
     case UOR_B200_GELU: return 0.5f * v * erfcf(-0.70710678118654752f * v);  // 1 + erf, its tail included
     case UOR_B200_GELU_TANH:  // (1 + tanh z) / 2 = 1 / (1 + exp(-2 z))
-        return v / (1.0f + expf(-1.5957691216057308f * fmaf(0.044715f * v * v, v, v)));
-    case UOR_B200_SILU: return silu(v);
+        return over_one_and(v, expf(-1.5957691216057308f * fmaf(0.044715f * v * v, v, v)));
+    case UOR_B200_SILU: return over_one_and(v, expf(-v));
     default: return v;
     }
 }
-// The output at (i, j) from its product.
+// The output at (i, j) from its product. What it reads is asked for before anything waits for it.
 __device__ __forceinline__ float follow_up(const Epilogue& e, int type, int64_t i, int64_t j, float v) {
-    if (e.bias) v += load_f32(e.bias, j, e.bias_type);
+    const float bias = e.bias ? load_f32(e.bias, j, e.bias_type) : 0.0f;
+    const float residual = e.residual.p ? load_f32(e.residual.p, i * e.residual.rs + j * e.residual.cs, type) : 0.0f;
+    if (e.bias) v += bias;
     v = activate(v, e.act);
-    if (e.residual.p) v += load_f32(e.residual.p, i * e.residual.rs + j * e.residual.cs, type);
-    return v;
+    return e.residual.p ? v + residual : v;
 }
 
 // y (m x n) = x (m x k of elem) dequant(w)^T, and what follows it.
