@@ -25,25 +25,47 @@
 // nothing. For an f32 result they are two 16-bit numbers, a rounded one and what that left (2^-17
 // together). They are bfloat16 whatever the cache's type is: float16 would lose the small ones.
 //
-// The work is cut evenly: tiles of 64 tokens of every sequence, head and eight (or sixteen) rows are
-// numbered by the lengths, which the device alone knows, and each block of threads has as many of them
-// as any other. What a sequence's share is cut into is joined by a second kernel in the order of the
-// tokens; so is nothing that one block had whole.
+// The work is cut evenly: tiles of 64 tokens of every item (a sequence, head and eight or sixteen rows)
+// are numbered by the lengths, which the device alone knows, and each block of threads has as many of them
+// as any other. What an item is cut into is joined by a second kernel in a fixed order; nothing is that one
+// block had whole. Cutting the last third of the work smaller and letting blocks take it as they come free
+// evened their ends out (83 to 165 us after the start) but cost as much in beginnings: 178 us, not 167.
+//
+// 64 contexts of 8192, 8 heads of 128 channels with 8 queries each, bfloat16: 167 us, 4.0 TB/s of codes
+// and scales; 351 instructions a block of 16 tokens and warp, of which the half-rate integer pipe has 64 %
+// of its cycles full on a processor with four blocks, the tensor pipe 32. One token in 4096: 12.4 us, of
+// which the sequences' scan takes 1.8, a table entry and then a block's arrival 2, three blocks to a warp
+// and their sums 4.5, and the second kernel 2.5 behind the last block.
 #pragma once
 #include "kv4_math.cuh"
+
+#include <algorithm>
 
 namespace uor {
 
 namespace {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS, STAGES = 4;
+constexpr int JOINERS = 256;  // threads of a block that joins
+// Tiles that a block takes at least, unless an item has fewer: what it saves in its own time a smaller
+// share costs in parts to join (one token, 4096 in the cache, 8 heads: 13.3 us with one, 12.4 with two
+// to four, 13.5 with six).
+constexpr int LEAST = 3;
+
 
 struct FewAttend {
     AttendArgs a;
     float* part;   // [2 grid][8 NT][dim]
     float2* stat;  // [2 grid][8 NT]: maximum, sum
-    int4* split;   // [grid]: sequence, head, row tile and parts of what block i begins and does not end
+    // [grid]: sequence, head, row tile and parts of what block i begins and does not end; and the block
+    // that began what block i begins with, i where that is itself.
+    int4* split;
+    int* from;
 };
+
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {  // of numbers that are mostly small
+    return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
+}
 
 // A word's nibbles i and 4 + i, i = 0 .. 3: of values as bfloat16 1 + code / 16; of keys as float16 the
 // same, or (FAST) 1 + code / 1024 of even i and 1 + code / 64 of odd ones.
@@ -124,6 +146,15 @@ __device__ __forceinline__ uint32_t mul_bf16(uint32_t a, uint32_t b) {
     return r;
 }
 
+__device__ __forceinline__ float weight(float2 s, float most) { return s.x == -INFINITY ? (s.y == 0.0f ? 0.0f : 1.0f) : ex2(s.x - most); }
+// A sum and its statistics with one part more.
+__device__ __forceinline__ void take(float4& sum, float2& both, const float4& add, float2 s) {
+    const float most = fmaxf(both.x, s.x), by = weight(both, most), of = weight(s, most);
+    if (both.y != 0.0f) sum.x *= by, sum.y *= by, sum.z *= by, sum.w *= by;
+    if (s.y != 0.0f) sum.x = fmaf(of, add.x, sum.x), sum.y = fmaf(of, add.y, sum.y), sum.z = fmaf(of, add.z, sum.z), sum.w = fmaf(of, add.w, sum.w);
+    both = make_float2(most, fmaf(of, s.y, by * both.y));
+}
+
 // NT: rows in eights. GP: 32s of channels in a group. EXACT: weights in two parts, for an f32 result.
 template <typename T, int D, int GP, int NT, bool EXACT>
 __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kernel(const __grid_constant__ FewAttend p) {
@@ -132,12 +163,13 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
     using B = __nv_bfloat16;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t scan[WARPS];
+    __shared__ int scan_items[WARPS];
     __shared__ float2 stat[WARPS][ROWS];
     const AttendArgs& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     uint8_t* ring = smem + warp * STAGES * block_bytes;
     const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-    int64_t* before = reinterpret_cast<int64_t*>(smem + WARPS * STAGES * block_bytes);  // [seqs + 1] tiles before each sequence's
+    int64_t* before = reinterpret_cast<int64_t*>(smem + WARPS * STAGES * block_bytes);  // [seqs + 1] tiles before each sequence's, padded
     // The middles' product: reduction positions 2 c, 2 c + 1 (and 8 + them) are a pair of groups of a
     // part of sum(q); pairs beyond the groups and parts beyond the third are 0.
     constexpr int PAIRS = (G + 1) / 2, SPAN = PAIRS == 1 ? 1 : PAIRS == 2 ? 2 : 4;  // lanes of a part
@@ -147,10 +179,38 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     int64_t total = 0;
+    int items = 0, own_items = 0, own_tiles = 0;
+    for (int s = threadIdx.x; s < a.batch.seqs; s += THREADS) {
+        const Share share(Sequence(a.batch, s), a, ROWS, WARPS);
+        own_items = share.row_tiles * a.kv.heads, own_tiles = share.tiles;
+        items += own_items, total += static_cast<int64_t>(own_items) * own_tiles;
+    }
+    items = __reduce_add_sync(0xffffffffu, items);
+    const int low = __reduce_add_sync(0xffffffffu, static_cast<int>(total & 0xFFFFF)), high = __reduce_add_sync(0xffffffffu, static_cast<int>(total >> 20));
+    if (lane == 0) scan[warp] = low + (static_cast<int64_t>(high) << 20), scan_items[warp] = items;
+    __syncthreads();
+    total = items = 0;
+    for (int w = 0; w < WARPS; ++w) total += scan[w], items += scan_items[w];
+    const int blocks = gridDim.x;
+    // Tiles of a block. Where there are two blocks to an item, an item's tiles count as many as whole blocks
+    // of them have, so that no block has parts of two: a part's beginning and end cost as much as four tiles
+    // (29 x 5 drafted tokens 23.9 -> 18.1 us, 8 contexts of 8192 40.2 -> 36.0, 32 of them 95.4 -> 97.3).
+    const bool padded = 2 * items <= blocks;
+    const int64_t each = max(static_cast<int64_t>(LEAST), padded ? quotient(total + blocks - items - 1, blocks - items) : quotient(total + blocks - 1, blocks));
+    const int pad = padded ? static_cast<int>(each) : 1;
+    auto whole_pads = [&](int tiles) { return (tiles + pad - 1) / pad * pad; };
+    total = 0;
     for (int s0 = 0; s0 < a.batch.seqs; s0 += THREADS) {
         const int s = s0 + threadIdx.x;
-        int64_t mine = s < a.batch.seqs ? Share(Sequence(a.batch, s), a, ROWS, WARPS).work(a.kv.heads) : 0;
-        const int64_t own = mine;
+        if (a.batch.seqs > THREADS) {
+            own_items = 0;
+            if (s < a.batch.seqs) {
+                const Share share(Sequence(a.batch, s), a, ROWS, WARPS);
+                own_items = share.row_tiles * a.kv.heads, own_tiles = share.tiles;
+            }
+        }
+        const int64_t own = static_cast<int64_t>(own_items) * whole_pads(own_tiles);
+        int64_t mine = own;
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t v = __shfl_up_sync(0xffffffffu, mine, o);
             if (lane >= o) mine += v;
@@ -165,10 +225,12 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
         }
         if (s < a.batch.seqs) before[s] = at;
     }
-    if (threadIdx.x == 0) before[a.batch.seqs] = total;
-    if (threadIdx.x == 0) p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0) {
+        before[a.batch.seqs] = total;
+        p.split[blockIdx.x] = make_int4(0, 0, 0, 0);
+        p.from[blockIdx.x] = blockIdx.x;
+    }
     __syncthreads();
-    const int64_t each = (total + gridDim.x - 1) / gridDim.x;
     int64_t x = blockIdx.x * each;
     const int64_t end = min(total, x + each);
 
@@ -183,8 +245,12 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
         const Sequence seq(a.batch, lo);
         const Share share(seq, a, ROWS, WARPS);
         const int64_t rel = x - before[lo];
-        const int item = static_cast<int>(rel / share.tiles), tile0 = static_cast<int>(rel - static_cast<int64_t>(item) * share.tiles);
-        const int tile1 = static_cast<int>(min(static_cast<int64_t>(share.tiles), tile0 + end - x));
+        const int padded_tiles = whole_pads(share.tiles);
+        const int item = static_cast<int>(quotient(rel, padded_tiles)), from = static_cast<int>(rel - static_cast<int64_t>(item) * padded_tiles);
+        const int to = static_cast<int>(min(static_cast<int64_t>(padded_tiles), from + end - x));
+        // padded: as many tiles as the item's other blocks have, or one less
+        const int span = padded ? (share.tiles - 1) / (padded_tiles / pad) + 1 : 1;
+        const int tile0 = padded ? from / pad * span : from, tile1 = padded ? min(share.tiles, tile0 + span) : to;
         const int row_tile = item / a.kv.heads, head = item - row_tile * a.kv.heads;
 
         // This warp's blocks: first, first + WARPS, ..
@@ -527,8 +593,8 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
             }
         }
         __syncthreads();
-        const bool whole = tile0 == 0 && tile1 == share.tiles;
-        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (tile0 == 0);
+        const bool whole = from == 0 && to == padded_tiles;
+        const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (from == 0);
         for (int v = threadIdx.x; v < ROWS * D / 4; v += THREADS) {
             const int r = v / (D / 4), ch = (v - r * (D / 4)) * 4;
             float most = -INFINITY;
@@ -551,40 +617,56 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
                 if (ch == 0) p.stat[slot * ROWS + r] = make_float2(most, all);
             }
         }
-        if (!whole && tile0 == 0 && threadIdx.x == 0) {
-            const int64_t item_end = x + share.tiles;  // of its tiles, numbered with all
-            p.split[blockIdx.x] = make_int4(lo, head, row_tile, static_cast<int>((item_end - 1) / each - blockIdx.x + 1));
+        if (!whole && threadIdx.x == 0) {
+            const int64_t begun = x - from;  // its first tile's number
+            if (from == 0)
+                p.split[blockIdx.x] = make_int4(lo, head, row_tile, static_cast<int>(quotient(begun + padded_tiles - 1, each)) - blockIdx.x + 1);
+            else
+                p.from[blockIdx.x] = static_cast<int>(quotient(begun, each));
         }
-        x += tile1 - tile0;
+        x += to - from;
         __syncthreads();  // before the next copies into the rings
     }
 }
 
-// What several blocks had a part of each, in the order of the tokens.
-__global__ void __launch_bounds__(THREADS) join_kernel(const __grid_constant__ FewAttend p, int tile_rows) {
+// What several blocks had a part of each. As many blocks as had one join it, each some of its outputs;
+// a block's threads take those, four channels each, beside one another and the parts in turn, and what
+// they have is added in a fixed order.
+__global__ void __launch_bounds__(JOINERS) join_kernel(const __grid_constant__ FewAttend p, int tile_rows) {
+    __shared__ float4 sums[JOINERS];
+    __shared__ float2 stats[JOINERS];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 it = p.split[blockIdx.x];
-    if (it.w == 0) return;
     const AttendArgs& a = p.a;
-    const Sequence seq(a.batch, it.x);
-    const int dim = a.kv.dim, rows = seq.count * a.share, quads = dim / 4;
-    auto slot = [&](int i) { return 2 * (static_cast<int64_t>(blockIdx.x) + i) + (i == 0); };
-    for (int v = threadIdx.x; v < tile_rows * quads; v += THREADS) {
-        const int r = v / quads, ch = (v - r * quads) * 4, row = it.z * tile_rows + r;
-        if (row >= rows) continue;
-        float most = -INFINITY;
-        for (int i = 0; i < it.w; ++i) most = fmaxf(most, p.stat[slot(i) * tile_rows + r].x);
-        float4 sum = make_float4(0, 0, 0, 0);
-        float all = 0;
+    const int quads = a.kv.dim / 4, from = p.from[blockIdx.x];
+    for (int k = 0; k < 2; ++k) {  // what the block ended, what it began
+        const int begin = k ? blockIdx.x : from;
+        if (k == 0 && begin == blockIdx.x) continue;
+        const int4 it = p.split[begin];
+        if (it.w == 0) continue;
+        const Sequence seq(a.batch, it.x);
+        const int outs = min(tile_rows, seq.count * a.share - it.z * tile_rows) * quads, each = (outs + it.w - 1) / it.w;
+        const int first = (blockIdx.x - begin) * each, upto = min(outs, first + each);
+        int abreast = 1;  // parts that are read beside one another
+        while (abreast < it.w && abreast < 32) abreast <<= 1;
+        const int width = JOINERS / abreast, column = threadIdx.x & (width - 1), row = threadIdx.x / width;
+        auto slot = [&](int i) { return 2 * (static_cast<int64_t>(begin) + i) + (i == 0); };
+        for (int o = first; o < upto; o += width) {
+            const int out = o + column, r = out / quads, ch = (out - r * quads) * 4;
+            float2 both = make_float2(-INFINITY, 0);
+            float4 sum = make_float4(0, 0, 0, 0);
+            if (out < upto) {
 #pragma unroll 4
-        for (int i = 0; i < it.w; ++i) {
-            const float2 s = p.stat[slot(i) * tile_rows + r];
-            const float4 add = *reinterpret_cast<const float4*>(p.part + (slot(i) * tile_rows + r) * dim + ch);
-            const float by = s.x == -INFINITY ? (s.y == 0.0f ? 0.0f : 1.0f) : ex2(s.x - most);
-            if (s.y != 0.0f) sum.x = fmaf(by, add.x, sum.x), sum.y = fmaf(by, add.y, sum.y), sum.z = fmaf(by, add.z, sum.z), sum.w = fmaf(by, add.w, sum.w);
-            all = fmaf(by, s.y, all);
+                for (int i = row; i < it.w; i += abreast)
+                    take(sum, both, *reinterpret_cast<const float4*>(p.part + (slot(i) * tile_rows + r) * a.kv.dim + ch), p.stat[slot(i) * tile_rows + r]);
+            }
+            sums[threadIdx.x] = sum, stats[threadIdx.x] = both;
+            __syncthreads();
+            if (row == 0 && out < upto) {
+                for (int i = 1; i < min(abreast, it.w); ++i) take(sum, both, sums[i * width + column], stats[i * width + column]);
+                finish(a, seq, it.y, it.z * tile_rows + r, ch, sum, both.x, both.y);
+            }
+            __syncthreads();
         }
-        finish(a, seq, it.y, row, ch, sum, most, all);
     }
 }
 
@@ -602,22 +684,28 @@ int launch_few(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route) {
             return UOR_B200_DEVICE_ERROR;
         per_sm = found;
     }
-    const int64_t grid = static_cast<int64_t>(ctx->sm_count) * per_sm;
+    // As many blocks as the table's whole length gives work.
+    const int64_t tiles = std::max(1, (a.batch.capacity + KV_BLOCK * WARPS - 1) / (KV_BLOCK * WARPS));
+    const int64_t items = (a.batch.seqs + static_cast<int64_t>(a.batch.rows) * a.share / (8 * NT)) * a.kv.heads;
+    const int64_t most = static_cast<int64_t>(ctx->sm_count) * per_sm;
+    if (items > INT32_MAX) return UOR_B200_UNSUPPORTED;
+    const int64_t grid = std::min(most, items >= most ? most : items * ((tiles + LEAST - 1) / LEAST));
     const size_t parts = static_cast<size_t>(2 * grid) * 8 * NT;
     int st = UOR_B200_OK;
-    auto* ws = static_cast<uint8_t*>(ctx_buffer(ctx, SLOT_WS, parts * (D * 4 + 8) + grid * 16, &st));
+    auto* ws = static_cast<uint8_t*>(ctx_buffer(ctx, SLOT_WS, parts * (D * 4 + 8) + grid * 20, &st));
     if (!ws) return st;
     FewAttend p{};
     p.a = a;
     p.part = reinterpret_cast<float*>(ws);
     p.stat = reinterpret_cast<float2*>(ws + parts * D * 4);
     p.split = reinterpret_cast<int4*>(ws + parts * (D * 4 + 8));
+    p.from = reinterpret_cast<int*>(p.split + grid);
     route->tile_m = 8 * NT, route->tile_n = KV_BLOCK * WARPS, route->tile_k = D;
     route->ctas = static_cast<uint32_t>(grid);
     kernel<<<static_cast<unsigned>(grid), THREADS, smem, ctx->stream>>>(p);
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(static_cast<unsigned>(grid));
-    c.blockDim = dim3(THREADS);
+    c.blockDim = dim3(JOINERS);
     c.stream = ctx->stream;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
