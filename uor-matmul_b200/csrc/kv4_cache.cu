@@ -1,14 +1,19 @@
 // kv4_cache.cu -- tokens into and out of the 4-bit cache of keys and values.
 //
-// Bound by memory: a prompt's rows are read once, the rotated queries and the codes written. A warp
-// has one row and steps through its heads, a lane eight neighbouring channels of a head, so that its
-// cosines and sines are read once a row. A group's extremes meet by shuffles.
+// A prompt's rows are read once, the rotated queries and the codes written. A warp has one row and steps
+// through its heads, a lane eight neighbouring channels of a head, so that its cosines and sines are read
+// once a row. A group's extremes meet by shuffles.
 //
-// A rotated value is the exact x cos - y sin rounded to f32 and then to 16 bits; a code that comes out
-// one off would be a whole step of the range off, so both are computed as their definition has them,
-// at the price of single precision: two fused multiply-adds give x cos - y sin to 2^-23 of its parts,
-// and only where that leaves the 16 bits open (once in some ten thousand values) doubles decide. A
-// code is a multiplication by the scale's reciprocal but where that comes near a half.
+// A rotated value is the exact x cos - y sin rounded to f32 and then to 16 bits; a code that comes out one
+// off would be a whole step of the range off, so both are computed as their definition has them. The
+// products are exact in 64 bits, where this processor multiplies at half its 32-bit rate. (In 32 bits, by
+// two fused multiply-adds with a bound of what they leave open and doubles where that matters: the same
+// 96 us.) A code is a multiplication by the scale's reciprocal but where that comes near a half; its eight
+// and their exceptions are one branch.
+//
+// 8192 tokens, 32 heads of queries, 8 of keys and values, 128 channels, all rotated: 96 us, 2.4 TB/s, and
+// 13 us to read them back. Bound by issue slots and what a processor's 20 warps have under way (61 % of
+// its cycles issue; with 16 warps of 128 registers 109 us); one token: 3.8 us, a launch's own time.
 #include "kv4.cuh"
 
 #include <cstring>
@@ -67,31 +72,31 @@ struct Half<__half> {
     }
 };
 
-// T(f32(x c - y s)), the difference exact but for one rounding to double where it has more bits.
-template <typename T>
-__device__ __noinline__ float turned_slow(float x, float c, float y, float s) {
-    const double v = __dsub_rn(__dmul_rn(x, c), __dmul_rn(y, s));
-    return to_f32(from_f32<T>(__double2float_rn(v)));
-}
-template <typename T>
-__device__ __forceinline__ float turned(float x, float c, float y, float s) {
-    const float p = __fmul_rn(y, s), e = __fmaf_rn(y, s, -p), d = __fmaf_rn(x, c, -p), f = __fsub_rn(d, e);
-    // f is off by half a unit of d and of itself, and by what underflow takes from e
-    const float off = __fmaf_rn(fabsf(d) + fabsf(f), 0x1p-23f, 0x1p-146f);
-    const uint32_t both = Half<T>::pair(f - off, f + off);
-    if ((both & 0xFFFFu) == both >> 16 && fabsf(f) <= 3e38f) return Half<T>::first(both);
-    return turned_slow<T>(x, c, y, s);
+// f32(x c - y s): the products are exact in 64 bits, their difference is rounded there once.
+__device__ __forceinline__ float turned(float x, double c, float y, double s) {
+    return __double2float_rn(__fma_rn(x, c, -__dmul_rn(y, s)));
 }
 
 __device__ __noinline__ uint32_t code_slow(float t, float scale) {
     return static_cast<uint32_t>(fminf(fmaxf(rintf(__fadd_rn(__fdiv_rn(t, scale), 7.5f)), 0.0f), 15.0f));
 }
-// The integer nearest to t / scale + 7.5, the quotient and the sum each rounded, within 0 .. 15.
-// inverse: 1 / scale, or 0 for one so small that it has none.
-__device__ __forceinline__ uint32_t code_of(float t, float scale, float inverse) {
-    const float z = __fmaf_rn(t, inverse, 7.5f), n = rintf(z);
-    if (inverse == 0.0f || fabsf(z - n) > 0.4999f) return code_slow(t, scale);
-    return static_cast<uint32_t>(fminf(fmaxf(n, 0.0f), 15.0f));
+// Eight codes: the integers nearest to (r - mid) / scale + 7.5, the quotient and the sum each rounded,
+// within 0 .. 15. inverse: 1 / scale, or 0 for one so small that it has none.
+__device__ __forceinline__ uint32_t codes_of(const float (&r)[8], float mid, float scale, float inverse) {
+    uint32_t codes = 0, hard = inverse == 0.0f ? 0xFFu : 0u;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // 1.5 2^23 more leaves the nearest integer in the lowest bits; within 0 .. 15 before, which it is but for rounding
+        const float z = fminf(fmaxf(__fmaf_rn(__fsub_rn(r[i], mid), inverse, 7.5f), 0.0f), 15.0f), n = __fadd_rn(z, 12582912.0f);
+        if (fabsf(z - __fsub_rn(n, 12582912.0f)) > 0.4999f) hard |= 1u << i;
+        codes |= (__float_as_uint(n) & 15u) << (4 * i);
+    }
+    if (hard) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (hard >> i & 1) codes = (codes & ~(15u << (4 * i))) | code_slow(__fsub_rn(r[i], mid), scale) << (4 * i);
+    }
+    return codes;
 }
 
 // Eight channels of 16 bits from `p`; vec: as one vector.
@@ -122,10 +127,11 @@ enum Turn {
     TURN_ANY = 3      // some of them, or with channels that do not lie so: one by one
 };
 
-constexpr int AHEAD = 4;  // a lane's heads under way
+constexpr int AHEAD = 2;  // a lane's heads under way; four take the registers of a fifth block: 104 us
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) append_kernel(const __grid_constant__ AppendArgs a, int slices) {
+// VEC: every row of heads begins at a multiple of 16 bytes.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(WARPS * 32, 5) append_kernel(const __grid_constant__ AppendArgs a, int slices) {
     const int lane = threadIdx.x & 31;
     const int64_t item = static_cast<int64_t>(blockIdx.x) * WARPS + (threadIdx.x >> 5);
     const int row = static_cast<int>(item / slices), slice = static_cast<int>(item - static_cast<int64_t>(row) * slices);
@@ -145,7 +151,7 @@ __global__ void __launch_bounds__(WARPS * 32) append_kernel(const __grid_constan
     const int t = at & 15, g = channel >> a.kv.group_shift, per_group = 1 << (a.kv.group_shift - 3);
     // The rotation of this lane's channels.
     int turn = TURN_NONE, other = 0;
-    float c[8], sn[8];
+    double c[8], sn[8];
     if (channel < a.turned && mine) {
         const float *cos = a.cos + at * a.turn_rs, *sin = a.sin + at * a.turn_rs;
         const int half = a.turned / 2;
@@ -183,8 +189,8 @@ __global__ void __launch_bounds__(WARPS * 32) append_kernel(const __grid_constan
             int local;
             place(h, &from, &local);
             const uint16_t* p = static_cast<const uint16_t*>(from->p) + row * from->rs + local * dim + channel;
-            x[u] = load8(p, from->vec);
-            if (turn == TURN_HALVES && h < a.q_heads + a.kv.heads) y[u] = load8(p + other, from->vec);
+            x[u] = load8(p, VEC || from->vec);
+            if (turn == TURN_HALVES && h < a.q_heads + a.kv.heads) y[u] = load8(p + other, VEC || from->vec);
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
@@ -194,22 +200,18 @@ __global__ void __launch_bounds__(WARPS * 32) append_kernel(const __grid_constan
             const bool query = h < a.q_heads, value = h >= a.q_heads + a.kv.heads;
             uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
             float r[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[2 * i] = Half<T>::first(w[i]), r[2 * i + 1] = Half<T>::second(w[i]);
             if (live && !value && turn != TURN_NONE) {
                 if (turn == TURN_HALVES) {
                     const uint32_t v[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        r[2 * i] = turned<T>(r[2 * i], c[2 * i], Half<T>::first(v[i]), sn[2 * i]);
-                        r[2 * i + 1] = turned<T>(r[2 * i + 1], c[2 * i + 1], Half<T>::second(v[i]), sn[2 * i + 1]);
-                    }
+                    for (int i = 0; i < 4; ++i)
+                        w[i] = Half<T>::pair(turned(Half<T>::first(w[i]), c[2 * i], Half<T>::first(v[i]), sn[2 * i]),
+                                             turned(Half<T>::second(w[i]), c[2 * i + 1], Half<T>::second(v[i]), sn[2 * i + 1]));
                 } else if (turn == TURN_PAIRS) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float p = r[2 * i], o = r[2 * i + 1];
-                        r[2 * i] = turned<T>(p, c[i], o, sn[i]);
-                        r[2 * i + 1] = turned<T>(o, c[i], p, -sn[i]);
+                        const float even = Half<T>::first(w[i]), odd = Half<T>::second(w[i]);
+                        w[i] = Half<T>::pair(turned(even, c[i], odd, sn[i]), turned(odd, c[i], even, -sn[i]));
                     }
                 } else {
                     const Rows* from;
@@ -219,25 +221,30 @@ __global__ void __launch_bounds__(WARPS * 32) append_kernel(const __grid_constan
                     const float *cos = a.cos + at * a.turn_rs, *sin = a.sin + at * a.turn_rs;
                     const int half = a.turned / 2;
 #pragma unroll
+                    for (int i = 0; i < 4; ++i) r[2 * i] = Half<T>::first(w[i]), r[2 * i + 1] = Half<T>::second(w[i]);
+#pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         const int ch = channel + i;
                         if (ch >= a.turned) break;
                         const bool low = a.interleaved ? ch % 2 == 0 : ch < half;
                         const int pair = a.interleaved ? ch / 2 : low ? ch : ch - half;
                         const int with = a.interleaved ? ch ^ 1 : low ? ch + half : ch - half;
-                        r[i] = turned<T>(r[i], cos[pair], to_f32(head[with]), low ? sin[pair] : -sin[pair]);
+                        r[i] = turned(r[i], cos[pair], to_f32(head[with]), low ? sin[pair] : -sin[pair]);
                     }
-                }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = Half<T>::pair(r[2 * i], r[2 * i + 1]);
+                    for (int i = 0; i < 4; ++i) w[i] = Half<T>::pair(r[2 * i], r[2 * i + 1]);
+                }
             }
             __syncwarp();  // queries may turn in place: no lane writes what another still reads
             if (live && query) {
                 store8(static_cast<uint16_t*>(a.q_out.p) + row * a.q_out.rs + h * dim + channel, make_uint4(w[0], w[1], w[2], w[3]),
-                       a.q_out.vec);
+                       VEC || a.q_out.vec);
             }
+            if (h0 + (u + 1) * abreast <= a.q_heads) continue;  // of the whole warp
             // Extremes of the group, by all lanes: those of other kinds take part and are not used.
             float high, low;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[2 * i] = Half<T>::first(w[i]), r[2 * i + 1] = Half<T>::second(w[i]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 r[i] = r[i] != r[i] ? 0.0f : fminf(fmaxf(r[i], -Half<T>::MOST), Half<T>::MOST);
@@ -254,11 +261,7 @@ __global__ void __launch_bounds__(WARPS * 32) append_kernel(const __grid_constan
             // half of the largest float and 7.5 halves of the scale: what is held stays within the type
             if (fmaf(3.75f, scale, 0.5f * fabsf(mid)) > 0.5f * Half<T>::MOST) scale = Half<T>::below(scale);
             const float inverse = scale > 0x1p-120f ? __frcp_rn(scale) : 0.0f;
-            uint32_t codes = 0;
-            if (scale > 0.0f) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) codes |= code_of(__fsub_rn(r[i], mid), scale, inverse) << (4 * i);
-            }
+            const uint32_t codes = scale > 0.0f ? codes_of(r, mid, scale, inverse) : 0u;
             const int head = h - a.q_heads - (value ? a.kv.heads : 0);
             uint8_t* to = block + head * a.kv.head_bytes;
             if (value) {
@@ -353,7 +356,9 @@ int run_kv4_append(uor_b200_ctx* ctx, const AppendArgs& a, uor_b200_route* route
     const int slices = slices_for(ctx, a.batch.rows, a.q_heads + 2 * a.kv.heads, 32 / (a.kv.dim / 8));
     const int64_t blocks = (static_cast<int64_t>(a.batch.rows) * slices + WARPS - 1) / WARPS;
     if (blocks > INT32_MAX) return UOR_B200_UNSUPPORTED;
-    auto* kernel = a.elem == UOR_B200_BF16 ? append_kernel<__nv_bfloat16> : append_kernel<__half>;
+    const bool vec = a.k.vec && a.v.vec && (a.q_heads == 0 || (a.q.vec && a.q_out.vec));
+    auto* kernel = a.elem == UOR_B200_BF16 ? (vec ? append_kernel<__nv_bfloat16, true> : append_kernel<__nv_bfloat16, false>)
+                                           : (vec ? append_kernel<__half, true> : append_kernel<__half, false>);
     kernel<<<static_cast<unsigned>(blocks), WARPS * 32, 0, ctx->stream>>>(a, slices);
     return UOR_B200_OK;
 }
