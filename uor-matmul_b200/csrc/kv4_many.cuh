@@ -45,14 +45,16 @@ struct Shape {
     static constexpr int TOKENS = 64;                    // of a step
     static constexpr int BLOCKS = TOKENS / KV_BLOCK;
     static constexpr int ATOMS = (D + 63) / 64;          // of 64 channels, the 128 bytes that a swizzle spans
-    static constexpr int KSTAGES = D <= 128 ? 4 : 2, VSTAGES = D <= 128 ? 4 : D <= 192 ? 2 : 1;
-    static constexpr int RING = 3;                       // blocks' keys, or values, under way of each decoding warp
+    static constexpr int KSTAGES = D <= 128 ? 2 : 1, VSTAGES = D <= 128 ? 3 : D <= 192 ? 2 : 1;
+    static constexpr int RING = D <= 192 ? 3 : 2;        // blocks' keys, or values, under way of each decoding warp
     static constexpr int THERE = 8;                      // steps that the decoders' notes are kept for
-    static constexpr int Q_ATOM = 128 * 128, Q_HALF = ATOMS * Q_ATOM;
-    static constexpr int T_ATOM = TOKENS * 128, T_BYTES = ATOMS * T_ATOM;  // a step's keys, or values
+    static constexpr int Q_ATOM = 128 * 128, Q_SUMS = ATOMS * Q_ATOM, Q_HALF = Q_SUMS + 128 * 32;
+    static constexpr int T_ATOM = TOKENS * 128, T_BYTES = ATOMS * T_ATOM;  // a step's values
+    // A step's keys without their middles, rounded, what that left, and the middles.
+    static constexpr int K_MIDS = 2 * T_BYTES, K_BYTES = K_MIDS + TOKENS * 32;
     static constexpr int S_AT = 0, O_AT = 2 * HALVES * TOKENS;  // tensor-memory columns: scores, sums
     static constexpr int BARS = HALVES + 3 + 2 * KSTAGES + 2 * VSTAGES + 6 * HALVES + 2 + 2 * DECODERS * RING;
-    static constexpr int FIXED = HALVES * Q_HALF + KSTAGES * T_BYTES + VSTAGES * T_BYTES;
+    static constexpr int FIXED = HALVES * Q_HALF + KSTAGES * K_BYTES + VSTAGES * T_BYTES;
     static_assert(BLOCKS == DECODERS, "a block of a step to each decoding warp");
     static_assert(O_AT + HALVES * D <= 512, "tensor memory");
     static int smem(int groups) { return 1024 + FIXED + DECODERS * RING * kv_block_bytes(D, groups) + BARS * 8 + THERE * BLOCKS; }
@@ -87,6 +89,17 @@ __device__ __forceinline__ uint32_t fma_half2(uint32_t a, uint32_t b, uint32_t c
     else
         asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
     return r;
+}
+// x: the product of scale and x, rounded; left: exactly what that left, four bits at most.
+template <typename T>
+__device__ __forceinline__ void product(uint32_t scale, uint32_t& x, uint32_t& left) {
+    uint32_t p, minus;
+    if constexpr (std::is_same<T, __half>::value)
+        asm("mul.rn.f16x2 %0, %2, %3;\n neg.f16x2 %1, %0;" : "=&r"(p), "=r"(minus) : "r"(scale), "r"(x));
+    else
+        asm("mul.rn.bf16x2 %0, %2, %3;\n neg.bf16x2 %1, %0;" : "=&r"(p), "=r"(minus) : "r"(scale), "r"(x));
+    left = fma_half2<T>(scale, x, minus);
+    x = p;
 }
 // Into the tensor cores' operands, which no thread reads: reads of the rings may pass it.
 __device__ __forceinline__ void sts128(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -188,7 +201,7 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
     const AttendArgs& a = p.a;
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
     uint8_t* keys_at = smem + Z::HALVES * Z::Q_HALF;
-    uint8_t* values_at = keys_at + Z::KSTAGES * Z::T_BYTES;
+    uint8_t* values_at = keys_at + Z::KSTAGES * Z::K_BYTES;
     uint8_t* rings = values_at + Z::VSTAGES * Z::T_BYTES;
     uint64_t* bars = reinterpret_cast<uint64_t*>(rings + DECODERS * Z::RING * a.kv.block_bytes);
     uint8_t* there = reinterpret_cast<uint8_t*>(bars + Z::BARS);  // [THERE][BLOCKS]: whether a step's blocks are
@@ -268,27 +281,66 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
             const bool live = r < share.rows;
             const int at = live ? seq.at + r / a.share : -1;
             const int row = seq.first + (live ? r / a.share : 0), col = it.head * a.share + (live ? r % a.share : 0);
-            // The row's query, its channels in each eight as the keys' words have them, and negated
-            // where the scale is, so that the largest score is the largest product.
+            // The row's query below 2 by a power of two, its channels in each eight as the keys' words have
+            // them, and negated where the scale is, so that the largest score is the largest product; and
+            // its groups' sums, that the middles multiply, in two parts.
+            float up;
             {
                 const uint16_t* from = static_cast<const uint16_t*>(a.q.p) + row * a.q.rs + static_cast<int64_t>(col) * D;
-                const uint32_t to = smem_u32(smem) + half * Z::Q_HALF + t * 128, flip = a.scale < 0 ? 0x80008000u : 0u;
+                const uint32_t to = smem_u32(smem) + half * Z::Q_HALF + t * 128, sums_to = smem_u32(smem) + half * Z::Q_HALF + Z::Q_SUMS + (t >> 3) * 256 + (t & 7) * 16;
+                auto eight = [&](int i, uint32_t (&w)[4]) {
+                    w[0] = w[1] = w[2] = w[3] = 0;
+                    if (!live) return;
+                    if (a.q.vec) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(from + 8 * i);
+                        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                    } else {
 #pragma unroll
+                        for (int k = 0; k < 4; ++k) w[k] = from[8 * i + 2 * k] | static_cast<uint32_t>(from[8 * i + 2 * k + 1]) << 16;
+                    }
+                };
+                float most = 0;
+#pragma unroll 8
                 for (int i = 0; i < D / 8; ++i) {
-                    uint32_t w[4] = {0, 0, 0, 0};
-                    if (live) {
-                        if (a.q.vec) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(from + 8 * i);
-                            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-                        } else {
+                    uint32_t w[4];
+                    eight(i, w);
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) w[k] = from[8 * i + 2 * k] | static_cast<uint32_t>(from[8 * i + 2 * k + 1]) << 16;
-                        }
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 v = two<T>(w[k]);
+                        most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
+                    }
+                }
+                const uint32_t power = min(max(__float_as_uint(most) >> 23, 1u), 253u);  // most is 1 to 2 times 2^(power - 127)
+                const float down = __uint_as_float((254 - power) << 23 | (a.scale < 0 ? 0x80000000u : 0u));
+                up = __uint_as_float(power << 23);
+                float sum = 0;
+#pragma unroll 4
+                for (int i = 0; i < D / 8; ++i) {
+                    uint32_t w[4];
+                    eight(i, w);
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) w[k] ^= flip;
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 v = two<T>(w[k]);
+                        const float x = v.x * down, y = v.y * down;
+                        sum += x + y;
+                        w[k] = pack<T>(x, y);
                     }
                     sts128(to + (i >> 3) * Z::Q_ATOM + (((i & 7) ^ (t & 7)) << 4), __byte_perm(w[0], w[2], 0x5410), __byte_perm(w[0], w[2], 0x7632),
                            __byte_perm(w[1], w[3], 0x5410), __byte_perm(w[1], w[3], 0x7632));
+                    const int per = 1 << (a.kv.group_shift - 3);
+                    if ((i & (per - 1)) == per - 1) {
+                        const int group = i / per;
+                        const uint32_t high = pack<T>(sum, 0.0f) & 0xFFFFu;
+                        const float held = two<T>(high).x;  // of what is not finite nothing is left
+                        const uint32_t low = fabsf(held) < INFINITY ? pack<T>(sum - held, 0.0f) & 0xFFFFu : 0u;
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(sums_to + group * 2), "h"(static_cast<uint16_t>(high)));
+                        asm volatile("st.shared.u16 [%0], %1;" ::"r"(sums_to + 128 + group * 2), "h"(static_cast<uint16_t>(low)));
+                        sum = 0;
+                    }
+                }
+                for (int group = a.kv.groups; group < 8; ++group) {
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(sums_to + group * 2), "h"(static_cast<uint16_t>(0)));
+                    asm volatile("st.shared.u16 [%0], %1;" ::"r"(sums_to + 128 + group * 2), "h"(static_cast<uint16_t>(0)));
                 }
                 fence_proxy_async();
                 __syncwarp();
@@ -298,7 +350,7 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
             const int first_row = it.tile * 128 * Z::HALVES + half * 128, last_row = min(first_row + 127, share.rows - 1);
             const int nearest = min(seq.at + first_row / a.share, seq.keys - 1);
             const int behind = a.window ? seq.at + last_row / a.share - a.window : -1;
-            const float k = fmaxf(fabsf(a.scale) * LOG2E, 1e-38f);  // of a scale of 0 still what -inf becomes -inf by
+            const float k = fmaxf(fabsf(a.scale) * LOG2E * up, 1e-38f);  // of a scale of 0 still what -inf becomes -inf by
             const uint64_t kk = pair_of(k, k);
             float m = -INFINITY;
             uint64_t l = 0;
@@ -497,20 +549,30 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
                     const uint32_t odd = (t & 1) ? 0x3232 : 0x1010;
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t to = smem_u32(keys_at) + stage * Z::T_BYTES + (row + h * 8 + t) * 128;
+                        const uint32_t to = smem_u32(keys_at) + stage * Z::K_BYTES + (row + h * 8 + t) * 128;
                         uint32_t v[N32];
-                        uint2 q[N32];
+                        uint32_t q[N32];
+                        const uint8_t* params = part + 8 * D + (h * 4 + (t >> 1)) * groups * 8;
                         words<N32>(part + ((h * 8 + t) * 4 + c) * N32 * 4, v);
 #pragma unroll
-                        for (int n = 0; n < N32; ++n) q[n] = *reinterpret_cast<const uint2*>(part + 8 * D + ((h * 4 + (t >> 1)) * groups + (n >> to_group)) * 8);
+                        for (int n = 0; n < N32; ++n) q[n] = *reinterpret_cast<const uint32_t*>(params + (n >> to_group) * 8);
+                        // the token's middles of groups 2 c and 2 c + 1, once for each part of the queries' sums
+                        const uint32_t m0 = 2 * c < groups ? *reinterpret_cast<const uint32_t*>(params + 2 * c * 8 + 4) : 0u;
+                        const uint32_t m1 = 2 * c + 1 < groups ? *reinterpret_cast<const uint32_t*>(params + (2 * c + 1) * 8 + 4) : 0u;
+                        const uint32_t mids = __byte_perm(m0, m1, (t & 1) ? 0x7632 : 0x5410);
+                        const uint32_t mids_to = smem_u32(keys_at) + stage * Z::K_BYTES + Z::K_MIDS + (2 * w + h) * 256 + t * 16 + c * 4;
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(mids_to), "r"(mids));
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(mids_to + 128), "r"(mids));
 #pragma unroll
                         for (int n = 0; n < N32; ++n) {
-                            const uint32_t scale = __byte_perm(q[n].x, 0, odd), mid = __byte_perm(q[n].y, 0, odd);
-                            uint32_t x[4];
+                            const uint32_t scale = __byte_perm(q[n], 0, odd);
+                            uint32_t x[4], left[4];
                             centred<T>(v[n], x);
 #pragma unroll
-                            for (int b = 0; b < 4; ++b) x[b] = fma_half2<T>(scale, x[b], mid);
-                            sts128(to + (n >> 1) * Z::T_ATOM + ((((n & 1) * 4 + c) ^ t) << 4), x[0], x[1], x[2], x[3]);
+                            for (int b = 0; b < 4; ++b) product<T>(scale, x[b], left[b]);
+                            const uint32_t piece = to + (n >> 1) * Z::T_ATOM + ((((n & 1) * 4 + c) ^ t) << 4);
+                            sts128(piece, x[0], x[1], x[2], x[3]);
+                            sts128(piece + Z::T_BYTES, left[0], left[1], left[2], left[3]);
                         }
                     }
                 } else {
@@ -564,13 +626,17 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
                 Item it;
                 constexpr uint32_t QK = idesc_f16(128, Z::TOKENS, BF16), PV = idesc_f16(128, D, BF16, true);
                 const uint64_t q_at = smem_desc_sw128(smem_u32(smem), 16, 1024), k_at = smem_desc_sw128(smem_u32(keys_at), 16, 1024);
+                const uint64_t qs_at = smem_desc_plain(smem_u32(smem) + Z::Q_SUMS, 128, 256), ks_at = smem_desc_plain(smem_u32(keys_at) + Z::K_MIDS, 128, 256);
                 const uint64_t v_at = smem_desc_sw128(smem_u32(values_at), Z::T_ATOM, 1024);
                 auto scores = [&](uint32_t g) {
                     const uint32_t side = 2 * half + (g & 1), ks = g % Z::KSTAGES;
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-                        mma_f16(tmem + Z::S_AT + side * Z::TOKENS, q_at + ((half * Z::Q_HALF + i / 4 * Z::Q_ATOM + i % 4 * 32) >> 4),
-                                k_at + (ks * Z::T_BYTES + i / 4 * Z::T_ATOM + i % 4 * 32) / 16, QK, i != 0);
+                    for (int part = 0; part < 2; ++part)
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i)
+                            mma_f16(tmem + Z::S_AT + side * Z::TOKENS, q_at + ((half * Z::Q_HALF + i / 4 * Z::Q_ATOM + i % 4 * 32) >> 4),
+                                    k_at + (ks * Z::K_BYTES + part * Z::T_BYTES + i / 4 * Z::T_ATOM + i % 4 * 32) / 16, QK, i != 0 || part != 0);
+                    mma_f16(tmem + Z::S_AT + side * Z::TOKENS, qs_at + (half * Z::Q_HALF >> 4), ks_at + ks * Z::K_BYTES / 16, QK, true);
                     mma_commit(sfull + 8 * side);
                 };
                 auto values = [&](uint32_t g, bool first) {  // sums (+)= weights values

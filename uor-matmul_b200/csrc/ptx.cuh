@@ -273,6 +273,13 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo
     return d;
 }
 
+// The same without a swizzle, of a K-major tile: core matrices of 8 rows by 16 bytes, lbo_bytes apart along
+// K and sbo_bytes apart along the rows.
+__device__ __forceinline__ uint64_t smem_desc_plain(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+    return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFFu) << 16 |
+           static_cast<uint64_t>((sbo_bytes >> 4) & 0x3FFFu) << 32 | static_cast<uint64_t>(1) << 46;
+}
+
 // Instruction descriptor for kind::i8 with a 32-bit signed accumulator.
 //   bits 4-5: D format (2 = s32); 7-9: A format (1 = s8, 0 = u8); 10-12: B format;
 //   15: A major (1 = MN); 16: B major; 17-22: N >> 3; 24-28: M >> 4.
