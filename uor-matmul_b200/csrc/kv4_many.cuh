@@ -631,11 +631,11 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
                 auto scores = [&](uint32_t g) {
                     const uint32_t side = 2 * half + (g & 1), ks = g % Z::KSTAGES;
 #pragma unroll
-                    for (int part = 0; part < 2; ++part)
-#pragma unroll
-                        for (int i = 0; i < D / 16; ++i)
-                            mma_f16(tmem + Z::S_AT + side * Z::TOKENS, q_at + ((half * Z::Q_HALF + i / 4 * Z::Q_ATOM + i % 4 * 32) >> 4),
-                                    k_at + (ks * Z::K_BYTES + part * Z::T_BYTES + i / 4 * Z::T_ATOM + i % 4 * 32) / 16, QK, i != 0 || part != 0);
+                    for (int i = 0; i < D / 16; ++i) {
+                        const uint64_t k0 = k_at + (ks * Z::K_BYTES + i / 4 * Z::T_ATOM + i % 4 * 32) / 16;
+                        mma_f16_twice(tmem + Z::S_AT + side * Z::TOKENS, q_at + ((half * Z::Q_HALF + i / 4 * Z::Q_ATOM + i % 4 * 32) >> 4), k0,
+                                      k0 + Z::T_BYTES / 16, QK, i != 0);
+                    }
                     mma_f16(tmem + Z::S_AT + side * Z::TOKENS, qs_at + (half * Z::Q_HALF >> 4), ks_at + ks * Z::K_BYTES / 16, QK, true);
                     mma_commit(sfull + 8 * side);
                 };
