@@ -23,7 +23,9 @@
 // Weights times scales, for a 16-bit result, are rounded twice, as weights and values that were each
 // brought to 16 bits would be; sum_j p_j scale_j is of the same rounded numbers, so the cancellation costs
 // nothing. For an f32 result they are two 16-bit numbers, a rounded one and what that left (2^-17
-// together). They are bfloat16 whatever the cache's type is: float16 would lose the small ones.
+// together), and values' codes are code - 7.5, an addition more for each pair: the tensor cores' sums of
+// u, five times as large as what is left of them, cut off more than that (1.4e-5 of the result, not
+// 2.5e-6). Weights are bfloat16 whatever the cache's type is: float16 would lose the small ones.
 //
 // The work is cut evenly: tiles of 64 tokens of every item (a sequence, head and eight or sixteen rows)
 // are numbered by the lengths, which the device alone knows, and each block of threads has as many of them
@@ -67,11 +69,17 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {  // of numbe
     return (a | b) >> 32 ? a / b : static_cast<int64_t>(static_cast<uint32_t>(a) / static_cast<uint32_t>(b));
 }
 
-// A word's nibbles i and 4 + i, i = 0 .. 3: of values as bfloat16 1 + code / 16; of keys as float16 the
+// A word's nibbles i and 4 + i, i = 0 .. 3: of values as bfloat16 1 + code / 16, or (EXACT) code - 7.5; of keys as float16 the
 // same, or (FAST) 1 + code / 1024 of even i and 1 + code / 64 of odd ones.
+template <bool EXACT>
 __device__ __forceinline__ void unpack_values(uint32_t w, uint32_t (&u)[4]) {
-    u[0] = and_or(w << 3, 0x00780078u, 0x3F803F80u), u[1] = and_or(w >> 1, 0x00780078u, 0x3F803F80u);
-    u[2] = and_or(w >> 5, 0x00780078u, 0x3F803F80u), u[3] = and_or(w >> 9, 0x00780078u, 0x3F803F80u);
+    constexpr uint32_t BASE = EXACT ? 0x41804180u : 0x3F803F80u;  // 16, or 1
+    u[0] = and_or(w << 3, 0x00780078u, BASE), u[1] = and_or(w >> 1, 0x00780078u, BASE);
+    u[2] = and_or(w >> 5, 0x00780078u, BASE), u[3] = and_or(w >> 9, 0x00780078u, BASE);
+    if constexpr (EXACT) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("add.rn.bf16x2 %0, %0, %1;" : "+r"(u[i]) : "r"(0xC1BCC1BCu));  // -23.5
+    }
 }
 template <bool FAST>
 __device__ __forceinline__ void unpack_keys(uint32_t w, uint32_t (&u)[4]) {
@@ -161,6 +169,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
     constexpr int N32 = D / 32, ROWS = 8 * NT, G = N32 / GP;
     constexpr int block_bytes = kv_block_bytes(D, G);
     using B = __nv_bfloat16;
+    constexpr float UNIT = EXACT ? 1.0f : 16.0f;  // of the values' products
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t scan[WARPS];
     __shared__ int scan_items[WARPS];
@@ -530,7 +539,7 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
 #pragma unroll
             for (int i = 0; i < N32; ++i) {
                 if (i % GP == 0) {
-                    const uint32_t minus = g == i / GP ? 0xC1BCC1BCu : 0u;  // -23.5 in the group's row
+                    [[maybe_unused]] const uint32_t minus = g == i / GP ? 0xC1BCC1BCu : 0u;  // -23.5 in the group's row
                     const uint32_t s0 = *reinterpret_cast<const uint32_t*>(params + (c * G + i / GP) * 8);
                     const uint32_t s1 = *reinterpret_cast<const uint32_t*>(params + ((4 + c) * G + i / GP) * 8);
 #pragma unroll
@@ -545,15 +554,14 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
                             if constexpr (EXACT) {
                                 const float2 r0 = two<B>(high[n][0]), r1 = two<B>(high[n][1]);
                                 low[n][0] = pack<B>(v[0] - r0.x, v[1] - r0.y), low[n][1] = pack<B>(v[2] - r1.x, v[3] - r1.y);
-                                mma<B>(rest[n], minus, 0, minus, 0, low[n][0], low[n][1]);
                             }
                         }
-                        mma<B>(rest[n], minus, 0, minus, 0, high[n][0], high[n][1]);
+                        if constexpr (!EXACT) mma<B>(rest[n], minus, 0, minus, 0, high[n][0], high[n][1]);
                     }
                 }
                 uint32_t u0[4], u1[4];
-                unpack_values(w[0][i], u0);
-                unpack_values(w[1][i], u1);
+                unpack_values<EXACT>(w[0][i], u0);
+                unpack_values<EXACT>(w[1][i], u1);
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -586,10 +594,10 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
                 }
                 float* to = sums + ((warp * ROWS + n * 8 + 2 * c) * D + 32 * i + 4 * g);
                 const auto& v = o[n][i];
-                *reinterpret_cast<float4*>(to) = make_float4(fmaf(16.0f, v[0][0], mid0), fmaf(16.0f, v[0][2], mid0),
-                                                             fmaf(16.0f, v[1][0], mid0), fmaf(16.0f, v[1][2], mid0));
-                *reinterpret_cast<float4*>(to + D) = make_float4(fmaf(16.0f, v[0][1], mid1), fmaf(16.0f, v[0][3], mid1),
-                                                                 fmaf(16.0f, v[1][1], mid1), fmaf(16.0f, v[1][3], mid1));
+                *reinterpret_cast<float4*>(to) = make_float4(fmaf(UNIT, v[0][0], mid0), fmaf(UNIT, v[0][2], mid0),
+                                                             fmaf(UNIT, v[1][0], mid0), fmaf(UNIT, v[1][2], mid0));
+                *reinterpret_cast<float4*>(to + D) = make_float4(fmaf(UNIT, v[0][1], mid1), fmaf(UNIT, v[0][3], mid1),
+                                                                 fmaf(UNIT, v[1][1], mid1), fmaf(UNIT, v[1][3], mid1));
             }
         }
         __syncthreads();
