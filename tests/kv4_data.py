@@ -9,14 +9,16 @@ Scores: sums of dim products in f32, none chained more than dim / 8 + 16 times: 
 sum divides them). Values: weights times scales travel as two bfloat16, 2^-17 together, and f32 sums
 chain at most a block of 16 tokens at a time: (n / 16 + 64) 2^-23.
 
-For a 16-bit result the products of codes run with offsets of up to 64 |q| until a group's end: terms
-of 16 * 65 scale |q| <= 150 M |q|, in sums of 32 channels that are added four times at most, 4 2^-23
+For a 16-bit result the products of codes run with offsets of up to 4 |q| until a group's end: terms
+of 16 * 5 scale |q| <= 12 M |q|, in sums of 32 channels that are added eight times at most, 8 2^-23
 of them more. Queries are float16 then, of 2^-25 of a row's largest where they are less than 2^-14 of
 it. And weights times scales are rounded twice to bfloat16, 2 2^-8 of scale |code - 7.5| <= 1.1 M, and
 once, half a unit, beside the middles.
 
-Where keys, values and weights are rounded to 16 bits (many rows), half a unit of that type is added to
-each: to the scores of |q| |k|, to the weights and to the values. The output's own rounding is half a unit more."""
+Where values and weights are rounded to 16 bits (many rows), half a unit of that type is added to each. The
+keys' codes times their scales are exact there; the middles multiply a group's sum of queries in two parts of
+16 bits, which is off by 2^-17 of it, and queries below 2 lose 2^-25 of a row's largest in float16, as do the
+parts and the products' second ones. The output's own rounding is half a unit more."""
 import math
 
 import numpy as np
@@ -147,10 +149,11 @@ def attention(cache, q, share, scale, out, window=0, sinks=0, rounded=False, key
             lse[start:start + n, h] = (top + torch.log(total))[:, 0]
             off = (dim / 8 + 16) * 2.0 ** -23 * abs(scale) * (x.abs() @ biggest(k).T)
             if out != U.F32:
-                off = off + abs(scale) * (4 * 2.0 ** -23 * (x.abs() @ (25 * biggest(k)).T)
+                off = off + abs(scale) * (8 * 2.0 ** -23 * (x.abs() @ (2 * biggest(k)).T)
                                           + 2.0 ** -25 * x.abs().amax(1, keepdim=True) * biggest(k).sum(1)[None])
             if rounded:
-                off = off + unit * abs(scale) * (x.abs() @ k.abs().T)
+                off = off + abs(scale) * (2.0 ** -17 * (x.abs() @ (biggest(k) / 6).T)
+                                          + 3 * 2.0 ** -25 * x.abs().amax(1, keepdim=True) * (biggest(k) / 6).sum(1)[None])
             off = off.masked_fill(~ok, 0.0) + s.abs().masked_fill(~ok, 0.0) * 2.0 ** -22
             worst = off.amax(1, keepdim=True) if there else torch.zeros(n, 1, device="cuda").double()
             by = 2 * torch.expm1(worst) + 2.0 ** -19 + 2.0 ** -16 + (there / 16 + 64) * 2.0 ** -23 + (3 * unit if rounded else 0.0)
@@ -161,7 +164,7 @@ def attention(cache, q, share, scale, out, window=0, sinks=0, rounded=False, key
                 y_off[start:start + n, h] = ((2 * torch.expm1(worst) + 3 * unit) * (share_of @ v.abs())
                                              + (2.0 ** -16 + (there / 16 + 64) * 2.0 ** -23) * (share_of @ biggest(v)))
             lse_off[start:start + n, h] = (worst[:, 0] + 2.0 ** -18 + (there / 16 + 64) * 2.0 ** -23
-                                           + (unit if rounded else 0.0) + 2.0 ** -22 * lse[start:start + n, h].abs().nan_to_num(0, 0, 0))
+                                           + 2.0 ** -22 * lse[start:start + n, h].abs().nan_to_num(0, 0, 0))
         start += n
     y, y_off = y.view(rows, -1), y_off.view(rows, -1)
     return y, y_off + round_bound(y.abs() + y_off, out), lse, lse_off

@@ -15,10 +15,12 @@
 // lie behind one another in the reduction.
 //
 // Queries are brought below 2 by a power of two, which makes float16 of either type (what lies 2^-14
-// below a row's largest keeps 2^-25 of it). Float16's ten bits hold two codes: for a 16-bit result u is
-// 1 + code / 1024 of the even channels and 1 + code / 64 of the odd ones, which takes five instructions
-// for eight codes, not eight, and the queries 64 and 4 times as large; the sums are f32 of some 64 |q|
-// and lose 2^-17 of |q|, where weights keep 2^-8 anyway. For an f32 result u is 1 + code / 16.
+// below a row's largest keeps 2^-25 of it). Float16's ten bits hold two codes: for a 16-bit result they
+// come as 1 + code / 1024 of the even channels, of which one multiplication makes what the odd ones are
+// at once, 1 + code / 64, with queries 4 times as large; that is five instructions of the integer pipe for
+// eight codes and two of another, not eight. (With the even ones as they come and queries 64 times as
+// large, 3 us of 167 less, the sums' roundings reached 2e-5 of lse, now 1.5e-6.) For an f32 result u is
+// 1 + code / 16.
 //
 // Weights times scales, for a 16-bit result, are rounded twice, as weights and values that were each
 // brought to 16 bits would be; sum_j p_j scale_j is of the same rounded numbers, so the cancellation costs
@@ -70,7 +72,7 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {  // of numbe
 }
 
 // A word's nibbles i and 4 + i, i = 0 .. 3: of values as bfloat16 1 + code / 16, or (EXACT) code - 7.5; of keys as float16 the
-// same, or (FAST) 1 + code / 1024 of even i and 1 + code / 64 of odd ones.
+// same, or (FAST) 1 + code / 64.
 template <bool EXACT>
 __device__ __forceinline__ void unpack_values(uint32_t w, uint32_t (&u)[4]) {
     constexpr uint32_t BASE = EXACT ? 0x41804180u : 0x3F803F80u;  // 16, or 1
@@ -87,6 +89,9 @@ __device__ __forceinline__ void unpack_keys(uint32_t w, uint32_t (&u)[4]) {
         const uint32_t v = w >> 8;
         u[0] = and_or(w, 0x000F000Fu, 0x3C003C00u), u[1] = and_or(w, 0x00F000F0u, 0x3C003C00u);
         u[2] = and_or(v, 0x000F000Fu, 0x3C003C00u), u[3] = and_or(v, 0x00F000F0u, 0x3C003C00u);
+        // 1 + code / 1024, times 16, less 15
+        asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(u[0]) : "r"(0x4C004C00u), "r"(0xCB80CB80u));
+        asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(u[2]) : "r"(0x4C004C00u), "r"(0xCB80CB80u));
     } else {
         u[0] = and_or(w << 6, 0x03C003C0u, 0x3C003C00u), u[1] = and_or(w << 2, 0x03C003C0u, 0x3C003C00u);
         u[2] = and_or(w >> 2, 0x03C003C0u, 0x3C003C00u), u[3] = and_or(w >> 6, 0x03C003C0u, 0x3C003C00u);
@@ -172,7 +177,6 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
     constexpr float UNIT = EXACT ? 1.0f : 16.0f;  // of the values' products
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t scan[WARPS];
-    __shared__ int scan_items[WARPS];
     __shared__ float2 stat[WARPS][ROWS];
     const AttendArgs& a = p.a;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
@@ -187,26 +191,28 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
     const uint32_t odd = g & 1, mid_half = odd ? 0x7632 : 0x5410;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+    // Items and their tiles, each thread's cut off at 2^20 (starts that do not rise may count rows often);
+    // where they matter there are few.
+    constexpr int MANY = 1 << 20;
     int64_t total = 0;
-    int items = 0, own_items = 0, own_tiles = 0;
+    int items = 0, work = 0, own_items = 0, own_tiles = 0;
     for (int s = threadIdx.x; s < a.batch.seqs; s += THREADS) {
         const Share share(Sequence(a.batch, s), a, ROWS, WARPS);
         own_items = share.row_tiles * a.kv.heads, own_tiles = share.tiles;
-        items += own_items, total += static_cast<int64_t>(own_items) * own_tiles;
+        items = min(MANY, items + min(MANY, own_items));
+        work = static_cast<int>(min(static_cast<int64_t>(MANY * 16), work + static_cast<int64_t>(own_items) * own_tiles));
     }
-    items = __reduce_add_sync(0xffffffffu, items);
-    const int low = __reduce_add_sync(0xffffffffu, static_cast<int>(total & 0xFFFFF)), high = __reduce_add_sync(0xffffffffu, static_cast<int>(total >> 20));
-    if (lane == 0) scan[warp] = low + (static_cast<int64_t>(high) << 20), scan_items[warp] = items;
+    items = __reduce_add_sync(0xffffffffu, items), work = __reduce_add_sync(0xffffffffu, work);
+    if (lane == 0) scan[warp] = static_cast<int64_t>(work) << 32 | items;
     __syncthreads();
-    total = items = 0;
-    for (int w = 0; w < WARPS; ++w) total += scan[w], items += scan_items[w];
+    items = 0;
+    for (int w = 0; w < WARPS; ++w) items += static_cast<int>(scan[w]), total += scan[w] >> 32;
     const int blocks = gridDim.x;
-    // Tiles of a block. Where there are two blocks to an item, an item's tiles count as many as whole blocks
-    // of them have, so that no block has parts of two: a part's beginning and end cost as much as four tiles
-    // (29 x 5 drafted tokens 23.9 -> 18.1 us, 8 contexts of 8192 40.2 -> 36.0, 32 of them 95.4 -> 97.3).
-    const bool padded = 2 * items <= blocks;
-    const int64_t each = max(static_cast<int64_t>(LEAST), padded ? quotient(total + blocks - items - 1, blocks - items) : quotient(total + blocks - 1, blocks));
-    const int pad = padded ? static_cast<int>(each) : 1;
+    // Where there are two blocks to an item, an item's tiles count as many as whole blocks of them have, so
+    // that no block has parts of two: a part's beginning and end cost as much as four tiles (29 x 5 drafted
+    // tokens 23.9 -> 18.1 us, 8 contexts of 8192 40.2 -> 36.0, 32 of them 95.4 -> 97.3).
+    const bool padded = 2 * items <= blocks && total < MANY * 16;
+    const int pad = padded ? max(LEAST, static_cast<int>(quotient(total + blocks - items - 1, blocks - items))) : 1;
     auto whole_pads = [&](int tiles) { return (tiles + pad - 1) / pad * pad; };
     total = 0;
     for (int s0 = 0; s0 < a.batch.seqs; s0 += THREADS) {
@@ -240,6 +246,8 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
         p.from[blockIdx.x] = blockIdx.x;
     }
     __syncthreads();
+    // Tiles of a block.
+    const int64_t each = padded ? pad : max(static_cast<int64_t>(LEAST), quotient(total + blocks - 1, blocks));
     int64_t x = blockIdx.x * each;
     const int64_t end = min(total, x + each);
 
@@ -345,11 +353,10 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
                     const float2 w = two<T>(q[n][i][k]);
                     v[2 * k] = w.x * down, v[2 * k + 1] = w.y * down;
                 }
-                constexpr float EVEN = EXACT ? 1.0f : 64.0f, ODD = EXACT ? 1.0f : 4.0f;
+                constexpr float by = EXACT ? 1.0f : 4.0f;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     // channels (0, 4), (1, 5), (2, 6), (3, 7), as the nibbles come
-                    const float by = k % 2 ? ODD : EVEN;
                     q[n][i][k] = pack<__half>(v[k] * by, v[k + 4] * by);
                     sum += v[k] + v[k + 4];
                     by_code = fmaf(-(by + 7.5f / 16.0f), v[k] + v[k + 4], by_code);
@@ -647,13 +654,14 @@ __global__ void __launch_bounds__(JOINERS) join_kernel(const __grid_constant__ F
     const AttendArgs& a = p.a;
     const int quads = a.kv.dim / 4, from = p.from[blockIdx.x];
     for (int k = 0; k < 2; ++k) {  // what the block ended, what it began
-        const int begin = k ? blockIdx.x : from;
-        if (k == 0 && begin == blockIdx.x) continue;
-        const int4 it = p.split[begin];
-        if (it.w == 0) continue;
+        const int me = blockIdx.x, begin = k ? me : from;
+        if (k == 0 && begin == me) continue;
+        int4 it = p.split[begin];
+        it.w = min(it.w, static_cast<int>(gridDim.x) - begin);
+        if (it.w <= 0) continue;
         const Sequence seq(a.batch, it.x);
         const int outs = min(tile_rows, seq.count * a.share - it.z * tile_rows) * quads, each = (outs + it.w - 1) / it.w;
-        const int first = (blockIdx.x - begin) * each, upto = min(outs, first + each);
+        const int first = (me - begin) * each, upto = min(outs, first + each);
         int abreast = 1;  // parts that are read beside one another
         while (abreast < it.w && abreast < 32) abreast <<= 1;
         const int width = JOINERS / abreast, column = threadIdx.x & (width - 1), row = threadIdx.x / width;

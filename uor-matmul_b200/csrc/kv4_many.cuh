@@ -1,21 +1,35 @@
 // kv4_many.cuh -- attention over the 4-bit cache where many rows read it: prompts and their pieces.
 //
-// Bound by the tensor cores: 4 D operations for every pair of a row and a token that it sees. A work item
-// is a tile of 256 rows (128 of heads past 128 channels), tokens by the heads that share keys, against
-// the tokens that they see, 128 (64) at a time. One CTA a processor takes items in turn from a counter,
-// the longest of a sequence first.
+// A work item is a tile of 256 rows (128 of heads past 128 channels) by the heads that share keys, against
+// the tokens that they see, 64 at a time. One CTA a processor takes items in turn from a counter, the
+// longest of a sequence first.
 //
-// The roles of a CTA: a warpgroup turns codes into 16-bit floats, in shared memory as the tensor cores
-// read them, mid + scale (code - 7.5) rounded once; one thread issues the tcgen05.mma, of each half of
-// the rows in turn; a warpgroup for each half has a row to a thread, whose scores it reads from tensor
-// memory, and where it puts the weights in their place, as the next product's A side. While one half's
-// exponentials run the other half's products do. Sums keep the maximum that they were begun with until
-// it is passed by 2^8; only then a row's sums in tensor memory are multiplied.
+// The mathematics. With x = mid + scale (code - 7.5), of each group of channels
+//   q . k = sum q (scale (code - 7.5)) + mid sum(q).
+// A scale has eight bits (eleven in float16) and code - 7.5 four: their product is exactly two numbers of
+// the 16-bit type, what it is rounded to and what that leaves, and the middles multiply the groups' sums of
+// queries, two parts each, in a product of their own. So scores are f32's own, and so is lse. (Keys rounded
+// once to 16 bits, and half the products: 8192 of 8192 in 692 us, but lse 3e-5 to 4e-4 off in bfloat16, 4e-6
+// to 5e-5 in float16; now 4e-7.) Values and weights are rounded once to 16 bits, as their type has
+// them. Queries are brought below 2 by a power of two, for the sums' sake in float16.
 //
-// Why this shape: a tile of tokens' codes cost as much of the issue slots as its exponentials for 128
-// rows, so they serve 256; the two halves' scores and sums take all of tensor memory's 512 columns at 128
-// channels. Of 128 tokens the products are 2097 cycles; their operands' reads from shared memory 1536,
-// the codes' decoding 512 of writes, 32768 exponentials 2048 of the special units.
+// The roles of a CTA: a warpgroup turns keys' codes, and another values', into 16-bit floats in shared
+// memory as the tensor cores read them, from rings of blocks that bulk copies fill; a thread for each half
+// of the rows issues its tcgen05.mma; a warpgroup for each half has a row to a thread, whose scores it
+// reads from tensor memory, and where it puts the weights in their place, as the next product's A side.
+// Scores of odd and even steps have columns of their own, so that the next step's are at hand when a
+// step's weights are done (8192 of 8192, keys rounded once: 927 us -> 705). Sums keep the maximum that they
+// were begun with until it is passed by 2^8; only then a row's sums in tensor memory are multiplied.
+//
+// Why this shape. A step's codes cost as many issue slots as the exponentials of 128 rows, so they serve
+// 256; the two halves' scores and sums take all of tensor memory's 512 columns at 128 channels. A query tile
+// comes from shared memory for both parts of the keys at once (898 us -> 845): read for each, the
+// operands' 12 KB for 64 cycles of products pass its 128 bytes a cycle.
+//
+// 8192 of 8192 tokens, 32 heads over 8 of 128 channels, bfloat16: 845 us, 651 TFLOP/s of the 4 D operations
+// of each pair. A step of 64 tokens takes 1.9 us at the 1.56 GHz that the processors run at under it, 2900
+// cycles: 1600 of products, shared memory some 2000 for their operands, the decoded values and the rings.
+// 2048 of 4096: 189 us; six sequences of up to 300 of 2500: 67 us, where items are few and uneven.
 //
 // Every wait is bounded; a role that gives up records it, and all leave at the item's end.
 #pragma once
@@ -34,7 +48,7 @@ constexpr int DECODERS = 4;  // warps for the keys, and for the values
 struct ManyAttend {
     AttendArgs a;
     const int64_t* before;  // [seqs + 1] items before each sequence's
-    unsigned* next;         // the item that is taken next
+    unsigned long long* next;  // the item that is taken next
     int* status;
     uint64_t budget_ns;
 };
@@ -163,7 +177,7 @@ __device__ __forceinline__ void bulk_load(uint32_t to, const void* from, uint32_
 
 // The items before each sequence's, and the first to be taken.
 __global__ void __launch_bounds__(1024) items_kernel(const __grid_constant__ AttendArgs a, int tile_rows, int tile_blocks, int64_t* before,
-                                                     unsigned* next) {
+                                                     unsigned long long* next) {
     __shared__ int64_t sums[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -227,7 +241,7 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // Takes an item; none left: seq is -1.
     auto take = [&](int slot) {
-        const int64_t x = atomicAdd(p.next, 1u), total = p.before[a.batch.seqs];
+        const int64_t x = static_cast<int64_t>(atomicAdd(p.next, 1ull)), total = p.before[a.batch.seqs];
         Item it{-1, 0, 0};
         if (x < total) {
             int lo = 0, hi = a.batch.seqs;  // before[lo] <= x < before[hi]
@@ -716,7 +730,7 @@ int launch_many(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route) {
     p.a = a;
     auto* before = reinterpret_cast<int64_t*>(ws);
     p.before = before;
-    p.next = reinterpret_cast<unsigned*>(before + a.batch.seqs + 1);
+    p.next = reinterpret_cast<unsigned long long*>(before + a.batch.seqs + 1);
     p.status = ctx->d_status;
     p.budget_ns = ctx->budget_ns;
     items_kernel<<<1, 1024, 0, ctx->stream>>>(a, 128 * Z::HALVES, Z::BLOCKS, before, p.next);
