@@ -39,8 +39,9 @@ class Layer:
         flat = qkv.view(-1)
         U.kv4_append(self.elem, kv, batch, flat[wide[0]:], (rows, wide[1], n), flat[wide[0] + wide[1]:], (rows, wide[2], n),
                      q=qkv, qv=(rows, wide[0], n), q_out=q, ov=(rows, wide[0]), rotation=self.turn, **how)
+        self.route = U.Route()
         U.kv4_attention(self.elem, self.elem, kv, batch, q, (rows, wide[0]), y, (rows, wide[0]), window=self.window, sinks=self.sinks,
-                        lse=lse, lv=tuple(lse.shape), **how)
+                        lse=lse, lv=tuple(lse.shape), route=self.route, **how)
         U.q4_linear(self.elem, self.elem, y, (rows, wide[0]), self.back.q, x, (rows, self.width), residual=x, **how)
 
 
@@ -63,9 +64,8 @@ def _check(layer, cache, x0, x1, buffers, seen):
         seen[i] = tuple(torch.cat((old, now[first:first + new])) for old, now in zip(seen[i], (k, v)))
         first += new
     cache.k, cache.v = [s[0] for s in seen], [s[1] for s in seen]
-    mean_rows = rows * layer.share / len(cache.news)
     a, a_off, l, l_off = attention(cache, q[:rows], layer.share, layer.dim ** -0.5, layer.elem, layer.window, layer.sinks,
-                                   rounded=mean_rows > 64)
+                                   rounded=layer.route.tile_m > 16)
     assert_within(y[:rows], a, a_off)
     assert_within(lse[:rows], l, l_off)
     want = y[:rows].double() @ layer.back.value.T
@@ -75,17 +75,19 @@ def _check(layer, cache, x0, x1, buffers, seen):
     assert_within(x1[:rows], want, off + round_bound(want.abs() + off, layer.elem))
 
 
+@pytest.mark.parametrize("many", [False, True])  # a large batch, most of it padding
 @pytest.mark.parametrize("elem,heads,share,dim,group,window,sinks",
                          [(U.BF16, 2, 2, 64, 32, 0, 0), (U.F16, 1, 4, 128, 64, 0, 0), (U.BF16, 2, 3, 96, 32, 50, 4)])
-def test_prompt_and_steps(elem, heads, share, dim, group, window, sinks):
+def test_prompt_and_steps(elem, heads, share, dim, group, window, sinks, many):
     layer = Layer(elem, heads, share, dim, group, window, sinks)
-    cache = Cache([144, 144, 16], [90, 133, 1], 16, heads, dim, group, elem, pad=2)
+    cache = Cache([144, 144, 16], [90, 133, 1], 16, heads, dim, group, elem, pad=6500 // (heads * share) if many else 2)
     cache.lengths = [90, 133, 1]
     cache.batch = cache.batch_of(cache.news)
     seen = [tuple(torch.empty(0, heads, dim, dtype=torch.float64, device="cuda") for _ in range(2)) for _ in cache.news]
     x0 = cache.normal(cache.rows, layer.width).to(layer.kind)
     x1, buffers = x0.clone(), layer.buffers(cache.rows)
     layer.run(cache.kv, cache.batch, x1, buffers)
+    assert (layer.route.tile_m > 16) == many
     _check(layer, cache, x0, x1, buffers, seen)
     for _ in range(4):
         cache.news, cache.lengths, cache.rows = [1, 1, 1], [n + 1 for n in cache.lengths], 3
@@ -104,13 +106,13 @@ def _decoding(layer):
     return cache
 
 
-@pytest.mark.parametrize("news", [[1, 1], [3, 2], [60, 41]])
-def test_a_captured_step_follows_the_device(news):
+@pytest.mark.parametrize("news,pad", [([1, 1], 0), ([3, 2], 1), ([60, 41], 0), ([60, 41], 1600)])
+def test_a_captured_step_follows_the_device(news, pad):
     """One graph of the whole half, replayed over lengths and inputs that the device holds, is to the byte
     what eager calls give; a second graph of the same context between its replays changes nothing."""
     layer = Layer(U.BF16, 2, 2, 64, 32)
     eager, replayed = _decoding(layer), _decoding(layer)
-    rows = sum(news)
+    rows, live = sum(news) + pad, sum(news)
     inputs = [eager.normal(rows, layer.width).to(layer.kind) for _ in range(3)]
     ctx, stream = U.Context(0), torch.cuda.Stream()
     ctx.set_stream(stream.cuda_stream)
@@ -144,7 +146,7 @@ def test_a_captured_step_follows_the_device(news):
         mine, own = v.clone(), layer.buffers(rows)
         layer.run(eager.kv, eager.batch_of(news), mine, own)
         for a, b in zip(g, (mine, own[2], own[3])):
-            assert torch.equal(a, b)
+            assert torch.equal(a[:live], b[:live])
     assert torch.equal(eager.pool, replayed.pool)
     del graphs
     ctx.close()

@@ -108,7 +108,7 @@ struct AttendArgs {
     float scale;
     int window, sinks;
 };
-// Few rows (kv4_few.cuh). EXACT: for f32 results.
+// Few rows (kv4_few.cuh). EXACT: for f32 and float16 results.
 template <typename T, bool EXACT>
 int kv4_few(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route);
 // Many rows, 16-bit results (kv4_many.cuh).

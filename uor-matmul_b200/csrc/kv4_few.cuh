@@ -15,19 +15,21 @@
 // lie behind one another in the reduction.
 //
 // Queries are brought below 2 by a power of two, which makes float16 of either type (what lies 2^-14
-// below a row's largest keeps 2^-25 of it). Float16's ten bits hold two codes: for a 16-bit result they
+// below a row's largest keeps 2^-25 of it). Float16's ten bits hold two codes: for a bfloat16 result they
 // come as 1 + code / 1024 of the even channels, of which one multiplication makes what the odd ones are
 // at once, 1 + code / 64, with queries 4 times as large; that is five instructions of the integer pipe for
 // eight codes and two of another, not eight. (With the even ones as they come and queries 64 times as
-// large, 3 us of 167 less, the sums' roundings reached 2e-5 of lse, now 1.5e-6.) For an f32 result u is
+// large, 3 us of 167 less, the sums' roundings reached 2e-5 of lse, now 1.5e-6.) For the others u is
 // 1 + code / 16.
 //
-// Weights times scales, for a 16-bit result, are rounded twice, as weights and values that were each
+// Weights times scales, for a bfloat16 result, are rounded twice, as weights and values that were each
 // brought to 16 bits would be; sum_j p_j scale_j is of the same rounded numbers, so the cancellation costs
-// nothing. For an f32 result they are two 16-bit numbers, a rounded one and what that left (2^-17
-// together), and values' codes are code - 7.5, an addition more for each pair: the tensor cores' sums of
-// u, five times as large as what is left of them, cut off more than that (1.4e-5 of the result, not
-// 2.5e-6). Weights are bfloat16 whatever the cache's type is: float16 would lose the small ones.
+// nothing. For f32 and float16 results (EXACT) they are two 16-bit numbers, a rounded one and what that
+// left (2^-17 together), and values' codes are code - 7.5, an addition more for each pair: the tensor
+// cores' sums of u, five times as large as what is left of them, cut off more than that (1.4e-5 of the
+// result, not 2.5e-6). Weights are bfloat16 whatever the cache's type is: float16 would lose the small
+// ones. (64 contexts of 8192: 169 us with one, 204 with two. A float16 result is 2e-4 off its 64 bits with
+// two, its own rounding; with one 1.8e-3.)
 //
 // The work is cut evenly: tiles of 64 tokens of every item (a sequence, head and eight or sixteen rows)
 // are numbered by the lengths, which the device alone knows, and each block of threads has as many of them
@@ -168,12 +170,13 @@ __device__ __forceinline__ void take(float4& sum, float2& both, const float4& ad
     both = make_float2(most, fmaf(of, s.y, by * both.y));
 }
 
-// NT: rows in eights. GP: 32s of channels in a group. EXACT: weights in two parts, for an f32 result.
+// NT: rows in eights. GP: 32s of channels in a group. EXACT: weights in two parts, for f32 and float16 results.
 template <typename T, int D, int GP, int NT, bool EXACT>
 __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kernel(const __grid_constant__ FewAttend p) {
     constexpr int N32 = D / 32, ROWS = 8 * NT, G = N32 / GP;
     constexpr int block_bytes = kv_block_bytes(D, G);
     using B = __nv_bfloat16;
+    static_assert(EXACT || std::is_same<T, B>::value, "float16 results take two parts");
     constexpr float UNIT = EXACT ? 1.0f : 16.0f;  // of the values' products
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int64_t scan[WARPS];
@@ -534,9 +537,6 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
                     mma<T>(rest[n], mid0, 0, mid1, 0, left0, left1);
                     parts_of(add2(pair_of<T>(p0[n]), pair_of<T>(left0)), both[n][0], both[n][1]);
                     parts_of(add2(pair_of<T>(p1[n]), pair_of<T>(left1)), both[n][2], both[n][3]);
-                } else if constexpr (!std::is_same<T, B>::value) {
-                    parts_of(pair_of<T>(p0[n]), both[n][0], both[n][1]);
-                    parts_of(pair_of<T>(p1[n]), both[n][2], both[n][3]);
                 }
             }
             uint32_t w[2][N32];
@@ -551,17 +551,15 @@ __global__ void __launch_bounds__(THREADS, D <= 128 && NT == 1 ? 4 : 1) few_kern
                     const uint32_t s1 = *reinterpret_cast<const uint32_t*>(params + ((4 + c) * G + i / GP) * 8);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        if constexpr (!EXACT && std::is_same<T, B>::value) {
+                        if constexpr (!EXACT) {
                             high[n][0] = mul_bf16(p0[n], s0), high[n][1] = mul_bf16(p1[n], s1);
                         } else {
                             float v[4];
                             parts_of(mul2(pair_of(both[n][0], both[n][1]), pair_of<T>(s0)), v[0], v[1]);
                             parts_of(mul2(pair_of(both[n][2], both[n][3]), pair_of<T>(s1)), v[2], v[3]);
                             high[n][0] = pack<B>(v[0], v[1]), high[n][1] = pack<B>(v[2], v[3]);
-                            if constexpr (EXACT) {
-                                const float2 r0 = two<B>(high[n][0]), r1 = two<B>(high[n][1]);
-                                low[n][0] = pack<B>(v[0] - r0.x, v[1] - r0.y), low[n][1] = pack<B>(v[2] - r1.x, v[3] - r1.y);
-                            }
+                            const float2 r0 = two<B>(high[n][0]), r1 = two<B>(high[n][1]);
+                            low[n][0] = pack<B>(v[0] - r0.x, v[1] - r0.y), low[n][1] = pack<B>(v[2] - r1.x, v[3] - r1.y);
                         }
                         if constexpr (!EXACT) mma<B>(rest[n], minus, 0, minus, 0, high[n][0], high[n][1]);
                     }
