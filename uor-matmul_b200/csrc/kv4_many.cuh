@@ -1,6 +1,6 @@
 // kv4_many.cuh -- attention over the 4-bit cache where many rows read it: prompts and their pieces.
 //
-// A work item is a tile of 256 rows (128 of heads past 128 channels) by the heads that share keys, against
+// A work item is a tile of 256 rows (128 of heads past 128 channels, or where items are few) by the heads that share keys, against
 // the tokens that they see, 64 at a time. One CTA a processor takes items in turn from a counter, the
 // longest of a sequence first.
 //
@@ -53,9 +53,9 @@ struct ManyAttend {
     uint64_t budget_ns;
 };
 
-template <int D>
+template <int D, int H>
 struct Shape {
-    static constexpr int HALVES = D <= 128 ? 2 : 1;      // of 128 rows
+    static constexpr int HALVES = H;                     // of 128 rows
     static constexpr int TOKENS = 64;                    // of a step
     static constexpr int BLOCKS = TOKENS / KV_BLOCK;
     static constexpr int ATOMS = (D + 63) / 64;          // of 64 channels, the 128 bytes that a swizzle spans
@@ -204,9 +204,9 @@ __global__ void __launch_bounds__(1024) items_kernel(const __grid_constant__ Att
     if (threadIdx.x == 0) before[a.batch.seqs] = total, *next = 0;
 }
 
-template <typename T, int D>
+template <typename T, int D, int H>
 __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant__ ManyAttend p) {
-    using Z = Shape<D>;
+    using Z = Shape<D, H>;
     constexpr int N32 = D / 32;
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ uint8_t smem_raw[];
@@ -713,10 +713,10 @@ __global__ void __launch_bounds__(THREADS, 1) many_kernel(const __grid_constant_
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, int H>
 int launch_many(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route) {
-    using Z = Shape<D>;
-    auto* kernel = many_kernel<T, D>;
+    using Z = Shape<D, H>;
+    auto* kernel = many_kernel<T, D, H>;
     const int smem = Z::smem(a.kv.groups);
     static bool ready[64] = {};
     if (!ready[ctx->device & 63]) {
@@ -749,16 +749,25 @@ int launch_many(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route) {
     return cuda_status(cudaLaunchKernelEx(&c, kernel, p));
 }
 
+template <typename T, int D>
+int by_halves(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route) {
+    const int64_t mean = (static_cast<int64_t>(a.batch.rows) * a.share + a.batch.seqs - 1) / a.batch.seqs;
+    // Tiles of 128 rows where there are processors enough for them all: 1.6 us a step for one half, 1.85 for
+    // two (512 new tokens of 4096, 4 queries to each of 8 heads: 108 : 126 us, 1024: 184 : 128).
+    return a.batch.seqs * a.kv.heads * ((mean + 127) / 128) <= ctx->sm_count ? launch_many<T, D, 1>(ctx, a, route)
+                                                                             : launch_many<T, D, 2>(ctx, a, route);
+}
+
 }  // namespace
 
 template <typename T>
 int kv4_many(uor_b200_ctx* ctx, const AttendArgs& a, uor_b200_route* route) {
     switch (a.kv.dim) {
-    case 64: return launch_many<T, 64>(ctx, a, route);
-    case 96: return launch_many<T, 96>(ctx, a, route);
-    case 128: return launch_many<T, 128>(ctx, a, route);
-    case 192: return launch_many<T, 192>(ctx, a, route);
-    default: return launch_many<T, 256>(ctx, a, route);
+    case 64: return by_halves<T, 64>(ctx, a, route);
+    case 96: return by_halves<T, 96>(ctx, a, route);
+    case 128: return by_halves<T, 128>(ctx, a, route);
+    case 192: return launch_many<T, 192, 1>(ctx, a, route);
+    default: return launch_many<T, 256, 1>(ctx, a, route);
     }
 }
 
