@@ -666,7 +666,7 @@ def q4_linear(elem, out, a, av, w, c, cv, bias=None, activation=IDENTITY, residu
     of = _out_type(elem, out)
     (C, dc) = _placed(c, cv, of)
     (R, dr) = _placed(residual, cv if rv is None else rv, of) if residual is not None else (None, dc)
-    bias_type = F32 if bias is None or _fits(getattr(bias, "dtype", None), F32) else elem
+    bias_type = F32 if bias is None or str(getattr(bias, "dtype", "")).endswith("float32") else elem
     pb, lb, db = _typed(bias, bias_type if bias_type in (F32, BF16, F16) else None) if bias is not None else (None, 0, dc)
     call = make_call(NEAREST, _same_place(w.on_device, da, dc, dr, db), ctx, route, asynchronous)
     _check(lib().uor_b200_q4_linear(elem, out, A, w, pb, lb, bias_type, activation, R, C, call), "q4_linear")
