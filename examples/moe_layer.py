@@ -9,7 +9,9 @@ For a row x of hidden states the layer computes
     y = h + sum_s weights[s] FFN_ids[s](h)   experts in 4 bits (expert_q4_ffn)
 
 first for a batch, then token by token from a CUDA graph, as a decoder does, and then trains R
-with the experts held fixed, through expert_route_backward. Needs a CUDA GPU."""
+with the experts held fixed, through expert_route_backward. Last it puts an attention half before the
+layer, over keys and values in 4 bits (q4_linear, kv4_append, kv4_attention, q4_linear), and runs the two
+for a prompt and then token by token from one graph. Needs a CUDA GPU."""
 import argparse
 import os
 import sys
@@ -116,6 +118,79 @@ class MoELayer:
         return 0.5 * (y - target).square().sum() / t
 
 
+class Attention:
+    """The attention half before a layer, for one sequence: x + O attention(rotated heads of W x + b) over a
+    paged cache of 4-bit keys and values, whose length the device holds."""
+
+    def __init__(self, layer, heads=8, shared_by=4, dim=64, positions=512, group=64, seed=2):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        self.layer, self.heads, self.wide = layer, heads, heads * dim
+        self.keys = heads // shared_by * dim  # channels of a token's keys, and of its values
+        rows = self.wide + 2 * self.keys
+        self.into = quantize(torch.randn(rows, layer.d, generator=g, device="cuda") * layer.d ** -0.5, group)
+        self.bias = (torch.randn(rows, generator=g, device="cuda") * 0.1).bfloat16()
+        self.back = quantize(torch.randn(layer.d, self.wide, generator=g, device="cuda") * 0.5 * self.wide ** -0.5, group)
+        page = 64
+        pages = -(-positions // page)
+        self.pool = torch.zeros(pages * U.kv4_page_bytes(page, heads // shared_by, dim, 32, U.BF16), dtype=torch.uint8, device="cuda")
+        self.cache = U.KV4(self.pool, pages, page, heads // shared_by, dim, 32, U.BF16)
+        self.table = torch.arange(pages, dtype=torch.int32, device="cuda").view(1, pages)
+        self.length = torch.zeros(1, dtype=torch.int32, device="cuda")
+        angle = torch.arange(pages * page, device="cuda").double()[:, None] * 10000.0 ** (
+            -torch.arange(dim // 2, device="cuda").double() / (dim // 2))
+        self.turn = U.Rotation(torch.cos(angle).float(), torch.sin(angle).float(), pages * page, dim, False)
+
+    def batch(self, rows):
+        """The sequence's newest `rows` tokens."""
+        return U.Batch(torch.tensor([0, rows], dtype=torch.int32, device="cuda"), self.length, self.table, 1, self.table.shape[1])
+
+    def forward(self, x, batch):
+        """x (rows x d): the sequence's next tokens, on the layer's stream; its length grows by them."""
+        t, d = x.shape
+        self.length += t
+        how = dict(ctx=self.layer.ctx, asynchronous=True)
+        rows = self.wide + 2 * self.keys
+        heads = torch.empty(t, rows, dtype=torch.bfloat16, device="cuda")
+        U.q4_linear(U.BF16, U.BF16, x, (t, d), self.into, heads, (t, rows), bias=self.bias, **how)
+        q, k, v = heads, heads.view(-1)[self.wide:], heads.view(-1)[self.wide + self.keys:]
+        U.kv4_append(U.BF16, self.cache, batch, k, (t, self.keys, rows), v, (t, self.keys, rows), q=q, qv=(t, self.wide, rows),
+                     q_out=q, ov=(t, self.wide, rows), rotation=self.turn, **how)
+        y = torch.empty(t, self.wide, dtype=torch.bfloat16, device="cuda")
+        U.kv4_attention(U.BF16, U.BF16, self.cache, batch, q, (t, self.wide, rows), y, (t, self.wide), **how)
+        out = torch.empty_like(x)
+        U.q4_linear(U.BF16, U.BF16, y, (t, self.wide), self.back, out, (t, d), residual=x, **how)
+        return out
+
+
+def run_attention(layer, x, report=print):
+    """A prompt through an attention half and the layer, then its last tokens once more, one by one from a
+    graph; how far the two are apart in units of the largest output."""
+    half, last = Attention(layer, positions=x.shape[0] + 64), min(8, x.shape[0])
+    torch.cuda.synchronize()
+    with torch.cuda.stream(layer.stream):
+        batch = half.batch(x.shape[0])
+        y = layer.forward(half.forward(x, batch))
+        one, token = half.batch(1), x[:1].clone()
+        layer.forward(half.forward(token, one))  # the context's buffers grow to this shape before the capture
+        layer.done()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=layer.stream):
+            out = layer.forward(half.forward(token, one))
+        half.length.fill_(x.shape[0] - last)
+        found = []
+        for t in range(x.shape[0] - last, x.shape[0]):
+            token.copy_(x[t:t + 1])
+            graph.replay()
+            found.append(out.clone())
+        layer.done()
+    far = float((torch.cat(found).float() - y[-last:].float()).abs().max() / y.float().abs().max())
+    report(f"attention over 4-bit keys and values and the layer, {x.shape[0]} tokens, the last {last} again from a graph: "
+           f"{far:.4f} of the largest output apart")
+    del graph
+    return far, torch.cat(found), half
+
+
 class Decoder:
     """One token at a time: the layer's forward captured once in a CUDA graph and replayed."""
 
@@ -191,3 +266,6 @@ if __name__ == "__main__":
         p.add_argument("--" + name, type=int, default=value)
     a = p.parse_args()
     run(a.tokens, a.d, a.f, a.experts, a.top_k, a.steps)
+    whole = MoELayer(a.d, a.f, a.experts, a.top_k)
+    run_attention(whole, torch.randn(a.tokens, a.d, device="cuda").bfloat16())
+    whole.close()
