@@ -8,12 +8,13 @@
 // off would be a whole step of the range off, so both are computed as their definition has them. The
 // products are exact in 64 bits, where this processor multiplies at half its 32-bit rate. (In 32 bits, by
 // two fused multiply-adds with a bound of what they leave open and doubles where that matters: the same
-// 96 us.) A code is a multiplication by the scale's reciprocal but where that comes near a half; its eight
+// time.) A code is a multiplication by the scale's reciprocal but where that comes near a half; its eight
 // and their exceptions are one branch.
 //
-// 8192 tokens, 32 heads of queries, 8 of keys and values, 128 channels, all rotated: 96 us, 2.4 TB/s, and
-// 13 us to read them back. Bound by issue slots and what a processor's 20 warps have under way (61 % of
-// its cycles issue; with 16 warps of 128 registers 109 us); one token: 3.8 us, a launch's own time.
+// 8192 tokens, 32 heads of queries, 8 of keys and values, 128 channels, all rotated: 91 us, 2.5 TB/s, and
+// 13 us to read them back. Bound by what a processor's 20 warps have under way: half of its cycles issue,
+// 270 instructions for 512 values (16 warps of 128 registers: 103 us; 24 of 80, which spill, 90; two heads
+// at a time with nothing ahead of them 96). One token: 3.8 us, a launch's own time.
 #include "kv4.cuh"
 
 #include <cstring>
@@ -127,8 +128,6 @@ enum Turn {
     TURN_ANY = 3      // some of them, or with channels that do not lie so: one by one
 };
 
-constexpr int AHEAD = 2;  // a lane's heads under way; four take the registers of a fifth block: 104 us
-
 // VEC: every row of heads begins at a multiple of 16 bytes.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(WARPS * 32, 5) append_kernel(const __grid_constant__ AppendArgs a, int slices) {
@@ -178,104 +177,102 @@ __global__ void __launch_bounds__(WARPS * 32, 5) append_kernel(const __grid_cons
         *from = q ? &a.q : k ? &a.k : &a.v;
         *local = q ? h : k ? h - a.q_heads : h - a.q_heads - a.kv.heads;
     };
-    for (int h0 = slice * each; h0 < last; h0 += AHEAD * abreast) {
-        uint4 x[AHEAD], y[AHEAD];
+    // The next heads are on their way while these are worked on.
+    uint4 x, y;
+    auto load = [&](int h, uint4& own, uint4& with) {
+        own = with = make_uint4(0, 0, 0, 0);
+        if (!mine || h >= last) return;
+        const Rows* from;
+        int local;
+        place(h, &from, &local);
+        const uint16_t* p = static_cast<const uint16_t*>(from->p) + row * from->rs + local * dim + channel;
+        own = load8(p, VEC || from->vec);
+        if (turn == TURN_HALVES && h < a.q_heads + a.kv.heads) with = load8(p + other, VEC || from->vec);
+    };
+    load(slice * each + sub, x, y);
+    uint4 next_x, next_y;
+    for (int h0 = slice * each; h0 < last; h0 += abreast, x = next_x, y = next_y) {
+        load(h0 + abreast + sub, next_x, next_y);
+        const int h = h0 + sub;
+        const bool live = mine && h < last;
+        const bool query = h < a.q_heads, value = h >= a.q_heads + a.kv.heads;
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        float r[8];
+        if (live && !value && turn != TURN_NONE) {
+            if (turn == TURN_HALVES) {
+                const uint32_t v[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int h = h0 + u * abreast + sub;
-            x[u] = y[u] = make_uint4(0, 0, 0, 0);
-            if (!mine || h >= last) continue;
-            const Rows* from;
-            int local;
-            place(h, &from, &local);
-            const uint16_t* p = static_cast<const uint16_t*>(from->p) + row * from->rs + local * dim + channel;
-            x[u] = load8(p, VEC || from->vec);
-            if (turn == TURN_HALVES && h < a.q_heads + a.kv.heads) y[u] = load8(p + other, VEC || from->vec);
-        }
+                for (int i = 0; i < 4; ++i)
+                    w[i] = Half<T>::pair(turned(Half<T>::first(w[i]), c[2 * i], Half<T>::first(v[i]), sn[2 * i]),
+                                         turned(Half<T>::second(w[i]), c[2 * i + 1], Half<T>::second(v[i]), sn[2 * i + 1]));
+            } else if (turn == TURN_PAIRS) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int h = h0 + u * abreast + sub;
-            if (h0 + u * abreast >= last) break;  // of the whole warp
-            const bool live = mine && h < last;
-            const bool query = h < a.q_heads, value = h >= a.q_heads + a.kv.heads;
-            uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-            float r[8];
-            if (live && !value && turn != TURN_NONE) {
-                if (turn == TURN_HALVES) {
-                    const uint32_t v[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        w[i] = Half<T>::pair(turned(Half<T>::first(w[i]), c[2 * i], Half<T>::first(v[i]), sn[2 * i]),
-                                             turned(Half<T>::second(w[i]), c[2 * i + 1], Half<T>::second(v[i]), sn[2 * i + 1]));
-                } else if (turn == TURN_PAIRS) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float even = Half<T>::first(w[i]), odd = Half<T>::second(w[i]);
-                        w[i] = Half<T>::pair(turned(even, c[i], odd, sn[i]), turned(odd, c[i], even, -sn[i]));
-                    }
-                } else {
-                    const Rows* from;
-                    int local;
-                    place(h, &from, &local);
-                    const T* head = static_cast<const T*>(from->p) + row * from->rs + local * dim;
-                    const float *cos = a.cos + at * a.turn_rs, *sin = a.sin + at * a.turn_rs;
-                    const int half = a.turned / 2;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) r[2 * i] = Half<T>::first(w[i]), r[2 * i + 1] = Half<T>::second(w[i]);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int ch = channel + i;
-                        if (ch >= a.turned) break;
-                        const bool low = a.interleaved ? ch % 2 == 0 : ch < half;
-                        const int pair = a.interleaved ? ch / 2 : low ? ch : ch - half;
-                        const int with = a.interleaved ? ch ^ 1 : low ? ch + half : ch - half;
-                        r[i] = turned(r[i], cos[pair], to_f32(head[with]), low ? sin[pair] : -sin[pair]);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = Half<T>::pair(r[2 * i], r[2 * i + 1]);
+                for (int i = 0; i < 4; ++i) {
+                    const float even = Half<T>::first(w[i]), odd = Half<T>::second(w[i]);
+                    w[i] = Half<T>::pair(turned(even, c[i], odd, sn[i]), turned(odd, c[i], even, -sn[i]));
                 }
-            }
-            __syncwarp();  // queries may turn in place: no lane writes what another still reads
-            if (live && query) {
-                store8(static_cast<uint16_t*>(a.q_out.p) + row * a.q_out.rs + h * dim + channel, make_uint4(w[0], w[1], w[2], w[3]),
-                       VEC || a.q_out.vec);
-            }
-            if (h0 + (u + 1) * abreast <= a.q_heads) continue;  // of the whole warp
-            // Extremes of the group, by all lanes: those of other kinds take part and are not used.
-            float high, low;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[2 * i] = Half<T>::first(w[i]), r[2 * i + 1] = Half<T>::second(w[i]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                r[i] = r[i] != r[i] ? 0.0f : fminf(fmaxf(r[i], -Half<T>::MOST), Half<T>::MOST);
-                high = i ? fmaxf(high, r[i]) : r[0];
-                low = i ? fminf(low, r[i]) : r[0];
-            }
-            for (int o = 1; o < per_group; o <<= 1) {
-                high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
-                low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-            }
-            if (!live || query) continue;
-            const float mid = to_f32(from_f32<T>(__fadd_rn(high * 0.5f, low * 0.5f)));
-            float scale = to_f32(from_f32<T>(__fdiv_rn(__fsub_rn(high * 0.5f, low * 0.5f), 7.5f)));
-            // half of the largest float and 7.5 halves of the scale: what is held stays within the type
-            if (fmaf(3.75f, scale, 0.5f * fabsf(mid)) > 0.5f * Half<T>::MOST) scale = Half<T>::below(scale);
-            const float inverse = scale > 0x1p-120f ? __frcp_rn(scale) : 0.0f;
-            const uint32_t codes = scale > 0.0f ? codes_of(r, mid, scale, inverse) : 0u;
-            const int head = h - a.q_heads - (value ? a.kv.heads : 0);
-            uint8_t* to = block + head * a.kv.head_bytes;
-            if (value) {
-                *reinterpret_cast<uint16_t*>(to + kv_value_half(dim, a.kv.groups, t, channel)) = static_cast<uint16_t>(codes);
-                *reinterpret_cast<uint16_t*>(to + kv_value_half(dim, a.kv.groups, t, channel + 4)) = static_cast<uint16_t>(codes >> 16);
             } else {
-                *reinterpret_cast<uint32_t*>(to + kv_key_word(dim, t, channel)) = codes;
+                const Rows* from;
+                int local;
+                place(h, &from, &local);
+                const T* head = static_cast<const T*>(from->p) + row * from->rs + local * dim;
+                const float *cos = a.cos + at * a.turn_rs, *sin = a.sin + at * a.turn_rs;
+                const int half = a.turned / 2;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[2 * i] = Half<T>::first(w[i]), r[2 * i + 1] = Half<T>::second(w[i]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int ch = channel + i;
+                    if (ch >= a.turned) break;
+                    const bool low = a.interleaved ? ch % 2 == 0 : ch < half;
+                    const int pair = a.interleaved ? ch / 2 : low ? ch : ch - half;
+                    const int with = a.interleaved ? ch ^ 1 : low ? ch + half : ch - half;
+                    r[i] = turned(r[i], cos[pair], to_f32(head[with]), low ? sin[pair] : -sin[pair]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = Half<T>::pair(r[2 * i], r[2 * i + 1]);
             }
-            if ((channel & ((1 << a.kv.group_shift) - 1)) == 0) {
-                const uint32_t both = Half<T>::pair(scale, mid);
-                auto* p = reinterpret_cast<uint16_t*>(to + kv_scale(dim, a.kv.groups, t, g, value));
-                p[0] = static_cast<uint16_t>(both);
-                p[2] = static_cast<uint16_t>(both >> 16);
-            }
+        }
+        __syncwarp();  // queries may turn in place: no lane writes what another still reads
+        if (live && query) {
+            store8(static_cast<uint16_t*>(a.q_out.p) + row * a.q_out.rs + h * dim + channel, make_uint4(w[0], w[1], w[2], w[3]),
+                   VEC || a.q_out.vec);
+        }
+        if (h0 + abreast <= a.q_heads) continue;  // of the whole warp
+        // Extremes of the group, by all lanes: those of other kinds take part and are not used.
+        float high, low;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[2 * i] = Half<T>::first(w[i]), r[2 * i + 1] = Half<T>::second(w[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            r[i] = r[i] != r[i] ? 0.0f : fminf(fmaxf(r[i], -Half<T>::MOST), Half<T>::MOST);
+            high = i ? fmaxf(high, r[i]) : r[0];
+            low = i ? fminf(low, r[i]) : r[0];
+        }
+        for (int o = 1; o < per_group; o <<= 1) {
+            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, o));
+            low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+        }
+        if (!live || query) continue;
+        const float mid = to_f32(from_f32<T>(__fadd_rn(high * 0.5f, low * 0.5f)));
+        float scale = to_f32(from_f32<T>(__fdiv_rn(__fsub_rn(high * 0.5f, low * 0.5f), 7.5f)));
+        // half of the largest float and 7.5 halves of the scale: what is held stays within the type
+        if (fmaf(3.75f, scale, 0.5f * fabsf(mid)) > 0.5f * Half<T>::MOST) scale = Half<T>::below(scale);
+        const float inverse = scale > 0x1p-120f ? __frcp_rn(scale) : 0.0f;
+        const uint32_t codes = scale > 0.0f ? codes_of(r, mid, scale, inverse) : 0u;
+        const int head = h - a.q_heads - (value ? a.kv.heads : 0);
+        uint8_t* to = block + head * a.kv.head_bytes;
+        if (value) {
+            *reinterpret_cast<uint16_t*>(to + kv_value_half(dim, a.kv.groups, t, channel)) = static_cast<uint16_t>(codes);
+            *reinterpret_cast<uint16_t*>(to + kv_value_half(dim, a.kv.groups, t, channel + 4)) = static_cast<uint16_t>(codes >> 16);
+        } else {
+            *reinterpret_cast<uint32_t*>(to + kv_key_word(dim, t, channel)) = codes;
+        }
+        if ((channel & ((1 << a.kv.group_shift) - 1)) == 0) {
+            const uint32_t both = Half<T>::pair(scale, mid);
+            auto* p = reinterpret_cast<uint16_t*>(to + kv_scale(dim, a.kv.groups, t, g, value));
+            p[0] = static_cast<uint16_t>(both);
+            p[2] = static_cast<uint16_t>(both >> 16);
         }
     }
 }

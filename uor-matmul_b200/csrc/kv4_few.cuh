@@ -37,11 +37,11 @@
 // block had whole. Cutting the last third of the work smaller and letting blocks take it as they come free
 // evened their ends out (83 to 165 us after the start) but cost as much in beginnings: 178 us, not 167.
 //
-// 64 contexts of 8192, 8 heads of 128 channels with 8 queries each, bfloat16: 167 us, 4.0 TB/s of codes
-// and scales; 351 instructions a block of 16 tokens and warp, of which the half-rate integer pipe has 64 %
-// of its cycles full on a processor with four blocks, the tensor pipe 32. One token in 4096: 12.4 us, of
-// which the sequences' scan takes 1.8, a table entry and then a block's arrival 2, three blocks to a warp
-// and their sums 4.5, and the second kernel 2.5 behind the last block.
+// 64 contexts of 8192, 8 heads of 128 channels with 8 queries each, bfloat16: 169 us, 4.0 TB/s of codes
+// and scales; 388 instructions a block of 16 tokens and warp, 60 % of all issue slots (a tenth more on
+// processors with four blocks than on average; the half-rate integer pipe is as busy). One token in 4096:
+// 12.5 us, of which the sequences' scan takes 1.8, a table entry and then a block's arrival 2, three blocks
+// to a warp and their sums 4.5, and the second kernel 2.5 behind the last block.
 #pragma once
 #include "kv4_math.cuh"
 
