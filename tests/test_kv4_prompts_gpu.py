@@ -214,3 +214,18 @@ def test_two_streams_and_a_graph():
     del graph
     for ctx in ctxs:
         ctx.close()
+
+
+def test_pages_past_4_gb():
+    """The same pages at the end of a pool of more than 2^32 bytes: the same bytes."""
+    c = Cache([300, 40], [200, 40], 16, 2, 64, 32, U.BF16, seed=11).fill()
+    q = c.queries(2)
+    here = _run(c, q, 2)
+    size = U.kv4_page_bytes(16, 2, 64, 32, U.BF16)
+    behind = (1 << 32) // size + 1
+    pool = torch.empty((behind + c.pages) * size, dtype=torch.uint8, device="cuda")
+    pool[behind * size:] = c.pool
+    c.kv = U.KV4(pool, behind + c.pages, 16, 2, 64, 32, U.BF16)
+    c.table[c.table >= 0] += behind
+    there = _run(c, q, 2)
+    assert all(torch.equal(a, b) for a, b in zip(here, there))
