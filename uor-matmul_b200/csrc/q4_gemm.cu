@@ -330,8 +330,14 @@ int launch_combine(uor_b200_ctx* ctx, const float* part, int splits, const FfnAr
 // fit the processors many passes abreast: 2048 x 2048 with 64 rows 9.4 : 15.0, 128 14.6 : 17.8,
 // 256 40 : 18.5; 768 x 768 with 512 rows 12 : 17, 1024 20 : 17; 1000 x 1001 with 128 rows 11.5 : 34,
 // 512 30 : 35. That is up to 2^25 weights and passes together.
-bool few_rows(int64_t m, const Q4Dev& w) {
+//
+// What follows a product (q4_linear; with bias and residual) costs the few-rows kernel, which reads and
+// writes element by element, 7 us a million outputs and the other 2.5: 512 x 1856 outputs of 128 positions
+// 18.9 : 17.1, 1901 x 1856 85 : 29, 1900 x 512 of 512 26.5 : 21.5; 1000 x 704 of 256 20.0 : 21.0, 512 x 1024 of
+// 1024 18.9 : 22.0. That is up to 3 2^18 outputs.
+bool few_rows(int64_t m, const Q4Dev& w, bool followed) {
     const int64_t passes = (m + 15) / 16, cols = m < 16 ? m : 16;
+    if (followed && passes > 1 && m * w.rows > int64_t(3) << 18) return false;
     return m <= 2 || (cols * w.cols <= 57344 && (passes == 1 || (passes <= 65535 && passes * w.rows * w.cols <= int64_t(1) << 25)));
 }
 
@@ -357,7 +363,7 @@ int run_q4_gemm(uor_b200_ctx* ctx, int elem, const Mat& x, int64_t m, const Q4De
     route->kernel = UOR_B200_KERNEL_Q4;
     if (w.cols == 0) return zeros_out(ctx, m, w.rows, e, y);
     int st = UOR_B200_OK;
-    const bool few = few_rows(m, w);
+    const bool few = few_rows(m, w, e.on != 0);
     Pieces pieces;
     // The few-rows kernel reads any row whose elements follow one another.
     const bool own_rows = few ? x.cs != 1 : !x_in_place(x, w.cols);
