@@ -639,8 +639,9 @@ def _placed(buf, v, t):
 
 
 def _same_place(first, *others):
-    if any(o != first for o in others):
-        raise ValueError("operands must all be host arrays or all be CUDA tensors")
+    for o in others:
+        if o != first:
+            raise ValueError("operands must all be host arrays or all be CUDA tensors")
     return first
 
 
@@ -687,7 +688,8 @@ def kv4_append(elem, cache, batch, k, kv, v, vv, q=None, qv=None, q_out=None, ov
     positions, and q (rows x query heads * dim), where given, rotated into q_out (or in place)."""
     of = elem if elem in (BF16, F16) else None
     K, V = _rows_of(k, kv, of), _rows_of(v, vv, of)
-    Q, O = (None if x is None else _rows_of(x, xv, of) for x, xv in ((q, qv), (q_out, ov)))
+    Q = None if q is None else _rows_of(q, qv, of)
+    O = None if q_out is None else _rows_of(q_out, ov, of)  # noqa: E741
     call = make_call(NEAREST, True, ctx, route, asynchronous)
     _check(lib().uor_b200_kv4_append(elem, cache, batch, K, V, Q, O, rotation, call), "kv4_append")
 
